@@ -8,10 +8,15 @@ the module name ``fa2_with_4d_mask_b200`` by ``tilelang_fa2_4d_mask/__init__.py`
 
 from .fa2 import causal_mode, flash_attention_with_4d_mask
 from .modeling_attention import tilelang_attention_forward, tilelang_flash_attention
+from .rotary import MultiAxisRotary
+from .shared_prefix import evict_by_weight, shared_prefix_attention
 
 __all__ = [
     "flash_attention_with_4d_mask",
     "tilelang_attention_forward",
     "tilelang_flash_attention",
     "causal_mode",
+    "MultiAxisRotary",
+    "shared_prefix_attention",
+    "evict_by_weight",
 ]

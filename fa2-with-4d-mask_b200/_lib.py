@@ -10,6 +10,7 @@ point raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 from typing import Optional
@@ -54,8 +55,14 @@ EXPORTED_SYMBOLS = (
     "fa4d_bwd_workspace_size_ex",
     "fa4d_bwd_group_split",
     "fa4d_mask_prepare_docs",
+    "fa4d_rotary",
+    "fa4d_rotary_append",
+    "fa4d_prefix_attention",
+    "fa4d_prefix_attention_workspace",
+    "fa4d_evict",
 )
 DEV_TIMEOUT_FWD, DEV_TIMEOUT_BWD, DEV_TIMEOUT_CHECK = 1, 2, 4
+DEV_TIMEOUT_PREFIX, DEV_CACHE_FULL = 16, 32
 
 ABI_VERSION = 2
 BLOCK = 128  # rows / keys per block of the mask's block map
@@ -140,6 +147,83 @@ class BwdArgs(ctypes.Structure):
     ]
 
 
+ROTARY_MAX_PAIRS = 128
+PAIR_HALF, PAIR_ADJACENT = 0, 1
+_i64x2 = ctypes.c_int64 * 2
+
+
+class RotaryTable(ctypes.Structure):
+    """Mirror of ``fa4d_rotary_table``."""
+
+    _fields_ = [
+        ("turn", ctypes.c_uint64 * ROTARY_MAX_PAIRS),
+        ("axis", ctypes.c_uint8 * ROTARY_MAX_PAIRS),
+        ("D", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("pairing", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``fa4d_rotary_args``."""
+
+    _fields_ = [
+        ("table", RotaryTable),
+        *((n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "positions")),
+        *((n, _i64x3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride", "positions_stride")),
+        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "dtype", "positions_bits", "inverse")),
+    ]
+
+
+class RotaryAppendArgs(ctypes.Structure):
+    """Mirror of ``fa4d_rotary_append_args``."""
+
+    _fields_ = [
+        ("table", RotaryTable),
+        *((n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "weights", "positions",
+                                         "lengths", "lengths_out")),
+        *((n, _i64x3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_cache_stride",
+                                "v_cache_stride")),
+        ("weights_stride", _i64x2),
+        ("positions_stride", _i64x3),
+        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "C", "dtype", "positions_bits")),
+    ]
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    """Mirror of ``fa4d_prefix_attention_args``."""
+
+    _fields_ = [
+        *((n, ctypes.c_void_p) for n in ("q", "prefix_k", "prefix_v", "k", "v", "o", "lengths", "mask", "weights",
+                                         "workspace")),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("q_stride", _i64x3),
+        ("prefix_k_stride", _i64x2),
+        ("prefix_v_stride", _i64x2),
+        *((n, _i64x3) for n in ("k_stride", "v_stride", "o_stride", "mask_stride")),
+        ("weights_stride", _i64x2),
+        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "D", "P", "C", "dtype", "causal")),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of ``fa4d_evict_args``."""
+
+    _fields_ = [
+        *((n, ctypes.c_void_p) for n in ("k", "v", "weights", "lengths", "k_out", "v_out", "weights_out",
+                                         "lengths_out", "index_out")),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("weights_stride", _i64x2),
+        ("k_out_stride", _i64x3),
+        ("v_out_stride", _i64x3),
+        ("weights_out_stride", _i64x2),
+        *((n, ctypes.c_int32) for n in ("B", "C", "Hk", "D", "keep", "sinks", "recent")),
+    ]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -207,6 +291,13 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         ctypes.c_void_p,
     ]
     lib.fa4d_mask_prepare_docs.restype = ctypes.c_int
+    for name, args in (("fa4d_rotary", RotaryArgs), ("fa4d_rotary_append", RotaryAppendArgs),
+                       ("fa4d_prefix_attention", PrefixAttentionArgs), ("fa4d_evict", EvictArgs)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    lib.fa4d_prefix_attention_workspace.argtypes = [ctypes.c_int32] * 8
+    lib.fa4d_prefix_attention_workspace.restype = ctypes.c_size_t
     version = lib.fa4d_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"{p}: ABI version {version}, expected {ABI_VERSION}; rebuild with build.py")
@@ -563,8 +654,29 @@ def backward(
     return dq, dk, dv
 
 
+def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
+    """Enqueues entry point ``name`` with its args structure on the device's current stream."""
+    lib = load_library()
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != FA4D_OK:
+        _raise(lib, rc, name)
+
+
+@functools.lru_cache(maxsize=256)
+def prefix_attention_workspace(index: int, *sizes: int) -> int:
+    """Bytes of fa4d_prefix_attention's workspace on device ``index`` for (B, T, Hq, Hk, D,
+    P, C, weights); 0 for sizes it refuses."""
+    with torch.cuda.device(index):
+        return int(load_library().fa4d_prefix_attention_workspace(*sizes))
+
+
 def device_status(device: Optional[torch.device] = None, clear: bool = True) -> int:
-    """Synchronises the current stream and returns the kernels' timeout bits (0 = none)."""
+    """Synchronises the current stream and returns the kernels' status bits (0 = none)."""
     lib = load_library()
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     if device.index is None:

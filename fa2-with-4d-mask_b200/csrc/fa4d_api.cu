@@ -890,3 +890,16 @@ int fa4d_bwd_noalloc(const fa4d_bwd_args* a, void* stream) {
 }
 
 }  // extern "C"
+
+// What the other host files of the library (fa4d_cache_api.cu) use of this one.
+namespace fa4d {
+int host_fail(int code, const char* message) { return fail(code, "%s", message); }
+int host_ok() { return ok(); }
+int host_bind_device_of(const void* ptr, const char* name) { return bind_device_of(ptr, name); }
+int* host_status_word() { return status_word_ptr(); }
+int host_sm_count() { return sm_count(); }
+int host_encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
+                     bool bf16, const char* name) {
+  return encode_bthd(m, ptr, B, T, H, D, st, rows, bf16, name);
+}
+}  // namespace fa4d

@@ -6,6 +6,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "fa4d.h"
+
 namespace fa4d {
 
 // Forward: one CTA owns 2 x 128 query rows of one (batch, query head) and streams
@@ -230,6 +232,11 @@ cudaError_t launch_dq256(const DqParams& p, bool bf16, bool has_mask, bool has_s
 cudaError_t launch_mask_blocks(const MaskBlocksParams& p, cudaStream_t s);
 cudaError_t launch_mask_prepare(const MaskPrepParams& p, cudaStream_t s);
 cudaError_t launch_wait_timeout_check(int* status, long long limit, cudaStream_t s);
+// `vec`: every row is a multiple of 16 bytes from a 16-byte boundary (and, for the rotary
+// forms, the pairs and the copied rest divide into runs of 8).
+cudaError_t launch_rotary(const fa4d_rotary_args& a, bool vec, int sms, cudaStream_t s);
+cudaError_t launch_rotary_append(const fa4d_rotary_append_args& a, bool vec, int* status, cudaStream_t s);
+cudaError_t launch_evict(const fa4d_evict_args& a, bool vec, int sms, cudaStream_t s);
 cudaError_t launch_exp2_check(float* out, int n, float lo, float hi, cudaStream_t s);
 
 }  // namespace fa4d

@@ -230,7 +230,7 @@ class _flash_attention_with_4d_mask(torch.autograd.Function):
         if _CHECK_STATUS:
             # Opt-in: synchronise and raise if any kernel since the last check gave up a
             # bounded wait (its outputs are then garbage).
-            bits = _lib.device_status(q.device)
+            bits = _lib.device_status(q.device) & ~_lib.DEV_CACHE_FULL
             if bits:
                 raise RuntimeError(f"an attention kernel gave up a bounded wait (device status {bits:#x})")
         if ctx.bhsd_input:

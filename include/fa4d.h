@@ -253,6 +253,140 @@ int fa4d_mask_prepare(const uint8_t* mask, const int64_t mask_stride[3], int32_t
 int fa4d_mask_prepare_docs(const int32_t* doc_q, const int32_t* doc_k, const int64_t doc_stride[2], int32_t Bm,
                            int32_t Tq, int32_t Tk, void* prepared, void* stream);
 
+/* ------------------------------------------------------------------ around the attention
+ * Operators a serving or multi-axis-position user needs next to the attention above; none
+ * has a counterpart in the reference. */
+
+/* Rotary positions with several axes.  The first rotary_dim elements of a head form
+ * rotary_dim / 2 pairs, (i, i + rotary_dim / 2) or (2 i, 2 i + 1); pair i is turned by the
+ * angle positions[axis[i]][b][t] * turn[i], counted in 2^-64 turns modulo a turn, so it is
+ * exact for every 64-bit position.  Elements past rotary_dim are copied. */
+#define FA4D_ROTARY_MAX_PAIRS 128
+enum fa4d_pairing { FA4D_PAIR_HALF = 0, FA4D_PAIR_ADJACENT = 1 };
+
+typedef struct fa4d_rotary_table {
+  uint64_t turn[FA4D_ROTARY_MAX_PAIRS]; /* turns per position, in 2^-64 turns */
+  uint8_t axis[FA4D_ROTARY_MAX_PAIRS];  /* position axis of each pair, < axes */
+  int32_t D;                            /* head dim: even, <= 2 * FA4D_ROTARY_MAX_PAIRS */
+  int32_t rotary_dim;                   /* even, 2..D */
+  int32_t pairing;                      /* enum fa4d_pairing */
+  int32_t axes;
+} fa4d_rotary_table;
+
+typedef struct fa4d_rotary_args {
+  fa4d_rotary_table table;
+  const void* q;             /* [B, T, Hq, D] */
+  const void* k;             /* [B, T, Hk, D] */
+  void* q_out;               /* written; must not overlap an input */
+  void* k_out;
+  const void* positions;     /* [axes, B or 1, T] integers */
+  int64_t q_stride[3];       /* element strides (batch, seq, head), head-dim stride 1 */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  int64_t positions_stride[3]; /* (axis, batch, seq), 0 where broadcast */
+  int32_t B, T, Hq, Hk;
+  int32_t dtype;             /* enum fa4d_dtype */
+  int32_t positions_bits;    /* 32 or 64 */
+  int32_t inverse;           /* 1: turns by the negative angle (the gradient of the other) */
+} fa4d_rotary_args;
+
+/* q_out, k_out = the turned q, k. */
+int fa4d_rotary(const fa4d_rotary_args* args, void* stream);
+
+typedef struct fa4d_rotary_append_args {
+  fa4d_rotary_table table;
+  const void* q;             /* [B, T, Hq, D] new tokens */
+  const void* k;             /* [B, T, Hk, D] */
+  const void* v;             /* [B, T, Hk, D] */
+  void* q_out;               /* [B, T, Hq, D] written */
+  void* k_cache;             /* [B, C, Hk, D], slots lengths[b] + t written */
+  void* v_cache;
+  float* weights;            /* [B, Hk, C] or NULL: set to 0 at the written slots */
+  const void* positions;     /* [axes, B or 1, T] integers */
+  const int32_t* lengths;    /* [B] entries in each cache before the call */
+  int32_t* lengths_out;      /* [B] written: min(lengths + T, C); may not be `lengths` */
+  int64_t q_stride[3];       /* element strides (batch, seq, head) */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_cache_stride[3]; /* (batch, slot, head) */
+  int64_t v_cache_stride[3];
+  int64_t weights_stride[2]; /* (batch, head), slot stride 1 */
+  int64_t positions_stride[3];
+  int32_t B, T, Hq, Hk, C;
+  int32_t dtype;
+  int32_t positions_bits;
+} fa4d_rotary_append_args;
+
+/* The serving form: q_out = the turned q; the turned k and v go to the cache slots.  A token
+ * whose slot lies outside [0, C) is not stored and sets FA4D_DEV_CACHE_FULL. */
+int fa4d_rotary_append(const fa4d_rotary_append_args* args, void* stream);
+
+/* Attention of a few new tokens per request over a prefix that all requests share and the
+ * request's own cache, in one softmax:
+ *   keys of (b, t) = prefix 0..P-1 and own slots j < lengths[b], with causal also
+ *   j <= lengths[b] - T + t (the T new tokens are the cache's last), with mask also
+ *   mask[b, h, t, j] != 0;  o = softmax(scale q k^T) v, 0 where there is no key.
+ * weights (optional) gains, for each own slot, the probability it received, summed over the
+ * query heads of the KV head's group and the T tokens. */
+typedef struct fa4d_prefix_attention_args {
+  const void* q;             /* [B, T, Hq, D] */
+  const void* prefix_k;      /* [P, Hk, D]; NULL iff P == 0 */
+  const void* prefix_v;
+  const void* k;             /* [B, C, Hk, D] own caches */
+  const void* v;
+  void* o;                   /* [B, T, Hq, D], written */
+  const int32_t* lengths;    /* [B]: valid own slots, clamped to [0, C] */
+  const uint8_t* mask;       /* [B or 1, Hq or 1, T, C] or NULL; nonzero byte = keep */
+  float* weights;            /* [B, Hk, C] or NULL, added to */
+  void* workspace;           /* >= fa4d_prefix_attention_workspace() bytes, 256-B aligned */
+  size_t workspace_bytes;
+  int64_t q_stride[3];       /* element strides (batch, seq, head), head-dim stride 1 */
+  int64_t prefix_k_stride[2]; /* (seq, head) */
+  int64_t prefix_v_stride[2];
+  int64_t k_stride[3];       /* (batch, slot, head) */
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t mask_stride[3];    /* (batch, head, token), 0 where broadcast; slot stride 1 */
+  int64_t weights_stride[2]; /* (batch, head), slot stride 1 */
+  int32_t B, T, Hq, Hk, D, P, C;
+  int32_t dtype;
+  int32_t causal;            /* 0 or 1 */
+  float scale;
+} fa4d_prefix_attention_args;
+
+/* Bytes of scratch for these sizes on the current device (partial results of the key
+ * splits, and the logits of the own keys when `weights`); 0 for invalid sizes. */
+size_t fa4d_prefix_attention_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C,
+                                       int32_t weights);
+int fa4d_prefix_attention(const fa4d_prefix_attention_args* args, void* stream);
+
+/* Eviction by weight: with n = lengths[b] clamped to [0, C], a cache of n <= keep entries is
+ * copied; of a longer one each KV head keeps its first `sinks` and last `recent` entries and
+ * the keep - sinks - recent heaviest of the others (equal weights: the lower index first; NaN
+ * counts as the smallest), in their order.  Slots from min(n, keep) to keep-1 of the outputs
+ * are zero (index -1). */
+typedef struct fa4d_evict_args {
+  const void* k;             /* [B, C, Hk, D] 16-bit elements */
+  const void* v;
+  const float* weights;      /* [B, Hk, C] */
+  const int32_t* lengths;    /* [B] */
+  void* k_out;               /* [B, >= keep, Hk, D]; must not overlap an input */
+  void* v_out;
+  float* weights_out;        /* [B, Hk, >= keep] */
+  int32_t* lengths_out;      /* [B]: min(n, keep) */
+  int32_t* index_out;        /* [B, Hk, keep]: the slot each entry came from */
+  int64_t k_stride[3];       /* element strides (batch, slot, head), head-dim stride 1 */
+  int64_t v_stride[3];
+  int64_t weights_stride[2]; /* (batch, head), slot stride 1 */
+  int64_t k_out_stride[3];
+  int64_t v_out_stride[3];
+  int64_t weights_out_stride[2];
+  int32_t B, C, Hk, D, keep, sinks, recent;
+} fa4d_evict_args;
+int fa4d_evict(const fa4d_evict_args* args, void* stream);
+
 /* Message for the last non-zero return on this thread ("" if none). */
 const char* fa4d_last_error(void);
 
@@ -266,6 +400,9 @@ const char* fa4d_last_error(void);
 /* A kernel whose shared-memory layout leaves no alignment slack found its dynamic shared
  * memory base not 1024-byte aligned and returned without computing (not seen on B200). */
 #define FA4D_DEV_SMEM_ALIGN 8
+/* fa4d_prefix_attention gave up a bounded wait; fa4d_rotary_append found a cache full. */
+#define FA4D_DEV_TIMEOUT_PREFIX 16
+#define FA4D_DEV_CACHE_FULL 32
 int fa4d_device_status(int device, void* stream, int clear);
 
 /* Diagnostic (no counterpart in the reference): runs the kernels' bounded mbarrier

@@ -3,7 +3,7 @@
 Loads the implementation package from the ``fa2-with-4d-mask_b200`` directory
 next to this one under the module name ``fa2_with_4d_mask_b200`` and re-exports
 the reference's public names (tilelang_fa2_4d_mask/__init__.py:3-10 of the
-reference).
+reference), and beside them this library's own operators around the attention.
 """
 
 from __future__ import annotations
@@ -38,9 +38,15 @@ _impl = load_impl()
 flash_attention_with_4d_mask = _impl.flash_attention_with_4d_mask
 tilelang_attention_forward = _impl.tilelang_attention_forward
 tilelang_flash_attention = _impl.tilelang_flash_attention
+MultiAxisRotary = _impl.MultiAxisRotary
+shared_prefix_attention = _impl.shared_prefix_attention
+evict_by_weight = _impl.evict_by_weight
 
 __all__ = [
     "flash_attention_with_4d_mask",
     "tilelang_attention_forward",
     "tilelang_flash_attention",
+    "MultiAxisRotary",
+    "shared_prefix_attention",
+    "evict_by_weight",
 ]
