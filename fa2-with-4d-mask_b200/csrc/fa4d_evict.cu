@@ -16,7 +16,9 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;  // of a radix pass: 11, 11 and 10 bits of the weight
+constexpr int kEach = 16;                    // weights of a thread, kept in registers
+constexpr int kChunk = kThreads * kEach;     // weights of a CTA at a time
+constexpr int kBins = 2048;                  // of a radix pass: 11, 11 and 10 bits of the weight
 constexpr int kRowsInFlight = 4;
 
 // Larger weight, larger key; -0 as 0; NaN below everything.
@@ -39,9 +41,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
 
 struct Smem {
   alignas(16) uint32_t hist[kBins];
-  alignas(16) uint32_t counts[4];  // of this CTA's slice: kept for sure, equal to the threshold
-  uint32_t warp_sum[2][kWarps];
+  alignas(16) uint32_t counts[4];     // of this CTA's slice: kept for sure, equal to the threshold
+  uint32_t group[kEach * kWarps];     // of each 32 weights in order: both counts, 16 bits each
+  uint32_t warp_sum[kWarps];
   uint32_t found[2];
+  int32_t list[kChunk];               // slots of this CTA's share (selection without slices)
 };
 
 // Sum of x over the threads before this one; `all` is the sum over the CTA.
@@ -80,11 +84,16 @@ struct Piece<1> {
   static __device__ __forceinline__ T zero() { return 0; }
 };
 
+// Caches of up to kChunk entries are selected by every CTA of the cluster for itself (the
+// weights are a few hundredths of the rows, and nothing waits between CTAs); of longer ones
+// each CTA takes a slice of the weights.  Weights stay in registers across the passes
+// (re-read where a slice is longer than kChunk).
 template <int VEC>
-__global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__ fa4d_evict_args a) {
+__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constant__ fa4d_evict_args a) {
   __shared__ Smem sm;
   const int rank = static_cast<int>(cluster_rank()), ranks = static_cast<int>(cluster_size());
   const int item = static_cast<int>(blockIdx.x) / ranks;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int b = item / a.Hk, h = item - b * a.Hk;
   const int n = min(max(__ldg(a.lengths + b), 0), a.C);
   const int kept = min(n, a.keep);
@@ -93,45 +102,71 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
   int32_t* index = a.index_out + static_cast<int64_t>(item) * a.keep;
   if (h == 0 && rank == 0 && threadIdx.x == 0) a.lengths_out[b] = kept;
 
+  const bool sliced = n > kChunk;
+  const int share = (a.keep + ranks - 1) / ranks;
+  const int slot0 = min(rank * share, a.keep), slot1 = min(slot0 + share, a.keep);
+
   if (n > a.keep) {
     // The middle [a.sinks, late) gives its `want` heaviest entries.
     const int late = n - a.recent;
-    const uint32_t want_all = a.keep - a.sinks - a.recent;
-    const int per = (n + ranks - 1) / ranks;
-    const int lo = min(rank * per, n), hi = min(lo + per, n);
-    const int mid_lo = max(lo, a.sinks), mid_hi = min(hi, late);
+    uint32_t want = a.keep - a.sinks - a.recent, prefix = 0;
+    const bool none = want == 0;
+    const int per = sliced ? (n + ranks - 1) / ranks : n;
+    const int lo = sliced ? min(rank * per, n) : 0, hi = min(lo + per, n);
+    const bool once = hi - lo <= kChunk;
 
-    // Radix selection of the want_all-th largest key of the middle.
-    uint32_t want = want_all, prefix = 0;
-    if (want_all > 0) {
+    float x[kEach];  // the weights j = base + i * kThreads + threadIdx.x
+    auto load = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int j = base + i * kThreads + threadIdx.x;
+        x[i] = j < hi ? __ldg(w + j) : 0.f;
+      }
+    };
+    auto in_middle = [&](int j) { return j >= a.sinks && j < late && j < hi; };
+    load(lo);
+
+    // Radix selection of the want-th largest key of the middle, from the top bits down.
+    if (!none) {
       constexpr int kShift[3] = {21, 10, 0};
       constexpr int kBits[3] = {11, 11, 10};
 #pragma unroll
       for (int pass = 0; pass < 3; ++pass) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
+        *reinterpret_cast<uint4*>(&sm.hist[4 * threadIdx.x]) = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
-        for (int j = mid_lo + threadIdx.x; j < mid_hi; j += kThreads) {
-          const uint32_t key = order_key(__ldg(w + j));
-          if (pass == 0 || (key >> (kShift[pass] + kBits[pass])) == prefix)
-            atomicAdd(&sm.hist[(key >> kShift[pass]) & ((1u << kBits[pass]) - 1u)], 1u);
+        for (int base = lo; base < hi; base += kChunk) {
+          if (!once) load(base);
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            const uint32_t key = order_key(x[i]);
+            if (in_middle(base + i * kThreads + threadIdx.x) &&
+                (pass == 0 || (key >> (kShift[pass] + kBits[pass])) == prefix))
+              atomicAdd(&sm.hist[(key >> kShift[pass]) & ((1u << kBits[pass]) - 1u)], 1u);
+          }
         }
-        cluster_sync();
-        // Thread i has bins 4 i' .. 4 i' + 3 with i' counted from the top, so that scans run
-        // from the largest key down.
+        // Thread i has four bins, counted from the top, so that scans run from the largest
+        // key down.
         const int bin0 = kBins - 4 - 4 * threadIdx.x;
         uint4 c = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t mine = smem_u32(&sm.hist[bin0]);
-        for (int r = 0; r < ranks; ++r) {
-          const uint4 x = ld_cluster_v4(peer_addr(mine, r));
-          c.x += x.x;
-          c.y += x.y;
-          c.z += x.z;
-          c.w += x.w;
+        if (sliced) {
+          cluster_sync();
+          const uint32_t mine = smem_u32(&sm.hist[bin0]);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r >= ranks) break;
+            const uint4 y = ld_cluster_v4(peer_addr(mine, r));
+            c.x += y.x;
+            c.y += y.y;
+            c.z += y.z;
+            c.w += y.w;
+          }
+        } else {
+          __syncthreads();
+          c = *reinterpret_cast<const uint4*>(&sm.hist[bin0]);
         }
         uint32_t all;
-        const uint32_t above = scan_before(c.x + c.y + c.z + c.w, sm.warp_sum[0], all);
+        uint32_t upto = scan_before(c.x + c.y + c.z + c.w, sm.warp_sum, all);
         const uint32_t cnt[4] = {c.w, c.z, c.y, c.x};
-        uint32_t upto = above;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (upto < want && want <= upto + cnt[e]) {
@@ -140,61 +175,92 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
           }
           upto += cnt[e];
         }
-        cluster_sync();  // every CTA has read the histograms; `found` is written
+        // `found` is written, and the histograms are read.
+        if (sliced)
+          cluster_sync();
+        else
+          __syncthreads();
         prefix = (prefix << kBits[pass]) | sm.found[0];
         want = sm.found[1];
       }
     }
     // Kept: sinks, recent, keys above `prefix`, and the first `want` equal to it.
-    const bool none = want_all == 0;
-    auto state = [&](int j, float& x) {  // 1: kept for sure, 2: equal to the threshold
-      x = __ldg(w + j);
+    auto state = [&](int j, float v) {  // 1: kept for sure, 2: equal to the threshold
+      if (j >= hi) return 0;
       if (j < a.sinks || j >= late) return 1;
-      const uint32_t key = order_key(x);
+      const uint32_t key = order_key(v);
       return none ? 0 : key > prefix ? 1 : key == prefix ? 2 : 0;
     };
-    uint32_t sure = 0, equal = 0;
-    for (int j = lo + threadIdx.x; j < hi; j += kThreads) {
-      float x;
-      const int st = state(j, x);
-      sure += st == 1;
-      equal += st == 2;
-    }
-    uint32_t sure_all, equal_all;
-    scan_before(sure, sm.warp_sum[0], sure_all);
-    scan_before(equal, sm.warp_sum[1], equal_all);
-    if (threadIdx.x == 0) {
-      sm.counts[0] = sure_all;
-      sm.counts[1] = equal_all;
-    }
-    cluster_sync();
-    uint32_t sure_before = 0, equal_before = 0;  // of the entries before this chunk
-    for (int r = 0; r < rank; ++r) {
-      const uint4 x = ld_cluster_v4(peer_addr(smem_u32(sm.counts), r));
-      sure_before += x.x;
-      equal_before += x.y;
-    }
-    for (int j0 = lo; j0 < hi; j0 += kThreads) {
-      const int j = j0 + threadIdx.x;
-      float x = 0.f;
-      const int st = j < hi ? state(j, x) : 0;
-      uint32_t chunk;  // both counts in one scan: at most 512 each
-      const uint32_t before = scan_before((st == 1 ? 1u : 0u) | (st == 2 ? 0x10000u : 0u), sm.warp_sum[0], chunk);
-      const uint32_t s = sure_before + (before & 0xffffu), e = equal_before + (before >> 16);
-      if (st == 1 || (st == 2 && e < want)) {
-        const uint32_t slot = s + min(e, want);
-        index[slot] = j;
-        w_out[slot] = x;
+    uint32_t sure_before = 0, equal_before = 0;  // of the entries before the chunk
+    if (sliced) {
+      uint32_t sure = 0, equal = 0;
+      for (int base = lo; base < hi; base += kChunk) {
+        if (!once) load(base);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int st = state(base + i * kThreads + threadIdx.x, x[i]);
+          sure += st == 1;
+          equal += st == 2;
+        }
       }
-      sure_before += chunk & 0xffffu;
-      equal_before += chunk >> 16;
+      uint32_t sure_all, equal_all;
+      scan_before(sure, sm.warp_sum, sure_all);
+      scan_before(equal, sm.warp_sum, equal_all);
+      if (threadIdx.x == 0) {
+        sm.counts[0] = sure_all;
+        sm.counts[1] = equal_all;
+      }
+      cluster_sync();
+      for (int r = 0; r < rank; ++r) {
+        const uint4 y = ld_cluster_v4(peer_addr(smem_u32(sm.counts), r));
+        sure_before += y.x;
+        equal_before += y.y;
+      }
     }
-    cluster_sync();  // the whole index is written, and no CTA reads another's memory any more
+    // Slots in order: a warp's 32 weights of each i by ballots, the groups by one scan.
+    for (int base = lo; base < hi; base += kChunk) {
+      if (!once) load(base);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int st = state(base + i * kThreads + threadIdx.x, x[i]);
+        const uint32_t sure = __ballot_sync(0xffffffffu, st == 1), equal = __ballot_sync(0xffffffffu, st == 2);
+        if (lane == 0) sm.group[i * kWarps + wid] = __popc(sure) | (__popc(equal) << 16);
+      }
+      __syncthreads();
+      uint32_t all;  // at most kChunk in each half
+      const uint32_t before =
+          scan_before(threadIdx.x < kEach * kWarps ? sm.group[threadIdx.x] : 0u, sm.warp_sum, all);
+      if (threadIdx.x < kEach * kWarps) sm.group[threadIdx.x] = before;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int j = base + i * kThreads + threadIdx.x;
+        const int st = state(j, x[i]);
+        const uint32_t sure = __ballot_sync(0xffffffffu, st == 1), equal = __ballot_sync(0xffffffffu, st == 2);
+        const uint32_t below = (1u << lane) - 1u, group = sm.group[i * kWarps + wid];
+        const uint32_t s = sure_before + (group & 0xffffu) + __popc(sure & below);
+        const uint32_t e = equal_before + (group >> 16) + __popc(equal & below);
+        if (st == 1 || (st == 2 && e < want)) {
+          const int slot = static_cast<int>(s + min(e, want));
+          if (sliced || (slot >= slot0 && slot < slot1)) {
+            index[slot] = j;
+            w_out[slot] = x[i];
+            if (!sliced) sm.list[slot - slot0] = j;
+          }
+        }
+      }
+      sure_before += all & 0xffffu;
+      equal_before += all >> 16;
+      if (!once) __syncthreads();  // the groups have been read
+    }
+    // The whole index (the share's list) is written; no CTA reads another's memory any more.
+    if (sliced)
+      cluster_sync();
+    else
+      __syncthreads();
   }
 
   // Copy slots [slot0, slot1).
-  const int share = (a.keep + ranks - 1) / ranks;
-  const int slot0 = min(rank * share, a.keep), slot1 = min(slot0 + share, a.keep);
   using T = typename Piece<VEC>::T;
   const int pieces = a.D / VEC;
   const uint16_t* k = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + h * a.k_stride[2];
@@ -211,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
       const int s = i / pieces;
       slot[u] = i < all ? slot0 + s : -1;
       c[u] = (i - s * pieces) * VEC;
-      from[u] = slot[u] < 0 || slot[u] >= kept ? -1 : n > a.keep ? index[slot[u]] : slot[u];
+      from[u] = slot[u] < 0 || slot[u] >= kept ? -1 : n <= a.keep ? slot[u] : sliced ? index[slot[u]] : sm.list[s];
     }
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {

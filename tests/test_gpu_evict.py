@@ -43,6 +43,8 @@ CASES = [
     (2, 2, 5000, 128, 1234, 1, 1233, torch.float16, "bhsd"),  # no room for the middle
     (70, 8, 300, 64, 200, 2, 50, torch.bfloat16, "bshd"),  # one CTA a head
     (1, 2, 20011, 256, 9000, 4, 1000, torch.bfloat16, "bhsd"),
+    (1, 1, 140003, 16, 70000, 4, 999, torch.float16, "bhsd"),  # a slice is more than a CTA keeps
+    (1, 2, 8193, 64, 8192, 0, 0, torch.bfloat16, "bshd"),
     (2, 2, 400, 20, 300, 3, 30, torch.float16, "bhsd"),  # rows that are no multiple of 16 bytes
 ]
 
