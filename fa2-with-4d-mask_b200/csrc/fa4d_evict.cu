@@ -16,10 +16,10 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kEach = 16;                    // weights of a thread, kept in registers
-constexpr int kChunk = kThreads * kEach;     // weights of a CTA at a time
-constexpr int kBins = 2048;                  // of a radix pass: 11, 11 and 10 bits of the weight
+constexpr int kChunk = 8192;  // weights of a CTA at a time
+constexpr int kBins = 2048;   // of a radix pass: 11, 11 and 10 bits of the weight
 constexpr int kRowsInFlight = 4;
+constexpr int kAhead = 4;     // shared-memory reads of a thread in flight
 
 // Larger weight, larger key; -0 as 0; NaN below everything.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -33,6 +33,12 @@ __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void add_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -41,11 +47,13 @@ __device__ __forceinline__ uint32_t cluster_size() {
 
 struct Smem {
   alignas(16) uint32_t hist[kBins];
-  alignas(16) uint32_t counts[4];     // of this CTA's slice: kept for sure, equal to the threshold
-  uint32_t group[kEach * kWarps];     // of each 32 weights in order: both counts, 16 bits each
+  alignas(16) uint32_t counts[4];  // of this CTA's slice: kept for sure, equal to the threshold
   uint32_t warp_sum[kWarps];
   uint32_t found[2];
-  int32_t list[kChunk];               // slots of this CTA's share (selection without slices)
+  alignas(16) uint32_t total[2][kBins];  // rank 0's, of slices: the cluster's histogram of even and odd passes
+  uint2 ballot[kChunk / 32];  // of each 32 entries: kept for sure, equal to the threshold
+  uint32_t key[kChunk];   // order_key of the weights
+  uint16_t list[kChunk];  // slots of this CTA's share (selection without slices)
 };
 
 // Sum of x over the threads before this one; `all` is the sum over the CTA.
@@ -86,11 +94,17 @@ struct Piece<1> {
 
 // Caches of up to kChunk entries are selected by every CTA of the cluster for itself (the
 // weights are a few hundredths of the rows, and nothing waits between CTAs); of longer ones
-// each CTA takes a slice of the weights.  Weights stay in registers across the passes
-// (re-read where a slice is longer than kChunk).
+// each CTA takes a slice of the weights.  Their order keys stay in shared memory across the
+// passes (re-read where a slice is longer than kChunk).  The loops are left rolled: with the
+// keys in registers and every loop over them unrolled, each instruction ran once per CTA and
+// its fetch was the time (2700 to 3300 clocks a radix pass and 8000 to 18000 for the slots at
+// 1024 to 2304 entries; 2000 and 2400 now).  What is left is the copy: 63000 of 78000 clocks
+// of a CTA at B32 Hk8 D128, 2304 slots to 1536 (75.5 us in all, 5.1 TB/s, 79% of the measured
+// copy rate), 155000 of 195000 at B4 Hk8 D64, 65536 to 32768 (119 us, 4.7 TB/s, 72%).
 template <int VEC>
 __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constant__ fa4d_evict_args a) {
-  __shared__ Smem sm;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int rank = static_cast<int>(cluster_rank()), ranks = static_cast<int>(cluster_size());
   const int item = static_cast<int>(blockIdx.x) / ranks;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -109,106 +123,175 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
   if (n > a.keep) {
     // The middle [a.sinks, late) gives its `want` heaviest entries.
     const int late = n - a.recent;
-    uint32_t want = a.keep - a.sinks - a.recent, prefix = 0;
+    uint32_t want = a.keep - a.sinks - a.recent, threshold = 0;
     const bool none = want == 0;
     const int per = sliced ? (n + ranks - 1) / ranks : n;
     const int lo = sliced ? min(rank * per, n) : 0, hi = min(lo + per, n);
     const bool once = hi - lo <= kChunk;
 
-    float x[kEach];  // the weights j = base + i * kThreads + threadIdx.x
+    auto sync = [&]() {  // of everyone who works on this selection
+      if (sliced)
+        cluster_sync();
+      else
+        __syncthreads();
+    };
     auto load = [&](int base) {
+      const int end = min(hi, base + kChunk);
+      for (int j0 = base + threadIdx.x; j0 < end; j0 += kAhead * kThreads) {
+        float x[kAhead];
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int j = base + i * kThreads + threadIdx.x;
-        x[i] = j < hi ? __ldg(w + j) : 0.f;
+        for (int u = 0; u < kAhead; ++u) x[u] = j0 + u * kThreads < end ? __ldg(w + j0 + u * kThreads) : 0.f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (j0 + u * kThreads < end) sm.key[j0 + u * kThreads - base] = order_key(x[u]);
       }
     };
-    auto in_middle = [&](int j) { return j >= a.sinks && j < late && j < hi; };
     load(lo);
 
-    // Radix selection of the want-th largest key of the middle, from the top bits down.
+    // Radix selection of the want-th largest key of the middle, from the top bits down.  With
+    // slices, the CTAs add the bins that are not empty to rank 0's, which finds the digit for
+    // all (each CTA adding all bins of all others cost 5 us a pass).
     if (!none) {
-      constexpr int kShift[3] = {21, 10, 0};
-      constexpr int kBits[3] = {11, 11, 10};
-#pragma unroll
+      constexpr int kMine = 4;  // bins of a thread in scans
+      static_assert(kMine * kThreads == kBins, "");
+      auto clear = [&](uint32_t* hist) {
+        *reinterpret_cast<uint4*>(&hist[kMine * threadIdx.x]) = make_uint4(0u, 0u, 0u, 0u);
+      };
+      if (sliced) {
+        clear(sm.total[0]);
+        cluster_sync();
+      }
+#pragma unroll 1
       for (int pass = 0; pass < 3; ++pass) {
-        *reinterpret_cast<uint4*>(&sm.hist[4 * threadIdx.x]) = make_uint4(0u, 0u, 0u, 0u);
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        clear(sm.hist);
         __syncthreads();
         for (int base = lo; base < hi; base += kChunk) {
-          if (!once) load(base);
+          if (!once) load(base);  // every thread reads only what it wrote
+          const int end = min(min(hi, late), base + kChunk);
+          for (int j0 = base + threadIdx.x; j0 < end; j0 += kAhead * kThreads) {
+            uint32_t key[kAhead];
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            const uint32_t key = order_key(x[i]);
-            if (in_middle(base + i * kThreads + threadIdx.x) &&
-                (pass == 0 || (key >> (kShift[pass] + kBits[pass])) == prefix))
-              atomicAdd(&sm.hist[(key >> kShift[pass]) & ((1u << kBits[pass]) - 1u)], 1u);
+            for (int u = 0; u < kAhead; ++u) key[u] = sm.key[min(j0 + u * kThreads, end - 1) - base];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+              const int j = j0 + u * kThreads;
+              // Bits above this digit equal to the threshold's (pass 0 has none).
+              if (j < end && j >= a.sinks && (pass == 0 || (key[u] >> (shift + bits)) == threshold))
+                atomicAdd(&sm.hist[(key[u] >> shift) & ((1u << bits) - 1u)], 1u);
+            }
           }
         }
-        // Thread i has four bins, counted from the top, so that scans run from the largest
-        // key down.
-        const int bin0 = kBins - 4 - 4 * threadIdx.x;
-        uint4 c = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+        uint32_t* total = sm.hist;
         if (sliced) {
+          total = sm.total[pass & 1];
+          const uint32_t at = peer_addr(smem_u32(total), 0);
+          const uint4 four = *reinterpret_cast<const uint4*>(&sm.hist[kMine * threadIdx.x]);
+          const uint32_t mine = at + 4 * kMine * threadIdx.x;
+          if (four.x) add_cluster(mine, four.x);
+          if (four.y) add_cluster(mine + 4, four.y);
+          if (four.z) add_cluster(mine + 8, four.z);
+          if (four.w) add_cluster(mine + 12, four.w);
+          clear(sm.total[(pass + 1) & 1]);  // read in the pass before, added to in the next
           cluster_sync();
-          const uint32_t mine = smem_u32(&sm.hist[bin0]);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            if (r >= ranks) break;
-            const uint4 y = ld_cluster_v4(peer_addr(mine, r));
-            c.x += y.x;
-            c.y += y.y;
-            c.z += y.z;
-            c.w += y.w;
-          }
-        } else {
-          __syncthreads();
-          c = *reinterpret_cast<const uint4*>(&sm.hist[bin0]);
         }
-        uint32_t all;
-        uint32_t upto = scan_before(c.x + c.y + c.z + c.w, sm.warp_sum, all);
-        const uint32_t cnt[4] = {c.w, c.z, c.y, c.x};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (upto < want && want <= upto + cnt[e]) {
-            sm.found[0] = bin0 + 3 - e;
+        if (!sliced || rank == 0) {
+          // Thread i has kMine bins counted from the top, so that scans run from the largest
+          // key down.
+          const int top = kBins - 1 - kMine * static_cast<int>(threadIdx.x);
+          const uint4 four = *reinterpret_cast<const uint4*>(&total[top - 3]);
+          const uint32_t mine = four.x + four.y + four.z + four.w;
+          uint32_t all;
+          uint32_t upto = scan_before(mine, sm.warp_sum, all);
+          if (upto < want && want <= upto + mine) {
+            int e = 0;
+            for (; want > upto + total[top - e]; ++e) upto += total[top - e];
+            sm.found[0] = top - e;
             sm.found[1] = want - upto;
+            for (int r = 1; sliced && r < ranks; ++r) {
+              st_cluster(peer_addr(smem_u32(&sm.found[0]), r), top - e);
+              st_cluster(peer_addr(smem_u32(&sm.found[1]), r), want - upto);
+            }
           }
-          upto += cnt[e];
         }
-        // `found` is written, and the histograms are read.
-        if (sliced)
-          cluster_sync();
-        else
-          __syncthreads();
-        prefix = (prefix << kBits[pass]) | sm.found[0];
+        sync();  // `found` is written, and the histograms are read
+        threshold = (threshold << bits) | sm.found[0];
         want = sm.found[1];
       }
+    } else {
+      __syncthreads();  // the keys are written
     }
-    // Kept: sinks, recent, keys above `prefix`, and the first `want` equal to it.
-    auto state = [&](int j, float v) {  // 1: kept for sure, 2: equal to the threshold
-      if (j >= hi) return 0;
+    // Kept: sinks, recent, keys above the threshold, and the first `want` equal to it.
+    auto state = [&](int j, uint32_t key) {  // 1: kept for sure, 2: equal to the threshold
       if (j < a.sinks || j >= late) return 1;
-      const uint32_t key = order_key(v);
-      return none ? 0 : key > prefix ? 1 : key == prefix ? 2 : 0;
+      return none ? 0 : key > threshold ? 1 : key == threshold ? 2 : 0;
     };
+    // Slots in order: each warp takes a run of the chunk, notes for each 32 entries which are
+    // kept and counts them; after one scan it walks its notes.
     uint32_t sure_before = 0, equal_before = 0;  // of the entries before the chunk
-    if (sliced) {
+    uint32_t before, all;                        // both counts, 16 bits each: before the run, of the chunk
+    int run;                                     // groups of 32 of a warp
+    auto note = [&](int base) {
+      const int count = min(hi - base, kChunk);
+      run = (count + 32 * kWarps - 1) / (32 * kWarps);
+      uint32_t mine = 0;
+      for (int g0 = wid * run; g0 < (wid + 1) * run && 32 * g0 < count; g0 += kAhead) {
+        int st[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = 32 * (g0 + u) + lane;
+          st[u] = g0 + u < (wid + 1) * run && i < count ? state(base + i, sm.key[i]) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const uint2 bits = make_uint2(__ballot_sync(0xffffffffu, st[u] == 1), __ballot_sync(0xffffffffu, st[u] == 2));
+          if (lane == 0 && g0 + u < (wid + 1) * run && 32 * (g0 + u) < count) sm.ballot[g0 + u] = bits;
+          mine += __popc(bits.x) | (__popc(bits.y) << 16);
+        }
+      }
+      before = __shfl_sync(0xffffffffu, scan_before(lane == 0 ? mine : 0u, sm.warp_sum, all), 0);
+    };
+    auto emit = [&](int base) {
+      const int count = min(hi - base, kChunk);
+      uint32_t s = sure_before + (before & 0xffffu), e = equal_before + (before >> 16);
+      const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
+      for (int g = wid * run; g < min((wid + 1) * run, (count + 31) / 32); ++g) {
+        const uint2 bits = sm.ballot[g];
+        const uint32_t equal_at = e + __popc(bits.y & below);
+        const int slot = static_cast<int>(s + __popc(bits.x & below) + min(equal_at, want));
+        const bool keeps = ((bits.x >> lane) & 1u) || (((bits.y >> lane) & 1u) && equal_at < want);
+        if (keeps && (sliced || (slot >= slot0 && slot < slot1))) {
+          const int j = base + 32 * g + lane;
+          index[slot] = j;
+          if (!sliced) sm.list[slot - slot0] = static_cast<uint16_t>(j);
+        }
+        s += __popc(bits.x);
+        e += __popc(bits.y);
+      }
+      sure_before += all & 0xffffu;
+      equal_before += all >> 16;
+    };
+    if (once) {
+      note(lo);
+    } else {
       uint32_t sure = 0, equal = 0;
       for (int base = lo; base < hi; base += kChunk) {
-        if (!once) load(base);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int st = state(base + i * kThreads + threadIdx.x, x[i]);
+        load(base);
+        for (int j = base + threadIdx.x; j < min(hi, base + kChunk); j += kThreads) {
+          const int st = state(j, sm.key[j - base]);
           sure += st == 1;
           equal += st == 2;
         }
       }
-      uint32_t sure_all, equal_all;
-      scan_before(sure, sm.warp_sum, sure_all);
-      scan_before(equal, sm.warp_sum, equal_all);
+      scan_before(sure, sm.warp_sum, before);
+      scan_before(equal, sm.warp_sum, all);
+    }
+    if (sliced) {
       if (threadIdx.x == 0) {
-        sm.counts[0] = sure_all;
-        sm.counts[1] = equal_all;
+        sm.counts[0] = once ? all & 0xffffu : before;
+        sm.counts[1] = once ? all >> 16 : all;
       }
       cluster_sync();
       for (int r = 0; r < rank; ++r) {
@@ -217,47 +300,18 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
         equal_before += y.y;
       }
     }
-    // Slots in order: a warp's 32 weights of each i by ballots, the groups by one scan.
-    for (int base = lo; base < hi; base += kChunk) {
-      if (!once) load(base);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int st = state(base + i * kThreads + threadIdx.x, x[i]);
-        const uint32_t sure = __ballot_sync(0xffffffffu, st == 1), equal = __ballot_sync(0xffffffffu, st == 2);
-        if (lane == 0) sm.group[i * kWarps + wid] = __popc(sure) | (__popc(equal) << 16);
+    if (once) {
+      emit(lo);
+    } else {
+      for (int base = lo; base < hi; base += kChunk) {
+        __syncthreads();  // the keys and notes of the chunk before have been read
+        load(base);
+        __syncthreads();
+        note(base);
+        emit(base);
       }
-      __syncthreads();
-      uint32_t all;  // at most kChunk in each half
-      const uint32_t before =
-          scan_before(threadIdx.x < kEach * kWarps ? sm.group[threadIdx.x] : 0u, sm.warp_sum, all);
-      if (threadIdx.x < kEach * kWarps) sm.group[threadIdx.x] = before;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int j = base + i * kThreads + threadIdx.x;
-        const int st = state(j, x[i]);
-        const uint32_t sure = __ballot_sync(0xffffffffu, st == 1), equal = __ballot_sync(0xffffffffu, st == 2);
-        const uint32_t below = (1u << lane) - 1u, group = sm.group[i * kWarps + wid];
-        const uint32_t s = sure_before + (group & 0xffffu) + __popc(sure & below);
-        const uint32_t e = equal_before + (group >> 16) + __popc(equal & below);
-        if (st == 1 || (st == 2 && e < want)) {
-          const int slot = static_cast<int>(s + min(e, want));
-          if (sliced || (slot >= slot0 && slot < slot1)) {
-            index[slot] = j;
-            w_out[slot] = x[i];
-            if (!sliced) sm.list[slot - slot0] = j;
-          }
-        }
-      }
-      sure_before += all & 0xffffu;
-      equal_before += all >> 16;
-      if (!once) __syncthreads();  // the groups have been read
     }
-    // The whole index (the share's list) is written; no CTA reads another's memory any more.
-    if (sliced)
-      cluster_sync();
-    else
-      __syncthreads();
+    sync();  // the whole index (the share's list) is written; no CTA reads another's memory any more
   }
 
   // Copy slots [slot0, slot1).
@@ -270,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
   const int all = (slot1 - slot0) * pieces;
   for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kRowsInFlight) {
     T x[kRowsInFlight], y[kRowsInFlight];
+    float wt[kRowsInFlight];
     int slot[kRowsInFlight], from[kRowsInFlight], c[kRowsInFlight];
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {
@@ -282,7 +337,9 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {
       x[u] = y[u] = Piece<VEC>::zero();
+      wt[u] = 0.f;
       if (from[u] >= 0) {
+        if (c[u] == 0) wt[u] = __ldg(w + from[u]);
         x[u] = __ldg(reinterpret_cast<const T*>(k + from[u] * a.k_stride[1] + c[u]));
         y[u] = __ldg(reinterpret_cast<const T*>(v + from[u] * a.v_stride[1] + c[u]));
       }
@@ -292,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
       if (slot[u] < 0) continue;
       *reinterpret_cast<T*>(ko + slot[u] * a.k_out_stride[1] + c[u]) = x[u];
       *reinterpret_cast<T*>(vo + slot[u] * a.v_out_stride[1] + c[u]) = y[u];
-      if (c[u] == 0 && (n <= a.keep || from[u] < 0)) {  // where no selection wrote them
-        index[slot[u]] = from[u];
-        w_out[slot[u]] = from[u] < 0 ? 0.f : __ldg(w + from[u]);
+      if (c[u] == 0) {
+        w_out[slot[u]] = wt[u];
+        if (n <= a.keep) index[slot[u]] = from[u];
       }
     }
   }
@@ -302,9 +359,12 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
 
 template <int VEC>
 cudaError_t launch_evict_t(const fa4d_evict_args& a, int ranks, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(evict_kernel<VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ranks) * a.B * a.Hk);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -318,9 +378,11 @@ cudaError_t launch_evict_t(const fa4d_evict_args& a, int ranks, cudaStream_t s) 
 }  // namespace
 
 cudaError_t launch_evict(const fa4d_evict_args& a, bool vec, int sms, cudaStream_t s) {
-  // CTAs per (request, KV head): the fewest that give every SM two, at most 8.
+  // CTAs per (request, KV head): the fewest that give every SM one, at most 8 (B32 Hk8, 2304
+  // slots to 1536: 75.5 us with 1, 79 with 2, 104 with 8; B4 Hk8, 65536 to 32768: 484 with 1,
+  // 164 with 4, 119 with 8).
   int ranks = 1;
-  while (ranks < 8 && static_cast<int64_t>(a.B) * a.Hk * ranks < 2LL * sms) ranks *= 2;
+  while (ranks < 8 && static_cast<int64_t>(a.B) * a.Hk * ranks < sms) ranks *= 2;
   return vec ? launch_evict_t<8>(a, ranks, s) : launch_evict_t<1>(a, ranks, s);
 }
 
