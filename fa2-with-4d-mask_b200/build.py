@@ -24,7 +24,7 @@ BUILD = HERE / "_build"
 LIB = HERE / "libfa4d.so"
 
 SOURCES = ["fa4d_api.cu", "fa4d_fwd.cu", "fa4d_bwd.cu", "fa4d_bwd256.cu", "fa4d_mask.cu", "fa4d_dq.cu", "fa4d_dq256.cu",
-           "fa4d_rotary.cu", "fa4d_decode.cu", "fa4d_evict.cu", "fa4d_cache_api.cu"]
+           "fa4d_rotary.cu", "fa4d_decode.cu", "fa4d_prefix.cu", "fa4d_evict.cu", "fa4d_cache_api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"]
 
@@ -49,7 +49,7 @@ def _stale(target: Path, inputs: list[Path]) -> bool:
 
 # Kernels that rebalance registers with setmaxnreg assume this exact allocation per
 # thread at launch; fewer would make a setmaxnreg.inc wait forever.
-LAUNCH_REGS = {"bwd_kernel": 128, "bwd256_kernel": 168, "fwd_kernel": 168}
+LAUNCH_REGS = {"bwd_kernel": 128, "bwd256_kernel": 168, "fwd_kernel": 168, "prefix_kernel": 168}
 
 
 def _check_launch_regs(src: Path, log: str) -> None:

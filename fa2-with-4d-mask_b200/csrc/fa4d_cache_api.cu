@@ -66,8 +66,36 @@ bool table_vec(const fa4d_rotary_table& t) { return t.rotary_dim % 16 == 0 && t.
 struct Plan {
   fa4d::DecodeParams p;
   int ctas;
-  size_t seg_o, seg_ml, logits, total;
+  int splits;        // runs of key tiles of the prefix kernel; 0: decode_kernel does the prefix
+  bool split_keys;
+  size_t seg_o, seg_ml, logits, pre_o, pre_ml, total;
 };
+
+// Runs per (row tile, KV head) of the prefix kernel: the number that shortens the estimate
+// waves x (tiles of a run x time of a tile + fixed time of a CTA) + the partial rows written
+// and read back.
+int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, bool split_keys, int sms) {
+  // Microseconds: a key tile of a CTA (two at a time with split_keys), and its fill, drain and
+  // output rows; measured on B200.
+  const double tile = D == 256 ? 2.2 : D == 64 ? 1.8 : 2.0, fixed = 6.0;
+  const int step = split_keys ? 2 : 1;
+  double best = 0.0;
+  int best_s = 1;
+  for (int s = 1; s <= tiles && s <= 64; ++s) {
+    const double waves = std::ceil(static_cast<double>(row_tiles) * Hk * s / sms);
+    const int run = (tiles + s - 1) / s;
+    const double t = waves * ((run + step - 1) / step * tile + fixed) + 1.6e-6 * step * s * rows * Hk * D;
+    if (s == 1 || t < best) {
+      best = t;
+      best_s = s;
+    }
+  }
+  return best_s;
+}
+
+// Up to this many rows of a KV head the prefix goes through decode_kernel, which reads it once
+// per 16 rows.
+constexpr int64_t kDecodeRows = 32;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -87,10 +115,19 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   p.G = Hq / Hk;
   p.R = T * p.G;
   p.tiles = (p.R + 15) / 16;
-  p.prefix_tiles = P ? static_cast<int>((rows + 15) / 16) : 0;
+  const int sms = fa4d::host_sm_count();
+  if (P && rows > kDecodeRows) {
+    out->split_keys = D != 256 && rows <= 128;
+    const int64_t row_tiles = D == 256 || out->split_keys ? (rows + 127) / 128 : (rows + 255) / 256;
+    out->splits = prefix_splits(row_tiles, Hk, (P + 127) / 128, rows, D, out->split_keys, sms);
+    p.splits = out->splits * (out->split_keys ? 2 : 1);
+    p.pre_rows = static_cast<int>(rows);
+  } else {
+    p.prefix_tiles = P ? static_cast<int>((rows + 15) / 16) : 0;
+  }
   p.prefix_units = (P + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys;
   p.seg_rows = static_cast<int>(std::min<int64_t>(16, p.prefix_tiles ? rows : p.R));
-  out->ctas = fa4d::host_sm_count() * fa4d::decode_ctas_per_sm(D);
+  out->ctas = sms * fa4d::decode_ctas_per_sm(D);
   p.warps = out->ctas * fa4d::kDecodeWarps;
   p.min_units = 2;
   p.logits_ld = (C + 3) / 4 * 4;
@@ -100,8 +137,10 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   out->seg_o = 0;
   out->seg_ml = align256(seg * D * sizeof(float));
   out->logits = out->seg_ml + align256(seg * sizeof(float2));
-  out->total = out->logits;
-  if (weights) out->total += align256(static_cast<size_t>(B) * Hk * p.R * p.logits_ld * sizeof(float));
+  out->pre_o = out->logits + (weights ? align256(static_cast<size_t>(B) * Hk * p.R * p.logits_ld * sizeof(float)) : 0);
+  const size_t pre = static_cast<size_t>(p.splits) * Hk * p.pre_rows;
+  out->pre_ml = out->pre_o + align256(pre * D * sizeof(float));
+  out->total = out->pre_ml + align256(pre * sizeof(float2));
   return FA4D_OK;
 }
 
@@ -212,9 +251,34 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   p.seg_o = reinterpret_cast<float*>(ws + plan.seg_o);
   p.seg_ml = reinterpret_cast<float2*>(ws + plan.seg_ml);
   p.logits = a->weights ? reinterpret_cast<float*>(ws + plan.logits) : nullptr;
+  p.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
+  p.pre_ml = reinterpret_cast<float2*>(ws + plan.pre_ml);
   const bool bf16 = a->dtype == FA4D_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if ((rc = launched(fa4d::launch_decode(p, a->D, bf16, plan.ctas, false, s), "decode attention"))) return rc;
+  if (plan.splits) {
+    fa4d::PrefixParams x;
+    memset(&x, 0, sizeof(x));
+    const int64_t ks[3] = {0, a->prefix_k_stride[0], a->prefix_k_stride[1]};
+    const int64_t vs[3] = {0, a->prefix_v_stride[0], a->prefix_v_stride[1]};
+    if ((rc = fa4d::host_encode_bthd(&x.tm_k, a->prefix_k, 1, a->P, a->Hk, a->D, ks, 128, bf16, "prefix_k"))) return rc;
+    if ((rc = fa4d::host_encode_bthd(&x.tm_v, a->prefix_v, 1, a->P, a->Hk, a->D, vs, 128, bf16, "prefix_v"))) return rc;
+    x.q = a->q;
+    for (int i = 0; i < 3; ++i) x.q_stride[i] = a->q_stride[i];
+    x.T = a->T;
+    x.G = p.G;
+    x.P = a->P;
+    x.rows = p.pre_rows;
+    x.parts = p.splits;
+    x.d_in = a->D;
+    x.scale_log2 = p.scale_log2;
+    x.o = p.pre_o;
+    x.ml = p.pre_ml;
+    x.status = fa4d::host_status_word();
+    if (!x.status) return fail(FA4D_ERR_CUDA, "device status word is not available");
+    if ((rc = launched(fa4d::launch_prefix(x, a->D, bf16, a->Hk, plan.splits, plan.split_keys, s), "prefix attention")))
+      return rc;
+  }
+  if ((rc = launched(fa4d::launch_decode(p, a->D, bf16, plan.ctas, plan.splits > 0, s), "decode attention"))) return rc;
   return launched(fa4d::launch_join(p, a->D, bf16, s), "attention join");
 }
 

@@ -486,7 +486,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll 4
       for (int i = 0; i < z.n; ++i) {
         const int64_t row = z.first + i * z.step;
-        const float f = ex2(z.ml[row].x - all.x);
+        const float m = z.ml[row].x;
+        if (m == kNegInf) continue;  // no key in this part (its row may not even be written)
+        const float f = ex2(m - all.x);
         float v[D / 32];
         load_row<D>(z.o + row * D, lane, v);
 #pragma unroll

@@ -51,10 +51,28 @@ struct DecodeParams {
   int* status;
 };
 
+// Attention of all rows of each KV head over the prefix (fa4d_prefix.cu).
+struct PrefixParams {
+  CUtensorMap tm_k;  // dims (D, P, Hk, 1), box (64, 128, 1, 1), 128-B swizzle
+  CUtensorMap tm_v;
+  const void* q;
+  int64_t q_stride[3];
+  int32_t T, G, P, rows;  // rows of a KV head
+  int32_t parts;          // partial results per row
+  int32_t d_in;           // head dim of the tensors (96 computes at 128)
+  float scale_log2;
+  float* o;               // [Hk][parts][rows][d_in]
+  float2* ml;             // [Hk][parts][rows]
+  int* status;
+};
+
 constexpr int kDecodeWarps = 4;   // warps of a decode_kernel CTA
 constexpr int kUnitKeys = 16;
 
 cudaError_t launch_decode(const DecodeParams& p, int D, bool bf16, int ctas, bool after_prefix, cudaStream_t s);
+// `split_keys`: the rows of a KV head fit one slot (at most 128), and a run's slots take even
+// and odd key tiles; two parts per run then, one otherwise.
+cudaError_t launch_prefix(const PrefixParams& p, int D, bool bf16, int Hk, int splits, bool split_keys, cudaStream_t s);
 cudaError_t launch_join(const DecodeParams& p, int D, bool bf16, cudaStream_t s);
 int decode_ctas_per_sm(int D);
 

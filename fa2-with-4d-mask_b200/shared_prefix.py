@@ -118,7 +118,10 @@ def shared_prefix_attention(
     pk_ptr = pv_ptr = None
     pk_stride = pv_stride = (0, 0)
     if P:
-        prefix_key, prefix_value = _rows16(prefix_key), _rows16(prefix_value)
+        # The prefix also goes through tensor maps, which have no stride of 0.
+        prefix_key, prefix_value = (
+            _rows16(x if all(s > 0 or n == 1 for s, n in zip(x.stride(), x.shape)) else x.contiguous())
+            for x in (prefix_key, prefix_value))
         pk_ptr, pv_ptr = prefix_key.data_ptr(), prefix_value.data_ptr()
         s, z = prefix_key.stride(), prefix_value.stride()
         pk_stride, pv_stride = ((s[1], s[0]), (z[1], z[0])) if layout == "bhsd" else (s[:2], z[:2])
