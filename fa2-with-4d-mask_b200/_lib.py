@@ -10,7 +10,7 @@ point raises.
 from __future__ import annotations
 
 import ctypes
-import functools
+import importlib.util
 import os
 from pathlib import Path
 from typing import Optional
@@ -149,79 +149,6 @@ class BwdArgs(ctypes.Structure):
 
 ROTARY_MAX_PAIRS = 128
 PAIR_HALF, PAIR_ADJACENT = 0, 1
-_i64x2 = ctypes.c_int64 * 2
-
-
-class RotaryTable(ctypes.Structure):
-    """Mirror of ``fa4d_rotary_table``."""
-
-    _fields_ = [
-        ("turn", ctypes.c_uint64 * ROTARY_MAX_PAIRS),
-        ("axis", ctypes.c_uint8 * ROTARY_MAX_PAIRS),
-        ("D", ctypes.c_int32),
-        ("rotary_dim", ctypes.c_int32),
-        ("pairing", ctypes.c_int32),
-        ("axes", ctypes.c_int32),
-    ]
-
-
-class RotaryArgs(ctypes.Structure):
-    """Mirror of ``fa4d_rotary_args``."""
-
-    _fields_ = [
-        ("table", RotaryTable),
-        *((n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "positions")),
-        *((n, _i64x3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride", "positions_stride")),
-        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "dtype", "positions_bits", "inverse")),
-    ]
-
-
-class RotaryAppendArgs(ctypes.Structure):
-    """Mirror of ``fa4d_rotary_append_args``."""
-
-    _fields_ = [
-        ("table", RotaryTable),
-        *((n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "weights", "positions",
-                                         "lengths", "lengths_out")),
-        *((n, _i64x3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_cache_stride",
-                                "v_cache_stride")),
-        ("weights_stride", _i64x2),
-        ("positions_stride", _i64x3),
-        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "C", "dtype", "positions_bits")),
-    ]
-
-
-class PrefixAttentionArgs(ctypes.Structure):
-    """Mirror of ``fa4d_prefix_attention_args``."""
-
-    _fields_ = [
-        *((n, ctypes.c_void_p) for n in ("q", "prefix_k", "prefix_v", "k", "v", "o", "lengths", "mask", "weights",
-                                         "workspace")),
-        ("workspace_bytes", ctypes.c_size_t),
-        ("q_stride", _i64x3),
-        ("prefix_k_stride", _i64x2),
-        ("prefix_v_stride", _i64x2),
-        *((n, _i64x3) for n in ("k_stride", "v_stride", "o_stride", "mask_stride")),
-        ("weights_stride", _i64x2),
-        *((n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hk", "D", "P", "C", "dtype", "causal")),
-        ("scale", ctypes.c_float),
-    ]
-
-
-class EvictArgs(ctypes.Structure):
-    """Mirror of ``fa4d_evict_args``."""
-
-    _fields_ = [
-        *((n, ctypes.c_void_p) for n in ("k", "v", "weights", "lengths", "k_out", "v_out", "weights_out",
-                                         "lengths_out", "index_out")),
-        ("k_stride", _i64x3),
-        ("v_stride", _i64x3),
-        ("weights_stride", _i64x2),
-        ("k_out_stride", _i64x3),
-        ("v_out_stride", _i64x3),
-        ("weights_out_stride", _i64x2),
-        *((n, ctypes.c_int32) for n in ("B", "C", "Hk", "D", "keep", "sinks", "recent")),
-    ]
 
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -291,13 +218,6 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         ctypes.c_void_p,
     ]
     lib.fa4d_mask_prepare_docs.restype = ctypes.c_int
-    for name, args in (("fa4d_rotary", RotaryArgs), ("fa4d_rotary_append", RotaryAppendArgs),
-                       ("fa4d_prefix_attention", PrefixAttentionArgs), ("fa4d_evict", EvictArgs)):
-        fn = getattr(lib, name)
-        fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
-        fn.restype = ctypes.c_int
-    lib.fa4d_prefix_attention_workspace.argtypes = [ctypes.c_int32] * 8
-    lib.fa4d_prefix_attention_workspace.restype = ctypes.c_size_t
     version = lib.fa4d_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"{p}: ABI version {version}, expected {ABI_VERSION}; rebuild with build.py")
@@ -654,25 +574,23 @@ def backward(
     return dq, dk, dv
 
 
-def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
-    """Enqueues entry point ``name`` with its args structure on the device's current stream."""
-    lib = load_library()
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != FA4D_OK:
-        _raise(lib, rc, name)
+_HOST = None
 
 
-@functools.lru_cache(maxsize=256)
-def prefix_attention_workspace(index: int, *sizes: int) -> int:
-    """Bytes of fa4d_prefix_attention's workspace on device ``index`` for (B, T, Hq, Hk, D,
-    P, C, weights); 0 for sizes it refuses."""
-    with torch.cuda.device(index):
-        return int(load_library().fa4d_prefix_attention_workspace(*sizes))
+def host():
+    """The native binding of the operators around the attention (_fa4d_host.so), which checks
+    their arguments, allocates and launches; imported on first use."""
+    global _HOST
+    if _HOST is None:
+        load_library()
+        path = HERE / "_fa4d_host.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python {HERE / 'build.py'}` (there is no fallback)")
+        spec = importlib.util.spec_from_file_location("_fa4d_host", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _HOST = module
+    return _HOST
 
 
 def device_status(device: Optional[torch.device] = None, clear: bool = True) -> int:

@@ -1,7 +1,9 @@
-"""Builds libfa4d.so (the sm_100a kernels behind include/fa4d.h) in place.
+"""Builds libfa4d.so (the sm_100a kernels behind include/fa4d.h) and _fa4d_host.so (the host
+binding of the operators around the attention) in place.
 
-The library is compiled with nvcc for ``sm_100a`` only and written next to this
-file, so it travels with the source tree.  Objects go to ``_build/`` beside it.
+The library is compiled with nvcc for ``sm_100a`` only, the binding with the host compiler
+against the installed torch, and both are written next to this file, so they travel with the
+source tree.  Objects go to ``_build/`` beside them.
 Run ``python build.py`` (add ``--ptxas-info`` to print register / spill counts).
 """
 
@@ -14,6 +16,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -22,6 +25,8 @@ CSRC = HERE / "csrc"
 INCLUDE = REPO / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "libfa4d.so"
+HOST_SOURCE = CSRC / "fa4d_torch.cpp"
+HOST_LIB = HERE / "_fa4d_host.so"
 
 SOURCES = ["fa4d_api.cu", "fa4d_fwd.cu", "fa4d_bwd.cu", "fa4d_bwd256.cu", "fa4d_mask.cu", "fa4d_dq.cu", "fa4d_dq256.cu",
            "fa4d_rotary.cu", "fa4d_decode.cu", "fa4d_prefix.cu", "fa4d_evict.cu", "fa4d_cache_api.cu"]
@@ -76,6 +81,27 @@ def _compile(nvcc: str, src: Path, obj: Path, ptxas_info: bool) -> str:
     return res.stdout + res.stderr
 
 
+def _build_host() -> None:
+    """The binding links libfa4d.so beside it and torch's own libraries (loaded by ``import
+    torch`` before it)."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    tmp = HOST_LIB.with_suffix(".so.tmp")
+    # The system's g++ (nvcc's host compiler): its libstdc++ is the one torch has loaded.
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in (root / "include", root / "include/torch/csrc/api/include", cuda / "include", INCLUDE,
+                                sysconfig.get_paths()["include"])),
+           str(HOST_SOURCE), "-o", str(tmp), f"-L{HERE}", "-l:libfa4d.so", f"-L{root / 'lib'}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"host binding failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, HOST_LIB)
+
+
 def build(force: bool = False, ptxas_info: bool = False, jobs: int | None = None) -> Path:
     nvcc = _nvcc()
     BUILD.mkdir(exist_ok=True)
@@ -100,6 +126,8 @@ def build(force: bool = False, ptxas_info: bool = False, jobs: int | None = None
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    if force or _stale(HOST_LIB, [HOST_SOURCE, INCLUDE / "fa4d.h"]):
+        _build_host()
     if ptxas_info:
         for log in logs:
             sys.stdout.write(log)
