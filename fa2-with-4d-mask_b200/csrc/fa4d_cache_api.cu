@@ -68,7 +68,7 @@ struct Plan {
   int ctas;
   int splits;        // runs of key tiles of the prefix kernel; 0: decode_kernel does the prefix
   bool split_keys;
-  size_t seg_o, seg_ml, logits, pre_o, pre_ml, total;
+  size_t seg_o, seg_ml, logits, pre_o, pre_ml, pre_used, total;
 };
 
 // Runs per (row tile, KV head) of the prefix kernel: the number that shortens the estimate
@@ -77,7 +77,8 @@ struct Plan {
 int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, bool split_keys, int sms) {
   // Microseconds: a key tile of a CTA (two at a time with split_keys), and its fill, drain and
   // output rows; measured on B200.
-  const double tile = D == 256 ? 2.2 : D == 64 ? 1.8 : 2.0, fixed = 6.0;
+  const double fixed = fa4d::kRunMicros;
+  const double tile = D == 256 ? fa4d::kTileMicros<256> : D == 64 ? fa4d::kTileMicros<64> : fa4d::kTileMicros<128>;
   const int step = split_keys ? 2 : 1;
   double best = 0.0;
   int best_s = 1;
@@ -122,12 +123,14 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
     out->splits = prefix_splits(row_tiles, Hk, (P + 127) / 128, rows, D, out->split_keys, sms);
     p.splits = out->splits * (out->split_keys ? 2 : 1);
     p.pre_rows = static_cast<int>(rows);
+    p.load = fa4d::PrefixLoad{static_cast<int>(row_tiles) * Hk, out->splits, (P + 127) / 128, out->split_keys ? 2 : 1, sms,
+                               p.tiles};
   } else {
     p.prefix_tiles = P ? static_cast<int>((rows + 15) / 16) : 0;
   }
   p.prefix_units = (P + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys;
   p.seg_rows = static_cast<int>(std::min<int64_t>(16, p.prefix_tiles ? rows : p.R));
-  out->ctas = sms * fa4d::decode_ctas_per_sm(D);
+  out->ctas = sms * (D == 256 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
   p.warps = out->ctas * fa4d::kDecodeWarps;
   p.min_units = 2;
   p.logits_ld = (C + 3) / 4 * 4;
@@ -140,7 +143,8 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   out->pre_o = out->logits + (weights ? align256(static_cast<size_t>(B) * Hk * p.R * p.logits_ld * sizeof(float)) : 0);
   const size_t pre = static_cast<size_t>(p.splits) * Hk * p.pre_rows;
   out->pre_ml = out->pre_o + align256(pre * D * sizeof(float));
-  out->total = out->pre_ml + align256(pre * sizeof(float2));
+  out->pre_used = out->pre_ml + align256(pre * sizeof(float2));
+  out->total = out->pre_used + 256;  // the runs made, and the shares
   return FA4D_OK;
 }
 
@@ -226,26 +230,16 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   fa4d::DecodeParams& p = plan.p;
   char* ws = static_cast<char*>(a->workspace);
   p.q = a->q;
-  p.pk = a->prefix_k;
-  p.pv = a->prefix_v;
-  p.k = a->k;
-  p.v = a->v;
   p.o = a->o;
   p.lengths = a->lengths;
   p.mask = a->mask;
   p.weights = a->weights;
   for (int i = 0; i < 3; ++i) {
     p.q_stride[i] = a->q_stride[i];
-    p.k_stride[i] = a->k_stride[i];
-    p.v_stride[i] = a->v_stride[i];
     p.o_stride[i] = a->o_stride[i];
     p.mask_stride[i] = a->mask_stride[i];
   }
-  for (int i = 0; i < 2; ++i) {
-    p.pk_stride[i] = a->prefix_k_stride[i];
-    p.pv_stride[i] = a->prefix_v_stride[i];
-    p.weights_stride[i] = a->weights_stride[i];
-  }
+  for (int i = 0; i < 2; ++i) p.weights_stride[i] = a->weights_stride[i];
   p.causal = a->causal;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.seg_o = reinterpret_cast<float*>(ws + plan.seg_o);
@@ -253,15 +247,29 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   p.logits = a->weights ? reinterpret_cast<float*>(ws + plan.logits) : nullptr;
   p.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
   p.pre_ml = reinterpret_cast<float2*>(ws + plan.pre_ml);
+  int32_t* used = reinterpret_cast<int32_t*>(ws + plan.pre_used);
+  p.pre_used = used;
+  p.shares = reinterpret_cast<fa4d::Shares*>(used + 16);
+  p.status = fa4d::host_status_word();
+  if (!p.status) return fail(FA4D_ERR_CUDA, "device status word is not available");
   const bool bf16 = a->dtype == FA4D_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto encode = [&](CUtensorMap* m, const void* ptr, int B, int T, const int64_t st[3], int rows, const char* name) {
+    return fa4d::host_encode_bthd(m, ptr, B, T, a->Hk, a->D, st, rows, bf16, name);
+  };
+  if ((rc = encode(&p.tm_k, a->k, a->B, a->C, a->k_stride, fa4d::kUnitKeys, "k"))) return rc;
+  if ((rc = encode(&p.tm_v, a->v, a->B, a->C, a->v_stride, fa4d::kUnitKeys, "v"))) return rc;
+  const int64_t ks[3] = {0, a->prefix_k_stride[0], a->prefix_k_stride[1]};
+  const int64_t vs[3] = {0, a->prefix_v_stride[0], a->prefix_v_stride[1]};
+  if (p.prefix_tiles) {
+    if ((rc = encode(&p.tm_pk, a->prefix_k, 1, a->P, ks, fa4d::kUnitKeys, "prefix_k"))) return rc;
+    if ((rc = encode(&p.tm_pv, a->prefix_v, 1, a->P, vs, fa4d::kUnitKeys, "prefix_v"))) return rc;
+  }
   if (plan.splits) {
     fa4d::PrefixParams x;
     memset(&x, 0, sizeof(x));
-    const int64_t ks[3] = {0, a->prefix_k_stride[0], a->prefix_k_stride[1]};
-    const int64_t vs[3] = {0, a->prefix_v_stride[0], a->prefix_v_stride[1]};
-    if ((rc = fa4d::host_encode_bthd(&x.tm_k, a->prefix_k, 1, a->P, a->Hk, a->D, ks, 128, bf16, "prefix_k"))) return rc;
-    if ((rc = fa4d::host_encode_bthd(&x.tm_v, a->prefix_v, 1, a->P, a->Hk, a->D, vs, 128, bf16, "prefix_v"))) return rc;
+    if ((rc = encode(&x.tm_k, a->prefix_k, 1, a->P, ks, 128, "prefix_k"))) return rc;
+    if ((rc = encode(&x.tm_v, a->prefix_v, 1, a->P, vs, 128, "prefix_v"))) return rc;
     x.q = a->q;
     for (int i = 0; i < 3; ++i) x.q_stride[i] = a->q_stride[i];
     x.T = a->T;
@@ -270,16 +278,21 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
     x.rows = p.pre_rows;
     x.parts = p.splits;
     x.d_in = a->D;
+    x.lengths = a->lengths;
+    x.B = a->B;
+    x.C = a->C;
+    x.Hk = a->Hk;
+    x.load = p.load;
+    x.used = used;
     x.scale_log2 = p.scale_log2;
     x.o = p.pre_o;
     x.ml = p.pre_ml;
-    x.status = fa4d::host_status_word();
-    if (!x.status) return fail(FA4D_ERR_CUDA, "device status word is not available");
+    x.status = p.status;
     if ((rc = launched(fa4d::launch_prefix(x, a->D, bf16, a->Hk, plan.splits, plan.split_keys, s), "prefix attention")))
       return rc;
   }
   if ((rc = launched(fa4d::launch_decode(p, a->D, bf16, plan.ctas, plan.splits > 0, s), "decode attention"))) return rc;
-  return launched(fa4d::launch_join(p, a->D, bf16, s), "attention join");
+  return launched(fa4d::launch_join(p, a->D, bf16, fa4d::host_sm_count(), s), "attention join");
 }
 
 int fa4d_evict(const fa4d_evict_args* a, void* stream) {

@@ -16,24 +16,19 @@ constexpr float kNegInf = -INFINITY;
 
 template <int D>
 struct DecodeShape {
-  // Bytes of a key's row in shared memory: a power of two, so that the 16-byte chunks of
-  // eight rows, each stored at (chunk ^ row % 8), lie in different banks.
-  static constexpr int kPitch = D == 96 ? 256 : 2 * D;
-  static constexpr int kTile = kUnitKeys * kPitch;  // K or V of a unit
+  static constexpr int kBoxes = (D + 63) / 64;       // TMA boxes of 64 columns (96: zeros past it)
+  static constexpr int kBox = kUnitKeys * 128;       // 128-byte rows, 16-byte chunks swizzled
+  static constexpr int kTile = kBoxes * kBox;        // K or V of a unit
   static constexpr int kStage = 2 * kTile;
   static constexpr int kStages = D == 64 ? 6 : 3;
-  static constexpr int kBytes = kDecodeWarps * kStages * kStage;
-  static constexpr int kCtas = D == 256 ? 1 : 2;  // on an SM
+  static constexpr int kBars = kDecodeWarps * kStages * kStage;
+  static constexpr int kBytes = kBars + kDecodeWarps * kStages * 8 + 8 + 1024;  // aligned to 1024
+  // 16-byte chunk c of row `row` of a tile.
+  static __device__ __forceinline__ uint32_t at(int row, int c) {
+    return (c >> 3) * kBox + row * 128 + (((c ^ row) & 7) << 4);
+  }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -61,21 +56,34 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__device__ __forceinline__ int length_of(const DecodeParams& p, int b) { return min(max(__ldg(p.lengths + b), 0), p.C); }
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnitKeys - 1) / kUnitKeys; }
-
-// Units of the requests before b (all of them for b = B), per KV head and row tile.
-__device__ __forceinline__ int64_t units_before(const DecodeParams& p, int b, int lane) {
-  int64_t n = 0;
-  for (int i = lane; i < b; i += 32) n += units_of(length_of(p, i));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
+__device__ __forceinline__ int length_of(const DecodeParams& p, int b) { return length_at(p.lengths, b, p.C); }
+// The division of `total` units.  Beside a prefix kernel the warps of the SMs that it leaves
+// free start at once, and the others when it is done: those get less, by its estimated time.
+template <int D>
+__device__ __forceinline__ Shares shares_of(const DecodeParams& p, int64_t total, int lane) {
+  const int least = p.min_units;
+  auto up = [](int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); };
+  if (p.load.items) {
+    const RunChoice c = choose_runs<D == 96 ? 128 : D>(p.load, total, lane);
+    const int free_sms = p.load.sms - p.load.items * c.runs;
+    if (free_sms > 0) {
+      const int early = p.warps / p.load.sms * free_sms, rest = p.warps - early;
+      // When all SMs work on the own keys; the late warps' part of that.
+      const float late_us = fmaxf(c.total_us - c.prefix_us - kDecodeMicros, 0.f);
+      const float part = fminf(late_us * c.rate * rest / p.warps, static_cast<float>(total));
+      const int late = static_cast<int>(part / max(rest, 1));
+      return Shares{early, max(up(total - static_cast<int64_t>(late) * rest, early), least), late};
+    }
+  }
+  return Shares{p.warps, max(up(total, p.warps), least), 0};
 }
 
-// Units of a warp, from the number of units in all.
-__device__ __forceinline__ int64_t share_of(const DecodeParams& p, int64_t total) {
-  return max(static_cast<int64_t>(p.min_units), (total + p.warps - 1) / p.warps);
+__device__ __forceinline__ int64_t warp_start(const Shares& s, int64_t warp) {
+  return min(warp, static_cast<int64_t>(s.early)) * s.each + max(warp - s.early, static_cast<int64_t>(0)) * s.late;
+}
+__device__ __forceinline__ int64_t warp_of(const Shares& s, int64_t unit) {
+  const int64_t early = static_cast<int64_t>(s.early) * s.each;
+  return unit < early ? unit / s.each : s.early + (unit - early) / max(s.late, 1);
 }
 
 // A place on the line of units.
@@ -157,47 +165,55 @@ __device__ __forceinline__ Place find_place(const DecodeParams& p, int64_t at, i
   return w;
 }
 
-// One warp: its units in order, each 16 keys of K and V brought by cp.async into the warp's
-// own ring (no barrier between warps), x = Q K^T and P V by m16n8k16 products with the
-// fp32 output row tile in registers.  Memory-bound: a row tile of 16 needs 16 FLOP per byte
+// One warp: its units in order, each 16 keys of K and V brought by TMA into the warp's own ring
+// (no barrier between warps), x = Q K^T and P V by m16n8k16 products with the fp32 output row
+// tile in registers.  Memory-bound: a row tile of 16 needs 16 FLOP per byte
 // of K and V.
 template <int D, bool kBF16, bool kMask>
-__global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) decode_kernel(
+__global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kernel(
     const __grid_constant__ DecodeParams p) {
   using S = DecodeShape<D>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kDecodeWarps + (threadIdx.x >> 5);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kDecodeWarps + wid;
   pdl_launch();
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars) + wid * S::kStages;
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kBars + kDecodeWarps * S::kStages * 8);
+  if (lane < S::kStages) mbar_init(&full[lane], 1);
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    prefetch_tmap(&p.tm_k);
+    prefetch_tmap(&p.tm_v);
+  }
+  fence_mbar_init();
+  __syncthreads();
 
   const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
-                        units_before(p, p.B, lane) * p.Hk * p.tiles;
-  const int64_t share = share_of(p, total);
-  const int64_t first = warp * share;
-  const int n = static_cast<int>(max(min(share, total - first), static_cast<int64_t>(0)));
+                        units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.tiles;
+  const Shares shares = shares_of<D>(p, total, lane);
+  if (warp == 0 && lane == 0) *p.shares = shares;
+  const int64_t first = warp_start(shares, warp);
+  const int n = static_cast<int>(max(min(warp_start(shares, warp + 1), total) - first, static_cast<int64_t>(0)));
   if (n > 0) {
-    const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * S::kStages * S::kStage;
+    uint8_t* ring = smem + wid * S::kStages * S::kStage;
     Place in = find_place(p, first, lane);
     Place at = in;
 
-    // K and V of the unit at `in` into a stage; rows past the item's keys are zeros.
+    // K and V of the unit at `in` into a stage.  Rows past the item's keys come along (zeros past
+    // the cache's end).
     auto bring = [&](int stage) {
-      const int64_t ks = in.prefix ? p.pk_stride[0] : p.k_stride[1], vs = in.prefix ? p.pv_stride[0] : p.v_stride[1];
-      const uint16_t* kb = in.prefix ? static_cast<const uint16_t*>(p.pk) + in.hk * p.pk_stride[1]
-                                     : static_cast<const uint16_t*>(p.k) + in.b * p.k_stride[0] + in.hk * p.k_stride[2];
-      const uint16_t* vb = in.prefix ? static_cast<const uint16_t*>(p.pv) + in.hk * p.pv_stride[1]
-                                     : static_cast<const uint16_t*>(p.v) + in.b * p.v_stride[0] + in.hk * p.v_stride[2];
-      const int key0 = in.u * kUnitKeys;
-      const uint32_t base = ring + stage * S::kStage;
-      constexpr int kChunks = D / 8;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[stage], S::kStage);
+        uint8_t* dst = ring + stage * S::kStage;
+        const CUtensorMap* k = in.prefix ? &p.tm_pk : &p.tm_k;
+        const CUtensorMap* v = in.prefix ? &p.tm_pv : &p.tm_v;
+        const int b = in.prefix ? 0 : in.b;
 #pragma unroll
-      for (int i = 0; i < kUnitKeys * kChunks / 32; ++i) {
-        const int id = i * 32 + lane, row = id / kChunks, c = id - row * kChunks;
-        const bool valid = key0 + row < in.keys;
-        const int64_t key = valid ? key0 + row : key0;
-        const uint32_t dst = base + row * S::kPitch + ((c ^ (row & 7)) << 4);
-        cp_async16(dst, kb + key * ks + c * 8, valid);
-        cp_async16(dst + S::kTile, vb + key * vs + c * 8, valid);
+        for (int c = 0; c < S::kBoxes; ++c) {
+          tma_load_4d(dst + c * S::kBox, k, &full[stage], c * 64, in.u * kUnitKeys, in.hk, b);
+          tma_load_4d(dst + S::kTile + c * S::kBox, v, &full[stage], c * 64, in.u * kUnitKeys, in.hk, b);
+        }
       }
     };
 
@@ -208,11 +224,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
         ++brought;
         if (brought < n) in.advance(p);
       }
-      cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) bring_next();
-
     uint32_t qf[D / 16][4];
     float acc[D / 8][4];
     float m[2], l[2];
@@ -272,12 +284,43 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
       }
     };
 
+    // Mask bits of a unit for this thread's two rows: bit 4 i + 2 nt + e for row i, key
+    // 8 nt + col + e.  They are loaded a unit ahead.
+    auto mask_bits = [&](int u) {
+      uint32_t bits = 0xffu;
+      if constexpr (kMask) {
+        if (at.prefix) return bits;
+        uint8_t v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int j = min(u * kUnitKeys + 8 * ((x >> 1) & 1) + col + (x & 1), at.keys - 1);
+          v[x] = mrow[x >> 2] ? __ldg(mrow[x >> 2] + j) : 0;
+        }
+        bits = 0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) bits |= (v[x] != 0 ? 1u : 0u) << x;
+      }
+      return bits;
+    };
+
+    uint32_t keep_next = 0;
+    // The first rounds only bring (one copy of that code: a CTA runs for microseconds, and
+    // instructions fetched for the first time are a good part of its start).
+#pragma unroll 1
+    for (int i = 0; i < S::kStages - 1; ++i) bring_next();
     begin_item();
+    keep_next = mask_bits(at.u);
+#pragma unroll 1
     for (int it = 0; it < n; ++it) {
-      cp_async_wait<S::kStages - 2>();
-      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[it % S::kStages], (it / S::kStages) & 1, abort_flag))) {
+        // Given up: what is still on its way must land before the CTA ends.
+        for (int j = it; j < brought; ++j) mbar_wait_short(&full[j % S::kStages], (j / S::kStages) & 1);
+        break;
+      }
       bring_next();  // into the stage of the unit before this one
-      const uint32_t sk = ring + (it % S::kStages) * S::kStage, sv = sk + S::kTile;
+      const uint32_t keep_bits = keep_next;
+      if (kMask && at.u + 1 < at.units) keep_next = mask_bits(at.u + 1);
+      const uint32_t sk = smem_u32(ring) + (it % S::kStages) * S::kStage, sv = sk + S::kTile;
 
       float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       {
@@ -285,7 +328,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t kf[4];
-          ldsm4(sk + row * S::kPitch + (((2 * kk + half) ^ (row & 7)) << 4), kf);
+          ldsm4(sk + S::at(row, 2 * kk + half), kf);
           mma16816<kBF16>(x[0], qf[kk], kf[0], kf[1]);
           mma16816<kBF16>(x[1], qf[kk], kf[2], kf[3]);
         }
@@ -298,8 +341,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = e >> 1, kj = 8 * nt + col + (e & 1), j = key0 + kj;
-          bool keep = j < lim[i];
-          if (kMask && keep && mrow[i]) keep = mrow[i][j] != 0;
+          const bool keep = j < lim[i] && (!kMask || ((keep_bits >> (4 * i + 2 * nt + (e & 1))) & 1u));
           x[nt][e] = keep ? x[nt][e] * p.scale_log2 : kNegInf;
           if (keep) dead &= ~(1u << kj);
         }
@@ -319,10 +361,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
         for (int id = lane; id < kUnitKeys * kChunks; id += 32) {
           const int row = id / kChunks, c = id - row * kChunks;
           if ((dead >> row) & 1)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + row * S::kPitch + ((c ^ (row & 7)) << 4)),
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(row, c)),
                          "r"(0)
                          : "memory");
         }
+        fence_async_smem();  // before a copy into the stage
         __syncwarp();
       }
 
@@ -364,19 +407,23 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, DecodeShape<D>::kCtas) deco
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           uint32_t vf[4];
-          ldsm4_t(sv + row * S::kPitch + (((2 * c + half) ^ (row & 7)) << 4), vf);
+          ldsm4_t(sv + S::at(row, 2 * c + half), vf);
           mma16816<kBF16>(acc[2 * c], pf, vf[0], vf[1]);
           mma16816<kBF16>(acc[2 * c + 1], pf, vf[2], vf[3]);
         }
       }
       if (at.u + 1 == at.units || it + 1 == n) end_item();
-      if (it + 1 < n && at.advance(p)) begin_item();
+      if (it + 1 < n && at.advance(p)) {
+        begin_item();
+        keep_next = mask_bits(at.u);
+      }
     }
-    cp_async_wait<0>();
   }
-  // The join may start once this grid is through; it must then also find what the prefix
-  // kernel before this one wrote.
-  pdl_wait();
+  if (lane == 0 && *reinterpret_cast<volatile int*>(abort_flag)) atomicOr(p.status, FA4D_DEV_TIMEOUT_PREFIX);
+  // The join may start once this grid is through, and must then also find what the prefix
+  // kernel before it wrote: one CTA stays until that is done (all of them staying would keep
+  // the SMs from the CTAs still to come).
+  if (blockIdx.x + 1 == gridDim.x) pdl_wait();
 }
 
 // ------------------------------------------------------------------ join
@@ -412,13 +459,18 @@ __device__ __forceinline__ void load_row(const float* row, int lane, float (&v)[
   }
 }
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinRows = 4;                 // rows of weights taken together
 constexpr int kJoinKeys = 4 * kJoinThreads;  // own keys of a block that adds weights
+constexpr int kJoinAhead = 8;                // partial rows of a warp in flight
 
-// Blocks x < row_blocks join the output, a warp a row; the others add the weights of
-// kJoinKeys own keys.
+// Blocks x < row_blocks join the output, row_warps warps a row, each a share of its parts; the
+// others add the weights of kJoinKeys own keys.  Everything here is latency: what does not
+// depend on the row's maximum and sum (logits, weights, partial rows) is loaded ahead of it.
 template <int D, bool kBF16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_blocks) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_blocks,
+                                                             int row_warps) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int hk = blockIdx.y, b = blockIdx.z;
   const bool adds = static_cast<int>(blockIdx.x) >= row_blocks;
@@ -428,17 +480,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 
   const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units;
   const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
-  const int64_t share = share_of(p, prefix_all + units_before(p, p.B, lane) * each);
   const int units = units_of(keys);
-  const int64_t first_unit = prefix_all + units_before(p, b, lane) * each;
+  const int64_t first_unit = prefix_all + units_before(p.lengths, p.C, b, lane) * each;
   pdl_wait();
+  const Shares shares = *p.shares;
 
   // The parts of row r: of its own keys, and of the prefix.
   auto parts_of_units = [&](int64_t from, int count, int64_t item, int row) {
     Parts x{p.seg_o, p.seg_ml, 0, p.seg_rows, 0};
     if (count > 0) {
-      const int64_t w0 = from / share;
-      x.n = static_cast<int>((from + count - 1) / share - w0 + 1);
+      const int64_t w0 = warp_of(shares, from);
+      x.n = static_cast<int>(warp_of(shares, from + count - 1) - w0 + 1);
       x.first = (w0 + item) * p.seg_rows + row;
     }
     return x;
@@ -450,7 +502,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   auto prefix_parts = [&](int r) {
     const int64_t row = static_cast<int64_t>(b) * p.R + r;
     if (p.splits) {
-      return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, p.splits};
+      return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, *p.pre_used};
     }
     const int64_t i = static_cast<int64_t>(hk) * p.prefix_tiles + row / 16;
     return parts_of_units(i * p.prefix_units, p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
@@ -475,32 +527,86 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   };
 
   if (!adds) {
-    const int r = blockIdx.x * (kJoinThreads / 32) + wid;
-    if (r >= p.R) return;
-    const Parts x = prefix_parts(r), y = own_parts(r);
-    const float2 all = total_of(x, y);
+    const int r = (blockIdx.x * kJoinWarps + wid) / row_warps;
+    Parts x{}, y{};
+    if (r < p.R) {
+      x = prefix_parts(r);
+      y = own_parts(r);
+    }
+    const int share = (x.n + y.n + row_warps - 1) / row_warps;
+    const int n0 = min(wid % row_warps * share, x.n + y.n), n = min(n0 + share, x.n + y.n);
     float acc[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-    auto add = [&](const Parts& z) {
-#pragma unroll 4
-      for (int i = 0; i < z.n; ++i) {
-        const int64_t row = z.first + i * z.step;
-        const float m = z.ml[row].x;
-        if (m == kNegInf) continue;  // no key in this part (its row may not even be written)
-        const float f = ex2(m - all.x);
-        float v[D / 32];
-        load_row<D>(z.o + row * D, lane, v);
+    float m_all = kNegInf, l_all = 0.f;
+    // 32 parts at a time, lane i with the maximum of part i; their rows kJoinAhead at a time.
+    for (int i0 = n0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      float2 ml = make_float2(kNegInf, 0.f);
+      if (i < n) ml = i < x.n ? x.ml[x.first + i * x.step] : y.ml[y.first + (i - x.n) * y.step];
+      float l, f;
+      auto settle = [&]() {  // this batch's maximum, factors and sum; the output so far rescaled
+        float mx = ml.x;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] += f * v[e];
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(mx, m_all);
+        f = ml.x == kNegInf ? 0.f : ex2(ml.x - mx);
+        l = ml.y * f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float old = m_all == kNegInf ? 0.f : ex2(m_all - mx);
+        l_all = l_all * old + l;
+        m_all = mx;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) acc[e] *= old;
+      };
+      const int batch = min(32, n - i0);
+      for (int j0 = 0; j0 < batch; j0 += kJoinAhead) {
+        float v[kJoinAhead][D / 32];
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+          const int j = min(i0 + j0 + u, n - 1);
+          const float* row = j < x.n ? x.o + (x.first + j * x.step) * D : y.o + (y.first + (j - x.n) * y.step) * D;
+          load_row<D>(row, lane, v[u]);
+        }
+        if (j0 == 0) settle();
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+          // A part without a key (maximum -inf) may not even have its row written.
+          const float fu = __shfl_sync(0xffffffffu, f, j0 + u), mu = __shfl_sync(0xffffffffu, ml.x, j0 + u);
+          if (j0 + u < batch && mu != kNegInf) {
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) acc[e] += fu * v[u][e];
+          }
+        }
       }
-    };
-    if (all.x != kNegInf) {
-      add(x);
-      add(y);
     }
+    if (row_warps > 1) {  // the row's first warp adds the others'
+      __shared__ float others[kJoinWarps][D];
+      __shared__ float2 others_ml[kJoinWarps];
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) others[wid][(D / 32) * lane + e] = acc[e];
+      if (lane == 0) others_ml[wid] = make_float2(m_all, l_all);
+      __syncthreads();
+      if (wid % row_warps) return;
+      float mx = kNegInf;
+      for (int i = 0; i < row_warps; ++i) mx = fmaxf(mx, others_ml[wid + i].x);
+      l_all = 0.f;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+      for (int i = 0; i < row_warps; ++i) {
+        const float2 ml = others_ml[wid + i];
+        if (ml.x == kNegInf) continue;
+        const float fi = ex2(ml.x - mx);
+        l_all += fi * ml.y;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) acc[e] += fi * others[wid + i][(D / 32) * lane + e];
+      }
+      m_all = mx;
+    }
+    if (r >= p.R) return;
     // A row without a key: 0.  (A NaN maximum or sum stays one.)
-    const float inv = all.x == kNegInf ? 0.f : 1.f / all.y;
+    const float inv = m_all == kNegInf ? 0.f : 1.f / l_all;
     const int t = r / p.G, h = hk * p.G + r % p.G;
     uint16_t* dst = static_cast<uint16_t*>(p.o) + b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
     if constexpr (D == 96) {
@@ -521,33 +627,41 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   constexpr int kRows = 64;
   __shared__ float lse[kRows];
   const int j = key0 + 4 * threadIdx.x;
-  float got[4] = {0.f, 0.f, 0.f, 0.f};
+  float* w = p.weights + b * p.weights_stride[0] + hk * p.weights_stride[1] + j;
+  float got[4] = {0.f, 0.f, 0.f, 0.f}, had[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) had[e] = j + e < keys ? w[e] : 0.f;
   for (int r0 = 0; r0 < p.R; r0 += kRows) {
     const int rows = min(kRows, p.R - r0);
+    const float* row = p.logits + ((static_cast<int64_t>(b) * p.Hk + hk) * p.R + r0) * p.logits_ld + j;
+    float4 x[kJoinRows];
+    auto load = [&](int r) {
+#pragma unroll
+      for (int u = 0; u < kJoinRows; ++u)
+        if (j < keys) x[u] = *reinterpret_cast<const float4*>(row + static_cast<int64_t>(min(r + u, rows - 1)) * p.logits_ld);
+    };
+    load(0);
     __syncthreads();
-    for (int r = wid; r < rows; r += kJoinThreads / 32) {
+    for (int r = wid; r < rows; r += kJoinWarps) {
       const float2 all = total_of(prefix_parts(r0 + r), own_parts(r0 + r));
       if (lane == 0) lse[r] = all.x == kNegInf ? INFINITY : all.x + log2f(all.y);
     }
     __syncthreads();
-    if (j < keys) {
-      const float* row = p.logits + ((static_cast<int64_t>(b) * p.Hk + hk) * p.R + r0) * p.logits_ld + j;
-      for (int r = 0; r < rows; ++r, row += p.logits_ld) {
-        const float4 x = *reinterpret_cast<const float4*>(row);
-        const float sub = lse[r];
-        got[0] += ex2(x.x - sub);
-        got[1] += ex2(x.y - sub);
-        got[2] += ex2(x.z - sub);
-        got[3] += ex2(x.w - sub);
+    for (int r = 0; r < rows; r += kJoinRows) {
+      if (r) load(r);
+#pragma unroll
+      for (int u = 0; u < kJoinRows; ++u) {
+        const float sub = r + u < rows ? lse[r + u] : INFINITY;
+        got[0] += ex2(x[u].x - sub);
+        got[1] += ex2(x[u].y - sub);
+        got[2] += ex2(x[u].z - sub);
+        got[3] += ex2(x[u].w - sub);
       }
     }
   }
-  if (j < keys) {
-    float* w = p.weights + b * p.weights_stride[0] + hk * p.weights_stride[1] + j;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (j + e < keys) w[e] += got[e];
-  }
+  for (int e = 0; e < 4; ++e)
+    if (j + e < keys) w[e] = had[e] + got[e];
 }
 
 // `overlap`: the grid may start before the kernel ahead of it in the stream is through.
@@ -583,17 +697,19 @@ cudaError_t launch_decode_d(const DecodeParams& p, bool bf16, int ctas, bool aft
 }
 
 template <int D>
-cudaError_t launch_join_d(const DecodeParams& p, bool bf16, cudaStream_t s) {
-  const int rows = (p.R + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+cudaError_t launch_join_d(const DecodeParams& p, bool bf16, int sms, cudaStream_t s) {
+  // Warps a row: as many as leave the grid about one block an SM (B32 Hq32 took 4 us longer
+  // with four of them and four times the blocks; one request 2 us less with eight).
+  int row_warps = 1;
+  while (row_warps < kJoinWarps && 2LL * row_warps * p.R * p.Hk * p.B <= 8LL * sms) row_warps *= 2;
+  const int rows = (p.R * row_warps + kJoinWarps - 1) / kJoinWarps;
   const int adds = p.weights ? (p.C + kJoinKeys - 1) / kJoinKeys : 0;
   const dim3 grid(rows + adds, p.Hk, p.B);
-  return bf16 ? launch_with(join_kernel<D, true>, grid, kJoinThreads, 0, true, s, p, rows)
-              : launch_with(join_kernel<D, false>, grid, kJoinThreads, 0, true, s, p, rows);
+  return bf16 ? launch_with(join_kernel<D, true>, grid, kJoinThreads, 0, true, s, p, rows, row_warps)
+              : launch_with(join_kernel<D, false>, grid, kJoinThreads, 0, true, s, p, rows, row_warps);
 }
 
 }  // namespace
-
-int decode_ctas_per_sm(int D) { return D == 256 ? DecodeShape<256>::kCtas : DecodeShape<128>::kCtas; }
 
 cudaError_t launch_decode(const DecodeParams& p, int D, bool bf16, int ctas, bool after_prefix, cudaStream_t s) {
   if (D == 64) return launch_decode_d<64>(p, bf16, ctas, after_prefix, s);
@@ -602,11 +718,11 @@ cudaError_t launch_decode(const DecodeParams& p, int D, bool bf16, int ctas, boo
   return launch_decode_d<256>(p, bf16, ctas, after_prefix, s);
 }
 
-cudaError_t launch_join(const DecodeParams& p, int D, bool bf16, cudaStream_t s) {
-  if (D == 64) return launch_join_d<64>(p, bf16, s);
-  if (D == 96) return launch_join_d<96>(p, bf16, s);
-  if (D == 128) return launch_join_d<128>(p, bf16, s);
-  return launch_join_d<256>(p, bf16, s);
+cudaError_t launch_join(const DecodeParams& p, int D, bool bf16, int sms, cudaStream_t s) {
+  if (D == 64) return launch_join_d<64>(p, bf16, sms, s);
+  if (D == 96) return launch_join_d<96>(p, bf16, sms, s);
+  if (D == 128) return launch_join_d<128>(p, bf16, sms, s);
+  return launch_join_d<256>(p, bf16, sms, s);
 }
 
 }  // namespace fa4d

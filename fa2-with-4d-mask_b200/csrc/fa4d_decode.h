@@ -14,22 +14,34 @@ namespace fa4d {
 // decode_kernel works on *units* of 16 keys of an *item* (a row tile with its keys), laid in
 // one line: first the prefix items (KV head, row tile; none when the prefix kernel does
 // them), then the requests' items (request, KV head, row tile), each with
-// ceil(length / 16) units.  Warp w takes units [w q, (w + 1) q), so ragged lengths divide
-// evenly without the host knowing them.  What warp w computes of an item is *segment*
+// ceil(length / 16) units.  Each warp takes a run of the line (Shares), so ragged lengths
+// divide evenly without the host knowing them.  What warp w computes of an item is *segment*
 // w + item (unique: along the line one of the two grows), an unnormalised fp32 output row
 // with the running maximum (log2) and sum of its exponentials.
+// The units of a warp: the first `early` warps have `each`, the others `late` (0: none).
+struct Shares {
+  int32_t early, each, late;
+};
+
+// What the prefix kernel takes of the GPU (see choose_runs).
+struct PrefixLoad {
+  int32_t items;  // CTAs per run of key tiles; 0: there is no prefix kernel
+  int32_t most;   // runs of its grid
+  int32_t tiles;  // 128-key tiles of the prefix
+  int32_t step;   // key tiles that a CTA takes side by side
+  int32_t sms;
+  int32_t row_tiles;  // of a (request, KV head)
+};
+
 struct DecodeParams {
+  CUtensorMap tm_k, tm_v;    // dims (D, C, Hk, B), box (64, 16, 1, 1), 128-B swizzle
+  CUtensorMap tm_pk, tm_pv;  // the prefix (D, P, Hk, 1), where decode_kernel does it
   const void* q;
-  const void* pk;
-  const void* pv;
-  const void* k;
-  const void* v;
   void* o;
   const int32_t* lengths;
   const uint8_t* mask;
   float* weights;
-  int64_t q_stride[3], pk_stride[2], pv_stride[2], k_stride[3], v_stride[3], o_stride[3], mask_stride[3],
-      weights_stride[2];
+  int64_t q_stride[3], o_stride[3], mask_stride[3], weights_stride[2];
   int32_t B, T, Hq, Hk, P, C;
   int32_t G, R;
   int32_t tiles;         // row tiles of a (request, KV head)
@@ -38,6 +50,8 @@ struct DecodeParams {
   int32_t seg_rows;      // rows kept of a segment: min(16, R or the batch's rows)
   int32_t warps;         // warps of decode_kernel's grid
   int32_t min_units;     // least units of a warp
+  PrefixLoad load;
+  Shares* shares;        // written by decode_kernel, read by join_kernel
   int32_t causal;
   float scale_log2;      // scale * log2(e)
   float* seg_o;          // [segments][seg_rows][D]
@@ -48,6 +62,7 @@ struct DecodeParams {
   int32_t splits, pre_rows;
   float* pre_o;
   float2* pre_ml;
+  const int32_t* pre_used;  // parts that the prefix kernel made, at most `splits`
   int* status;
 };
 
@@ -58,7 +73,11 @@ struct PrefixParams {
   const void* q;
   int64_t q_stride[3];
   int32_t T, G, P, rows;  // rows of a KV head
-  int32_t parts;          // partial results per row
+  int32_t parts;          // partial results per row, at most
+  const int32_t* lengths;  // of the own keys that the decode kernel reads meanwhile
+  int32_t B, C, Hk;
+  PrefixLoad load;
+  int32_t* used;          // partial results per row, written
   int32_t d_in;           // head dim of the tensors (96 computes at 128)
   float scale_log2;
   float* o;               // [Hk][parts][rows][d_in]
@@ -69,11 +88,80 @@ struct PrefixParams {
 constexpr int kDecodeWarps = 4;   // warps of a decode_kernel CTA
 constexpr int kUnitKeys = 16;
 
+// Measured on B200, in microseconds: a key tile of a prefix kernel CTA (two of them, taken side
+// by side, where the slots split the keys) and a CTA's fill, drain and output rows; a unit of a
+// decode_kernel warp beside the SM's others, and the time until its first unit.
+template <int D>
+constexpr float kTileMicros = D == 256 ? 2.2f : D == 64 ? 1.8f : 2.0f;
+constexpr float kRunMicros = 6.0f;
+template <int D>
+constexpr float kUnitMicros = D == 256 ? 2.0f : D == 64 ? 0.65f : 1.2f;
+constexpr float kDecodeMicros = 5.0f;
+constexpr float kReadRate = 6.0f;  // MB per microsecond that decode_kernel reads, of the GPU
+template <int D>
+constexpr int kDecodeCtas = D == 256 ? 1 : 2;  // of an SM
+
+#ifdef __CUDACC__
+struct RunChoice {
+  int runs;
+  float prefix_us, total_us;  // of the prefix kernel, of both
+  float rate;                 // units per microsecond of the whole GPU
+};
+
+__device__ __forceinline__ int length_at(const int32_t* lengths, int b, int C) { return min(max(__ldg(lengths + b), 0), C); }
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnitKeys - 1) / kUnitKeys; }
+
+// Units of the requests before b (all of them for b = B), per KV head and row tile.
+__device__ __forceinline__ int64_t units_before(const int32_t* lengths, int C, int b, int lane) {
+  int64_t n = 0;
+  for (int i = lane; i < b; i += 32) n += units_of(length_at(lengths, i, C));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+
+// How many runs the prefix's key tiles are divided into, at most the grid's.  A run fills an SM
+// (shared memory and registers), and the decode kernel, launched right behind, streams the own
+// keys (`units` of them) on the SMs that are left: fewer, longer runs let the tensor work and
+// the memory work go on side by side.  Only the lengths, on the device, tell how much that is,
+// so it is worked out there by one warp (lane l for l + 1, l + 33, ... runs).
+template <int D>
+__device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t units, int lane) {
+  const float all = static_cast<float>(units);
+  const float sm_rate = kDecodeCtas<D> * kDecodeWarps / kUnitMicros<D>;
+  // Row tiles of a request read the same keys, mostly from L2.
+  const float gpu_rate = fminf(w.sms * sm_rate, kReadRate * 1e6f / (kUnitKeys * 4 * D) * w.row_tiles);
+  RunChoice best{1, 0.f, INFINITY, gpu_rate};
+  for (int s = lane + 1; s <= w.most; s += 32) {
+    const int ctas = w.items * s, run = (w.tiles + s - 1) / s;
+    const float mine = ((ctas + w.sms - 1) / w.sms) * (((run + w.step - 1) / w.step) * kTileMicros<D> + kRunMicros);
+    const float beside = fminf(gpu_rate, sm_rate * max(w.sms - ctas, 0)) * fmaxf(mine - kDecodeMicros, 0.f);
+    const float total = mine + (all > beside ? kDecodeMicros + (all - beside) / gpu_rate : 0.f);
+    if (total < best.total_us) {
+      best.runs = s;
+      best.prefix_us = mine;
+      best.total_us = total;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const int s = __shfl_xor_sync(0xffffffffu, best.runs, o);
+    const float mine = __shfl_xor_sync(0xffffffffu, best.prefix_us, o);
+    const float total = __shfl_xor_sync(0xffffffffu, best.total_us, o);
+    if (total < best.total_us || (total == best.total_us && s > best.runs)) {
+      best.runs = s;
+      best.prefix_us = mine;
+      best.total_us = total;
+    }
+  }
+  return best;
+}
+#endif
+
 cudaError_t launch_decode(const DecodeParams& p, int D, bool bf16, int ctas, bool after_prefix, cudaStream_t s);
 // `split_keys`: the rows of a KV head fit one slot (at most 128), and a run's slots take even
 // and odd key tiles; two parts per run then, one otherwise.
 cudaError_t launch_prefix(const PrefixParams& p, int D, bool bf16, int Hk, int splits, bool split_keys, cudaStream_t s);
-cudaError_t launch_join(const DecodeParams& p, int D, bool bf16, cudaStream_t s);
-int decode_ctas_per_sm(int D);
+cudaError_t launch_join(const DecodeParams& p, int D, bool bf16, int sms, cudaStream_t s);
 
 }  // namespace fa4d

@@ -75,10 +75,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y;
   const int row0 = blockIdx.x * 128 * L::kQTiles;
-  // Key tiles of this run, [kt0, kt0 + n): n >= 1.
   const int tiles = (p.P + 127) / 128;
-  const int kt0 = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.z / gridDim.z);
-  const int n = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.z + 1) / gridDim.z) - kt0;
+  int* runs_shared = reinterpret_cast<int*>(smem + L::kMisc + 8);
+  if (warp == 0) {
+    const int64_t units = units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.load.row_tiles;
+    const int r = choose_runs<D>(p.load, units, lane).runs;
+    if (lane == 0) *runs_shared = r;
+  }
+  __syncthreads();
+  const int runs = *runs_shared;
+  if (static_cast<int>(blockIdx.z) >= runs) return;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) *p.used = runs * (kSplitKeys ? 2 : 1);
+  // Key tiles of this run, [kt0, kt0 + n): n >= 1.
+  const int kt0 = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.z / runs);
+  const int n = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.z + 1) / runs) - kt0;
   // Whether slot 1 has rows (or tiles) of its own.
   const bool two = !kDoubleS && (kSplitKeys ? n > 1 : row0 + 128 < p.rows);
 

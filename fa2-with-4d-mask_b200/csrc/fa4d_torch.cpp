@@ -404,11 +404,11 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   q = rows16(q);
   Tensor out = at::empty_like(q);
   if (out.numel() == 0) return THPVariable_Wrap(out);
-  k = rows16(k);
-  v = rows16(v);
+  k = rows16(k, true);  // keys and values go through tensor maps
+  v = rows16(v, true);
   fa4d_prefix_attention_args a;
   memset(&a, 0, sizeof(a));
-  if (P) {  // the prefix also goes through tensor maps
+  if (P) {
     pk = rows16(pk, true);
     pv = rows16(pv, true);
     a.prefix_k = pk.data_ptr();
