@@ -6,6 +6,7 @@
 // 2^(m - m_all).
 #include "fa4d.h"
 #include "fa4d_decode.h"
+#include "fa4d_launch.cuh"
 #include "fa4d_ptx.cuh"
 
 namespace fa4d {
@@ -53,9 +54,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ int length_of(const DecodeParams& p, int b) { return length_at(p.lengths, b, p.C); }
 // The division of `total` units.  Beside a prefix kernel the warps of the SMs that it leaves
 // free start at once, and the others when it is done: those get less, by its estimated time.
@@ -171,13 +169,12 @@ __device__ __forceinline__ Place find_place(const DecodeParams& p, int64_t at, i
 // of K and V.
 template <int D, bool kBF16, bool kMask>
 __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kernel(
-    const __grid_constant__ DecodeParams p) {
+    const __grid_constant__ DecodeParams p, bool after_prefix) {
   using S = DecodeShape<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t warp = static_cast<int64_t>(blockIdx.x) * kDecodeWarps + wid;
-  pdl_launch();
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars) + wid * S::kStages;
   int* abort_flag = reinterpret_cast<int*>(smem + S::kBars + kDecodeWarps * S::kStages * 8);
   if (lane < S::kStages) mbar_init(&full[lane], 1);
@@ -188,6 +185,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   }
   fence_mbar_init();
   __syncthreads();
+  // Behind the prefix kernel, which itself started only when everything ahead was through and
+  // writes nothing that is read here, there is nothing to wait for.
+  if (!after_prefix) pdl_wait();
+  pdl_launch();
 
   const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
                         units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.tiles;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   // The join may start once this grid is through, and must then also find what the prefix
   // kernel before it wrote: one CTA stays until that is done (all of them staying would keep
   // the SMs from the CTAs still to come).
-  if (blockIdx.x + 1 == gridDim.x) pdl_wait();
+  if (after_prefix && blockIdx.x + 1 == gridDim.x) pdl_wait();
 }
 
 // ------------------------------------------------------------------ join
@@ -471,6 +472,7 @@ constexpr int kJoinAhead = 8;                // partial rows of a warp in flight
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_blocks,
                                                              int row_warps) {
+  pdl_launch();
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int hk = blockIdx.y, b = blockIdx.z;
   const bool adds = static_cast<int>(blockIdx.x) >= row_blocks;
@@ -664,28 +666,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (j + e < keys) w[e] = had[e] + got[e];
 }
 
-// `overlap`: the grid may start before the kernel ahead of it in the stream is through.
-template <typename K, typename... Args>
-cudaError_t launch_with(K kernel, dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = overlap ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int D, bool kBF16, bool kMask>
 cudaError_t launch_decode_t(const DecodeParams& p, int ctas, bool after_prefix, cudaStream_t s) {
   auto kern = decode_kernel<D, kBF16, kMask>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D>::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_with(kern, dim3(ctas), 32 * kDecodeWarps, DecodeShape<D>::kBytes, after_prefix, s, p);
+  return launch_chained(kern, dim3(ctas), 32 * kDecodeWarps, DecodeShape<D>::kBytes, 1, s, p, after_prefix);
 }
 
 template <int D>
@@ -705,8 +691,8 @@ cudaError_t launch_join_d(const DecodeParams& p, bool bf16, int sms, cudaStream_
   const int rows = (p.R * row_warps + kJoinWarps - 1) / kJoinWarps;
   const int adds = p.weights ? (p.C + kJoinKeys - 1) / kJoinKeys : 0;
   const dim3 grid(rows + adds, p.Hk, p.B);
-  return bf16 ? launch_with(join_kernel<D, true>, grid, kJoinThreads, 0, true, s, p, rows, row_warps)
-              : launch_with(join_kernel<D, false>, grid, kJoinThreads, 0, true, s, p, rows, row_warps);
+  return bf16 ? launch_chained(join_kernel<D, true>, grid, kJoinThreads, 0, 1, s, p, rows, row_warps)
+              : launch_chained(join_kernel<D, false>, grid, kJoinThreads, 0, 1, s, p, rows, row_warps);
 }
 
 }  // namespace

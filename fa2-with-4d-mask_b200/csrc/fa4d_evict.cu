@@ -8,6 +8,7 @@
 // (4 D bytes each way), against 4 bytes of weight an entry.
 #include "fa4d.h"
 #include "fa4d_kernels.h"
+#include "fa4d_launch.cuh"
 #include "fa4d_ptx.cuh"
 
 namespace fa4d {
@@ -109,6 +110,8 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
   const int item = static_cast<int>(blockIdx.x) / ranks;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int b = item / a.Hk, h = item - b * a.Hk;
+  pdl_wait();
+  pdl_launch();
   const int n = min(max(__ldg(a.lengths + b), 0), a.C);
   const int kept = min(n, a.keep);
   const float* w = a.weights + b * a.weights_stride[0] + h * a.weights_stride[1];
@@ -361,18 +364,7 @@ template <int VEC>
 cudaError_t launch_evict_t(const fa4d_evict_args& a, int ranks, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(evict_kernel<VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ranks) * a.B * a.Hk);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Smem);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, evict_kernel<VEC>, a);
+  return launch_chained(evict_kernel<VEC>, dim3(static_cast<unsigned>(ranks) * a.B * a.Hk), kThreads, sizeof(Smem), ranks, s, a);
 }
 
 }  // namespace

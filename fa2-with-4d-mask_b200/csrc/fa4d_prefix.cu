@@ -20,6 +20,7 @@
 // (16-bit, rounded to the type of V as the product takes it) overwrites S.
 #include "fa4d.h"
 #include "fa4d_decode.h"
+#include "fa4d_launch.cuh"
 #include "fa4d_mma.cuh"
 #include "fa4d_ptx.cuh"
 
@@ -35,6 +36,13 @@ constexpr float kNegInf = -INFINITY;
 // O is rescaled only when a running maximum grows by more than this (log2 units).
 constexpr float kRescaleThreshold = 8.0f;
 
+// A whole 32-byte sector.
+__device__ __forceinline__ void st_sector(float* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <int D, bool kSplitKeys>
 struct PrefixLayout {
   static constexpr int kTile = 128 * D * 2;
@@ -45,7 +53,7 @@ struct PrefixLayout {
   static constexpr int kK = kQ + kQTiles * kTile;
   static constexpr int kV = kK + kStages * kTile;
   static constexpr int kBar = kV + kStages * kTile;
-  static constexpr int kNumBars = 10 + 4 * kStages;
+  static constexpr int kNumBars = 8 + 4 * kStages;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kAlloc = kMisc + 16 + 1024;  // slack to align the base to 1024 B
   static_assert(kAlloc <= 232448, "shared memory beyond the 227 KB per-block limit");
@@ -59,13 +67,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* q_full = bars + 0;   // [2] per slot, 128 arrivals
-  uint64_t* s_full = bars + 2;   // [2] per slot (per S buffer at D = 256)
-  uint64_t* p_full = bars + 4;   // [2]
-  uint64_t* o_full = bars + 6;   // [2]
-  uint64_t* mma_drain = bars + 8;
-  uint64_t* pv_done = bars + 9;  // D = 256: PV of a tile completed
-  uint64_t* k_full = bars + 10;
+  uint64_t* s_full = bars + 0;   // [2] per slot (per S buffer at D = 256)
+  uint64_t* p_full = bars + 2;   // [2]
+  uint64_t* o_full = bars + 4;   // [2]
+  uint64_t* mma_drain = bars + 6;
+  uint64_t* pv_done = bars + 7;  // D = 256: PV of a tile completed
+  uint64_t* k_full = bars + 8;
   uint64_t* k_empty = k_full + KVS;
   uint64_t* v_full = k_empty + KVS;
   uint64_t* v_empty = v_full + KVS;
@@ -77,49 +84,72 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   const int row0 = blockIdx.x * 128 * L::kQTiles;
   const int tiles = (p.P + 127) / 128;
   int* runs_shared = reinterpret_cast<int*>(smem + L::kMisc + 8);
+  // The start, side by side: the number of runs, barriers, tensor memory, Q.
   if (warp == 0) {
+    pdl_wait();
     const int64_t units = units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.load.row_tiles;
     const int r = choose_runs<D>(p.load, units, lane).runs;
     if (lane == 0) *runs_shared = r;
+  } else if (warp == 1) {
+    if (lane == 0) {
+      prefetch_tmap(&p.tm_k);
+      prefetch_tmap(&p.tm_v);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 128);
+        mbar_init(&o_full[i], 1);
+      }
+      mbar_init(mma_drain, 1);
+      mbar_init(pv_done, 1);
+      for (int i = 0; i < KVS; ++i) {
+        mbar_init(&k_full[i], 1);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], 1);
+        mbar_init(&v_empty[i], 1);
+      }
+      *abort_flag = 0;
+      fence_mbar_init();
+    }
+  } else if (warp == 2) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (warp >= 4 && (warp - 4) / 4 < L::kQTiles) {
+    // Q rows into the swizzled tile, D / 8 lanes a row; lane i knows where row i lies.
+    pdl_wait();
+    const int t = (warp - 4) / 4, first = (warp & 3) * 32, row = row0 + 128 * t + first + lane;
+    const int token = row / p.G, h = hk * p.G + row % p.G;
+    const int b = token / p.T, tt = token - b * p.T;
+    const int64_t mine = b * p.q_stride[0] + tt * p.q_stride[1] + h * p.q_stride[2];
+    constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
+    const int c = lane % kLanes;
+    uint8_t* dst = smem + L::kQ + t * L::kTile + (c >> 3) * 16384;
+#pragma unroll 8
+    for (int i = 0; i < 32; i += kRowsAtOnce) {
+      const int r = i + lane / kLanes;
+      const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row0 + 128 * t + first + r < p.rows && 8 * c < p.d_in)
+        v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at) + c);
+      *reinterpret_cast<uint4*>(dst + (first + r) * 128 + (((c ^ r) & 7) << 4)) = v;
+    }
+    fence_async_smem();
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   const int runs = *runs_shared;
-  if (static_cast<int>(blockIdx.z) >= runs) return;
+  if (static_cast<int>(blockIdx.z) >= runs) {
+    if (warp == 2) tmem_dealloc(tmem, 512);
+    return;
+  }
   if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) *p.used = runs * (kSplitKeys ? 2 : 1);
   // Key tiles of this run, [kt0, kt0 + n): n >= 1.
   const int kt0 = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.z / runs);
   const int n = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.z + 1) / runs) - kt0;
   // Whether slot 1 has rows (or tiles) of its own.
   const bool two = !kDoubleS && (kSplitKeys ? n > 1 : row0 + 128 < p.rows);
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 128);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_full[i], 1);
-    }
-    mbar_init(mma_drain, 1);
-    mbar_init(pv_done, 1);
-    for (int i = 0; i < KVS; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
-    }
-    *abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == 2) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  // The decode kernel may take over SMs as these CTAs end.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  pdl_launch();  // the decode kernel takes the SMs that are left, and these as their CTAs end
 
   if (warp < 4) {
     regs_dec<kRegsCtl>();
@@ -138,8 +168,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     };
     if (warp == 0) {
       if (lane == 0) {
-        prefetch_tmap(&p.tm_k);
-        prefetch_tmap(&p.tm_v);
         int uk = 0, uv = 0;
         bool ok = true;
         for (int u = 0; ok && u < n; ++u) {
@@ -169,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       auto pv = [&](int t, int u, bool accumulate) {
         issue_pv<D, kBF16>(kDoubleS ? tmem + 256 : tmem + 256 + D * t, tmem + 128 * t, sV + (u % KVS) * L::kTile, accumulate);
       };
-      bool ok = wait(&q_full[0], 0) && (!two || kSplitKeys || wait(&q_full[1], 0)) && wait(&k_full[0], 0);
+      bool ok = wait(&k_full[0], 0);
       if (ok) {
         tc_fence_after();
         if (elect_one()) {
@@ -274,23 +302,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       const bool warp_valid = row - lane < p.rows;  // some lane has a row
       const uint32_t lane_base = static_cast<uint32_t>(quad) << 16;
 
-      // Q rows of the slot (both slots have the same ones with kSplitKeys: slot 0 loads them).
-      if (!kSplitKeys || t == 0) {
-        const int token = row / p.G, h = hk * p.G + row % p.G;
-        const int b = token / p.T, tt = token - b * p.T;
-        const uint16_t* q =
-            static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + tt * p.q_stride[1] + h * p.q_stride[2];
-        uint8_t* dst = smem + L::kQ + t * L::kTile + at * 128;
-#pragma unroll 8
-        for (int c = 0; c < D / 8; ++c) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (valid && 8 * c < p.d_in) v = __ldg(reinterpret_cast<const uint4*>(q) + c);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (at & 7)) << 4)) = v;
-        }
-        fence_async_smem();
-        mbar_arrive(&q_full[t]);
-      }
-
       const int count = kSplitKeys ? (n - t + 1) / 2 : n;
       const uint32_t tO = tmem + lane_base + 256 + (kDoubleS ? 0 : D * t);
       float m_run = kNegInf, l_run = 0.f;
@@ -391,9 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             tmem_ld32(tO + 32 * c, o);
             tmem_wait_ld();
             if (valid && 32 * c < p.d_in) {
-              uint4* dst = reinterpret_cast<uint4*>(p.o + out * p.d_in + 32 * c);
+              float* dst = p.o + out * p.d_in + 32 * c;
 #pragma unroll
-              for (int v = 0; v < 8; ++v) dst[v] = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+              for (int v = 0; v < 4; ++v) st_sector(dst + 8 * v, &o[8 * v]);
             }
           }
         }
@@ -417,8 +428,7 @@ cudaError_t launch_prefix_t(const PrefixParams& p, int Hk, int splits, cudaStrea
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   if (e != cudaSuccess) return e;
   const dim3 grid((p.rows + 128 * L::kQTiles - 1) / (128 * L::kQTiles), Hk, splits);
-  kern<<<grid, kThreads, L::kAlloc, s>>>(p);
-  return cudaGetLastError();
+  return launch_chained(kern, grid, kThreads, L::kAlloc, 1, s, p);
 }
 
 template <int D, bool kBF16>

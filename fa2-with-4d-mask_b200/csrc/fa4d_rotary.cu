@@ -10,6 +10,7 @@
 // Both are bound by memory: each element is read once and written once.
 #include "fa4d.h"
 #include "fa4d_kernels.h"
+#include "fa4d_launch.cuh"
 #include "fa4d_ptx.cuh"
 
 namespace fa4d {
@@ -108,6 +109,8 @@ constexpr int kHeads = 4;
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ fa4d_rotary_args a, int chunks,
                                                           int heads_each) {
+  pdl_wait();
+  pdl_launch();
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t n = id / chunks;
   if (n >= static_cast<int64_t>(a.B) * a.T) return;
@@ -147,6 +150,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_constant__ fa4d_rotary_append_args a,
                                                                  int chunks, int* status) {
+  pdl_wait();
+  pdl_launch();
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int heads = a.Hq + 2 * a.Hk;
   const int64_t row = id / chunks, n = row / heads;
@@ -201,11 +206,8 @@ cudaError_t launch_rotary_t(const fa4d_rotary_args& a, int sms, cudaStream_t s) 
   const int split = static_cast<int>(min(want, static_cast<int64_t>((heads + kHeads - 1) / kHeads)));
   const int each = (heads + split - 1) / split;
   const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads), (heads + each - 1) / each);
-  if (a.table.pairing == FA4D_PAIR_ADJACENT)
-    rotary_kernel<kBF16, true, VEC><<<grid, kThreads, 0, s>>>(a, chunks, each);
-  else
-    rotary_kernel<kBF16, false, VEC><<<grid, kThreads, 0, s>>>(a, chunks, each);
-  return cudaGetLastError();
+  auto kern = a.table.pairing == FA4D_PAIR_ADJACENT ? rotary_kernel<kBF16, true, VEC> : rotary_kernel<kBF16, false, VEC>;
+  return launch_chained(kern, grid, kThreads, 0, 1, s, a, chunks, each);
 }
 
 template <int VEC, bool kBF16>
@@ -213,11 +215,9 @@ cudaError_t launch_append_t(const fa4d_rotary_append_args& a, int* status, cudaS
   const int chunks = chunks_of(a.table, VEC);
   const int64_t threads = static_cast<int64_t>(a.B) * a.T * (a.Hq + 2 * a.Hk) * chunks;
   const unsigned grid = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
-  if (a.table.pairing == FA4D_PAIR_ADJACENT)
-    rotary_append_kernel<kBF16, true, VEC><<<grid, kThreads, 0, s>>>(a, chunks, status);
-  else
-    rotary_append_kernel<kBF16, false, VEC><<<grid, kThreads, 0, s>>>(a, chunks, status);
-  return cudaGetLastError();
+  auto kern =
+      a.table.pairing == FA4D_PAIR_ADJACENT ? rotary_append_kernel<kBF16, true, VEC> : rotary_append_kernel<kBF16, false, VEC>;
+  return launch_chained(kern, dim3(grid), kThreads, 0, 1, s, a, chunks, status);
 }
 
 }  // namespace
