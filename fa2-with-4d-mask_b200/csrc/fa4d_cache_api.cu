@@ -68,7 +68,7 @@ struct Plan {
   int ctas;
   int splits;        // runs of key tiles of the prefix kernel; 0: decode_kernel does the prefix
   bool split_keys;
-  size_t seg_o, seg_ml, logits, pre_o, pre_ml, pre_used, total;
+  size_t seg_o, seg_ml, logits, pre_o, pre_ml, shares, total;
 };
 
 // Runs per (row tile, KV head) of the prefix kernel: the number that shortens the estimate
@@ -143,8 +143,8 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   out->pre_o = out->logits + (weights ? align256(static_cast<size_t>(B) * Hk * p.R * p.logits_ld * sizeof(float)) : 0);
   const size_t pre = static_cast<size_t>(p.splits) * Hk * p.pre_rows;
   out->pre_ml = out->pre_o + align256(pre * D * sizeof(float));
-  out->pre_used = out->pre_ml + align256(pre * sizeof(float2));
-  out->total = out->pre_used + 256;  // the runs made, and the shares
+  out->shares = out->pre_ml + align256(pre * sizeof(float2));
+  out->total = out->shares + 256;
   return FA4D_OK;
 }
 
@@ -240,6 +240,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
     p.mask_stride[i] = a->mask_stride[i];
   }
   for (int i = 0; i < 2; ++i) p.weights_stride[i] = a->weights_stride[i];
+  p.weights_vec = aligned16(a->weights) && a->weights_stride[0] % 4 == 0 && a->weights_stride[1] % 4 == 0;
   p.causal = a->causal;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.seg_o = reinterpret_cast<float*>(ws + plan.seg_o);
@@ -247,9 +248,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   p.logits = a->weights ? reinterpret_cast<float*>(ws + plan.logits) : nullptr;
   p.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
   p.pre_ml = reinterpret_cast<float2*>(ws + plan.pre_ml);
-  int32_t* used = reinterpret_cast<int32_t*>(ws + plan.pre_used);
-  p.pre_used = used;
-  p.shares = reinterpret_cast<fa4d::Shares*>(used + 16);
+  p.shares = reinterpret_cast<fa4d::Shares*>(ws + plan.shares);
   p.status = fa4d::host_status_word();
   if (!p.status) return fail(FA4D_ERR_CUDA, "device status word is not available");
   const bool bf16 = a->dtype == FA4D_BF16;
@@ -283,7 +282,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
     x.C = a->C;
     x.Hk = a->Hk;
     x.load = p.load;
-    x.used = used;
+    x.shares = p.shares;
     x.scale_log2 = p.scale_log2;
     x.o = p.pre_o;
     x.ml = p.pre_ml;

@@ -70,10 +70,10 @@ __device__ __forceinline__ Shares shares_of(const DecodeParams& p, int64_t total
       const float late_us = fmaxf(c.total_us - c.prefix_us - kDecodeMicros, 0.f);
       const float part = fminf(late_us * c.rate * rest / p.warps, static_cast<float>(total));
       const int late = static_cast<int>(part / max(rest, 1));
-      return Shares{early, max(up(total - static_cast<int64_t>(late) * rest, early), least), late};
+      return Shares{early, max(up(total - static_cast<int64_t>(late) * rest, early), least), late, 0};
     }
   }
-  return Shares{p.warps, max(up(total, p.warps), least), 0};
+  return Shares{p.warps, max(up(total, p.warps), least), 0, 0};
 }
 
 __device__ __forceinline__ int64_t warp_start(const Shares& s, int64_t warp) {
@@ -134,30 +134,36 @@ __device__ __forceinline__ Place find_place(const DecodeParams& p, int64_t at, i
   }
   at -= prefix_all;
   const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    const int mine = b < p.B ? units_of(length_of(p, b)) : 0;
-    int64_t upto = mine;
+  for (int b0 = 0; b0 < p.B; b0 += 128) {
+    int mine[4];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t left = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += left;
+    for (int x = 0; x < 4; ++x) mine[x] = units_of(length_of(p, min(b0 + 32 * x + lane, p.B - 1)));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (b0 + 32 * x >= p.B) break;
+      if (b0 + 32 * x + lane >= p.B) mine[x] = 0;
+      int64_t upto = mine[x];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t left = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += left;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto * each > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        at -= (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine[x], l)) * each;
+        w.prefix = false;
+        w.b = b0 + 32 * x + l;
+        w.keys = length_of(p, w.b);
+        w.units = units_of(w.keys);
+        const int64_t item = at / w.units;
+        w.hk = static_cast<int>(item / p.tiles);
+        w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * p.tiles);
+        w.u = static_cast<int>(at - item * w.units);
+        return w;
+      }
+      at -= __shfl_sync(0xffffffffu, upto, 31) * each;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, upto * each > at);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      at -= (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine, l)) * each;
-      w.prefix = false;
-      w.b = b0 + l;
-      w.keys = length_of(p, w.b);
-      w.units = units_of(w.keys);
-      const int64_t item = at / w.units;
-      w.hk = static_cast<int>(item / p.tiles);
-      w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * p.tiles);
-      w.u = static_cast<int>(at - item * w.units);
-      return w;
-    }
-    at -= __shfl_sync(0xffffffffu, upto, 31) * each;
   }
   w.to_request(p, p.B);
   return w;
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   }
   fence_mbar_init();
   __syncthreads();
-  // Behind the prefix kernel, which itself started only when everything ahead was through and
+  // Behind the prefix kernel, every CTA of which has seen everything ahead complete, and which
   // writes nothing that is read here, there is nothing to wait for.
   if (!after_prefix) pdl_wait();
   pdl_launch();
@@ -193,7 +199,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
                         units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.tiles;
   const Shares shares = shares_of<D>(p, total, lane);
-  if (warp == 0 && lane == 0) *p.shares = shares;
+  if (warp == 0 && lane == 0) {
+    p.shares->early = shares.early;
+    p.shares->each = shares.each;
+    p.shares->late = shares.late;
+  }
   const int64_t first = warp_start(shares, warp);
   const int n = static_cast<int>(max(min(warp_start(shares, warp + 1), total) - first, static_cast<int64_t>(0)));
   if (n > 0) {
@@ -257,8 +267,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
             static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + col;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][i] = valid ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * kk)) : 0u;
-          qf[kk][i + 2] = valid ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * kk + 8)) : 0u;
+          qf[kk][i] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * kk)) : 0u;
+          qf[kk][i + 2] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * kk + 8)) : 0u;
         }
         m[i] = kNegInf;
         l[i] = 0.f;
@@ -295,7 +305,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const int j = min(u * kUnitKeys + 8 * ((x >> 1) & 1) + col + (x & 1), at.keys - 1);
-          v[x] = mrow[x >> 2] ? __ldg(mrow[x >> 2] + j) : 0;
+          v[x] = mrow[x >> 2] ? __ldcg(mrow[x >> 2] + j) : 0;
         }
         bits = 0;
 #pragma unroll
@@ -462,33 +472,27 @@ __device__ __forceinline__ void load_row(const float* row, int lane, float (&v)[
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinRows = 4;                 // rows of weights taken together
-constexpr int kJoinKeys = 4 * kJoinThreads;  // own keys of a block that adds weights
-constexpr int kJoinAhead = 8;                // partial rows of a warp in flight
+constexpr int kJoinAhead = 8;                 // partial rows of a warp in flight
+constexpr int kWeighRows = 4;                 // rows of weights taken together
+constexpr int kWeighKeys = 4 * kJoinThreads;  // own keys of a block of weigh_kernel at a time
+constexpr int kWeighTimes = 4;
 
-// Blocks x < row_blocks join the output, row_warps warps a row, each a share of its parts; the
-// others add the weights of kJoinKeys own keys.  Everything here is latency: what does not
-// depend on the row's maximum and sum (logits, weights, partial rows) is loaded ahead of it.
-template <int D, bool kBF16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_blocks,
-                                                             int row_warps) {
-  pdl_launch();
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int hk = blockIdx.y, b = blockIdx.z;
-  const bool adds = static_cast<int>(blockIdx.x) >= row_blocks;
-  const int keys = length_of(p, b);
-  const int key0 = (static_cast<int>(blockIdx.x) - row_blocks) * kJoinKeys;
-  if (adds && key0 >= keys) return;
+// The partial results of the rows of (request b, KV head hk).
+struct Joined {
+  const DecodeParams& p;
+  int b, hk, keys, units;
+  int64_t each, first_unit;
+  Shares shares;
 
-  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units;
-  const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
-  const int units = units_of(keys);
-  const int64_t first_unit = prefix_all + units_before(p.lengths, p.C, b, lane) * each;
-  pdl_wait();
-  const Shares shares = *p.shares;
-
-  // The parts of row r: of its own keys, and of the prefix.
-  auto parts_of_units = [&](int64_t from, int count, int64_t item, int row) {
+  // Before the partial results are there: what the lengths tell.
+  __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane) : p(params), b(b_), hk(hk_) {
+    keys = length_of(p, b);
+    units = units_of(keys);
+    each = static_cast<int64_t>(p.Hk) * p.tiles;
+    first_unit = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
+                 units_before(p.lengths, p.C, b, lane) * each;
+  }
+  __device__ __forceinline__ Parts of_units(int64_t from, int count, int64_t item, int row) const {
     Parts x{p.seg_o, p.seg_ml, 0, p.seg_rows, 0};
     if (count > 0) {
       const int64_t w0 = warp_of(shares, from);
@@ -496,174 +500,210 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       x.first = (w0 + item) * p.seg_rows + row;
     }
     return x;
-  };
-  auto own_parts = [&](int r) {
-    const int64_t i = static_cast<int64_t>(hk) * p.tiles + r / 16;
-    return parts_of_units(first_unit + i * units, units, static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
-  };
-  auto prefix_parts = [&](int r) {
-    const int64_t row = static_cast<int64_t>(b) * p.R + r;
-    if (p.splits) {
-      return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, *p.pre_used};
-    }
-    const int64_t i = static_cast<int64_t>(hk) * p.prefix_tiles + row / 16;
-    return parts_of_units(i * p.prefix_units, p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
-  };
-  // Maximum and sum over all parts of a row.
-  auto total_of = [&](const Parts& x, const Parts& y) {
-    float m = kNegInf, l = 0.f;
-    for (int i = lane; i < x.n + y.n; i += 32) {
-      const float2 ml = i < x.n ? x.ml[x.first + i * x.step] : y.ml[y.first + (i - x.n) * y.step];
-      const float mx = fmaxf(m, ml.x);
-      if (mx != kNegInf) l = l * ex2(m - mx) + ml.y * ex2(ml.x - mx);
-      m = mx;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-      const float mx = fmaxf(m, m2);
-      if (mx != kNegInf) l = l * ex2(m - mx) + l2 * ex2(m2 - mx);
-      m = mx;
-    }
-    return make_float2(m, l);
-  };
-
-  if (!adds) {
-    const int r = (blockIdx.x * kJoinWarps + wid) / row_warps;
-    Parts x{}, y{};
-    if (r < p.R) {
-      x = prefix_parts(r);
-      y = own_parts(r);
-    }
-    const int share = (x.n + y.n + row_warps - 1) / row_warps;
-    const int n0 = min(wid % row_warps * share, x.n + y.n), n = min(n0 + share, x.n + y.n);
-    float acc[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-    float m_all = kNegInf, l_all = 0.f;
-    // 32 parts at a time, lane i with the maximum of part i; their rows kJoinAhead at a time.
-    for (int i0 = n0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      float2 ml = make_float2(kNegInf, 0.f);
-      if (i < n) ml = i < x.n ? x.ml[x.first + i * x.step] : y.ml[y.first + (i - x.n) * y.step];
-      float l, f;
-      auto settle = [&]() {  // this batch's maximum, factors and sum; the output so far rescaled
-        float mx = ml.x;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mx = fmaxf(mx, m_all);
-        f = ml.x == kNegInf ? 0.f : ex2(ml.x - mx);
-        l = ml.y * f;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const float old = m_all == kNegInf ? 0.f : ex2(m_all - mx);
-        l_all = l_all * old + l;
-        m_all = mx;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] *= old;
-      };
-      const int batch = min(32, n - i0);
-      for (int j0 = 0; j0 < batch; j0 += kJoinAhead) {
-        float v[kJoinAhead][D / 32];
-#pragma unroll
-        for (int u = 0; u < kJoinAhead; ++u) {
-          const int j = min(i0 + j0 + u, n - 1);
-          const float* row = j < x.n ? x.o + (x.first + j * x.step) * D : y.o + (y.first + (j - x.n) * y.step) * D;
-          load_row<D>(row, lane, v[u]);
-        }
-        if (j0 == 0) settle();
-#pragma unroll
-        for (int u = 0; u < kJoinAhead; ++u) {
-          // A part without a key (maximum -inf) may not even have its row written.
-          const float fu = __shfl_sync(0xffffffffu, f, j0 + u), mu = __shfl_sync(0xffffffffu, ml.x, j0 + u);
-          if (j0 + u < batch && mu != kNegInf) {
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) acc[e] += fu * v[u][e];
-          }
-        }
-      }
-    }
-    if (row_warps > 1) {  // the row's first warp adds the others'
-      __shared__ float others[kJoinWarps][D];
-      __shared__ float2 others_ml[kJoinWarps];
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) others[wid][(D / 32) * lane + e] = acc[e];
-      if (lane == 0) others_ml[wid] = make_float2(m_all, l_all);
-      __syncthreads();
-      if (wid % row_warps) return;
-      float mx = kNegInf;
-      for (int i = 0; i < row_warps; ++i) mx = fmaxf(mx, others_ml[wid + i].x);
-      l_all = 0.f;
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-      for (int i = 0; i < row_warps; ++i) {
-        const float2 ml = others_ml[wid + i];
-        if (ml.x == kNegInf) continue;
-        const float fi = ex2(ml.x - mx);
-        l_all += fi * ml.y;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] += fi * others[wid + i][(D / 32) * lane + e];
-      }
-      m_all = mx;
-    }
-    if (r >= p.R) return;
-    // A row without a key: 0.  (A NaN maximum or sum stays one.)
-    const float inv = m_all == kNegInf ? 0.f : 1.f / l_all;
-    const int t = r / p.G, h = hk * p.G + r % p.G;
-    uint16_t* dst = static_cast<uint16_t*>(p.o) + b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
-    if constexpr (D == 96) {
-#pragma unroll
-      for (int e = 0; e < 3; ++e) dst[3 * lane + e] = static_cast<uint16_t>(pack2<kBF16>(acc[e] * inv, 0.f));
-    } else {
-      uint32_t w[D / 64];
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) w[e] = pack2<kBF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-      if constexpr (D == 64) *reinterpret_cast<uint32_t*>(dst + 2 * lane) = w[0];
-      if constexpr (D == 128) *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(w[0], w[1]);
-      if constexpr (D == 256) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    return;
   }
+  __device__ __forceinline__ void load_shares() {
+    const int4 s = __ldcg(reinterpret_cast<const int4*>(p.shares));
+    shares = Shares{s.x, s.y, s.z, s.w};
+  }
+  // The parts of row r: of its own keys, and of the prefix.
+  __device__ __forceinline__ Parts own(int r) const {
+    const int64_t i = static_cast<int64_t>(hk) * p.tiles + r / 16;
+    return of_units(first_unit + i * units, units, static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
+  }
+  __device__ __forceinline__ Parts prefix(int r) const {
+    const int64_t row = static_cast<int64_t>(b) * p.R + r;
+    if (p.splits)
+      return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, shares.parts};
+    const int64_t i = static_cast<int64_t>(hk) * p.prefix_tiles + row / 16;
+    return of_units(i * p.prefix_units, p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
+  }
+};
 
-  // Weights: sum over the rows of 2^(x - lse), lse = +inf for a row without a key.
+// Joins the output: row_warps warps a row, each a share of its parts.  Everything here is
+// latency: partial rows are loaded ahead of the maximum that scales them.
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_warps) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  Joined at(p, blockIdx.z, blockIdx.y, lane);
+  pdl_wait();
+  pdl_launch();
+  at.load_shares();
+
+  const int r = (blockIdx.x * kJoinWarps + wid) / row_warps;
+  Parts x{}, y{};
+  if (r < p.R) {
+    x = at.prefix(r);
+    y = at.own(r);
+  }
+  const int share = (x.n + y.n + row_warps - 1) / row_warps;
+  const int n0 = min(wid % row_warps * share, x.n + y.n), n = min(n0 + share, x.n + y.n);
+  float acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  float m_all = kNegInf, l_all = 0.f;
+  // 32 parts at a time, lane i with the maximum of part i; their rows kJoinAhead at a time.
+  for (int i0 = n0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    float2 ml = make_float2(kNegInf, 0.f);
+    if (i < n) ml = i < x.n ? x.ml[x.first + i * x.step] : y.ml[y.first + (i - x.n) * y.step];
+    float f;
+    auto settle = [&]() {  // this batch's maximum, factors and sum; the output so far rescaled
+      float mx = ml.x;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = fmaxf(mx, m_all);
+      f = ml.x == kNegInf ? 0.f : ex2(ml.x - mx);
+      float l = ml.y * f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const float old = m_all == kNegInf ? 0.f : ex2(m_all - mx);
+      l_all = l_all * old + l;
+      m_all = mx;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] *= old;
+    };
+    const int batch = min(32, n - i0);
+    for (int j0 = 0; j0 < batch; j0 += kJoinAhead) {
+      float v[kJoinAhead][D / 32];
+#pragma unroll
+      for (int u = 0; u < kJoinAhead; ++u) {
+        const int j = min(i0 + j0 + u, n - 1);
+        const float* row = j < x.n ? x.o + (x.first + j * x.step) * D : y.o + (y.first + (j - x.n) * y.step) * D;
+        load_row<D>(row, lane, v[u]);
+      }
+      if (j0 == 0) settle();
+#pragma unroll
+      for (int u = 0; u < kJoinAhead; ++u) {
+        // A part without a key (maximum -inf) may not even have its row written.
+        const float fu = __shfl_sync(0xffffffffu, f, j0 + u), mu = __shfl_sync(0xffffffffu, ml.x, j0 + u);
+        if (j0 + u < batch && mu != kNegInf) {
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) acc[e] += fu * v[u][e];
+        }
+      }
+    }
+  }
+  if (row_warps > 1) {  // the row's first warp adds the others'
+    __shared__ float others[kJoinWarps][D];
+    __shared__ float2 others_ml[kJoinWarps];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) others[wid][(D / 32) * lane + e] = acc[e];
+    if (lane == 0) others_ml[wid] = make_float2(m_all, l_all);
+    __syncthreads();
+    if (wid % row_warps) return;
+    float mx = kNegInf;
+    for (int i = 0; i < row_warps; ++i) mx = fmaxf(mx, others_ml[wid + i].x);
+    l_all = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    for (int i = 0; i < row_warps; ++i) {
+      const float2 ml = others_ml[wid + i];
+      if (ml.x == kNegInf) continue;
+      const float fi = ex2(ml.x - mx);
+      l_all += fi * ml.y;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] += fi * others[wid + i][(D / 32) * lane + e];
+    }
+    m_all = mx;
+  }
+  if (r >= p.R) return;
+  // A row without a key: 0.  (A NaN maximum or sum stays one.)
+  const float inv = m_all == kNegInf ? 0.f : 1.f / l_all;
+  const int t = r / p.G, h = at.hk * p.G + r % p.G;
+  uint16_t* dst = static_cast<uint16_t*>(p.o) + at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
+  if constexpr (D == 96) {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) dst[3 * lane + e] = static_cast<uint16_t>(pack2<kBF16>(acc[e] * inv, 0.f));
+  } else {
+    uint32_t w[D / 64];
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) w[e] = pack2<kBF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    if constexpr (D == 64) *reinterpret_cast<uint32_t*>(dst + 2 * lane) = w[0];
+    if constexpr (D == 128) *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(w[0], w[1]);
+    if constexpr (D == 256) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Adds to the weights of a request's own keys: the sum over the rows of 2^(x - lse), lse = +inf
+// for a row without a key.  A kernel of its own beside join_kernel, whose registers would leave
+// it two blocks an SM (33 us in one kernel at B128 Hk8, 4096 slots; 95 MB).  It starts when
+// every block of join_kernel has found the partial results complete, so they are complete here,
+// works beside it, and its last block waits so that this kernel is over only when that one is.
+__global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kRows = 64;
   __shared__ float lse[kRows];
-  const int j = key0 + 4 * threadIdx.x;
-  float* w = p.weights + b * p.weights_stride[0] + hk * p.weights_stride[1] + j;
-  float got[4] = {0.f, 0.f, 0.f, 0.f}, had[4];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  Joined at(p, blockIdx.z, blockIdx.y, lane);
+  const int key0 = blockIdx.x * kWeighTimes * kWeighKeys + 4 * threadIdx.x;
+  float* weights = p.weights + at.b * p.weights_stride[0] + at.hk * p.weights_stride[1];
+  if (blockIdx.x * kWeighTimes * kWeighKeys < at.keys) {
+    at.load_shares();
+    for (int r0 = 0; r0 < p.R; r0 += kRows) {
+      const int rows = min(kRows, p.R - r0);
+      const float* logits = p.logits + ((static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r0) * p.logits_ld;
+      float4 x[kWeighRows];
+      auto load = [&](int j, int r) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) had[e] = j + e < keys ? w[e] : 0.f;
-  for (int r0 = 0; r0 < p.R; r0 += kRows) {
-    const int rows = min(kRows, p.R - r0);
-    const float* row = p.logits + ((static_cast<int64_t>(b) * p.Hk + hk) * p.R + r0) * p.logits_ld + j;
-    float4 x[kJoinRows];
-    auto load = [&](int r) {
+        for (int u = 0; u < kWeighRows; ++u)
+          x[u] = __ldcg(reinterpret_cast<const float4*>(logits + static_cast<int64_t>(min(r + u, rows - 1)) * p.logits_ld + j));
+      };
+      __syncthreads();
+      for (int r = wid; r < rows; r += kJoinWarps) {
+        // Maximum and sum over all parts of the row.
+        const Parts px = at.prefix(r0 + r), py = at.own(r0 + r);
+        float m = kNegInf, l = 0.f;
+        for (int i = lane; i < px.n + py.n; i += 32) {
+          const float2 ml = __ldcg(i < px.n ? px.ml + px.first + i * px.step : py.ml + py.first + (i - px.n) * py.step);
+          const float mx = fmaxf(m, ml.x);
+          if (mx != kNegInf) l = l * ex2(m - mx) + ml.y * ex2(ml.x - mx);
+          m = mx;
+        }
 #pragma unroll
-      for (int u = 0; u < kJoinRows; ++u)
-        if (j < keys) x[u] = *reinterpret_cast<const float4*>(row + static_cast<int64_t>(min(r + u, rows - 1)) * p.logits_ld);
-    };
-    load(0);
-    __syncthreads();
-    for (int r = wid; r < rows; r += kJoinWarps) {
-      const float2 all = total_of(prefix_parts(r0 + r), own_parts(r0 + r));
-      if (lane == 0) lse[r] = all.x == kNegInf ? INFINITY : all.x + log2f(all.y);
-    }
-    __syncthreads();
-    for (int r = 0; r < rows; r += kJoinRows) {
-      if (r) load(r);
+        for (int o = 16; o; o >>= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+          const float mx = fmaxf(m, m2);
+          if (mx != kNegInf) l = l * ex2(m - mx) + l2 * ex2(m2 - mx);
+          m = mx;
+        }
+        if (lane == 0) lse[r] = m == kNegInf ? INFINITY : m + log2f(l);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 0; i < kWeighTimes; ++i) {
+        const int j = key0 + i * kWeighKeys;
+        if (j >= at.keys) break;
+        float got[4];
+        const bool whole = p.weights_vec && j + 4 <= at.keys;
+        if (whole) {
+          const float4 w = __ldcg(reinterpret_cast<const float4*>(weights + j));
+          got[0] = w.x, got[1] = w.y, got[2] = w.z, got[3] = w.w;
+        } else {
 #pragma unroll
-      for (int u = 0; u < kJoinRows; ++u) {
-        const float sub = r + u < rows ? lse[r + u] : INFINITY;
-        got[0] += ex2(x[u].x - sub);
-        got[1] += ex2(x[u].y - sub);
-        got[2] += ex2(x[u].z - sub);
-        got[3] += ex2(x[u].w - sub);
+          for (int e = 0; e < 4; ++e) got[e] = j + e < at.keys ? __ldcg(weights + j + e) : 0.f;
+        }
+        for (int r = 0; r < rows; r += kWeighRows) {
+          load(j, r);
+#pragma unroll
+          for (int u = 0; u < kWeighRows; ++u) {
+            const float sub = r + u < rows ? lse[r + u] : INFINITY;
+            got[0] += ex2(x[u].x - sub);
+            got[1] += ex2(x[u].y - sub);
+            got[2] += ex2(x[u].z - sub);
+            got[3] += ex2(x[u].w - sub);
+          }
+        }
+        if (whole) {
+          *reinterpret_cast<float4*>(weights + j) = make_float4(got[0], got[1], got[2], got[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j + e < at.keys) weights[j + e] = got[e];
+        }
       }
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (j + e < keys) w[e] = had[e] + got[e];
+  pdl_launch();
+  if (blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z) pdl_wait();
 }
 
 template <int D, bool kBF16, bool kMask>
@@ -688,11 +728,12 @@ cudaError_t launch_join_d(const DecodeParams& p, bool bf16, int sms, cudaStream_
   // with four of them and four times the blocks; one request 2 us less with eight).
   int row_warps = 1;
   while (row_warps < kJoinWarps && 2LL * row_warps * p.R * p.Hk * p.B <= 8LL * sms) row_warps *= 2;
-  const int rows = (p.R * row_warps + kJoinWarps - 1) / kJoinWarps;
-  const int adds = p.weights ? (p.C + kJoinKeys - 1) / kJoinKeys : 0;
-  const dim3 grid(rows + adds, p.Hk, p.B);
-  return bf16 ? launch_chained(join_kernel<D, true>, grid, kJoinThreads, 0, 1, s, p, rows, row_warps)
-              : launch_chained(join_kernel<D, false>, grid, kJoinThreads, 0, 1, s, p, rows, row_warps);
+  const dim3 grid((p.R * row_warps + kJoinWarps - 1) / kJoinWarps, p.Hk, p.B);
+  auto kern = bf16 ? join_kernel<D, true> : join_kernel<D, false>;
+  const cudaError_t e = launch_chained(kern, grid, kJoinThreads, 0, 1, s, p, row_warps);
+  if (e != cudaSuccess || !p.weights) return e;
+  const dim3 weigh((p.C + kWeighTimes * kWeighKeys - 1) / (kWeighTimes * kWeighKeys), p.Hk, p.B);
+  return launch_chained(weigh_kernel, weigh, kJoinThreads, 0, 1, s, p);
 }
 
 }  // namespace

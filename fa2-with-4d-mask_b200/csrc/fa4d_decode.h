@@ -18,9 +18,10 @@ namespace fa4d {
 // divide evenly without the host knowing them.  What warp w computes of an item is *segment*
 // w + item (unique: along the line one of the two grows), an unnormalised fp32 output row
 // with the running maximum (log2) and sum of its exponentials.
-// The units of a warp: the first `early` warps have `each`, the others `late` (0: none).
-struct Shares {
-  int32_t early, each, late;
+// The units of a warp: the first `early` warps have `each`, the others `late` (0: none); and
+// the parts of a row that the prefix kernel made.  16 bytes, read together.
+struct alignas(16) Shares {
+  int32_t early, each, late, parts;
 };
 
 // What the prefix kernel takes of the GPU (see choose_runs).
@@ -51,18 +52,18 @@ struct DecodeParams {
   int32_t warps;         // warps of decode_kernel's grid
   int32_t min_units;     // least units of a warp
   PrefixLoad load;
-  Shares* shares;        // written by decode_kernel, read by join_kernel
+  Shares* shares;        // written by decode_kernel (parts: by prefix_kernel), read by the join
   int32_t causal;
   float scale_log2;      // scale * log2(e)
   float* seg_o;          // [segments][seg_rows][D]
   float2* seg_ml;        // [segments][seg_rows]: maximum (log2 units), sum
   float* logits;         // [B, Hk, R, logits_ld] of the own keys, log2 units; null without weights
   int32_t logits_ld;
+  int32_t weights_vec;   // rows of weights start on 16-byte boundaries
   // Partial results of the prefix kernel: [Hk][splits][pre_rows] rows, splits 0: none.
   int32_t splits, pre_rows;
   float* pre_o;
   float2* pre_ml;
-  const int32_t* pre_used;  // parts that the prefix kernel made, at most `splits`
   int* status;
 };
 
@@ -77,7 +78,7 @@ struct PrefixParams {
   const int32_t* lengths;  // of the own keys that the decode kernel reads meanwhile
   int32_t B, C, Hk;
   PrefixLoad load;
-  int32_t* used;          // partial results per row, written
+  Shares* shares;         // `parts` written: the partial results per row, at most p.parts
   int32_t d_in;           // head dim of the tensors (96 computes at 128)
   float scale_log2;
   float* o;               // [Hk][parts][rows][d_in]
@@ -108,13 +109,21 @@ struct RunChoice {
   float rate;                 // units per microsecond of the whole GPU
 };
 
-__device__ __forceinline__ int length_at(const int32_t* lengths, int b, int C) { return min(max(__ldg(lengths + b), 0), C); }
+// Read past L1 (as is everything that a kernel of the chain reads without a wait of its own):
+// what is complete is in L2, and an SM's L1 may still hold what an earlier kernel read there.
+__device__ __forceinline__ int length_at(const int32_t* lengths, int b, int C) { return min(max(__ldcg(lengths + b), 0), C); }
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnitKeys - 1) / kUnitKeys; }
 
 // Units of the requests before b (all of them for b = B), per KV head and row tile.
 __device__ __forceinline__ int64_t units_before(const int32_t* lengths, int C, int b, int lane) {
   int64_t n = 0;
-  for (int i = lane; i < b; i += 32) n += units_of(length_at(lengths, i, C));
+  for (int i = lane; i < b; i += 128) {  // four loads in flight
+    int u[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) u[x] = units_of(length_at(lengths, min(i + 32 * x, b - 1), C));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) n += i + 32 * x < b ? u[x] : 0;
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n;

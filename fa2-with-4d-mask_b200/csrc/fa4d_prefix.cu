@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     if (warp == 2) tmem_dealloc(tmem, 512);
     return;
   }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) *p.used = runs * (kSplitKeys ? 2 : 1);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.shares->parts = runs * (kSplitKeys ? 2 : 1);
   // Key tiles of this run, [kt0, kt0 + n): n >= 1.
   const int kt0 = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.z / runs);
   const int n = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.z + 1) / runs) - kt0;

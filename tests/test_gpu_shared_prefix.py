@@ -198,6 +198,35 @@ def test_repeats_bit_for_bit_in_a_graph_and_on_another_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,P", [(2, 0), (40, 500)])
+def test_inputs_changed_in_place_between_calls(B, P):
+    """Back-to-back calls with no synchronisation, each after kernels that rewrite lengths, query,
+    caches and mask in the same memory: every call sees its own inputs."""
+    g = torch.Generator().manual_seed(10)
+    q, pk, pv, k, v = make(g, B, 2, 8, 2, 64, P, 70, torch.bfloat16, "bhsd")
+    steps = []
+    for i in range(6):
+        steps.append((torch.randn(q.shape, generator=g).to(q), torch.randn(k.shape, generator=g).to(k),
+                      torch.randint(0, 71, (B,), generator=g, dtype=torch.int32).to(DEV),
+                      (torch.rand(B, 1, 2, 70, generator=g) < 0.7).to(DEV)))
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    mask = torch.zeros(B, 1, 2, 70, dtype=torch.bool, device=DEV)
+    w = torch.zeros(B, 2, 70, device=DEV)
+    got = []
+    for q1, k1, n1, m1 in steps:
+        for dst, src in ((q, q1), (k, k1), (lengths, n1), (mask, m1)):
+            dst.copy_(src)
+        w.zero_()
+        got.append((api.shared_prefix_attention(q, pk, pv, k, v, lengths, mask=mask, weights=w), w.clone()))
+    for (q1, k1, n1, m1), (out, w1) in zip(steps, got):
+        torch.cuda.synchronize()
+        w.zero_()
+        again = api.shared_prefix_attention(q1, pk, pv, k1, v, n1, mask=m1, weights=w)
+        torch.cuda.synchronize()
+        assert torch.equal(out, again) and torch.equal(w1, w)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     store = torch.empty(2 ** 31 + 65536, dtype=torch.bfloat16, device=DEV)
     k = store.as_strided((2, 1, 200, 64), (2 ** 31 + 8, 64 * 200, 64, 1))
