@@ -84,88 +84,122 @@ __device__ __forceinline__ int64_t warp_of(const Shares& s, int64_t unit) {
   return unit < early ? unit / s.each : s.early + (unit - early) / max(s.late, 1);
 }
 
-// A place on the line of units.
+// The lengths of the first 128 requests in a warp's registers (lane l: l, l + 32, ...), the
+// others in memory.
+struct Lengths {
+  int n[4];
+  __device__ __forceinline__ void load(const DecodeParams& p, int lane) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) n[x] = length_of(p, min(32 * x + lane, p.B - 1));
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (32 * x + lane >= p.B) n[x] = 0;
+  }
+  __device__ __forceinline__ int of(const DecodeParams& p, int b) const {
+    if (b >= 128) return length_of(p, b);
+    return __shfl_sync(0xffffffffu, b < 64 ? (b < 32 ? n[0] : n[1]) : (b < 96 ? n[2] : n[3]), b & 31);
+  }
+  // What all requests take of the line, per KV head and row tile.
+  __device__ __forceinline__ int64_t line(const DecodeParams& p, int lane) const {
+    int64_t all = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) all += line_of(n[x]);
+    for (int i = 128 + lane; i < p.B; i += 32) all += line_of(length_of(p, i));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    return all;
+  }
+};
+
+// A place on the line, in a run with `left` of it to go.
 struct Place {
   bool prefix;
   int b, hk, tile;  // the item (b unused in the prefix)
   int u, units;     // unit within the item, units of the item
   int keys;         // keys of the item
+  int64_t left;
 
+  __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ int item(const DecodeParams& p) const {
     return prefix ? hk * p.prefix_tiles + tile : (p.prefix_tiles + b * p.tiles) * p.Hk + hk * p.tiles + tile;
   }
-  // First request at or after b that has keys (B: none).
-  __device__ __forceinline__ void to_request(const DecodeParams& p, int from) {
+  __device__ __forceinline__ void next_item(const DecodeParams& p, const Lengths& lengths) {
+    u = 0;
+    if (++tile < (prefix ? p.prefix_tiles : p.tiles)) return;
+    tile = 0;
+    if (++hk < p.Hk) return;
+    hk = 0;
+    b = prefix ? 0 : b + 1;
     prefix = false;
-    u = hk = tile = 0;
-    keys = units = 0;
-    for (b = from; b < p.B; ++b) {
-      keys = length_of(p, b);
+    for (; b < p.B; ++b) {  // the next request with keys
+      keys = lengths.of(p, b);
       units = units_of(keys);
-      if (units) break;
+      if (units) return;
     }
+    left = 0;
   }
   // To the next unit; true if it is of another item.
-  __device__ __forceinline__ bool advance(const DecodeParams& p) {
+  __device__ __forceinline__ bool advance(const DecodeParams& p, const Lengths& lengths) {
+    --left;
     if (++u < units) return false;
-    u = 0;
-    if (++tile < (prefix ? p.prefix_tiles : p.tiles)) return true;
-    tile = 0;
-    if (++hk < p.Hk) return true;
-    to_request(p, prefix ? 0 : b + 1);
+    left -= kItemUnits;
+    next_item(p, lengths);
     return true;
   }
 };
 
-// The place of unit `at` (which exists).
-__device__ __forceinline__ Place find_place(const DecodeParams& p, int64_t at, int lane) {
+// The first unit at or after `at` on the line, in a run of `left`.
+__device__ __forceinline__ Place find_place(const DecodeParams& p, const Lengths& lengths, int64_t at, int64_t left,
+                                            int lane) {
   Place w;
-  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units;
-  if (at < prefix_all) {
-    const int64_t item = at / p.prefix_units;
-    w.prefix = true;
-    w.b = 0;
-    w.hk = static_cast<int>(item / p.prefix_tiles);
-    w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * p.prefix_tiles);
-    w.u = static_cast<int>(at - item * p.prefix_units);
-    w.units = p.prefix_units;
+  w.left = left;
+  w.b = 0;
+  int64_t line = p.prefix_units + kItemUnits;
+  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * line;
+  int tiles = p.tiles;
+  w.prefix = at < prefix_all;
+  if (w.prefix) {
     w.keys = p.P;
-    return w;
-  }
-  at -= prefix_all;
-  const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
-  for (int b0 = 0; b0 < p.B; b0 += 128) {
-    int mine[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) mine[x] = units_of(length_of(p, min(b0 + 32 * x + lane, p.B - 1)));
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (b0 + 32 * x >= p.B) break;
-      if (b0 + 32 * x + lane >= p.B) mine[x] = 0;
-      int64_t upto = mine[x];
+    tiles = p.prefix_tiles;
+  } else {
+    at -= prefix_all;
+    const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
+    bool found = false;
+    auto search = [&](int b0, int mine) {  // among the 32 requests from b0
+      int64_t upto = line_of(mine);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t left = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += left;
+        const int64_t before = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += before;
       }
       const unsigned past = __ballot_sync(0xffffffffu, upto * each > at);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        at -= (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine[x], l)) * each;
-        w.prefix = false;
-        w.b = b0 + 32 * x + l;
-        w.keys = length_of(p, w.b);
-        w.units = units_of(w.keys);
-        const int64_t item = at / w.units;
-        w.hk = static_cast<int>(item / p.tiles);
-        w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * p.tiles);
-        w.u = static_cast<int>(at - item * w.units);
-        return w;
+      found = past != 0;
+      const int l = found ? __ffs(past) - 1 : 31;
+      const int64_t to = __shfl_sync(0xffffffffu, upto, l);
+      if (!found) {
+        at -= to * each;
+        return;
       }
-      at -= __shfl_sync(0xffffffffu, upto, 31) * each;
-    }
+      w.b = b0 + l;
+      w.keys = __shfl_sync(0xffffffffu, mine, l);
+      line = line_of(w.keys);
+      at -= (to - line) * each;
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (!found && 32 * x < p.B) search(32 * x, lengths.n[x]);
+    for (int b0 = 128; !found && b0 < p.B; b0 += 32)
+      search(b0, b0 + lane < p.B ? length_of(p, b0 + lane) : 0);
   }
-  w.to_request(p, p.B);
+  w.units = units_of(w.keys);
+  const int64_t item = at / line;
+  w.hk = static_cast<int>(item / tiles);
+  w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * tiles);
+  w.u = static_cast<int>(at - item * line);
+  if (w.u >= w.units) {  // in the item's change of rows
+    w.left -= line - w.u;
+    w.next_item(p, lengths);
+  }
   return w;
 }
 
@@ -196,8 +230,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   if (!after_prefix) pdl_wait();
   pdl_launch();
 
-  const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
-                        units_before(p.lengths, p.C, p.B, lane) * p.Hk * p.tiles;
+  Lengths lengths;
+  lengths.load(p, lane);
+  const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kItemUnits) +
+                        lengths.line(p, lane) * p.Hk * p.tiles;
   const Shares shares = shares_of<D>(p, total, lane);
   if (warp == 0 && lane == 0) {
     p.shares->early = shares.early;
@@ -205,11 +241,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
     p.shares->late = shares.late;
   }
   const int64_t first = warp_start(shares, warp);
-  const int n = static_cast<int>(max(min(warp_start(shares, warp + 1), total) - first, static_cast<int64_t>(0)));
-  if (n > 0) {
+  const int64_t run = min(warp_start(shares, warp + 1), total) - first;
+  Place at;
+  at.left = 0;
+  if (run > 0) at = find_place(p, lengths, first, run, lane);
+  if (at.more()) {
     uint8_t* ring = smem + wid * S::kStages * S::kStage;
-    Place in = find_place(p, first, lane);
-    Place at = in;
+    Place in = at;
 
     // K and V of the unit at `in` into a stage.  Rows past the item's keys come along (zeros past
     // the cache's end).
@@ -230,12 +268,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
 
     int brought = 0;
     auto bring_next = [&]() {
-      if (brought < n) {
+      if (in.more()) {
         bring(brought % S::kStages);
         ++brought;
-        if (brought < n) in.advance(p);
+        in.advance(p, lengths);
       }
     };
+
     uint32_t qf[D / 16][4];
     float acc[D / 8][4];
     float m[2], l[2];
@@ -322,7 +361,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
     begin_item();
     keep_next = mask_bits(at.u);
 #pragma unroll 1
-    for (int it = 0; it < n; ++it) {
+    for (int it = 0; at.more(); ++it) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full[it % S::kStages], (it / S::kStages) & 1, abort_flag))) {
         // Given up: what is still on its way must land before the CTA ends.
         for (int j = it; j < brought; ++j) mbar_wait_short(&full[j % S::kStages], (j / S::kStages) & 1);
@@ -423,8 +462,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
           mma16816<kBF16>(acc[2 * c + 1], pf, vf[2], vf[3]);
         }
       }
-      if (at.u + 1 == at.units || it + 1 == n) end_item();
-      if (it + 1 < n && at.advance(p)) {
+      if (at.u + 1 == at.units || at.left == 1) end_item();
+      if (at.advance(p, lengths) && at.more()) {
         begin_item();
         keep_next = mask_bits(at.u);
       }
@@ -480,18 +519,18 @@ constexpr int kWeighTimes = 4;
 // The partial results of the rows of (request b, KV head hk).
 struct Joined {
   const DecodeParams& p;
-  int b, hk, keys, units;
-  int64_t each, first_unit;
+  int b, hk, keys;
+  int64_t each, first;
   Shares shares;
 
   // Before the partial results are there: what the lengths tell.
   __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane) : p(params), b(b_), hk(hk_) {
     keys = length_of(p, b);
-    units = units_of(keys);
     each = static_cast<int64_t>(p.Hk) * p.tiles;
-    first_unit = static_cast<int64_t>(p.prefix_tiles) * p.Hk * p.prefix_units +
-                 units_before(p.lengths, p.C, b, lane) * each;
+    first = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kItemUnits) +
+            line_before(p.lengths, p.C, b, lane) * each;
   }
+  // Of an item of `count` units that starts at `from` on the line.
   __device__ __forceinline__ Parts of_units(int64_t from, int count, int64_t item, int row) const {
     Parts x{p.seg_o, p.seg_ml, 0, p.seg_rows, 0};
     if (count > 0) {
@@ -508,14 +547,14 @@ struct Joined {
   // The parts of row r: of its own keys, and of the prefix.
   __device__ __forceinline__ Parts own(int r) const {
     const int64_t i = static_cast<int64_t>(hk) * p.tiles + r / 16;
-    return of_units(first_unit + i * units, units, static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
+    return of_units(first + i * line_of(keys), units_of(keys), static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
   }
   __device__ __forceinline__ Parts prefix(int r) const {
     const int64_t row = static_cast<int64_t>(b) * p.R + r;
     if (p.splits)
       return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, shares.parts};
     const int64_t i = static_cast<int64_t>(hk) * p.prefix_tiles + row / 16;
-    return of_units(i * p.prefix_units, p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
+    return of_units(i * (p.prefix_units + kItemUnits), p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
   }
 };
 

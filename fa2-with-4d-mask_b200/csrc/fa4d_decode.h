@@ -14,11 +14,12 @@ namespace fa4d {
 // decode_kernel works on *units* of 16 keys of an *item* (a row tile with its keys), laid in
 // one line: first the prefix items (KV head, row tile; none when the prefix kernel does
 // them), then the requests' items (request, KV head, row tile), each with
-// ceil(length / 16) units.  Each warp takes a run of the line (Shares), so ragged lengths
-// divide evenly without the host knowing them.  What warp w computes of an item is *segment*
+// ceil(length / 16) units and the time of kItemUnits more, which a change of rows costs (its
+// output written, the next item's queries read).  Each warp takes a run of the line (Shares),
+// so ragged lengths divide evenly without the host knowing them.  What warp w computes of an item is *segment*
 // w + item (unique: along the line one of the two grows), an unnormalised fp32 output row
 // with the running maximum (log2) and sum of its exponentials.
-// The units of a warp: the first `early` warps have `each`, the others `late` (0: none); and
+// The run of a warp: the first `early` warps have `each` units, the others `late` (0: none); and
 // the parts of a row that the prefix kernel made.  16 bytes, read together.
 struct alignas(16) Shares {
   int32_t early, each, late, parts;
@@ -88,6 +89,7 @@ struct PrefixParams {
 
 constexpr int kDecodeWarps = 4;   // warps of a decode_kernel CTA
 constexpr int kUnitKeys = 16;
+constexpr int kItemUnits = 2;
 
 // Measured on B200, in microseconds: a key tile of a prefix kernel CTA (two of them, taken side
 // by side, where the slots split the keys) and a CTA's fill, drain and output rows; a unit of a
@@ -114,13 +116,16 @@ struct RunChoice {
 __device__ __forceinline__ int length_at(const int32_t* lengths, int b, int C) { return min(max(__ldcg(lengths + b), 0), C); }
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnitKeys - 1) / kUnitKeys; }
 
-// Units of the requests before b (all of them for b = B), per KV head and row tile.
-__device__ __forceinline__ int64_t units_before(const int32_t* lengths, int C, int b, int lane) {
+// What an item of so many keys takes of the line.
+__device__ __forceinline__ int line_of(int keys) { return keys > 0 ? units_of(keys) + kItemUnits : 0; }
+
+// What the requests before b (all of them for b = B) take of the line, per KV head and row tile.
+__device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, int b, int lane) {
   int64_t n = 0;
   for (int i = lane; i < b; i += 128) {  // four loads in flight
     int u[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) u[x] = units_of(length_at(lengths, min(i + 32 * x, b - 1), C));
+    for (int x = 0; x < 4; ++x) u[x] = line_of(length_at(lengths, min(i + 32 * x, b - 1), C));
 #pragma unroll
     for (int x = 0; x < 4; ++x) n += i + 32 * x < b ? u[x] : 0;
   }
