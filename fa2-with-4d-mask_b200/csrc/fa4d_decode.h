@@ -95,11 +95,11 @@ constexpr int kItemUnits = 2;
 // by side, where the slots split the keys) and a CTA's fill, drain and output rows; a unit of a
 // decode_kernel warp beside the SM's others, and the time until its first unit.
 template <int D>
-constexpr float kTileMicros = D == 256 ? 2.2f : D == 64 ? 1.8f : 2.0f;
+constexpr float kTileMicros = D == 256 ? 1.4f : D == 64 ? 1.9f : 2.1f;
 constexpr float kRunMicros = 6.0f;
 template <int D>
-constexpr float kUnitMicros = D == 256 ? 2.0f : D == 64 ? 0.65f : 1.2f;
-constexpr float kDecodeMicros = 5.0f;
+constexpr float kUnitMicros = D == 256 ? 1.6f : D == 64 ? 0.6f : 1.0f;
+constexpr float kDecodeMicros = 3.5f;
 constexpr float kReadRate = 6.0f;  // MB per microsecond that decode_kernel reads, of the GPU
 template <int D>
 constexpr int kDecodeCtas = D == 256 ? 1 : 2;  // of an SM
