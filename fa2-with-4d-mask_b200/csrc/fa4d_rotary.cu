@@ -17,7 +17,7 @@ namespace fa4d {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // VEC pairs of one head: two runs of VEC elements.  VEC = 8 moves them as two 16-byte
 // vectors; VEC = 1 serves sizes and addresses that are not multiples of 16 bytes.

@@ -54,6 +54,13 @@ struct Layout {
   int head() const { return bhsd ? 1 : 2; }
 };
 
+// Whether two elements share memory through a stride of 0, which a tensor that is written may not.
+bool repeats(const Tensor& x) {
+  for (int i = 0; i < x.dim(); ++i)
+    if (x.size(i) > 1 && x.stride(i) == 0) return true;
+  return false;
+}
+
 void set3(int64_t (&out)[3], const Tensor& x, Layout l) {
   out[0] = x.stride(0);
   out[1] = x.stride(l.seq());
@@ -311,6 +318,8 @@ PyObject* rotary_append(PyObject* const* args) {
   const int64_t C = check_cache(kc, vc, lengths, weights, l, B, Hk, table->t.D, q);
   no_gradient("append", {&q, &k, &v});
   if (kc.stride(3) != 1 || vc.stride(3) != 1) refuse("the caches are written in place and need unit head-dim stride");
+  if (repeats(kc) || repeats(vc) || (weights.defined() && repeats(weights)))
+    refuse("the caches and weights are written in place and may not repeat memory");
   need_cuda("MultiAxisRotary", q);
   q = unit_rows(q);
   k = unit_rows(k);
@@ -360,6 +369,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   if (D != 64 && D != 96 && D != 128 && D != 256) refuse(cat("head dim ", D, " is not built (64, 96, 128, 256)"));
   const Tensor lengths = any_tensor(args[5], kLengths), weights = optional_arg(args[7], kWeights);
   const int64_t C = check_cache(k, v, lengths, weights, l, B, Hk, D, q);
+  if (weights.defined() && repeats(weights)) refuse("weights are written in place and may not repeat memory");
   if ((args[1] == Py_None) != (args[2] == Py_None)) refuse("prefix_key and prefix_value go together");
   Tensor pk, pv;
   int64_t P = 0;
@@ -487,6 +497,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
     wo = any_tensor(PyTuple_GET_ITEM(args[7], 2), what);
     if (check_cache(ko, vo, lengths, wo, l, B, Hk, D, k) < keep) refuse(what);
     if (ko.stride(3) != 1 || vo.stride(3) != 1) refuse("out is written in place and needs unit head-dim stride");
+    if (repeats(ko) || repeats(vo) || repeats(wo)) refuse("out is written in place and may not repeat memory");
     for (const Tensor* x : std::initializer_list<const Tensor*>{&ko, &vo, &wo})
       for (const Tensor* y : std::initializer_list<const Tensor*>{&k, &v, &weights, &lengths})
         if (meet(*x, *y)) refuse("out may not share memory with the inputs");

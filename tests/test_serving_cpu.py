@@ -90,6 +90,8 @@ def test_no_cpu_fallback():
     (dict(w=torch.zeros(2, 8, 2).transpose(1, 2)), "weights must be"),
     (dict(w=torch.zeros(2, 2, 8, dtype=torch.float64)), "weights must be"),
     (dict(k=_new().requires_grad_()), "no gradient"),
+    (dict(vc=_new(B=1, T=8).expand(2, -1, -1, -1)), "may not repeat memory"),
+    (dict(w=torch.zeros(1, 2, 8).expand(2, -1, -1)), "may not repeat memory"),
     (dict(kc=_new(D=8, T=64).transpose(2, 3)), "expected batch|unit head-dim"),
     (dict(vc=torch.zeros(2, 2, 64, 8, dtype=torch.bfloat16).transpose(2, 3)), "unit head-dim"),
 ])
@@ -120,6 +122,7 @@ PRE = torch.zeros(2, 5, 64, dtype=torch.bfloat16)
     (dict(mask=torch.ones(2, 2, 3, 3)), "mask must be a bool tensor"),
     (dict(mask=torch.ones(2, 3, 3, 3, dtype=torch.bool)), "mask must be a bool tensor"),
     (dict(weights=torch.zeros(2, 2, 4)), "weights must be"),
+    (dict(weights=torch.zeros(2, 1, 3).expand(-1, 2, -1)), "may not repeat memory"),
     (dict(scale=float("nan")), "scale must be finite"),
     (dict(layout="sbhd"), "unsupported layout"),
     (dict(q=_new().requires_grad_()), "no gradient"),
@@ -141,6 +144,7 @@ def test_shared_prefix_refusals(change, msg):
     (dict(weights=torch.zeros(2, 2, 9)), "weights must be"),
     (dict(out=(_new(T=3), _new(T=3), torch.zeros(2, 2, 3))), "at least keep = 4"),
     (dict(out=(_new(T=4), _new(T=5), torch.zeros(2, 2, 4))), "value cache has shape"),
+    (dict(out=(_new(H=1, T=4).expand(-1, 2, -1, -1), _new(T=4), torch.zeros(2, 2, 4))), "may not repeat memory"),
 ])
 def test_evict_refusals(change, msg):
     a = dict(key=_new(T=8), value=_new(T=8), weights=torch.zeros(2, 2, 8), lengths=torch.zeros(2, dtype=torch.int32), keep=4)
