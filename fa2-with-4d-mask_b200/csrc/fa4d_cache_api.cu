@@ -94,9 +94,13 @@ int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, boo
   return best_s;
 }
 
-// Up to this many rows of a KV head the prefix goes through decode_kernel, which reads it once
-// per 16 rows.
-constexpr int64_t kDecodeRows = 32;
+// decode_kernel reads the prefix once per 16 rows, from L2 after the first time, and spares the
+// prefix kernel's launch and start.  It takes the prefix while what it reads of K (V as much
+// again) is at most this many elements.  Both ways, in us, for Hq32 Hk8 D128 behind own caches
+// of 100: 16 rows 15.4 / 15.5 at P 2048 and 40 / 34 at 32768; 64 rows 15.6 / 16.3 at 512 and
+// 19.3 / 18.2 at 2048; Hq64 Hk1 D64, 128 rows: 11.9 / 13.0 at 2048 and 15.7 / 14.3 at 8192;
+// Hq16 Hk4 D256, 128 rows: 18.5 / 21.4 at 512 and 27.8 / 21.1 at 2048.
+constexpr int64_t kDecodePrefix = 1 << 22;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -117,7 +121,7 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   p.R = T * p.G;
   p.tiles = (p.R + 15) / 16;
   const int sms = fa4d::host_sm_count();
-  if (P && rows > kDecodeRows) {
+  if ((rows + 15) / 16 * P * Hk * D > kDecodePrefix) {
     out->split_keys = D != 256 && rows <= 128;
     const int64_t row_tiles = D == 256 || out->split_keys ? (rows + 127) / 128 : (rows + 255) / 256;
     out->splits = prefix_splits(row_tiles, Hk, (P + 127) / 128, rows, D, out->split_keys, sms);

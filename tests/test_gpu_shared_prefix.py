@@ -70,6 +70,17 @@ CASES = [
     (20, 1, 20, 2, 256, 257, 12, torch.float16, "bhsd"),
     (24, 2, 12, 2, 96, 400, 10, torch.bfloat16, "bshd"),
     (70, 1, 4, 2, 128, 1025, 5, torch.float16, "bhsd"),
+    # Prefixes long enough for the tensor-core kernel: at most 128 rows of a KV head and more,
+    # tiles that the prefix's end cuts.
+    (12, 1, 16, 2, 64, 6001, 20, torch.bfloat16, "bshd"),
+    (300, 1, 2, 2, 64, 2047, 7, torch.float16, "bhsd"),
+    (15, 1, 8, 2, 128, 4200, 33, torch.float16, "bshd"),
+    (40, 1, 8, 1, 128, 1793, 40, torch.bfloat16, "bhsd"),
+    (43, 3, 3, 1, 128, 1409, 9, torch.bfloat16, "bshd"),  # 387 rows: the last slot has none
+    (16, 2, 4, 2, 256, 2177, 30, torch.bfloat16, "bshd"),
+    (9, 1, 5, 1, 256, 6100, 8, torch.float16, "bhsd"),
+    (18, 1, 8, 2, 96, 4608, 11, torch.bfloat16, "bhsd"),
+    (100, 2, 1, 1, 96, 3601, 6, torch.float16, "bshd"),
 ]
 
 
@@ -126,7 +137,7 @@ def test_masks_rows_left_empty_and_garbage_in_masked_places(Bm, Hm, P):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 2.0])
-@pytest.mark.parametrize("B,P", [(2, 70), (64, 300)])
+@pytest.mark.parametrize("B,P", [(2, 70), (64, 300), (64, 4500)])
 def test_scales(scale, B, P):
     g = torch.Generator().manual_seed(4)
     args = make(g, B, 1, 4, 1, 64, P, 20, torch.float16, "bshd")
@@ -137,18 +148,19 @@ def test_scales(scale, B, P):
 def test_growing_logits():
     """Keys in order of rising logits, by a factor that moves the maximum at every tile."""
     g = torch.Generator().manual_seed(6)
-    for B in (2, 48):
-        q, pk, pv, k, v = make(g, B, 1, 4, 1, 64, 900, 40, torch.bfloat16, "bhsd")
+    for B, P in ((2, 900), (48, 900), (48, 6000)):
+        q, pk, pv, k, v = make(g, B, 1, 4, 1, 64, P, 40, torch.bfloat16, "bhsd")
         q = torch.ones_like(q)
-        pk = (torch.arange(900, device=DEV)[None, :, None] * 0.005).expand_as(pk).to(torch.bfloat16)
+        pk = (torch.arange(P, device=DEV)[None, :, None] * (4.5 / P)).expand_as(pk).to(torch.bfloat16)
         k = k * 0.1 + 4
         check(q, pk, pv, k, v, torch.full((B,), 40, dtype=torch.int32, device=DEV), "bhsd")
 
 
 @pytest.mark.gpu
-def test_strided_and_unaligned_inputs_give_the_same_bits():
+@pytest.mark.parametrize("P", [150, 33000])
+def test_strided_and_unaligned_inputs_give_the_same_bits(P):
     g = torch.Generator().manual_seed(8)
-    q, pk, pv, k, v = make(g, 3, 2, 4, 2, 64, 150, 50, torch.bfloat16, "bhsd")
+    q, pk, pv, k, v = make(g, 3, 2, 4, 2, 64, P, 50, torch.bfloat16, "bhsd")
     lengths = torch.tensor([50, 20, 2], dtype=torch.int32, device=DEV)
     want = api.shared_prefix_attention(q, pk, pv, k, v, lengths)
 
@@ -166,12 +178,17 @@ def test_strided_and_unaligned_inputs_give_the_same_bits():
     for f in (shifted, padded, seq_first):
         assert torch.equal(api.shared_prefix_attention(f(q), pk, pv, k, v, lengths), want)
         assert torch.equal(api.shared_prefix_attention(q, f(pk), f(pv), f(k), f(v), lengths), want)
+    # One head of the prefix and of the caches for all (a stride of 0).
+    one = [x[..., :1, :, :].expand(x.shape) for x in (pk, pv, k, v)]
+    whole = [x.contiguous() for x in one]
+    assert torch.equal(api.shared_prefix_attention(q, *one, lengths), api.shared_prefix_attention(q, *whole, lengths))
 
 
 @pytest.mark.gpu
-def test_repeats_bit_for_bit_in_a_graph_and_on_another_stream():
+@pytest.mark.parametrize("P", [600, 2000])
+def test_repeats_bit_for_bit_in_a_graph_and_on_another_stream(P):
     g = torch.Generator().manual_seed(9)
-    q, pk, pv, k, v = make(g, 40, 1, 8, 2, 128, 600, 90, torch.bfloat16, "bshd")
+    q, pk, pv, k, v = make(g, 40, 1, 8, 2, 128, P, 90, torch.bfloat16, "bshd")
     lengths = torch.randint(1, 91, (40,), generator=g, dtype=torch.int32).to(DEV)
     w0 = torch.zeros(40, 2, 90, device=DEV)
     call = lambda w: api.shared_prefix_attention(q, pk, pv, k, v, lengths, weights=w, layout="bshd")  # noqa: E731
@@ -198,7 +215,7 @@ def test_repeats_bit_for_bit_in_a_graph_and_on_another_stream():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,P", [(2, 0), (40, 500)])
+@pytest.mark.parametrize("B,P", [(2, 0), (40, 500), (40, 2000)])
 def test_inputs_changed_in_place_between_calls(B, P):
     """Back-to-back calls with no synchronisation, each after kernels that rewrite lengths, query,
     caches and mask in the same memory: every call sees its own inputs."""
