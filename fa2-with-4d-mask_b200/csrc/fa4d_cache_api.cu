@@ -68,7 +68,7 @@ struct Plan {
   int ctas;
   int splits;        // runs of key tiles of the prefix kernel; 0: decode_kernel does the prefix
   bool split_keys;
-  size_t seg_o, seg_ml, logits, pre_o, pre_ml, shares, total;
+  size_t seg_o, seg_ml, logits, lse, pre_o, pre_ml, shares, total;
 };
 
 // Runs per (row tile, KV head) of the prefix kernel: the number that shortens the estimate
@@ -144,7 +144,9 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   out->seg_o = 0;
   out->seg_ml = align256(seg * D * sizeof(float));
   out->logits = out->seg_ml + align256(seg * sizeof(float2));
-  out->pre_o = out->logits + (weights ? align256(static_cast<size_t>(B) * Hk * p.R * p.logits_ld * sizeof(float)) : 0);
+  const size_t own_rows = weights ? static_cast<size_t>(B) * Hk * p.R : 0;
+  out->lse = out->logits + align256(own_rows * p.logits_ld * sizeof(float));
+  out->pre_o = out->lse + align256(own_rows * sizeof(float));
   const size_t pre = static_cast<size_t>(p.splits) * Hk * p.pre_rows;
   out->pre_ml = out->pre_o + align256(pre * D * sizeof(float));
   out->shares = out->pre_ml + align256(pre * sizeof(float2));
@@ -250,6 +252,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   p.seg_o = reinterpret_cast<float*>(ws + plan.seg_o);
   p.seg_ml = reinterpret_cast<float2*>(ws + plan.seg_ml);
   p.logits = a->weights ? reinterpret_cast<float*>(ws + plan.logits) : nullptr;
+  p.lse = reinterpret_cast<float*>(ws + plan.lse);
   p.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
   p.pre_ml = reinterpret_cast<float2*>(ws + plan.pre_ml);
   p.shares = reinterpret_cast<fa4d::Shares*>(ws + plan.shares);

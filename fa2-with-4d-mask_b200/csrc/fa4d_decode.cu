@@ -515,6 +515,9 @@ constexpr int kJoinAhead = 8;                 // partial rows of a warp in fligh
 constexpr int kWeighRows = 4;                 // rows of weights taken together
 constexpr int kWeighKeys = 4 * kJoinThreads;  // own keys of a block of weigh_kernel at a time
 constexpr int kWeighTimes = 4;
+// Rows whose sums weigh_kernel works out itself, beside the join (24 rows: 40.1 us so, 41.6 behind
+// it; 64 rows: 56 and 49).
+constexpr int kWeighOwnRows = 32;
 
 // The partial results of the rows of (request b, KV head hk).
 struct Joined {
@@ -648,6 +651,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   if (r >= p.R) return;
   // A row without a key: 0.  (A NaN maximum or sum stays one.)
   const float inv = m_all == kNegInf ? 0.f : 1.f / l_all;
+  if (p.weights && lane == 0)
+    p.lse[(static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r] = m_all == kNegInf ? INFINITY : m_all + log2f(l_all);
   const int t = r / p.G, h = at.hk * p.G + r % p.G;
   uint16_t* dst = static_cast<uint16_t*>(p.o) + at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
   if constexpr (D == 96) {
@@ -668,6 +673,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // it two blocks an SM (33 us in one kernel at B128 Hk8, 4096 slots; 95 MB).  It starts when
 // every block of join_kernel has found the partial results complete, so they are complete here,
 // works beside it, and its last block waits so that this kernel is over only when that one is.
+// With more than kWeighOwnRows rows, a warp's turns at their sums take longer than waiting for
+// join_kernel, which has them all.
 __global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kRows = 64;
   __shared__ float lse[kRows];
@@ -676,7 +683,11 @@ __global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_con
   const int key0 = blockIdx.x * kWeighTimes * kWeighKeys + 4 * threadIdx.x;
   float* weights = p.weights + at.b * p.weights_stride[0] + at.hk * p.weights_stride[1];
   if (blockIdx.x * kWeighTimes * kWeighKeys < at.keys) {
-    at.load_shares();
+    const bool from_join = p.R > kWeighOwnRows;
+    if (from_join)
+      pdl_wait();
+    else
+      at.load_shares();
     for (int r0 = 0; r0 < p.R; r0 += kRows) {
       const int rows = min(kRows, p.R - r0);
       const float* logits = p.logits + ((static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r0) * p.logits_ld;
@@ -687,7 +698,9 @@ __global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_con
           x[u] = __ldcg(reinterpret_cast<const float4*>(logits + static_cast<int64_t>(min(r + u, rows - 1)) * p.logits_ld + j));
       };
       __syncthreads();
-      for (int r = wid; r < rows; r += kJoinWarps) {
+      if (from_join && threadIdx.x < rows)
+        lse[threadIdx.x] = p.lse[(static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r0 + threadIdx.x];
+      for (int r = wid; !from_join && r < rows; r += kJoinWarps) {
         // Maximum and sum over all parts of the row.
         const Parts px = at.prefix(r0 + r), py = at.own(r0 + r);
         float m = kNegInf, l = 0.f;

@@ -61,6 +61,7 @@ struct DecodeParams {
   float* logits;         // [B, Hk, R, logits_ld] of the own keys, log2 units; null without weights
   int32_t logits_ld;
   int32_t weights_vec;   // rows of weights start on 16-byte boundaries
+  float* lse;            // [B, Hk, R]: log2 of a row's sum, written by the join with weights; +inf without a key
   // Partial results of the prefix kernel: [Hk][splits][pre_rows] rows, splits 0: none.
   int32_t splits, pre_rows;
   float* pre_o;
