@@ -269,22 +269,45 @@ const char* kLengths = "lengths must be a contiguous int32 tensor";
 
 // ------------------------------------------------------------------ entry points
 
-// make_table(turn, axis, head_dim, rotary_dim, pairing, axes) -> capsule
+// make_table(base, sections, head_dim, rotary_dim, pairing) -> capsule.  Pair i turns by
+// base^(-2 i / rotary_dim) radians a position: as turns, modulo one, in units of 2^-64.
 PyObject* make_table(PyObject* const* args) {
   auto table = c10::make_intrusive<Table>();
-  memset(&table->t, 0, sizeof(table->t));
-  const Py_ssize_t n = PyTuple_Size(args[0]);
-  for (Py_ssize_t i = 0; i < n && i < FA4D_ROTARY_MAX_PAIRS; ++i) {
-    table->t.turn[i] = PyLong_AsUnsignedLongLongMask(PyTuple_GET_ITEM(args[0], i));
-    table->t.axis[i] = static_cast<uint8_t>(int_arg(PyTuple_GET_ITEM(args[1], i), "axis"));
+  fa4d_rotary_table& t = table->t;
+  memset(&t, 0, sizeof(t));
+  const double base = PyFloat_AsDouble(args[0]);
+  t.D = small(int_arg(args[2], "head_dim"), "head_dim");
+  t.rotary_dim = small(int_arg(args[3], "rotary_dim"), "rotary_dim");
+  t.pairing = small(int_arg(args[4], "pairing"), "pairing");
+  t.axes = small(PyTuple_Size(args[1]), "sections");
+  int i = 0;
+  for (int a = 0; a < t.axes; ++a) {
+    const int64_t n = int_arg(PyTuple_GET_ITEM(args[1], a), "sections");
+    for (int64_t j = 0; j < n && i < FA4D_ROTARY_MAX_PAIRS; ++j, ++i) {
+      const long double turns = std::pow(static_cast<long double>(base), -2.0L * i / t.rotary_dim) / 6.283185307179586476925287L;
+      t.turn[i] = static_cast<uint64_t>(std::ldexp(turns - std::floor(turns), 64));
+      t.axis[i] = static_cast<uint8_t>(a);
+    }
   }
-  table->t.D = small(int_arg(args[2], "head_dim"), "head_dim");
-  table->t.rotary_dim = small(int_arg(args[3], "rotary_dim"), "rotary_dim");
-  table->t.pairing = small(int_arg(args[4], "pairing"), "pairing");
-  table->t.axes = small(int_arg(args[5], "axes"), "axes");
   return PyCapsule_New(table.release(), kTableName, [](PyObject* o) {
     c10::intrusive_ptr<Table>::reclaim(static_cast<Table*>(PyCapsule_GetPointer(o, kTableName)));
   });
+}
+
+// table_turns(table) -> (turns per position of each pair in 2^-64 turns, axis of each pair)
+PyObject* table_turns(PyObject* const* args) {
+  const fa4d_rotary_table& t = table_arg(args[0])->t;
+  const int n = t.rotary_dim / 2;
+  PyObject* turns = PyTuple_New(n);
+  PyObject* axes = PyTuple_New(n);
+  for (int i = 0; i < n; ++i) {
+    PyTuple_SET_ITEM(turns, i, PyLong_FromUnsignedLongLong(t.turn[i]));
+    PyTuple_SET_ITEM(axes, i, PyLong_FromLong(t.axis[i]));
+  }
+  PyObject* out = PyTuple_Pack(2, turns, axes);
+  Py_DECREF(turns);
+  Py_DECREF(axes);
+  return out;
 }
 
 // rotary(table, query, key, positions, layout) -> (query, key)
@@ -569,7 +592,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define FA4D_ENTRY(name, n) \
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr }
-PyMethodDef kMethods[] = {FA4D_ENTRY(make_table, 6),      FA4D_ENTRY(rotary, 5),
+PyMethodDef kMethods[] = {FA4D_ENTRY(make_table, 5),      FA4D_ENTRY(table_turns, 1),
+                          FA4D_ENTRY(rotary, 5),
                           FA4D_ENTRY(rotary_append, 10),  FA4D_ENTRY(shared_prefix_attention, 11),
                           FA4D_ENTRY(evict_by_weight, 9), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fa4d_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

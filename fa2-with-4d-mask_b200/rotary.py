@@ -42,7 +42,7 @@ class MultiAxisRotary:
         if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > head_dim:
             raise ValueError(f"rotary_dim must be even and at most head_dim, got {rotary_dim}")
         sections = tuple(int(n) for n in sections)
-        if not sections or min(sections) < 0 or sum(sections) != rotary_dim // 2:
+        if not sections or len(sections) > 255 or min(sections) < 0 or sum(sections) != rotary_dim // 2:
             raise ValueError(f"sections must add up to rotary_dim / 2 = {rotary_dim // 2}, got {sections}")
         if pairing not in _PAIRINGS:
             raise ValueError(f"unsupported pairing: {pairing}")
@@ -50,17 +50,8 @@ class MultiAxisRotary:
             raise ValueError(f"base must be positive, got {base}")
         self.head_dim, self.sections, self.base = head_dim, sections, float(base)
         self.rotary_dim, self.pairing = rotary_dim, pairing
-        axis = tuple(a for a, n in enumerate(sections) for _ in range(n))
         self._host = _lib.host()
-        self._table = self._host.make_table(self._turns(), axis, head_dim, rotary_dim, _PAIRINGS[pairing], len(sections))
-
-    def _turns(self) -> tuple:
-        """Turns per position of each pair, modulo a turn, in 2^-64 turns."""
-        out = []
-        for i in range(self.rotary_dim // 2):
-            turns = self.base ** (-2.0 * i / self.rotary_dim) / (2.0 * math.pi)
-            out.append(int(math.fmod(turns, 1.0) * 2.0 ** 64) & (2 ** 64 - 1))
-        return tuple(out)
+        self._table = self._host.make_table(self.base, sections, head_dim, rotary_dim, _PAIRINGS[pairing])
 
     def __call__(self, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, *,
                  layout: Layout = "bhsd") -> tuple:

@@ -1,6 +1,7 @@
 /*
  * fa4d.h — C ABI of the B200 (sm_100a) FlashAttention-2 forward/backward with an
- * optional 4D bool mask and fp32 additive score.
+ * optional 4D bool mask and fp32 additive score, and of the operators around it (rotary
+ * positions, attention over a shared prefix and caches, eviction).
  *
  * Every entry point takes plain device pointers, element strides and sizes; no
  * framework types cross this boundary.  The caller owns every buffer (inputs,

@@ -94,7 +94,7 @@ def test_far_positions_lose_nothing():
     two_pi_scaled = 6283185307179586476925286766559005768394338798750211641949889184615632812572417997256069650684234135
     pos = torch.tensor([[[2 ** 40 + 12345, 2 ** 40 - 1, -(2 ** 39) - 7]]])
     exact = torch.tensor([((int(p) * 10 ** 99) % two_pi_scaled) / 10 ** 99 for p in pos.flatten()], dtype=torch.float64)
-    # turn holds 1 / (2 pi) to 2^-53 of itself: 2^40 positions bring that to 2^-15 turns.
+    # turn is exact to 2^-64 turns: 2^41 positions bring that to 2^-23; the rest is fp16's rounding.
     x = torch.zeros(1, 1, 3, 2, dtype=torch.float16)
     x[..., 0] = 1.0
     y, _ = api.MultiAxisRotary(2, (1,), base=1.0)(x.to(DEV), x.to(DEV), pos.to(DEV))

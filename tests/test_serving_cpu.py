@@ -16,8 +16,8 @@ from fa2_with_4d_mask_b200 import _lib
 @pytest.mark.parametrize("base,dim", [(1e4, 128), (5e5, 96), (0.5, 20)])
 def test_rotary_table(base, dim):
     rope = api.MultiAxisRotary(dim, (dim // 2 - 2, 0, 2), base=base)
-    turns = rope._turns()
-    assert len(turns) == dim // 2
+    turns, axes = _lib.host().table_turns(rope._table)
+    assert len(turns) == dim // 2 and axes == (0,) * (dim // 2 - 2) + (2, 2)
     for i in range(dim // 2):
         want = base ** (-2.0 * i / dim) / (2 * math.pi) % 1.0
         assert abs((turns[i] / 2.0 ** 64 - want + 0.5) % 1.0 - 0.5) < 2.0 ** -50
