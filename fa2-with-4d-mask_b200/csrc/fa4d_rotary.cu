@@ -7,7 +7,7 @@
 // 32-bit product of position and frequency is off by 4e-3 rad at position 65536), and the
 // fraction's top 32 bits go to sincospif, whose argument then needs no range reduction.
 //
-// Both are bound by memory: each element is read once and written once.
+// Bound by memory: each element is read once and written once.
 #include "fa4d.h"
 #include "fa4d_kernels.h"
 #include "fa4d_launch.cuh"
@@ -104,6 +104,9 @@ struct Chunk {
 
 // One thread: one chunk of a token, for a range of the q and k heads, so the angles are
 // computed once for kHeads heads and more; the loads of kHeads heads are in flight together.
+// Measured, one direction: B4 T8192 Hq32 Hk8 D128 106 us (6.3 TB/s, 98% of the measured copy
+// rate), B1 31.7 us (5.3 TB/s), B2 T16385 Hq16 Hk8 D256 139 us (5.8 TB/s).  Two heads at a time
+// took 36 us at B1, eight 35; 256 threads a block 32.5.
 constexpr int kHeads = 4;
 
 template <bool kBF16, bool kAdj, int VEC>
@@ -146,7 +149,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 }
 
 // One thread: one chunk of one head (q, k or v) of a new token.  A decode step has few
-// tokens, so everything is spread over threads and the angles are computed per head.
+// tokens, so everything is spread over threads and the angles are computed per head; latency
+// bounds it (one token 3.9 us, 160 tokens 5.2 us, back to back).
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_constant__ fa4d_rotary_append_args a,
                                                                  int chunks, int* status) {
