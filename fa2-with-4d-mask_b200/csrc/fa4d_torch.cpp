@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
+#include <cstring>
 #include <string>
 
 #include "fa4d.h"
@@ -98,17 +99,17 @@ Tensor tensor_arg(PyObject* o, const char* name, int dim) {
   if (x.dim() != dim) refuse(cat(name, " must be a rank-", dim, " tensor"));
   return x;
 }
-Tensor any_tensor(PyObject* o, const std::string& otherwise) {
+Tensor any_tensor(PyObject* o, const char* otherwise) {
   if (!THPVariable_Check(o)) refuse(otherwise);
   return THPVariable_Unpack(o);
 }
-Tensor optional_arg(PyObject* o, const std::string& otherwise) { return o == Py_None ? Tensor() : any_tensor(o, otherwise); }
+Tensor optional_arg(PyObject* o, const char* otherwise) { return o == Py_None ? Tensor() : any_tensor(o, otherwise); }
 
 Layout layout_arg(PyObject* o) {
   const char* s = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : "";
-  if (std::string(s) == "bhsd") return {true};
-  if (std::string(s) == "bshd") return {false};
-  refuse(cat("unsupported layout: ", s));
+  if (s && !strcmp(s, "bhsd")) return {true};
+  if (s && !strcmp(s, "bshd")) return {false};
+  refuse(cat("unsupported layout: ", s ? s : ""));
 }
 int64_t int_arg(PyObject* o, const char* name) {
   const int64_t v = PyLong_AsLongLong(o);
@@ -156,9 +157,9 @@ void check_tokens(const Tensor& q, const Tensor& k, const Tensor& v, Layout l, i
 
 // Integer positions [axes, B or 1, T], as int32 or int64.
 Tensor check_positions(PyObject* o, const Table& table, int64_t B, int64_t T, const Tensor& like) {
-  const std::string shape = cat("positions must be an integer tensor of shape [", table.t.axes, ", ", B, " or 1, ", T, "]");
-  Tensor p = any_tensor(o, shape);
-  if (p.dim() != 3 || p.size(0) != table.t.axes || (p.size(1) != 1 && p.size(1) != B) || p.size(2) != T) refuse(shape);
+  Tensor p = any_tensor(o, "positions must be an integer tensor");
+  if (p.dim() != 3 || p.size(0) != table.t.axes || (p.size(1) != 1 && p.size(1) != B) || p.size(2) != T)
+    refuse(cat("positions must be an integer tensor of shape [", table.t.axes, ", ", B, " or 1, ", T, "]"));
   if (!at::isIntegralType(p.scalar_type(), false)) refuse("positions must be an integer tensor");
   if (p.device() != like.device()) refuse(cat("positions must be on ", like.device(), ", got ", p.device()));
   return p.scalar_type() == at::kInt || p.scalar_type() == at::kLong ? p : p.to(at::kLong);
@@ -398,11 +399,10 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   int64_t P = 0;
   const int seq = l.bhsd ? 1 : 0;
   if (args[1] != Py_None) {
-    const std::string shape = l.bhsd ? cat("[", Hk, ", P, ", D, "]") : cat("[P, ", Hk, ", ", D, "]");
     auto one = [&](PyObject* o, const char* name) {
-      const Tensor x = any_tensor(o, cat(name, " must have shape ", shape));
-      if (x.dim() != 3 || x.size(1 - seq) != Hk || x.size(2) != D || (pk.defined() && x.size(seq) != pk.size(seq)))
-        refuse(cat(name, " must have shape ", shape));
+      const Tensor x = tensor_arg(o, name, 3);
+      if (x.size(1 - seq) != Hk || x.size(2) != D || (pk.defined() && x.size(seq) != pk.size(seq)))
+        refuse(cat(name, " must have shape ", l.bhsd ? cat("[", Hk, ", P, ", D, "]") : cat("[P, ", Hk, ", ", D, "]")));
       if (x.scalar_type() != q.scalar_type() || x.device() != q.device())
         refuse(cat(name, " must be ", name_of(q.scalar_type()), " on ", q.device()));
       return x;
@@ -413,11 +413,10 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   }
   Tensor mask;
   if (args[6] != Py_None) {
-    const std::string shape = cat("mask must be a bool tensor of shape [", B, " or 1, ", Hq, " or 1, ", T, ", ", C, "]");
-    mask = any_tensor(args[6], shape);
+    mask = any_tensor(args[6], "mask must be a bool tensor");
     if (mask.dim() != 4 || mask.scalar_type() != at::kBool || (mask.size(0) != 1 && mask.size(0) != B) ||
         (mask.size(1) != 1 && mask.size(1) != Hq) || mask.size(2) != T || mask.size(3) != C)
-      refuse(shape);
+      refuse(cat("mask must be a bool tensor of shape [", B, " or 1, ", Hq, " or 1, ", T, ", ", C, "]"));
     if (mask.device() != q.device()) refuse(cat("mask must be on ", q.device(), ", got ", mask.device()));
   }
   double scale = 1.0 / std::sqrt(static_cast<double>(D));
@@ -513,12 +512,12 @@ PyObject* evict_by_weight(PyObject* const* args) {
   no_gradient("evict_by_weight", {&k, &v, &weights});
   Tensor ko, vo, wo;
   if (args[7] != Py_None) {
-    const std::string what = cat("out must be (key, value, weights) with at least keep = ", keep, " slots");
+    const char* what = "out must be (key, value, weights)";
     if (!PyTuple_Check(args[7]) || PyTuple_GET_SIZE(args[7]) != 3) refuse(what);
     ko = tensor_arg(PyTuple_GET_ITEM(args[7], 0), "key cache", 4);
     vo = tensor_arg(PyTuple_GET_ITEM(args[7], 1), "value cache", 4);
     wo = any_tensor(PyTuple_GET_ITEM(args[7], 2), what);
-    if (check_cache(ko, vo, lengths, wo, l, B, Hk, D, k) < keep) refuse(what);
+    if (check_cache(ko, vo, lengths, wo, l, B, Hk, D, k) < keep) refuse(cat(what, " with at least keep = ", keep, " slots"));
     if (ko.stride(3) != 1 || vo.stride(3) != 1) refuse("out is written in place and needs unit head-dim stride");
     if (repeats(ko) || repeats(vo) || repeats(wo)) refuse("out is written in place and may not repeat memory");
     for (const Tensor* x : std::initializer_list<const Tensor*>{&ko, &vo, &wo})
