@@ -75,20 +75,22 @@ __device__ __forceinline__ uint64_t position_at(const void* positions, int bits,
                     : static_cast<uint64_t>(static_cast<int64_t>(__ldg(static_cast<const int*>(positions) + i)));
 }
 
-// Where chunk c of a head lies: its two runs, and the cosines and sines of its pairs for
-// token (b, t); chunks past the pairs cover the elements that are copied.
+// Where chunk c of a head lies: its two runs, and (after turn_to) the cosines and sines of its
+// pairs for token (b, t); chunks past the pairs cover the elements that are copied.
 template <int VEC, bool kAdj>
 struct Chunk {
   int at0, at1;
   bool copied;
   float cs[VEC], sn[VEC];
 
-  __device__ __forceinline__ Chunk(const fa4d_rotary_table& tab, const void* positions, int bits, const int64_t (&ps)[3],
-                                   int64_t b, int64_t t, int c, bool inverse) {
+  __device__ __forceinline__ Chunk(const fa4d_rotary_table& tab, int c) {
     const int pairs = tab.rotary_dim / 2, turned = pairs / VEC;
     copied = c >= turned;
     at0 = copied ? tab.rotary_dim + (c - turned) * 2 * VEC : (kAdj ? 2 * c * VEC : c * VEC);
     at1 = (kAdj || copied) ? at0 + VEC : pairs + c * VEC;
+  }
+  __device__ __forceinline__ void turn_to(const fa4d_rotary_table& tab, const void* positions, int bits,
+                                          const int64_t (&ps)[3], int64_t b, int64_t t, int c, bool inverse) {
     if (copied) return;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -104,9 +106,9 @@ struct Chunk {
 
 // One thread: one chunk of a token, for a range of the q and k heads, so the angles are
 // computed once for kHeads heads and more; the loads of kHeads heads are in flight together.
-// Measured, one direction: B4 T8192 Hq32 Hk8 D128 106 us (6.3 TB/s, 98% of the measured copy
-// rate), B1 31.7 us (5.3 TB/s), B2 T16385 Hq16 Hk8 D256 139 us (5.8 TB/s).  Two heads at a time
-// took 36 us at B1, eight 35; 256 threads a block 32.5.
+// Measured, one direction: B4 T8192 Hq32 Hk8 D128 104.6 us (6.4 TB/s, the measured copy rate),
+// B1 31.2 us (5.4 TB/s), B2 T16385 Hq16 Hk8 D256 129 us (6.2 TB/s; 139 with the angles worked out
+// before the first loads).  Two heads at a time took 135 us there, eight the same as four.
 constexpr int kHeads = 4;
 
 template <bool kBF16, bool kAdj, int VEC>
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   if (n >= static_cast<int64_t>(a.B) * a.T) return;
   const int c = static_cast<int>(id - n * chunks);
   const int64_t b = n / a.T, t = n - b * a.T;
-  const Chunk<VEC, kAdj> ch(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, c, a.inverse != 0);
+  Chunk<VEC, kAdj> ch(a.table, c);
 
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1];
   const uint16_t* k = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1];
@@ -136,6 +138,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       x[u] = Run<VEC>::load(src + ch.at0);
       y[u] = Run<VEC>::load(src + ch.at1);
     }
+    // The angles, while the first heads are on their way.
+    if (h0 == first) ch.turn_to(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, c, a.inverse != 0);
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       const int h = h0 + u;
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_co
     if (h == a.Hq && c == 0) atomicOr(status, FA4D_DEV_CACHE_FULL);
     return;
   }
-  const Chunk<VEC, kAdj> ch(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, c, false);
+  Chunk<VEC, kAdj> ch(a.table, c);
   const uint16_t* src;
   uint16_t* dst;
   if (h < a.Hq) {
@@ -192,7 +196,10 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_co
     if (a.weights && c == 0) a.weights[b * a.weights_stride[0] + hk * a.weights_stride[1] + slot] = 0.f;
   }
   typename Run<VEC>::T x = Run<VEC>::load(src + ch.at0), y = Run<VEC>::load(src + ch.at1);
-  if (!ch.copied && h < a.Hq + a.Hk) turn<kBF16, kAdj>(x, y, ch.cs, ch.sn);
+  if (!ch.copied && h < a.Hq + a.Hk) {
+    ch.turn_to(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, c, false);
+    turn<kBF16, kAdj>(x, y, ch.cs, ch.sn);
+  }
   Run<VEC>::store(dst + ch.at0, x);
   Run<VEC>::store(dst + ch.at1, y);
 }
