@@ -514,7 +514,10 @@ __device__ __forceinline__ void load_row(const float* row, int lane, float (&v)[
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinAhead = 8;                 // partial rows of a warp in flight
+// Partial rows of a warp in flight (16 at head dim 64: Hq64 Hk1 B48 35.3 -> 33.9 us; at 256 the
+// registers cost more: draft trees of B16 35.4 -> 36.7).
+template <int D>
+constexpr int kJoinAhead = D == 64 ? 16 : 8;
 constexpr int kWeighRows = 4;                 // rows of weights taken together
 constexpr int kWeighKeys = 4 * kJoinThreads;  // own keys of a block of weigh_kernel at a time
 constexpr int kWeighTimes = 4;
@@ -609,17 +612,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       for (int e = 0; e < D / 32; ++e) acc[e] *= old;
     };
     const int batch = min(32, n - i0);
-    for (int j0 = 0; j0 < batch; j0 += kJoinAhead) {
-      float v[kJoinAhead][D / 32];
+    for (int j0 = 0; j0 < batch; j0 += kJoinAhead<D>) {
+      float v[kJoinAhead<D>][D / 32];
 #pragma unroll
-      for (int u = 0; u < kJoinAhead; ++u) {
+      for (int u = 0; u < kJoinAhead<D>; ++u) {
         const int j = min(i0 + j0 + u, n - 1);
         const float* row = j < x.n ? x.o + (x.first + j * x.step) * D : y.o + (y.first + (j - x.n) * y.step) * D;
         load_row<D>(row, lane, v[u]);
       }
       if (j0 == 0) settle();
 #pragma unroll
-      for (int u = 0; u < kJoinAhead; ++u) {
+      for (int u = 0; u < kJoinAhead<D>; ++u) {
         // A part without a key (maximum -inf) may not even have its row written.
         const float fu = __shfl_sync(0xffffffffu, f, j0 + u), mu = __shfl_sync(0xffffffffu, ml.x, j0 + u);
         if (j0 + u < batch && mu != kNegInf) {
