@@ -46,6 +46,12 @@ __device__ __forceinline__ void st_sector(float* dst, const uint32_t* v) {
                : "memory");
 }
 
+// 16 bytes, the first `bytes` of them from src and the others zero.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 template <int D, bool kSplitKeys>
 struct PrefixLayout {
   static constexpr int kTile = 128 * D * 2;
@@ -116,25 +122,27 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   } else if (warp == 2) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
-  } else if (warp >= 4 && (warp - 4) / 4 < L::kQTiles) {
-    // Q rows into the swizzled tile, D / 8 lanes a row; lane i knows where row i lies.
+  } else if (warp >= 4) {
+    // Q rows into the swizzled tiles, D / 8 lanes a row, divided over the eight warps; lane i
+    // knows where row i lies.  All copies are in flight at once and take no registers (loads,
+    // eight a thread in flight: 1.2 to 2.9 us more a call at D 128 and 256).
     pdl_wait();
-    const int t = (warp - 4) / 4, first = (warp & 3) * 32, row = row0 + 128 * t + first + lane;
+    constexpr int kRowsOfWarp = 16 * L::kQTiles, kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
+    const int first = (warp - 4) * kRowsOfWarp, row = row0 + first + (lane & (kRowsOfWarp - 1));
     const int token = row / p.G, h = hk * p.G + row % p.G;
     const int b = token / p.T, tt = token - b * p.T;
     const int64_t mine = b * p.q_stride[0] + tt * p.q_stride[1] + h * p.q_stride[2];
-    constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
     const int c = lane % kLanes;
-    uint8_t* dst = smem + L::kQ + t * L::kTile + (c >> 3) * 16384;
+    uint8_t* dst = smem + L::kQ + (first >> 7) * L::kTile + (c >> 3) * 16384;
 #pragma unroll 8
-    for (int i = 0; i < 32; i += kRowsAtOnce) {
+    for (int i = 0; i < kRowsOfWarp; i += kRowsAtOnce) {
       const int r = i + lane / kLanes;
       const int64_t at = __shfl_sync(0xffffffffu, mine, r);
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row0 + 128 * t + first + r < p.rows && 8 * c < p.d_in)
-        v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at) + c);
-      *reinterpret_cast<uint4*>(dst + (first + r) * 128 + (((c ^ r) & 7) << 4)) = v;
+      const bool some = row0 + first + r < p.rows && 8 * c < p.d_in;
+      cp_async16(dst + ((first & 127) + r) * 128 + (((c ^ r) & 7) << 4), static_cast<const uint16_t*>(p.q) + (some ? at + 8 * c : 0),
+                 some ? 16 : 0);
     }
+    cp_async_wait_all();
     fence_async_smem();
   }
   tc_fence_before();
@@ -298,13 +306,30 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   } else {
     regs_inc<kRegsSoftmax>();
     const int t = (warp - 4) >> 2;
+    const int quad = (warp & 3) * 32;
+    const int row = row0 + (L::kQTiles == 2 ? 128 * t : 0) + quad + lane;
+    const bool valid = row < p.rows;
+    const bool warp_valid = row - lane < p.rows;  // some lane has a row
+    const uint32_t lane_base = static_cast<uint32_t>(quad) << 16;
+    // Columns of the output row, [c0, c0 + kCols): at D = 256 both warpgroups write the slot's.
+    constexpr int kCols = kDoubleS ? D / 2 : D;
+    auto write_row = [&](uint32_t tO, int64_t out, int c0) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&o_full[kDoubleS ? 0 : t], 0, abort_flag))) return;
+      tc_fence_after();
+      if (!warp_valid) return;
+#pragma unroll
+      for (int c = 0; c < kCols; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tO + c0 + c, o);
+        tmem_wait_ld();
+        if (valid && c0 + c < p.d_in) {
+          float* dst = p.o + out * p.d_in + c0 + c;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) st_sector(dst + 8 * v, &o[8 * v]);
+        }
+      }
+    };
     if (t < L::kSlots && (t == 0 || two || kSplitKeys)) {
-      const int quad = (warp & 3) * 32, at = quad + lane;
-      const int row = row0 + (kSplitKeys ? 0 : 128 * t) + at;
-      const bool valid = row < p.rows;
-      const bool warp_valid = row - lane < p.rows;  // some lane has a row
-      const uint32_t lane_base = static_cast<uint32_t>(quad) << 16;
-
       const int count = kSplitKeys ? (n - t + 1) / 2 : n;
       const uint32_t tO = tmem + lane_base + 256 + (kDoubleS ? 0 : D * t);
       float m_run = kNegInf, l_run = 0.f;
@@ -395,23 +420,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       const int part = kSplitKeys ? 2 * blockIdx.z + t : blockIdx.z;
       const int64_t out = (static_cast<int64_t>(hk) * p.parts + part) * p.rows + row;
       if (valid) p.ml[out] = make_float2(m_run, l_run);
-      if (count > 0 && ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[kDoubleS ? 0 : t], 0, abort_flag));
-        tc_fence_after();
-        if (warp_valid) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + 32 * c, o);
-            tmem_wait_ld();
-            if (valid && 32 * c < p.d_in) {
-              float* dst = p.o + out * p.d_in + 32 * c;
-#pragma unroll
-              for (int v = 0; v < 4; ++v) st_sector(dst + 8 * v, &o[8 * v]);
-            }
-          }
-        }
-      }
+      if (count > 0 && ok) write_row(tO, out, 0);
+      tc_fence_before();
+    } else if (kDoubleS) {
+      const int64_t out = (static_cast<int64_t>(hk) * p.parts + blockIdx.z) * p.rows + row;
+      write_row(tmem + lane_base + 256, out, kCols);
       tc_fence_before();
     }
   }
