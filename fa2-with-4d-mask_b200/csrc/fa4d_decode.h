@@ -96,12 +96,14 @@ constexpr int kItemUnits = 2;
 // by side, where the slots split the keys) and a CTA's fill, drain and output rows; a unit of a
 // decode_kernel warp beside the SM's others, and the time until its first unit.
 template <int D>
-constexpr float kTileMicros = D == 256 ? 1.4f : D == 64 ? 1.9f : 2.1f;
-constexpr float kRunMicros = 6.0f;
+constexpr float kTileMicros = D == 256 ? 1.75f : D == 64 ? 1.9f : 2.1f;
+constexpr float kRunMicros = 7.0f;
 template <int D>
-constexpr float kUnitMicros = D == 256 ? 1.6f : D == 64 ? 0.6f : 1.0f;
+constexpr float kUnitMicros = D == 256 ? 1.6f : D == 64 ? 0.8f : 1.2f;
 constexpr float kDecodeMicros = 3.5f;
 constexpr float kReadRate = 6.0f;  // MB per microsecond that decode_kernel reads, of the GPU
+constexpr float kBesideRate = 0.9f;   // of kReadRate, beside the prefix kernel
+constexpr float kPrefixWeight = 0.2f;  // see choose_runs
 template <int D>
 constexpr int kDecodeCtas = D == 256 ? 1 : 2;  // of an SM
 
@@ -139,20 +141,28 @@ __device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, in
 // (shared memory and registers), and the decode kernel, launched right behind, streams the own
 // keys (`units` of them) on the SMs that are left: fewer, longer runs let the tensor work and
 // the memory work go on side by side.  Only the lengths, on the device, tell how much that is,
-// so it is worked out there by one warp (lane l for l + 1, l + 33, ... runs).
+// so it is worked out there by one warp (lane l for l + 1, l + 33, ... runs).  Where the own
+// keys take longer than the prefix whatever its runs, the estimates of many divisions are
+// equal; what they leave out (the start of the CTAs that come late) goes with the prefix
+// kernel's time, a part of which is therefore added.  Over 18 calls (8 to 256 requests, 1024 to
+// 30000 prefix keys, head dims 64 to 256), each timed with every number of runs, the choice is
+// 0.7% above the best on average and at most 2.6% (5.3% and 33% without that part, with
+// estimates from the kernels alone).
 template <int D>
 __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t units, int lane) {
   const float all = static_cast<float>(units);
   const float sm_rate = kDecodeCtas<D> * kDecodeWarps / kUnitMicros<D>;
   // Row tiles of a request read the same keys, mostly from L2.
   const float gpu_rate = fminf(w.sms * sm_rate, kReadRate * 1e6f / (kUnitKeys * 4 * D) * w.row_tiles);
-  RunChoice best{1, 0.f, INFINITY, gpu_rate};
+  RunChoice best{1, 0.f, 0.f, gpu_rate};
+  float best_cost = INFINITY;
   for (int s = lane + 1; s <= w.most; s += 32) {
     const int ctas = w.items * s, run = (w.tiles + s - 1) / s;
     const float mine = ((ctas + w.sms - 1) / w.sms) * (((run + w.step - 1) / w.step) * kTileMicros<D> + kRunMicros);
-    const float beside = fminf(gpu_rate, sm_rate * max(w.sms - ctas, 0)) * fmaxf(mine - kDecodeMicros, 0.f);
+    const float beside = fminf(kBesideRate * gpu_rate, sm_rate * max(w.sms - ctas, 0)) * fmaxf(mine - kDecodeMicros, 0.f);
     const float total = mine + (all > beside ? kDecodeMicros + (all - beside) / gpu_rate : 0.f);
-    if (total < best.total_us) {
+    if (total + kPrefixWeight * mine < best_cost) {
+      best_cost = total + kPrefixWeight * mine;
       best.runs = s;
       best.prefix_us = mine;
       best.total_us = total;
@@ -161,9 +171,11 @@ __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t un
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const int s = __shfl_xor_sync(0xffffffffu, best.runs, o);
+    const float cost = __shfl_xor_sync(0xffffffffu, best_cost, o);
     const float mine = __shfl_xor_sync(0xffffffffu, best.prefix_us, o);
     const float total = __shfl_xor_sync(0xffffffffu, best.total_us, o);
-    if (total < best.total_us || (total == best.total_us && s > best.runs)) {
+    if (cost < best_cost || (cost == best_cost && s < best.runs)) {
+      best_cost = cost;
       best.runs = s;
       best.prefix_us = mine;
       best.total_us = total;
