@@ -135,11 +135,18 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   p.prefix_units = (P + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys;
   p.seg_rows = static_cast<int>(std::min<int64_t>(16, p.prefix_tiles ? rows : p.R));
   out->ctas = sms * (D == 256 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
-  p.warps = out->ctas * fa4d::kDecodeWarps;
   p.min_units = 2;
-  p.logits_ld = (C + 3) / 4 * 4;
   const int64_t items = static_cast<int64_t>(p.prefix_tiles) * Hk + static_cast<int64_t>(B) * Hk * p.tiles;
   if (items > (1 << 30)) return fail(FA4D_ERR_UNSUPPORTED, "too many row tiles");
+  if (!out->splits) {
+    // No more CTAs than full caches could occupy.
+    const int64_t line = static_cast<int64_t>(p.prefix_tiles) * Hk * (p.prefix_units + fa4d::kItemUnits) +
+                         static_cast<int64_t>(B) * Hk * p.tiles * ((C + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys + fa4d::kItemUnits);
+    const int64_t each = p.min_units * fa4d::kDecodeWarps;
+    out->ctas = static_cast<int>(std::min<int64_t>(out->ctas, (line + each - 1) / each));
+  }
+  p.warps = out->ctas * fa4d::kDecodeWarps;
+  p.logits_ld = (C + 3) / 4 * 4;
   const size_t seg = (static_cast<size_t>(items) + p.warps) * p.seg_rows;
   out->seg_o = 0;
   out->seg_ml = align256(seg * D * sizeof(float));
