@@ -22,8 +22,14 @@ struct DecodeShape {
   static constexpr int kTile = kBoxes * kBox;        // K or V of a unit
   static constexpr int kStage = 2 * kTile;
   static constexpr int kStages = D == 64 ? 6 : 3;
-  static constexpr int kBars = kDecodeWarps * kStages * kStage;
+  // At head dim 256 the queries stay in shared memory: in registers (64, beside 128 of output)
+  // they spilled, and no product's operands were loaded ahead of it (524 MB of own keys, B32
+  // Hq16 Hk16: 204 us so, 182 from shared memory; 16 requests of 6 tokens 43.8 and 38.0).
+  static constexpr bool kQShared = D == 256;
+  static constexpr int kQ = kDecodeWarps * kStages * kStage;
+  static constexpr int kBars = kQ + (kQShared ? kDecodeWarps * kTile : 0);
   static constexpr int kBytes = kBars + kDecodeWarps * kStages * 8 + 8 + 1024;  // aligned to 1024
+  static_assert(kBytes <= 232448, "shared memory beyond the 227 KB per-block limit");
   // 16-byte chunk c of row `row` of a tile.
   static __device__ __forceinline__ uint32_t at(int row, int c) {
     return (c >> 3) * kBox + row * 128 + (((c ^ row) & 7) << 4);
@@ -250,6 +256,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   if (run > 0) at = find_place(p, lengths, first, run, lane);
   if (at.more()) {
     uint8_t* ring = smem + wid * S::kStages * S::kStage;
+    uint8_t* queries = smem + S::kQ + wid * S::kTile;  // kQShared
     Place in = at;
 
     // K and V of the unit at `in` into a stage.  Rows past the item's keys come along (zeros past
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
       }
     };
 
-    uint32_t qf[D / 16][4];
+    uint32_t qf[S::kQShared ? 1 : D / 16][4];
     float acc[D / 8][4];
     float m[2], l[2];
     int lim[2];              // keys below lim[i] are seen by row i of this thread
@@ -305,15 +312,25 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
           if (kMask) mrow[i] = p.mask + b * p.mask_stride[0] + h * p.mask_stride[1] + t * p.mask_stride[2];
           if (p.logits) lrow[i] = p.logits + ((b * p.Hk + at.hk) * p.R + r) * p.logits_ld;
         }
-        const uint16_t* row =
-            static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + col;
+        const uint16_t* row = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2];
+        if constexpr (S::kQShared) {  // a row's four lanes take every fourth chunk
+          if (!valid) row = static_cast<const uint16_t*>(p.q);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][i] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * kk)) : 0u;
-          qf[kk][i + 2] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * kk + 8)) : 0u;
+          for (int c = lane & 3; c < D / 8; c += 4)
+            cp_async16(queries + S::at((lane >> 2) + 8 * i, c), row + 8 * c, valid ? 16 : 0);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][i] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + col + 16 * kk)) : 0u;
+            qf[kk][i + 2] = valid ? __ldcg(reinterpret_cast<const uint32_t*>(row + col + 16 * kk + 8)) : 0u;
+          }
         }
         m[i] = kNegInf;
         l[i] = 0.f;
+      }
+      if constexpr (S::kQShared) {
+        cp_async_wait_all();
+        __syncwarp();
       }
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
@@ -382,8 +399,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t kf[4];
           ldsm4(sk + S::at(row, 2 * kk + half), kf);
-          mma16816<kBF16>(x[0], qf[kk], kf[0], kf[1]);
-          mma16816<kBF16>(x[1], qf[kk], kf[2], kf[3]);
+          uint32_t(&q)[4] = qf[S::kQShared ? 0 : kk];
+          if constexpr (S::kQShared) ldsm4(smem_u32(queries) + S::at(lane & 15, 2 * kk + (lane >> 4)), q);
+          mma16816<kBF16>(x[0], q, kf[0], kf[1]);
+          mma16816<kBF16>(x[1], q, kf[2], kf[3]);
         }
       }
       // Scaled to log2 units; -inf where the row does not see the key.

@@ -46,12 +46,6 @@ __device__ __forceinline__ void st_sector(float* dst, const uint32_t* v) {
                : "memory");
 }
 
-// 16 bytes, the first `bytes` of them from src and the others zero.
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 template <int D, bool kSplitKeys>
 struct PrefixLayout {
   static constexpr int kTile = 128 * D * 2;

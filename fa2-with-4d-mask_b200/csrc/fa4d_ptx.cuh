@@ -487,6 +487,13 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : ((1u << n) - 1u));
 }
 
+// ------------------------------------------------------------------ asynchronous copies of a thread
+// 16 bytes (both addresses 16-B aligned), the first `bytes` of them from src and the others zero.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // ------------------------------------------------------------------ shared loads
 __device__ __forceinline__ float4 lds_f4(uint32_t saddr) {
   float4 v;
