@@ -19,8 +19,10 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 8192;  // weights of a CTA at a time
 constexpr int kBins = 2048;   // of a radix pass: 11, 11 and 10 bits of the weight
-constexpr int kRowsInFlight = 4;
-constexpr int kAhead = 4;     // shared-memory reads of a thread in flight
+// Pieces of a row of K and of V that a thread has in flight: 1024 threads an SM hold 98 KB, which
+// L1 has room for (B32 Hk8 D128, 2304 slots to 1536: 78 us with 2, 74 with 3, 75 with 4, 80 with 6).
+constexpr int kRowsInFlight = 3;
+constexpr int kAhead = 4;  // other reads of a thread in flight
 
 // Larger weight, larger key; -0 as 0; NaN below everything.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -100,7 +102,7 @@ struct Piece<1> {
 // keys in registers and every loop over them unrolled, each instruction ran once per CTA and
 // its fetch was the time (2700 to 3300 clocks a radix pass and 8000 to 18000 for the slots at
 // 1024 to 2304 entries; 2000 and 2400 now).  What is left is the copy: 63000 of 78000 clocks
-// of a CTA at B32 Hk8 D128, 2304 slots to 1536 (75.5 us in all, 5.1 TB/s, 79% of the measured
+// of a CTA at B32 Hk8 D128, 2304 slots to 1536 (74 us in all, 5.2 TB/s, 81% of the measured
 // copy rate), 155000 of 195000 at B4 Hk8 D64, 65536 to 32768 (119 us, 4.7 TB/s, 72%).
 template <int VEC>
 __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constant__ fa4d_evict_args a) {
@@ -324,25 +326,41 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
   const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2];
   uint16_t* ko = static_cast<uint16_t*>(a.k_out) + b * a.k_out_stride[0] + h * a.k_out_stride[2];
   uint16_t* vo = static_cast<uint16_t*>(a.v_out) + b * a.v_out_stride[0] + h * a.v_out_stride[2];
+  auto from_of = [&](int slot) { return n <= a.keep ? slot : sliced ? index[slot] : sm.list[slot - slot0]; };
+  // Weights by themselves: beside the rows they cost registers, and the spills' traffic was 3%.
+  for (int s0 = slot0 + threadIdx.x; s0 < slot1; s0 += kThreads * kAhead) {
+    int from[kAhead];
+    float wt[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int slot = s0 + u * kThreads;
+      from[u] = slot < min(slot1, kept) ? from_of(slot) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) wt[u] = from[u] < 0 ? 0.f : __ldg(w + from[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int slot = s0 + u * kThreads;
+      if (slot >= slot1) break;
+      w_out[slot] = wt[u];
+      if (n <= a.keep) index[slot] = from[u];
+    }
+  }
   const int all = (slot1 - slot0) * pieces;
   for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kRowsInFlight) {
     T x[kRowsInFlight], y[kRowsInFlight];
-    float wt[kRowsInFlight];
     int slot[kRowsInFlight], from[kRowsInFlight], c[kRowsInFlight];
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {
-      const int i = i0 + u * kThreads;
-      const int s = i / pieces;
+      const int i = i0 + u * kThreads, s = i / pieces;
       slot[u] = i < all ? slot0 + s : -1;
       c[u] = (i - s * pieces) * VEC;
-      from[u] = slot[u] < 0 || slot[u] >= kept ? -1 : n <= a.keep ? slot[u] : sliced ? index[slot[u]] : sm.list[s];
+      from[u] = slot[u] < 0 || slot[u] >= kept ? -1 : from_of(slot[u]);
     }
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {
       x[u] = y[u] = Piece<VEC>::zero();
-      wt[u] = 0.f;
       if (from[u] >= 0) {
-        if (c[u] == 0) wt[u] = __ldg(w + from[u]);
         x[u] = __ldg(reinterpret_cast<const T*>(k + from[u] * a.k_stride[1] + c[u]));
         y[u] = __ldg(reinterpret_cast<const T*>(v + from[u] * a.v_stride[1] + c[u]));
       }
@@ -352,10 +370,6 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
       if (slot[u] < 0) continue;
       *reinterpret_cast<T*>(ko + slot[u] * a.k_out_stride[1] + c[u]) = x[u];
       *reinterpret_cast<T*>(vo + slot[u] * a.v_out_stride[1] + c[u]) = y[u];
-      if (c[u] == 0) {
-        w_out[slot[u]] = wt[u];
-        if (n <= a.keep) index[slot[u]] = from[u];
-      }
     }
   }
 }
