@@ -96,10 +96,10 @@ int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, boo
 
 // decode_kernel reads the prefix once per 16 rows, from L2 after the first time, and spares the
 // prefix kernel's launch and start.  It takes the prefix while what it reads of K (V as much
-// again) is at most this many elements.  Both ways, in us, for Hq32 Hk8 D128 behind own caches
-// of 100: 16 rows 15.4 / 15.5 at P 2048 and 40 / 34 at 32768; 64 rows 15.6 / 16.3 at 512 and
-// 19.3 / 18.2 at 2048; Hq64 Hk1 D64, 128 rows: 11.9 / 13.0 at 2048 and 15.7 / 14.3 at 8192;
-// Hq16 Hk4 D256, 128 rows: 18.5 / 21.4 at 512 and 27.8 / 21.1 at 2048.
+// again) is at most this many elements.  Both ways (here / prefix kernel), in us, behind own
+// caches of 100, Hq32 Hk8 D128: 16 rows 14.0 / 15.2 at P 2048 and 23.2 / 19.8 at 8192; 64 rows
+// 15.5 / 15.5 at 512 and 19.0 / 17.3 at 2048; Hq64 Hk1 D64, 128 rows: 11.0 / 14.2 at 2048 and
+// 24.7 / 18.9 at 32768; Hq16 Hk4 D256, 128 rows: 16.9 / 18.1 at 512 and 24.5 / 21.8 at 2048.
 constexpr int64_t kDecodePrefix = 1 << 22;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }

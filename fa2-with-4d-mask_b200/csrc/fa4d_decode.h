@@ -97,13 +97,12 @@ constexpr int kItemUnits = 2;
 // decode_kernel warp beside the SM's others, and the time until its first unit.
 template <int D>
 constexpr float kTileMicros = D == 256 ? 1.75f : D == 64 ? 1.9f : 2.1f;
-constexpr float kRunMicros = 7.0f;
+constexpr float kRunMicros = 6.0f;
 template <int D>
-constexpr float kUnitMicros = D == 256 ? 1.6f : D == 64 ? 0.8f : 1.2f;
+constexpr float kUnitMicros = D == 256 ? 1.0f : D == 64 ? 0.8f : 1.1f;
 constexpr float kDecodeMicros = 3.5f;
 constexpr float kReadRate = 6.0f;  // MB per microsecond that decode_kernel reads, of the GPU
-constexpr float kBesideRate = 0.9f;   // of kReadRate, beside the prefix kernel
-constexpr float kPrefixWeight = 0.2f;  // see choose_runs
+constexpr float kPrefixWeight = 0.1f;  // see choose_runs
 template <int D>
 constexpr int kDecodeCtas = D == 256 ? 1 : 2;  // of an SM
 
@@ -144,10 +143,11 @@ __device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, in
 // so it is worked out there by one warp (lane l for l + 1, l + 33, ... runs).  Where the own
 // keys take longer than the prefix whatever its runs, the estimates of many divisions are
 // equal; what they leave out (the start of the CTAs that come late) goes with the prefix
-// kernel's time, a part of which is therefore added.  Over 18 calls (8 to 256 requests, 1024 to
-// 30000 prefix keys, head dims 64 to 256), each timed with every number of runs, the choice is
-// 0.7% above the best on average and at most 2.6% (5.3% and 33% without that part, with
-// estimates from the kernels alone).
+// kernel's time, a part of which is therefore added; of equal divisions the one with fewer
+// partial rows to join is taken.  Over 18 calls (8 to 256 requests, 1024 to 30000 prefix keys,
+// head dims 64 to 256), each timed with every number of runs, the choice is 1.0% above the best
+// on average and 4% at most (3.3% and 25% with the larger of equal numbers of runs and without
+// that part).
 template <int D>
 __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t units, int lane) {
   const float all = static_cast<float>(units);
@@ -159,7 +159,7 @@ __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t un
   for (int s = lane + 1; s <= w.most; s += 32) {
     const int ctas = w.items * s, run = (w.tiles + s - 1) / s;
     const float mine = ((ctas + w.sms - 1) / w.sms) * (((run + w.step - 1) / w.step) * kTileMicros<D> + kRunMicros);
-    const float beside = fminf(kBesideRate * gpu_rate, sm_rate * max(w.sms - ctas, 0)) * fmaxf(mine - kDecodeMicros, 0.f);
+    const float beside = fminf(gpu_rate, sm_rate * max(w.sms - ctas, 0)) * fmaxf(mine - kDecodeMicros, 0.f);
     const float total = mine + (all > beside ? kDecodeMicros + (all - beside) / gpu_rate : 0.f);
     if (total + kPrefixWeight * mine < best_cost) {
       best_cost = total + kPrefixWeight * mine;

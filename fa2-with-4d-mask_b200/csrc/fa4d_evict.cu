@@ -19,8 +19,8 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 8192;  // weights of a CTA at a time
 constexpr int kBins = 2048;   // of a radix pass: 11, 11 and 10 bits of the weight
-// Pieces of a row of K and of V that a thread has in flight: 1024 threads an SM hold 98 KB, which
-// L1 has room for (B32 Hk8 D128, 2304 slots to 1536: 78 us with 2, 74 with 3, 75 with 4, 80 with 6).
+// Pieces of a row of K and of V that a thread has in flight (B32 Hk8 D128, 2304 slots to 1536:
+// 78 us with 2, 74 with 3, 75 with 4, 80 with 6; less shared memory, for a larger L1: no change).
 constexpr int kRowsInFlight = 3;
 constexpr int kAhead = 4;  // other reads of a thread in flight
 
