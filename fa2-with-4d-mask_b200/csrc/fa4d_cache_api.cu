@@ -140,7 +140,7 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   if (items > (1 << 30)) return fail(FA4D_ERR_UNSUPPORTED, "too many row tiles");
   if (!out->splits) {
     // No more CTAs than full caches could occupy.
-    const int64_t line = static_cast<int64_t>(p.prefix_tiles) * Hk * (p.prefix_units + fa4d::kItemUnits) +
+    const int64_t line = static_cast<int64_t>(p.prefix_tiles) * Hk * (p.prefix_units + fa4d::kPrefixItemUnits) +
                          static_cast<int64_t>(B) * Hk * p.tiles * ((C + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys + fa4d::kItemUnits);
     const int64_t each = p.min_units * fa4d::kDecodeWarps;
     out->ctas = static_cast<int>(std::min<int64_t>(out->ctas, (line + each - 1) / each));

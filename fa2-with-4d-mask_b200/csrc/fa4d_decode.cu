@@ -148,7 +148,7 @@ struct Place {
   __device__ __forceinline__ bool advance(const DecodeParams& p, const Lengths& lengths) {
     --left;
     if (++u < units) return false;
-    left -= kItemUnits;
+    left -= prefix ? kPrefixItemUnits : kItemUnits;
     next_item(p, lengths);
     return true;
   }
@@ -160,7 +160,7 @@ __device__ __forceinline__ Place find_place(const DecodeParams& p, const Lengths
   Place w;
   w.left = left;
   w.b = 0;
-  int64_t line = p.prefix_units + kItemUnits;
+  int64_t line = p.prefix_units + kPrefixItemUnits;
   const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * line;
   int tiles = p.tiles;
   w.prefix = at < prefix_all;
@@ -214,7 +214,7 @@ __device__ __forceinline__ Place find_place(const DecodeParams& p, const Lengths
 // tile in registers.  Memory bounds it, at 16 FLOP per byte of K and V for a row tile of 16: 1208
 // MB of own keys (B128 Hk8 D128, 512 to 4096 entries) in 200-205 us with the join, 5.9-6.0 TB/s,
 // 92% of the measured copy rate.  Short calls are bound by the start: lengths, division, first
-// loads take about 4 us, a unit 0.6 to 1.6 us (head dim 64 to 256) when memory is idle.  A row
+// loads take about 4 us, a unit 0.6 to 1.0 us (head dim 64 to 256) when memory is idle.  A row
 // tile is the product's 16 rows: more tiles of a request read its keys again, from L2.
 template <int D, bool kBF16, bool kMask>
 __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kernel(
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
 
   Lengths lengths;
   lengths.load(p, lane);
-  const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kItemUnits) +
+  const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kPrefixItemUnits) +
                         lengths.line(p, lane) * p.Hk * p.tiles;
   const Shares shares = shares_of<D>(p, total, lane);
   if (warp == 0 && lane == 0) {
@@ -555,7 +555,7 @@ struct Joined {
   __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane) : p(params), b(b_), hk(hk_) {
     keys = length_of(p, b);
     each = static_cast<int64_t>(p.Hk) * p.tiles;
-    first = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kItemUnits) +
+    first = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kPrefixItemUnits) +
             line_before(p.lengths, p.C, b, lane) * each;
   }
   // Of an item of `count` units that starts at `from` on the line.
@@ -582,7 +582,7 @@ struct Joined {
     if (p.splits)
       return Parts{p.pre_o, p.pre_ml, static_cast<int64_t>(hk) * p.splits * p.pre_rows + row, p.pre_rows, shares.parts};
     const int64_t i = static_cast<int64_t>(hk) * p.prefix_tiles + row / 16;
-    return of_units(i * (p.prefix_units + kItemUnits), p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
+    return of_units(i * (p.prefix_units + kPrefixItemUnits), p.prefix_tiles ? p.prefix_units : 0, i, static_cast<int>(row % 16));
   }
 };
 

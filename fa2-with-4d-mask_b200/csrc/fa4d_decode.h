@@ -13,12 +13,13 @@ namespace fa4d {
 //
 // decode_kernel works on *units* of 16 keys of an *item* (a row tile with its keys), laid in
 // one line: first the prefix items (KV head, row tile; none when the prefix kernel does
-// them), then the requests' items (request, KV head, row tile), each with
-// ceil(length / 16) units and the time of kItemUnits more, which a change of rows costs (its
-// output written, the next item's queries read).  Each warp takes a run of the line (Shares),
-// so ragged lengths divide evenly without the host knowing them.  What warp w computes of an item is *segment*
-// w + item (unique: along the line one of the two grows), an unnormalised fp32 output row
-// with the running maximum (log2) and sum of its exponentials.
+// them), then the requests' items (request, KV head, row tile), each with ceil(length / 16)
+// units and the time of kItemUnits (of the prefix: kPrefixItemUnits) more, which a change of
+// rows costs (its output written, the next item's queries read).  Each warp takes a run of the
+// line (Shares), so ragged lengths divide evenly without the host knowing them.  What warp w
+// computes of an item is *segment*
+// w + item (unique: along the line one of the two grows), an unnormalised fp32 output row with
+// the running maximum (log2) and sum of its exponentials.
 // The run of a warp: the first `early` warps have `each` units, the others `late` (0: none); and
 // the parts of a row that the prefix kernel made.  16 bytes, read together.
 struct alignas(16) Shares {
@@ -91,6 +92,11 @@ struct PrefixParams {
 constexpr int kDecodeWarps = 4;   // warps of a decode_kernel CTA
 constexpr int kUnitKeys = 16;
 constexpr int kItemUnits = 2;
+// The prefix's items lie together at the front: with a short prefix the first warps do little but
+// change rows, each time with a wait as long as memory is busy (128 requests, 918 MB of own keys,
+// 16 prefix keys: 226 us with 2, 198 with 6, 177 with 12, 165 with 20; small calls lose 1% from 6
+// to 12 and again to 20).
+constexpr int kPrefixItemUnits = 8;
 
 // Measured on B200, in microseconds: a key tile of a prefix kernel CTA (two of them, taken side
 // by side, where the slots split the keys) and a CTA's fill, drain and output rows; a unit of a

@@ -16,9 +16,11 @@
 // and odd key tiles (kSplitKeys), since then the bytes of K and V bound the kernel: one slot
 // alone would take 64 KB per 3400 clocks, 5.5 TB/s over the GPU, two take 9.6 TB/s.  At
 // D = 256 tensor memory holds one slot with two S buffers.
-// Measured: 86 us for 512 rows a KV head x 32768 keys, Hk8 D128, with the join (69 GFLOP, 0.8
-// PFLOP/s; a tile of 256 rows 2.05 us), 18 us for 128 rows x 4096 keys; the chain bounds it, and
-// in short runs the start, Q and the output rows (6 us a CTA).
+// Measured, with the decode and join kernels behind: 86 us for 512 rows a KV head x 32768 keys,
+// Hk8 D128 (69 GFLOP, 0.8 PFLOP/s; a tile of 256 rows 2.05 us), 20 us for 128 rows x 4096 keys.  A
+// tile's time is neither the chain's alone (halves of a tile with S buffers of their own, the next
+// S always there ahead: no faster at D 64, 5% slower at D 128) nor the exponentials' (a third of
+// them by polynomial: no change).  In short runs the start, Q and the output rows count (6 us a CTA).
 // Tensor memory (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [256+D,256+2D); P
 // (16-bit, rounded to the type of V as the product takes it) overwrites S.
 #include "fa4d.h"

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 
 // One thread: one chunk of one head (q, k or v) of a new token.  A decode step has few
 // tokens, so everything is spread over threads and the angles are computed per head; latency
-// bounds it (one token 3.9 us, 160 tokens 5.2 us, back to back).
+// bounds it (one token 3.5 us, 160 tokens 5.0 us, back to back).
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_constant__ fa4d_rotary_append_args a,
                                                                  int chunks, int* status) {
