@@ -288,12 +288,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
     uint32_t qf[S::kQShared ? 1 : D / 16][4];
     float acc[D / 8][4];
     float m[2], l[2];
+    unsigned seen;           // bit i: row i has seen one of this thread's keys
     int lim[2];              // keys below lim[i] are seen by row i of this thread
     const uint8_t* mrow[2];  // its mask row
     float* lrow[2];          // its row of logits, null where there is none
     const int col = 2 * (lane & 3);
 
     auto begin_item = [&]() {
+      seen = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = at.tile * 16 + (lane >> 2) + 8 * i;
@@ -344,6 +346,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        // A maximum of -inf over keys that were seen (part_of_keys, fa4d_decode.h).
+        const unsigned saw = __ballot_sync(0xffffffffu, (seen >> i) & 1u);
+        if ((saw >> (lane & 28)) & 15u) part_of_keys(m[i], l[i]);
         const int r = (lane >> 2) + 8 * i;
         if (r >= p.seg_rows) continue;
         const int64_t row = seg * p.seg_rows + r;
@@ -415,7 +420,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
           const int i = e >> 1, kj = 8 * nt + col + (e & 1), j = key0 + kj;
           const bool keep = j < lim[i] && (!kMask || ((keep_bits >> (4 * i + 2 * nt + (e & 1))) & 1u));
           x[nt][e] = keep ? x[nt][e] * p.scale_log2 : kNegInf;
-          if (keep) dead &= ~(1u << kj);
+          if (keep) {
+            dead &= ~(1u << kj);
+            seen |= 1u << i;
+          }
         }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -586,6 +594,11 @@ struct Joined {
   }
 };
 
+// log2 of a row's sum from its maximum and sum; +inf for a row without a key.
+__device__ __forceinline__ float log2_sum(float m, float l) {
+  return m == kNegInf ? (l == 0.f ? INFINITY : NAN) : m + log2f(l);
+}
+
 // Joins the output: row_warps warps a row, each a share of its parts.  Everything here is
 // latency: partial rows are loaded ahead of the maximum that scales them (about 3 us for 42 parts
 // of 32 rows, 8 us behind a decode kernel of 296 CTAs at B32 Hq32).
@@ -609,6 +622,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
   float m_all = kNegInf, l_all = 0.f;
+  bool undefined = false;  // a part of keys of logit -inf
   // 32 parts at a time, lane i with the maximum of part i; their rows kJoinAhead at a time.
   for (int i0 = n0; i0 < n; i0 += 32) {
     const int i = i0 + lane;
@@ -621,6 +635,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       mx = fmaxf(mx, m_all);
       f = ml.x == kNegInf ? 0.f : ex2(ml.x - mx);
+      undefined = undefined || (ml.x == kNegInf && ml.y != 0.f);
       float l = ml.y * f;
 #pragma unroll
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -651,6 +666,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       }
     }
   }
+  if (__any_sync(0xffffffffu, undefined) && m_all == kNegInf) l_all = 1.f;
   if (row_warps > 1) {  // the row's first warp adds the others'
     __shared__ float others[kJoinWarps][D];
     __shared__ float2 others_ml[kJoinWarps];
@@ -666,7 +682,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
     for (int i = 0; i < row_warps; ++i) {
       const float2 ml = others_ml[wid + i];
-      if (ml.x == kNegInf) continue;
+      if (ml.x == kNegInf) {
+        if (mx == kNegInf) l_all = fmaxf(l_all, ml.y);
+        continue;
+      }
       const float fi = ex2(ml.x - mx);
       l_all += fi * ml.y;
 #pragma unroll
@@ -675,10 +694,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     m_all = mx;
   }
   if (r >= p.R) return;
-  // A row without a key: 0.  (A NaN maximum or sum stays one.)
-  const float inv = m_all == kNegInf ? 0.f : 1.f / l_all;
-  if (p.weights && lane == 0)
-    p.lse[(static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r] = m_all == kNegInf ? INFINITY : m_all + log2f(l_all);
+  // A row without a key: 0.  One whose every logit is -inf, or that saw a NaN (in l_all): NaN.
+  const float inv = m_all == kNegInf ? (l_all == 0.f ? 0.f : NAN) : 1.f / l_all;
+  if (p.weights && lane == 0) p.lse[(static_cast<int64_t>(at.b) * p.Hk + at.hk) * p.R + r] = log2_sum(m_all, l_all);
   const int t = r / p.G, h = at.hk * p.G + r % p.G;
   uint16_t* dst = static_cast<uint16_t*>(p.o) + at.b * p.o_stride[0] + t * p.o_stride[1] + h * p.o_stride[2];
   if constexpr (D == 96) {
@@ -693,6 +711,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if constexpr (D == 256) *reinterpret_cast<uint4*>(dst + 8 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
+
+// What a key of logit x gains: nothing where the row does not see it (-inf), even if the row's sum
+// is NaN.
+__device__ __forceinline__ float gain(float x, float lse) { return x == kNegInf ? 0.f : ex2(x - lse); }
 
 // Adds to the weights of a request's own keys: the sum over the rows of 2^(x - lse), lse = +inf
 // for a row without a key.  A kernel of its own beside join_kernel, whose registers would leave
@@ -733,17 +755,17 @@ __global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_con
         for (int i = lane; i < px.n + py.n; i += 32) {
           const float2 ml = __ldcg(i < px.n ? px.ml + px.first + i * px.step : py.ml + py.first + (i - px.n) * py.step);
           const float mx = fmaxf(m, ml.x);
-          if (mx != kNegInf) l = l * ex2(m - mx) + ml.y * ex2(ml.x - mx);
+          l = mx != kNegInf ? l * ex2(m - mx) + ml.y * ex2(ml.x - mx) : fmaxf(l, ml.y);
           m = mx;
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
           const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
           const float mx = fmaxf(m, m2);
-          if (mx != kNegInf) l = l * ex2(m - mx) + l2 * ex2(m2 - mx);
+          l = mx != kNegInf ? l * ex2(m - mx) + l2 * ex2(m2 - mx) : fmaxf(l, l2);
           m = mx;
         }
-        if (lane == 0) lse[r] = m == kNegInf ? INFINITY : m + log2f(l);
+        if (lane == 0) lse[r] = log2_sum(m, l);
       }
       __syncthreads();
 #pragma unroll 1
@@ -764,10 +786,10 @@ __global__ void __launch_bounds__(kJoinThreads, 6) weigh_kernel(const __grid_con
 #pragma unroll
           for (int u = 0; u < kWeighRows; ++u) {
             const float sub = r + u < rows ? lse[r + u] : INFINITY;
-            got[0] += ex2(x[u].x - sub);
-            got[1] += ex2(x[u].y - sub);
-            got[2] += ex2(x[u].z - sub);
-            got[3] += ex2(x[u].w - sub);
+            got[0] += gain(x[u].x, sub);
+            got[1] += gain(x[u].y, sub);
+            got[2] += gain(x[u].z, sub);
+            got[3] += gain(x[u].w, sub);
           }
         }
         if (whole) {

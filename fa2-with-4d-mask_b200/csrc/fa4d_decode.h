@@ -19,7 +19,8 @@ namespace fa4d {
 // line (Shares), so ragged lengths divide evenly without the host knowing them.  What warp w
 // computes of an item is *segment*
 // w + item (unique: along the line one of the two grows), an unnormalised fp32 output row with
-// the running maximum (log2) and sum of its exponentials.
+// the running maximum (log2) and sum of its exponentials: maximum -inf and sum 0 where the row saw
+// no key (its output row may then be missing), and as part_of_keys writes them where it did.
 // The run of a warp: the first `early` warps have `each` units, the others `late` (0: none); and
 // the parts of a row that the prefix kernel made.  16 bytes, read together.
 struct alignas(16) Shares {
@@ -113,6 +114,18 @@ template <int D>
 constexpr int kDecodeCtas = D == 256 ? 1 : 2;  // of an SM
 
 #ifdef __CUDACC__
+// The maximum and sum of a part that saw keys.  A maximum leaves NaN out, so a sum over keys of
+// logit NaN alone comes with the maximum -inf: it becomes 0, and the sum reaches every sum that it
+// is joined to.  Keys of logit -inf alone sum to 0: the part counts for nothing beside a finite
+// logit, but a row of such parts is undefined, which the sum 1 tells from a row without a key.
+__device__ __forceinline__ void part_of_keys(float& m, float& l) {
+  if (m != -INFINITY) return;
+  if (l != l)
+    m = 0.f;
+  else
+    l = 1.f;
+}
+
 struct RunChoice {
   int runs;
   float prefix_us, total_us;  // of the prefix kernel, of both

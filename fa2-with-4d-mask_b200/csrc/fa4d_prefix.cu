@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         mbar_arrive(&p_full[sb]);
       }
 
-      // This run's part of the row; one without a tile is marked by its maximum, -inf.
+      // This run's part of the row; one without a tile is marked by its maximum, -inf, and sum, 0.
+      if (count > 0) part_of_keys(m_run, l_run);
       const int part = kSplitKeys ? 2 * blockIdx.z + t : blockIdx.z;
       const int64_t out = (static_cast<int64_t>(hk) * p.parts + part) * p.rows + row;
       if (valid) p.ml[out] = make_float2(m_run, l_run);
