@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
   const int b = item / a.Hk, h = item - b * a.Hk;
   pdl_wait();
   pdl_launch();
-  const int n = min(max(__ldg(a.lengths + b), 0), a.C);
+  const int n = min(max(__ldcg(a.lengths + b), 0), a.C);
   const int kept = min(n, a.keep);
   const float* w = a.weights + b * a.weights_stride[0] + h * a.weights_stride[1];
   float* w_out = a.weights_out + b * a.weights_out_stride[0] + h * a.weights_out_stride[1];
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
       for (int j0 = base + threadIdx.x; j0 < end; j0 += kAhead * kThreads) {
         float x[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) x[u] = j0 + u * kThreads < end ? __ldg(w + j0 + u * kThreads) : 0.f;
+        for (int u = 0; u < kAhead; ++u) x[u] = j0 + u * kThreads < end ? __ldcg(w + j0 + u * kThreads) : 0.f;
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
           if (j0 + u * kThreads < end) sm.key[j0 + u * kThreads - base] = order_key(x[u]);
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
       from[u] = slot < min(slot1, kept) ? from_of(slot) : -1;
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) wt[u] = from[u] < 0 ? 0.f : __ldg(w + from[u]);
+    for (int u = 0; u < kAhead; ++u) wt[u] = from[u] < 0 ? 0.f : __ldcg(w + from[u]);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int slot = s0 + u * kThreads;
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
     for (int u = 0; u < kRowsInFlight; ++u) {
       x[u] = y[u] = Piece<VEC>::zero();
       if (from[u] >= 0) {
-        x[u] = __ldg(reinterpret_cast<const T*>(k + from[u] * a.k_stride[1] + c[u]));
-        y[u] = __ldg(reinterpret_cast<const T*>(v + from[u] * a.v_stride[1] + c[u]));
+        x[u] = __ldcg(reinterpret_cast<const T*>(k + from[u] * a.k_stride[1] + c[u]));
+        y[u] = __ldcg(reinterpret_cast<const T*>(v + from[u] * a.v_stride[1] + c[u]));
       }
     }
 #pragma unroll
