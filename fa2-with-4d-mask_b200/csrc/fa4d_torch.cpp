@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/python_headers.h>
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -68,7 +69,17 @@ void set3(int64_t (&out)[3], const Tensor& x, Layout l) {
   out[2] = x.stride(l.head());
 }
 
+// A tangent (torch.autograd.forward_ad) is not carried through, so a tensor with one is refused, as
+// the attention's autograd function does.  Such a tensor need not require a gradient.
+void no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* x : tensors)
+    if (x->defined() && x->_fw_grad(0).defined())
+      throw Refused{PyExc_NotImplementedError, cat(name, " has no forward-mode derivative")};
+}
+
 void no_gradient(const char* name, std::initializer_list<const Tensor*> tensors) {
+  no_tangent(name, tensors);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* x : tensors)
     if (x->defined() && x->requires_grad()) refuse(cat(name, " has no gradient: call it under torch.no_grad()"));
@@ -318,6 +329,7 @@ PyObject* rotary(PyObject* const* args) {
   const Tensor q = tensor_arg(args[1], "query", 4), k = tensor_arg(args[2], "key", 4);
   check_tokens(q, k, Tensor(), l, table->t.D);
   const Tensor positions = check_positions(args[3], *table, q.size(0), q.size(l.seq()), q);
+  no_tangent("MultiAxisRotary", {&q, &k});
   need_cuda("MultiAxisRotary", q);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
     auto holder = c10::intrusive_ptr<torch::CustomClassHolder>(c10::intrusive_ptr<Table>::unsafe_reclaim_from_nonowning(table));
@@ -340,6 +352,7 @@ PyObject* rotary_append(PyObject* const* args) {
   const Tensor kc = tensor_arg(args[5], "key cache", 4), vc = tensor_arg(args[6], "value cache", 4);
   const Tensor lengths = any_tensor(args[7], kLengths), weights = optional_arg(args[8], kWeights);
   const int64_t C = check_cache(kc, vc, lengths, weights, l, B, Hk, table->t.D, q);
+  no_tangent("append", {&kc, &vc, &weights});
   no_gradient("append", {&q, &k, &v});
   if (kc.stride(3) != 1 || vc.stride(3) != 1) refuse("the caches are written in place and need unit head-dim stride");
   if (repeats(kc) || repeats(vc) || (weights.defined() && repeats(weights)))
@@ -429,6 +442,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   }
   if (!std::isfinite(scale)) refuse("scale must be finite");
   const int causal = PyObject_IsTrue(args[9]);
+  no_tangent("shared_prefix_attention", {&weights});
   no_gradient("shared_prefix_attention", {&q, &pk, &pv, &k, &v});
   need_cuda("shared_prefix_attention", q);
 
