@@ -85,6 +85,12 @@ void no_gradient(const char* name, std::initializer_list<const Tensor*> tensors)
     if (x->defined() && x->requires_grad()) refuse(cat(name, " has no gradient: call it under torch.no_grad()"));
 }
 
+// Tells autograd that tensors have been written (an inference tensor has no version to tell).
+void written(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* x : tensors)
+    if (x->defined() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+}
+
 void need_cuda(const char* name, const Tensor& x) {
   if (!x.is_cuda()) throw Refused{PyExc_RuntimeError, cat(name, " runs on CUDA (sm_100a) tensors only")};
 }
@@ -352,8 +358,7 @@ PyObject* rotary_append(PyObject* const* args) {
   const Tensor kc = tensor_arg(args[5], "key cache", 4), vc = tensor_arg(args[6], "value cache", 4);
   const Tensor lengths = any_tensor(args[7], kLengths), weights = optional_arg(args[8], kWeights);
   const int64_t C = check_cache(kc, vc, lengths, weights, l, B, Hk, table->t.D, q);
-  no_tangent("append", {&kc, &vc, &weights});
-  no_gradient("append", {&q, &k, &v});
+  no_gradient("append", {&q, &k, &v, &kc, &vc, &weights});
   if (kc.stride(3) != 1 || vc.stride(3) != 1) refuse("the caches are written in place and need unit head-dim stride");
   if (repeats(kc) || repeats(vc) || (weights.defined() && repeats(weights)))
     refuse("the caches and weights are written in place and may not repeat memory");
@@ -391,6 +396,7 @@ PyObject* rotary_append(PyObject* const* args) {
   a.C = small(C, "cache");
   a.dtype = dtype_code(q);
   check(fa4d_rotary_append(&a, stream_of(q)), "fa4d_rotary_append");
+  written({&kc, &vc, &weights});
   return pair_of(qo, lengths_out);
 }
 
@@ -442,8 +448,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   }
   if (!std::isfinite(scale)) refuse("scale must be finite");
   const int causal = PyObject_IsTrue(args[9]);
-  no_tangent("shared_prefix_attention", {&weights});
-  no_gradient("shared_prefix_attention", {&q, &pk, &pv, &k, &v});
+  no_gradient("shared_prefix_attention", {&q, &pk, &pv, &k, &v, &weights});
   need_cuda("shared_prefix_attention", q);
 
   const c10::cuda::OptionalCUDAGuard guard(q.device());
@@ -497,6 +502,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   const Tensor workspace = at::empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
   a.workspace = workspace.data_ptr();
   check(fa4d_prefix_attention(&a, stream_of(q)), "fa4d_prefix_attention");
+  written({&weights});
   return THPVariable_Wrap(out);
 }
 
@@ -538,6 +544,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
       for (const Tensor* y : std::initializer_list<const Tensor*>{&k, &v, &weights, &lengths})
         if (meet(*x, *y)) refuse("out may not share memory with the inputs");
     if (meet(ko, vo)) refuse("out's keys and values may not share memory");
+    no_gradient("evict_by_weight", {&ko, &vo, &wo});
   }
   need_cuda("evict_by_weight", k);
   const c10::cuda::OptionalCUDAGuard guard(k.device());
@@ -574,6 +581,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
     a.sinks = small(sinks, "sinks");
     a.recent = small(recent, "recent");
     check(fa4d_evict(&a, stream_of(k)), "fa4d_evict");
+    written({&ko, &vo, &wo});
   }
   PyObject* out = PyTuple_New(5);
   if (!out) return nullptr;
