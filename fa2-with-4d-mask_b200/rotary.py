@@ -31,8 +31,11 @@ class MultiAxisRotary:
         pairing: "half" pairs element i with i + rotary_dim / 2, "adjacent" 2 i with 2 i + 1.
 
     Angles are exact for every position (fixed point modulo a turn); positions are integers
-    and may be negative.
+    and may be negative.  Objects can be copied and pickled.
     """
+
+    # Where a process that loads a pickle finds it: this package has no importable name of its own.
+    __module__ = "tilelang_fa2_4d_mask"
 
     def __init__(self, head_dim: int, sections: Sequence[int], *, base: float = 10000.0,
                  rotary_dim: Optional[int] = None, pairing: str = "half"):
@@ -50,8 +53,18 @@ class MultiAxisRotary:
             raise ValueError(f"base must be positive, got {base}")
         self.head_dim, self.sections, self.base = head_dim, sections, float(base)
         self.rotary_dim, self.pairing = rotary_dim, pairing
+        self._make_table()
+
+    def _make_table(self) -> None:
         self._host = _lib.host()
-        self._table = self._host.make_table(self.base, sections, head_dim, rotary_dim, _PAIRINGS[pairing])
+        self._table = self._host.make_table(self.base, self.sections, self.head_dim, self.rotary_dim, _PAIRINGS[self.pairing])
+
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k not in ("_host", "_table")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._make_table()
 
     def __call__(self, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, *,
                  layout: Layout = "bhsd") -> tuple:
