@@ -6,6 +6,7 @@ The directory name is not a Python identifier, so the package is loaded under
 the module name ``fa2_with_4d_mask_b200`` by ``tilelang_fa2_4d_mask/__init__.py``.
 """
 
+from ._lib import DEV_CACHE_FULL, device_status
 from .fa2 import causal_mode, flash_attention_with_4d_mask
 from .modeling_attention import tilelang_attention_forward, tilelang_flash_attention
 from .rotary import MultiAxisRotary
@@ -19,4 +20,6 @@ __all__ = [
     "MultiAxisRotary",
     "shared_prefix_attention",
     "evict_by_weight",
+    "device_status",
+    "DEV_CACHE_FULL",
 ]

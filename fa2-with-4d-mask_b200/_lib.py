@@ -594,7 +594,9 @@ def host():
 
 
 def device_status(device: Optional[torch.device] = None, clear: bool = True) -> int:
-    """Synchronises the current stream and returns the kernels' status bits (0 = none)."""
+    """Synchronises the current stream and returns the kernels' status bits on the device: waits
+    that gave up, and ``DEV_CACHE_FULL`` where a token did not fit its cache (0 = none).  With
+    ``clear`` all bits are reset."""
     lib = load_library()
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     if device.index is None:

@@ -230,9 +230,13 @@ class _flash_attention_with_4d_mask(torch.autograd.Function):
         if _CHECK_STATUS:
             # Opt-in: synchronise and raise if any kernel since the last check gave up a
             # bounded wait (its outputs are then garbage).
-            bits = _lib.device_status(q.device) & ~_lib.DEV_CACHE_FULL
-            if bits:
-                raise RuntimeError(f"an attention kernel gave up a bounded wait (device status {bits:#x})")
+            # The word also tells that a cache was full: that is left to its reader, except where
+            # this raises, which clears the word and passes it on.
+            if _lib.device_status(q.device, clear=False) & ~_lib.DEV_CACHE_FULL:
+                bits = _lib.device_status(q.device)
+                full = "; a cache was full too, and tokens were not stored" if bits & _lib.DEV_CACHE_FULL else ""
+                bits &= ~_lib.DEV_CACHE_FULL
+                raise RuntimeError(f"an attention kernel gave up a bounded wait (device status {bits:#x}){full}")
         if ctx.bhsd_input:
             dQ, dK, dV = dQ.transpose(1, 2), dK.transpose(1, 2), dV.transpose(1, 2)
         return dQ, dK, dV, None, None, None, None, None, None, None, None

@@ -93,7 +93,7 @@ class MultiAxisRotary:
 
         Returns:
             (turned query, new lengths).  Tokens past the capacity C are not stored: the new
-            length stays at C and ``FA4D_DEV_CACHE_FULL`` is set in the device status word.
+            length stays at C and ``DEV_CACHE_FULL`` is set in ``device_status()``.
         """
         return self._host.rotary_append(self._table, query, key, value, positions, key_cache, value_cache, lengths,
                                         weights, layout)

@@ -41,6 +41,8 @@ tilelang_flash_attention = _impl.tilelang_flash_attention
 MultiAxisRotary = _impl.MultiAxisRotary
 shared_prefix_attention = _impl.shared_prefix_attention
 evict_by_weight = _impl.evict_by_weight
+device_status = _impl.device_status
+DEV_CACHE_FULL = _impl.DEV_CACHE_FULL
 
 __all__ = [
     "flash_attention_with_4d_mask",
@@ -49,4 +51,6 @@ __all__ = [
     "MultiAxisRotary",
     "shared_prefix_attention",
     "evict_by_weight",
+    "device_status",
+    "DEV_CACHE_FULL",
 ]
