@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -506,16 +507,80 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   return THPVariable_Wrap(out);
 }
 
-// Whether the memory spans of two tensors meet.
-bool meet(const Tensor& x, const Tensor& y) {
-  if (x.numel() == 0 || y.numel() == 0) return false;
-  auto end = [](const Tensor& t) {
-    int64_t last = 0;
-    for (int i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+// Whether two tensors share a byte.  A byte of x lies at its base + the sum of index * stride +
+// the byte within its element, so they do where whole numbers c, each within the range that the
+// indices leave it, solve  sum c * stride = base of y - base of x  (c of x's dimensions from 0
+// up, of y's from 0 down).
+class Meeting {
+ public:
+  static bool of(const Tensor& x, const Tensor& y) {
+    if (x.numel() == 0 || y.numel() == 0) return false;
+    Meeting m;
+    m.add(x, 1);
+    m.add(y, -1);
+    m.terms.push_back({1, 1 - static_cast<int64_t>(y.element_size()), static_cast<int64_t>(x.element_size()) - 1});
+    return m.solve(static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(x.data_ptr()));
+  }
+
+ private:
+  struct Term {
+    int64_t stride, lo, hi;  // of the number that multiplies the stride
+    // Of the sums of this term and the shorter strides' behind it: the least and the largest, and
+    // whether every number between them is one.
+    int64_t least = 0, most = 0;
+    bool dense = false;
   };
-  return static_cast<const char*>(x.data_ptr()) < end(y) && static_cast<const char*>(y.data_ptr()) < end(x);
-}
+  c10::SmallVector<Term, 16> terms;
+  int steps = 0;
+
+  void add(const Tensor& x, int sign) {
+    for (int i = 0; i < x.dim(); ++i) {
+      if (x.size(i) == 1 || x.stride(i) == 0) continue;
+      const int64_t stride = x.stride(i) * static_cast<int64_t>(x.element_size()), last = x.size(i) - 1;
+      terms.push_back({stride, sign > 0 ? 0 : -last, sign > 0 ? last : 0});
+    }
+  }
+
+  bool solve(int64_t sum) {
+    std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.stride > b.stride; });
+    size_t n = 0;  // equal strides make one term
+    for (size_t i = 1; i < terms.size(); ++i) {
+      if (terms[i].stride == terms[n].stride) {
+        terms[n].lo += terms[i].lo;
+        terms[n].hi += terms[i].hi;
+      } else {
+        terms[++n] = terms[i];
+      }
+    }
+    terms.resize(n + 1);
+    int64_t least = 0, most = 0;
+    bool dense = true;
+    for (size_t i = terms.size(); i-- > 0;) {
+      Term& t = terms[i];
+      dense = dense && (t.lo == t.hi || t.stride <= most - least + 1);
+      t.least = least += t.lo * t.stride;
+      t.most = most += t.hi * t.stride;
+      t.dense = dense;
+    }
+    return search(0, sum);
+  }
+
+  // From the longest stride down.  Where strides are nested few numbers fit at each; what is not
+  // decided within the steps counts as shared.
+  bool search(size_t i, int64_t sum) {
+    if (i == terms.size()) return sum == 0;
+    const Term& t = terms[i];
+    if (sum < t.least || sum > t.most) return false;
+    if (t.dense || ++steps > 10000) return true;
+    const int64_t rest_least = t.least - t.lo * t.stride, rest_most = t.most - t.hi * t.stride;
+    auto down = [&](int64_t v) { return v / t.stride - (v % t.stride < 0); };
+    const int64_t from = std::max(t.lo, -down(rest_most - sum)), to = std::min(t.hi, down(sum - rest_least));
+    for (int64_t c = from; c <= to; ++c)
+      if (search(i + 1, sum - c * t.stride)) return true;
+    return false;
+  }
+};
+bool meet(const Tensor& x, const Tensor& y) { return Meeting::of(x, y); }
 
 // evict_by_weight(key, value, weights, lengths, keep, sinks, recent, out, layout) -> (key,
 // value, weights, lengths, index)
@@ -543,7 +608,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
     for (const Tensor* x : std::initializer_list<const Tensor*>{&ko, &vo, &wo})
       for (const Tensor* y : std::initializer_list<const Tensor*>{&k, &v, &weights, &lengths})
         if (meet(*x, *y)) refuse("out may not share memory with the inputs");
-    if (meet(ko, vo)) refuse("out's keys and values may not share memory");
+    if (meet(ko, vo) || meet(ko, wo) || meet(vo, wo)) refuse("out's tensors may not share memory with each other");
     no_gradient("evict_by_weight", {&ko, &vo, &wo});
   }
   need_cuda("evict_by_weight", k);
