@@ -98,6 +98,13 @@ void need_cuda(const char* name, const Tensor& x) {
 
 Tensor unit_rows(const Tensor& x) { return x.stride(3) == 1 ? x : x.contiguous(); }
 
+// A new tensor in x's order of strides, with whole rows: where the rows of x overlap (windows of
+// one another, which have no order), a contiguous one.
+Tensor new_rows(const Tensor& x) {
+  Tensor out = at::empty_like(x);
+  return out.stride(3) == 1 ? out : at::empty_like(x, at::MemoryFormat::Contiguous);
+}
+
 // x with rows that 16-byte accesses can reach: itself, or a copy.  `walked`: no dimension may
 // have stride 0 either.
 Tensor rows16(const Tensor& x, bool walked = false) {
@@ -194,7 +201,7 @@ void set_positions(Args& a, const Tensor& p) {
 std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, const Tensor& positions, const Table& table, Layout l, bool inverse) {
   q = unit_rows(q);
   k = unit_rows(k);
-  Tensor qo = at::empty_like(q), ko = at::empty_like(k);
+  Tensor qo = new_rows(q), ko = new_rows(k);
   if (q.numel() == 0 || k.numel() == 0) {
     if (q.numel() || k.numel()) refuse("query and key need at least one head");
     return {qo, ko};
@@ -367,7 +374,7 @@ PyObject* rotary_append(PyObject* const* args) {
   q = unit_rows(q);
   k = unit_rows(k);
   v = unit_rows(v);
-  Tensor qo = at::empty_like(q);
+  Tensor qo = new_rows(q);
   if (B == 0 || T == 0) return pair_of(qo, lengths.clone());
   Tensor lengths_out = at::empty_like(lengths);
   const c10::cuda::OptionalCUDAGuard guard(q.device());
@@ -454,7 +461,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
 
   const c10::cuda::OptionalCUDAGuard guard(q.device());
   q = rows16(q);
-  Tensor out = at::empty_like(q);
+  Tensor out = new_rows(q);
   if (out.numel() == 0) return THPVariable_Wrap(out);
   k = rows16(k, true);  // keys and values go through tensor maps
   v = rows16(v, true);
