@@ -597,6 +597,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
   if (!half_type(k)) refuse(cat("key cache must be fp16 or bf16, got ", name_of(k.scalar_type())));
   const Tensor weights = any_tensor(args[2], "weights are required"), lengths = any_tensor(args[3], kLengths);
   const int64_t B = k.size(0), D = k.size(3), Hk = k.size(l.head());
+  if (Hk == 0 || D == 0) refuse("the caches need at least one head of at least one element");
   const int64_t C = check_cache(k, v, lengths, weights, l, B, Hk, D, k);
   const int64_t keep = int_arg(args[4], "keep"), sinks = int_arg(args[5], "sinks"), recent = int_arg(args[6], "recent");
   if (keep < 1 || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
@@ -628,7 +629,7 @@ PyObject* evict_by_weight(PyObject* const* args) {
     wo = at::empty({B, Hk, keep}, weights.options());
   }
   Tensor lengths_out = at::empty_like(lengths), index = at::empty({B, Hk, keep}, lengths.options());
-  if (B && Hk && D) {
+  if (B) {
     fa4d_evict_args a;
     a.k = k.data_ptr();
     a.v = v.data_ptr();
