@@ -2,7 +2,8 @@
 binding of the operators around the attention) in place.
 
 The library is compiled with nvcc for ``sm_100a`` only, the binding with the host compiler
-against the installed torch, and both are written next to this file, so they travel with the
+against the installed torch (where there is none, it is left out: C callers do not need it), and
+both are written next to this file, so they travel with the
 source tree.  Objects go to ``_build/`` beside them.
 Run ``python build.py`` (add ``--ptxas-info`` to print register / spill counts).
 """
@@ -11,6 +12,8 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import re
 import shutil
@@ -81,9 +84,17 @@ def _compile(nvcc: str, src: Path, obj: Path, ptxas_info: bool) -> str:
     return res.stdout + res.stderr
 
 
-def _build_host() -> None:
+def _build_host(force: bool) -> None:
     """The binding links libfa4d.so beside it and torch's own libraries (loaded by ``import
-    torch`` before it)."""
+    torch`` before it); it is built again when its sources, or torch or Python, are others."""
+    if importlib.util.find_spec("torch") is None:
+        print(f"torch is not installed: {HOST_LIB.name} is not built", file=sys.stderr)
+        return
+    stamp = BUILD / "host_built_for.txt"
+    target = f"torch {importlib.metadata.version('torch')}, python {sys.version_info.major}.{sys.version_info.minor}"
+    known = stamp.read_text() if stamp.exists() else ""
+    if not force and known == target and not _stale(HOST_LIB, [HOST_SOURCE, INCLUDE / "fa4d.h"]):
+        return
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -100,6 +111,7 @@ def _build_host() -> None:
     if res.returncode != 0:
         raise RuntimeError(f"host binding failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, HOST_LIB)
+    stamp.write_text(target)
 
 
 def build(force: bool = False, ptxas_info: bool = False, jobs: int | None = None) -> Path:
@@ -126,8 +138,7 @@ def build(force: bool = False, ptxas_info: bool = False, jobs: int | None = None
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
-    if force or _stale(HOST_LIB, [HOST_SOURCE, INCLUDE / "fa4d.h"]):
-        _build_host()
+    _build_host(force)
     if ptxas_info:
         for log in logs:
             sys.stdout.write(log)
