@@ -3,9 +3,10 @@
 //
 // Pair i of a head is multiplied, as a complex number, by e^(i phi) with
 // phi = position(axis of i) * theta_i.  The angle is kept as a fraction of a turn in 64-bit
-// fixed point: position * turn_i modulo 2^64 is exact, so large positions lose nothing (a
-// 32-bit product of position and frequency is off by 4e-3 rad at position 65536), and the
-// fraction's top 32 bits go to sincospif, whose argument then needs no range reduction.
+// fixed point: position * turn_i modulo 2^64 is exact, so what a position adds to the error is
+// its multiple of turn_i's own rounding, about 2^-64 turns (a 32-bit product of position and
+// frequency is off by 4e-3 rad at position 65536), and the fraction's top 32 bits go to sincospif,
+// whose argument, rounded to 2^-25 turns, then needs no range reduction.
 //
 // Bound by memory: each element is read once and written once.
 #include "fa4d.h"

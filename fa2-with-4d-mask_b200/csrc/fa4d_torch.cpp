@@ -296,7 +296,8 @@ const char* kLengths = "lengths must be a contiguous int32 tensor";
 // ------------------------------------------------------------------ entry points
 
 // make_table(base, sections, head_dim, rotary_dim, pairing) -> capsule.  Pair i turns by
-// base^(-2 i / rotary_dim) radians a position: as turns, modulo one, in units of 2^-64.
+// base^(-2 i / rotary_dim) radians a position: as turns, modulo one, to the nearest 2^-64 (at
+// most 1.12 of these off, for a base of 1 or more).
 PyObject* make_table(PyObject* const* args) {
   auto table = c10::make_intrusive<Table>();
   fa4d_rotary_table& t = table->t;
@@ -311,7 +312,8 @@ PyObject* make_table(PyObject* const* args) {
     const int64_t n = int_arg(PyTuple_GET_ITEM(args[1], a), "sections");
     for (int64_t j = 0; j < n && i < FA4D_ROTARY_MAX_PAIRS; ++j, ++i) {
       const long double turns = std::pow(static_cast<long double>(base), -2.0L * i / t.rotary_dim) / 6.283185307179586476925287L;
-      t.turn[i] = static_cast<uint64_t>(std::ldexp(turns - std::floor(turns), 64));
+      const long double units = std::rint(std::ldexp(turns - std::floor(turns), 64));
+      t.turn[i] = units < 18446744073709551616.0L ? static_cast<uint64_t>(units) : 0;  // a whole turn
       t.axis[i] = static_cast<uint8_t>(a);
     }
   }

@@ -30,8 +30,9 @@ class MultiAxisRotary:
         rotary_dim: elements of a head that are turned (default all); the rest is copied.
         pairing: "half" pairs element i with i + rotary_dim / 2, "adjacent" 2 i with 2 i + 1.
 
-    Angles are exact for every position (fixed point modulo a turn); positions are integers
-    and may be negative.  Objects can be copied and pickled.
+    Positions are integers and may be negative.  The product of position and frequency is exact
+    modulo a turn, so an angle is off by at most 2**-25 turns, and ``1.2 * abs(position) * 2**-64``
+    for the rounding of the frequency (for a base of 1 or more).  Objects can be copied and pickled.
     """
 
     # Where a process that loads a pickle finds it: this package has no importable name of its own.

@@ -260,8 +260,10 @@ int fa4d_mask_prepare_docs(const int32_t* doc_q, const int32_t* doc_k, const int
 
 /* Rotary positions with several axes.  The first rotary_dim elements of a head form
  * rotary_dim / 2 pairs, (i, i + rotary_dim / 2) or (2 i, 2 i + 1); pair i is turned by the
- * angle positions[axis[i]][b][t] * turn[i], counted in 2^-64 turns modulo a turn, so it is
- * exact for every 64-bit position.  Elements past rotary_dim are copied. */
+ * angle positions[axis[i]][b][t] * turn[i], counted in 2^-64 turns modulo a turn: that product
+ * is exact for every 64-bit position, so the angle is off by |position| times the rounding of
+ * turn[i] (half a unit at best: 2^-25 turns at 2^40 positions, a quarter turn at 2^63), and by
+ * 2^-25 turns for the sine's and cosine's argument.  Elements past rotary_dim are copied. */
 #define FA4D_ROTARY_MAX_PAIRS 128
 enum fa4d_pairing { FA4D_PAIR_HALF = 0, FA4D_PAIR_ADJACENT = 1 };
 
