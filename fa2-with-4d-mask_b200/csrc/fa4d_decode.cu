@@ -517,12 +517,6 @@ struct Parts {
 };
 
 template <int D>
-struct RowAcc {
-  static constexpr int kEach = D / 32;  // elements of a lane: consecutive
-  float v[kEach];
-};
-
-template <int D>
 __device__ __forceinline__ void load_row(const float* row, int lane, float (&v)[D / 32]) {
   if constexpr (D == 64) {
     const float2 a = *reinterpret_cast<const float2*>(row + 2 * lane);
