@@ -24,7 +24,7 @@ struct DecodeShape {
   static constexpr int kStages = D == 64 ? 6 : 3;
   // At head dim 256 the queries stay in shared memory: in registers (64, beside 128 of output)
   // they spilled, and no product's operands were loaded ahead of it (524 MB of own keys, B32
-  // Hq16 Hk16: 204 us so, 182 from shared memory; 16 requests of 6 tokens 43.8 and 38.0).
+  // Hq16 Hk16: 204 us so, 182 from shared memory; 16 requests of 6 tokens: 5.8 us less a call).
   static constexpr bool kQShared = D == 256;
   static constexpr int kQ = kDecodeWarps * kStages * kStage;
   static constexpr int kBars = kQ + (kQShared ? kDecodeWarps * kTile : 0);
@@ -542,8 +542,8 @@ constexpr int kJoinAhead = D == 64 ? 16 : 8;
 constexpr int kWeighRows = 4;                 // rows of weights taken together
 constexpr int kWeighKeys = 4 * kJoinThreads;  // own keys of a block of weigh_kernel at a time
 constexpr int kWeighTimes = 4;
-// Rows whose sums weigh_kernel works out itself, beside the join (24 rows: 40.1 us so, 41.6 behind
-// it; 64 rows: 56 and 49).
+// Rows whose sums weigh_kernel works out itself, beside the join (16 requests, Hk4, prefix 2050, own
+// up to 770: 24 rows at D 256 33.0 us so, 34.5 behind it; 64 rows at D 128 49.1 and 42.7).
 constexpr int kWeighOwnRows = 32;
 
 // The partial results of the rows of (request b, KV head hk).
@@ -769,8 +769,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) weigh_kernel(const __grid_con
         const int j = key0 + i * kWeighKeys;
         if (j >= at.keys) break;
         // The gain, complete before it meets the weight: added to a large weight row by row, gains
-        // below its last place would be lost (64 rows of 3e-6 beside 100: all of them).  Between
-        // batches of rows it waits in the first row's place, whose logits have been read.
+        // below its last place would be lost (64 rows of 3e-6 beside 100: all of them).  The weight
+        // is on its way meanwhile (loaded after the rows: 1.3 us more a call).  Between batches of
+        // rows the gain waits in the first row's place, whose logits have been read.
         float4* sums = reinterpret_cast<float4*>(first_row + j);
         float got[4] = {0.f, 0.f, 0.f, 0.f}, had[4];
         const bool whole = p.weights_vec && j + 4 <= at.keys;

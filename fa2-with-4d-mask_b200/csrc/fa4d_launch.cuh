@@ -5,9 +5,10 @@
 // work; pdl_wait() returns when that one is complete and its writes are visible, so everything
 // that touches global memory comes after it, and no load is of the kind (__ldg, ld.global.nc) that
 // asks for data that stay as they are for the whole kernel, its time before the wait included: the
-// kernel ahead may write them, and the compiler may move such a load above the wait.  pdl_launch() lets the kernel behind start (up to
-// its own wait) once every CTA of this grid has called it or ended.  After an ordinary kernel,
-// or in front of one, both mean nothing and the stream's order holds as always.
+// kernel ahead may write them, and the compiler may move such a load above the wait.
+// pdl_launch() lets the kernel behind start (up to its own wait) once every CTA of this grid has
+// called it or ended.  After an ordinary kernel, or in front of one, both mean nothing and the
+// stream's order holds as always.
 #pragma once
 
 #include <cuda_runtime.h>

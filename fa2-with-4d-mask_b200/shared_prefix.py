@@ -44,14 +44,18 @@ def shared_prefix_attention(
         lengths: int32 ``[B]``, entries of each cache, the T new tokens included.
         mask: optional bool ``[B or 1, Hq or 1, T, C]`` over the own cache, True keeps.
         weights: optional fp32 ``[B, Hk, C]``; gains in place the probability each own entry
-            received, summed over the group's query heads and the T tokens.
+            received, summed over the group's query heads and the T tokens.  The workspace then
+            holds the own keys' logits, ``4 * B * Hq * T * C`` bytes by the caches' capacity C.
         scale: softmax scale, ``head_dim ** -0.5`` by default.
         is_causal: new token t sees the own entries up to its own, ``lengths - T + t``.
 
     Returns:
-        The output in the query's layout; rows that see no key are 0.
+        The output in the query's layout; rows that see no key are 0.  A row that sees a NaN, or
+        whose every logit is -inf, is NaN, as its softmax is; what no token of the request may see
+        can hold anything.
 
-    Rows that are not on 16-byte boundaries are copied first.  There is no gradient.
+    Rows that are not on 16-byte boundaries are copied first.  There is no gradient, in either
+    mode; ``weights`` is written as by an in-place operation.
     """
     return _lib.host().shared_prefix_attention(query, prefix_key, prefix_value, key, value, lengths, mask, weights, scale,
                                                is_causal, layout)
@@ -80,8 +84,8 @@ def evict_by_weight(
         weights: fp32 ``[B, Hk, C]`` with unit slot stride.
         lengths: int32 ``[B]`` entries of each cache.
         out: optional (key, value, weights) to write to, with at least ``keep`` slots and no
-            memory of the inputs (two sets of caches can take turns); slots past ``keep`` stay
-            as they are.  Default: new tensors of ``keep`` slots.
+            element of the inputs or of each other (two sets of caches can take turns); slots
+            past ``keep`` stay as they are.  Default: new tensors of ``keep`` slots.
 
     Returns:
         (key, value, weights, lengths, index): the caches, ``min(lengths, keep)``, and the

@@ -330,9 +330,10 @@ int fa4d_rotary_append(const fa4d_rotary_append_args* args, void* stream);
  * request's own cache, in one softmax:
  *   keys of (b, t) = prefix 0..P-1 and own slots j < lengths[b], with causal also
  *   j <= lengths[b] - T + t (the T new tokens are the cache's last), with mask also
- *   mask[b, h, t, j] != 0;  o = softmax(scale q k^T) v, 0 where there is no key.
+ *   mask[b, h, t, j] != 0;  o = softmax(scale q k^T) v, 0 where there is no key, NaN where the
+ *   softmax is undefined (a NaN among the logits, an infinite one at the top, all -inf).
  * weights (optional) gains, for each own slot, the probability it received, summed over the
- * query heads of the KV head's group and the T tokens. */
+ * query heads of the KV head's group and the T tokens, and then added. */
 typedef struct fa4d_prefix_attention_args {
   const void* q;             /* [B, T, Hq, D] */
   const void* prefix_k;      /* [P, Hk, D]; NULL iff P == 0 */
@@ -360,7 +361,8 @@ typedef struct fa4d_prefix_attention_args {
 } fa4d_prefix_attention_args;
 
 /* Bytes of scratch for these sizes on the current device (partial results of the key
- * splits, and the logits of the own keys when `weights`); 0 for invalid sizes. */
+ * splits, and with `weights` the logits of the own keys, 4 * B * Hq * T * C bytes by the caches'
+ * capacity C); 0 for invalid sizes. */
 size_t fa4d_prefix_attention_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C,
                                        int32_t weights);
 int fa4d_prefix_attention(const fa4d_prefix_attention_args* args, void* stream);
