@@ -10,7 +10,7 @@ from ._lib import DEV_CACHE_FULL, device_status
 from .fa2 import causal_mode, flash_attention_with_4d_mask
 from .modeling_attention import tilelang_attention_forward, tilelang_flash_attention
 from .rotary import MultiAxisRotary
-from .shared_prefix import evict_by_weight, shared_prefix_attention
+from .shared_prefix import cache_values, evict_by_weight, shared_prefix_attention
 
 __all__ = [
     "flash_attention_with_4d_mask",
@@ -19,6 +19,7 @@ __all__ = [
     "causal_mode",
     "MultiAxisRotary",
     "shared_prefix_attention",
+    "cache_values",
     "evict_by_weight",
     "device_status",
     "DEV_CACHE_FULL",

@@ -60,6 +60,13 @@ EXPORTED_SYMBOLS = (
     "fa4d_prefix_attention",
     "fa4d_prefix_attention_workspace",
     "fa4d_evict",
+    "fa4d_norm_rotary",
+    "fa4d_norm_rotary_bwd",
+    "fa4d_norm_rotary_bwd_workspace",
+    "fa4d_norm_append",
+    "fa4d_cache_values",
+    "fa4d_prefix_attention_8bit",
+    "fa4d_prefix_attention_8bit_workspace",
 )
 DEV_TIMEOUT_FWD, DEV_TIMEOUT_BWD, DEV_TIMEOUT_CHECK = 1, 2, 4
 DEV_TIMEOUT_PREFIX, DEV_CACHE_FULL = 16, 32

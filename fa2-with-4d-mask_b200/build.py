@@ -32,7 +32,7 @@ HOST_SOURCE = CSRC / "fa4d_torch.cpp"
 HOST_LIB = HERE / "_fa4d_host.so"
 
 SOURCES = ["fa4d_api.cu", "fa4d_fwd.cu", "fa4d_bwd.cu", "fa4d_bwd256.cu", "fa4d_mask.cu", "fa4d_dq.cu", "fa4d_dq256.cu",
-           "fa4d_rotary.cu", "fa4d_decode.cu", "fa4d_prefix.cu", "fa4d_evict.cu", "fa4d_cache_api.cu"]
+           "fa4d_rotary.cu", "fa4d_norm.cu", "fa4d_append.cu", "fa4d_decode.cu", "fa4d_decode8.cu", "fa4d_prefix.cu", "fa4d_evict.cu", "fa4d_cache_api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"]
 

@@ -85,35 +85,41 @@ int bind_device_of(const void* ptr, const char* name) {
   return FA4D_OK;
 }
 
-// Tensor map over a [B, T, H, D] 16-bit tensor given element strides (b, t, h):
-// dims (D, T, H, B), box (64, rows, 1, 1), 128-B swizzle, zero fill out of bounds.
-int encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
-                bool bf16, const char* name) {
+// Tensor map over a [B, T, H, D] tensor of `esize`-byte elements given element strides (b, t, h):
+// dims (D, T, H, B), box (box, rows, 1, 1), zero fill out of bounds.
+int encode_tokens(CUtensorMap* m, CUtensorMapDataType type, int esize, int box0, CUtensorMapSwizzle swizzle, const void* ptr,
+                  int B, int T, int H, int D, const int64_t st[3], int rows, const char* name) {
   auto enc = tensor_map_encoder();
   if (!enc) return fail(FA4D_ERR_DRIVER, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   if (!aligned(ptr, 16)) return fail(FA4D_ERR_LAYOUT, "%s: base address is not 16-byte aligned", name);
   const int64_t sz[3] = {B, T, H};
   int64_t bytes[3];
   for (int i = 0; i < 3; ++i) {
-    bytes[i] = st[i] * 2;
+    bytes[i] = st[i] * esize;
     // A size-1 dimension is never stepped over; give it a valid stride that is at
     // least as large as the whole tensor so no size rule can trip on it.
-    if (sz[i] == 1) bytes[i] = static_cast<int64_t>(D) * 2 * B * T * H;
+    if (sz[i] == 1) bytes[i] = static_cast<int64_t>(D) * esize * B * T * H;
     if (bytes[i] <= 0 || bytes[i] % 16 != 0 || bytes[i] >= (int64_t(1) << 40))
-      return fail(FA4D_ERR_LAYOUT, "%s: stride %lld (elements) is not a positive multiple of 8", name,
-                  static_cast<long long>(st[i]));
+      return fail(FA4D_ERR_LAYOUT, "%s: stride %lld (elements) is not a positive multiple of %d", name,
+                  static_cast<long long>(st[i]), 16 / esize);
   }
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(T), static_cast<cuuint64_t>(H),
                         static_cast<cuuint64_t>(B)};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(bytes[1]), static_cast<cuuint64_t>(bytes[2]),
                            static_cast<cuuint64_t>(bytes[0])};
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                   const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = enc(m, type, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FA4D_ERR_DRIVER, "%s: cuTensorMapEncodeTiled failed (%d)", name, int(r));
   return FA4D_OK;
+}
+
+// 16-bit elements: box (64, rows, 1, 1), 128-B swizzle.
+int encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
+                bool bf16, const char* name) {
+  return encode_tokens(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, 64,
+                       CU_TENSOR_MAP_SWIZZLE_128B, ptr, B, T, H, D, st, rows, name);
 }
 
 // Tensor map over a [B or 1, H or 1, Tq, Tk] mask (1-byte) or score (4-byte) tensor
@@ -901,5 +907,10 @@ int host_sm_count() { return sm_count(); }
 int host_encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
                      bool bf16, const char* name) {
   return encode_bthd(m, ptr, B, T, H, D, st, rows, bf16, name);
+}
+int host_encode_bthd8(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
+                      const char* name) {
+  return encode_tokens(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, D == 64 ? 64 : 128,
+                       D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, ptr, B, T, H, D, st, rows, name);
 }
 }  // namespace fa4d

@@ -1,5 +1,6 @@
 // fa4d_cache_api.cu — the C ABI of the operators around the attention: rotary positions and
-// their serving form, attention over a shared prefix and own caches, eviction.  Argument
+// their serving form, with and without norms, attention over a shared prefix and own caches of 16
+// or 8 bits, the values of 8-bit caches, eviction.  Argument
 // checks, the division of work and dispatch; nothing is allocated here.
 #include <algorithm>
 #include <cmath>
@@ -43,6 +44,15 @@ bool rows16(const void* p, const int64_t* st, int n) {
 int check_dtype(int dtype) {
   if (dtype != FA4D_BF16 && dtype != FA4D_F16) return fail(FA4D_ERR_INVALID, "dtype %d is not bf16/f16", dtype);
   return FA4D_OK;
+}
+
+int check_cache_type(int type) {
+  if (type != FA4D_CACHE_E4M3 && type != FA4D_CACHE_INT8) return fail(FA4D_ERR_INVALID, "cache_type %d is not e4m3/int8", type);
+  return FA4D_OK;
+}
+// Rows of an 8-bit cache that 16-byte accesses can reach.
+bool codes16(const void* p, const int64_t st[3]) {
+  return aligned16(p) && st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0;
 }
 
 int check_table(const fa4d_rotary_table& t, int positions_bits) {
@@ -104,7 +114,7 @@ constexpr int64_t kDecodePrefix = 1 << 22;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights, Plan* out) {
+int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights, bool cache8, Plan* out) {
   if (B < 1 || T < 1 || Hq < 1 || Hk < 1 || C < 1 || P < 0)
     return fail(FA4D_ERR_INVALID, "sizes must be positive (B=%d T=%d Hq=%d Hk=%d C=%d P=%d)", B, T, Hq, Hk, C, P);
   if (Hq % Hk != 0) return fail(FA4D_ERR_INVALID, "query heads (%d) must be divisible by key/value heads (%d)", Hq, Hk);
@@ -120,8 +130,9 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   p.G = Hq / Hk;
   p.R = T * p.G;
   p.tiles = (p.R + 15) / 16;
+  p.unit_shift = !cache8 ? fa4d::kUnitShift : D == 64 ? fa4d::kUnit8Shift<64> : D == 256 ? fa4d::kUnit8Shift<256> : fa4d::kUnit8Shift<128>;
   const int sms = fa4d::host_sm_count();
-  if ((rows + 15) / 16 * P * Hk * D > kDecodePrefix) {
+  if (cache8 ? P > 0 : (rows + 15) / 16 * P * Hk * D > kDecodePrefix) {
     out->split_keys = D != 256 && rows <= 128;
     const int64_t row_tiles = D == 256 || out->split_keys ? (rows + 127) / 128 : (rows + 255) / 256;
     out->splits = prefix_splits(row_tiles, Hk, (P + 127) / 128, rows, D, out->split_keys, sms);
@@ -134,14 +145,14 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   }
   p.prefix_units = (P + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys;
   p.seg_rows = static_cast<int>(std::min<int64_t>(16, p.prefix_tiles ? rows : p.R));
-  out->ctas = sms * (D == 256 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
+  out->ctas = sms * (D == 256 && !cache8 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
   p.min_units = 2;
   const int64_t items = static_cast<int64_t>(p.prefix_tiles) * Hk + static_cast<int64_t>(B) * Hk * p.tiles;
   if (items > (1 << 30)) return fail(FA4D_ERR_UNSUPPORTED, "too many row tiles");
   if (!out->splits) {
     // No more CTAs than full caches could occupy.
     const int64_t line = static_cast<int64_t>(p.prefix_tiles) * Hk * (p.prefix_units + fa4d::kPrefixItemUnits) +
-                         static_cast<int64_t>(B) * Hk * p.tiles * ((C + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys + fa4d::kItemUnits);
+                         static_cast<int64_t>(B) * Hk * p.tiles * (((C - 1) >> p.unit_shift) + 1 + fa4d::kItemUnits);
     const int64_t each = p.min_units * fa4d::kDecodeWarps;
     out->ctas = static_cast<int>(std::min<int64_t>(out->ctas, (line + each - 1) / each));
   }
@@ -161,56 +172,9 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   return FA4D_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int fa4d_rotary(const fa4d_rotary_args* a, void* stream) {
-  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
-  int rc = check_table(a->table, a->positions_bits);
-  if (!rc) rc = check_dtype(a->dtype);
-  if (rc) return rc;
-  if (!a->q || !a->k || !a->q_out || !a->k_out || !a->positions)
-    return fail(FA4D_ERR_INVALID, "q, k, q_out, k_out and positions are required");
-  if (a->B < 1 || a->T < 1 || a->Hq < 1 || a->Hk < 1 || a->Hq > (1 << 20) || a->Hk > (1 << 20))
-    return fail(FA4D_ERR_INVALID, "sizes must be positive (B=%d T=%d Hq=%d Hk=%d)", a->B, a->T, a->Hq, a->Hk);
-  if (static_cast<int64_t>(a->B) * a->T > (1LL << 31)) return fail(FA4D_ERR_UNSUPPORTED, "more than 2^31 tokens");
-  if ((rc = host_bind_device_of(a->q, "q"))) return rc;
-  const bool vec = table_vec(a->table) && rows16(a->q, a->q_stride, 3) && rows16(a->k, a->k_stride, 3) &&
-                   rows16(a->q_out, a->q_out_stride, 3) && rows16(a->k_out, a->k_out_stride, 3);
-  return launched(fa4d::launch_rotary(*a, vec, fa4d::host_sm_count(), static_cast<cudaStream_t>(stream)), "rotary");
-}
-
-int fa4d_rotary_append(const fa4d_rotary_append_args* a, void* stream) {
-  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
-  int rc = check_table(a->table, a->positions_bits);
-  if (!rc) rc = check_dtype(a->dtype);
-  if (rc) return rc;
-  if (!a->q || !a->k || !a->v || !a->q_out || !a->k_cache || !a->v_cache || !a->positions || !a->lengths ||
-      !a->lengths_out)
-    return fail(FA4D_ERR_INVALID, "q, k, v, q_out, the caches, positions, lengths and lengths_out are required");
-  if (a->lengths == a->lengths_out) return fail(FA4D_ERR_INVALID, "lengths_out may not be lengths");
-  if (a->B < 1 || a->T < 1 || a->Hq < 1 || a->Hk < 1 || a->C < 1)
-    return fail(FA4D_ERR_INVALID, "sizes must be positive (B=%d T=%d Hq=%d Hk=%d C=%d)", a->B, a->T, a->Hq, a->Hk, a->C);
-  if (static_cast<int64_t>(a->B) * a->T * (a->Hq + 2LL * a->Hk) > (1LL << 31))
-    return fail(FA4D_ERR_UNSUPPORTED, "more than 2^31 rows");
-  if ((rc = host_bind_device_of(a->q, "q"))) return rc;
-  int* status = fa4d::host_status_word();
-  if (!status) return fail(FA4D_ERR_CUDA, "device status word is not available");
-  const bool vec = table_vec(a->table) && rows16(a->q, a->q_stride, 3) && rows16(a->k, a->k_stride, 3) &&
-                   rows16(a->v, a->v_stride, 3) && rows16(a->q_out, a->q_out_stride, 3) &&
-                   rows16(a->k_cache, a->k_cache_stride, 3) && rows16(a->v_cache, a->v_cache_stride, 3);
-  return launched(fa4d::launch_rotary_append(*a, vec, status, static_cast<cudaStream_t>(stream)), "rotary append");
-}
-
-size_t fa4d_prefix_attention_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C,
-                                       int32_t weights) {
-  Plan plan;
-  return plan_prefix(B, T, Hq, Hk, D, P, C, weights != 0, &plan) ? 0 : plan.total;
-}
-
-int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
-  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+// `cache8`: the own caches are in 8 bits, described there.
+int prefix_attention(const fa4d_prefix_attention_args& args, const fa4d_prefix_attention_8bit_args* cache8, void* stream) {
+  const fa4d_prefix_attention_args* a = &args;
   int rc = check_dtype(a->dtype);
   if (rc) return rc;
   if (!a->q || !a->k || !a->v || !a->o || !a->lengths) return fail(FA4D_ERR_INVALID, "q, k, v, o and lengths are required");
@@ -220,7 +184,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   if (a->causal != 0 && a->causal != 1) return fail(FA4D_ERR_INVALID, "causal must be 0 or 1");
   if ((rc = host_bind_device_of(a->q, "q"))) return rc;
   Plan plan;
-  if ((rc = plan_prefix(a->B, a->T, a->Hq, a->Hk, a->D, a->P, a->C, a->weights != nullptr, &plan))) return rc;
+  if ((rc = plan_prefix(a->B, a->T, a->Hq, a->Hk, a->D, a->P, a->C, a->weights != nullptr, cache8 != nullptr, &plan))) return rc;
   if (!a->workspace || a->workspace_bytes < plan.total)
     return fail(FA4D_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", a->workspace_bytes, plan.total);
   if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0)
@@ -236,11 +200,16 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
               {a->o, a->o_stride, 3, "o"},
               {a->prefix_k, a->prefix_k_stride, 2, "prefix_k"},
               {a->prefix_v, a->prefix_v_stride, 2, "prefix_v"}};
-  for (const auto& r : rows)
-    if (r.p && !rows16(r.p, r.st, r.n))
+  for (const auto& r : rows) {
+    const bool codes = cache8 && (r.p == a->k || r.p == a->v);
+    if (r.p && !(codes ? codes16(r.p, r.st) : rows16(r.p, r.st, r.n)))
       return fail(FA4D_ERR_LAYOUT, "%s: rows must start on 16-byte boundaries", r.name);
+  }
 
-  fa4d::DecodeParams& p = plan.p;
+  fa4d::Decode8Params p8;
+  memset(&p8, 0, sizeof(p8));
+  p8.d = plan.p;
+  fa4d::DecodeParams& p = cache8 ? p8.d : plan.p;
   char* ws = static_cast<char*>(a->workspace);
   p.q = a->q;
   p.o = a->o;
@@ -270,8 +239,12 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
   auto encode = [&](CUtensorMap* m, const void* ptr, int B, int T, const int64_t st[3], int rows, const char* name) {
     return fa4d::host_encode_bthd(m, ptr, B, T, a->Hk, a->D, st, rows, bf16, name);
   };
-  if ((rc = encode(&p.tm_k, a->k, a->B, a->C, a->k_stride, fa4d::kUnitKeys, "k"))) return rc;
-  if ((rc = encode(&p.tm_v, a->v, a->B, a->C, a->v_stride, fa4d::kUnitKeys, "v"))) return rc;
+  auto encode_own = [&](CUtensorMap* m, const void* ptr, const int64_t st[3], const char* name) {
+    return cache8 ? fa4d::host_encode_bthd8(m, ptr, a->B, a->C, a->Hk, a->D, st, 1 << p.unit_shift, name)
+                  : encode(m, ptr, a->B, a->C, st, fa4d::kUnitKeys, name);
+  };
+  if ((rc = encode_own(&p.tm_k, a->k, a->k_stride, "k"))) return rc;
+  if ((rc = encode_own(&p.tm_v, a->v, a->v_stride, "v"))) return rc;
   const int64_t ks[3] = {0, a->prefix_k_stride[0], a->prefix_k_stride[1]};
   const int64_t vs[3] = {0, a->prefix_v_stride[0], a->prefix_v_stride[1]};
   if (p.prefix_tiles) {
@@ -295,6 +268,7 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
     x.B = a->B;
     x.C = a->C;
     x.Hk = a->Hk;
+    x.unit_shift = p.unit_shift;
     x.load = p.load;
     x.shares = p.shares;
     x.scale_log2 = p.scale_log2;
@@ -304,8 +278,193 @@ int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
     if ((rc = launched(fa4d::launch_prefix(x, a->D, bf16, a->Hk, plan.splits, plan.split_keys, s), "prefix attention")))
       return rc;
   }
-  if ((rc = launched(fa4d::launch_decode(p, a->D, bf16, plan.ctas, plan.splits > 0, s), "decode attention"))) return rc;
+  if (cache8) {
+    p8.k_scale = cache8->k_scale;
+    p8.v_scale = cache8->v_scale;
+    for (int i = 0; i < 2; ++i) {
+      p8.k_scale_stride[i] = cache8->k_scale_stride[i];
+      p8.v_scale_stride[i] = cache8->v_scale_stride[i];
+    }
+    p8.q_bf16 = bf16;
+    rc = launched(fa4d::launch_decode8(p8, a->D, cache8->cache_type == FA4D_CACHE_INT8, plan.ctas, plan.splits > 0, s),
+                  "8-bit decode attention");
+  } else {
+    rc = launched(fa4d::launch_decode(p, a->D, bf16, plan.ctas, plan.splits > 0, s), "decode attention");
+  }
+  if (rc) return rc;
   return launched(fa4d::launch_join(p, a->D, bf16, fa4d::host_sm_count(), s), "attention join");
+}
+
+// The norm's arguments, where there is one.
+int check_norm(const fa4d_head_norm& n) {
+  if (!n.q_weight || !n.k_weight) return fail(FA4D_ERR_INVALID, "q_weight and k_weight are required");
+  if (n.weight_f32 != 0 && n.weight_f32 != 1) return fail(FA4D_ERR_INVALID, "weight_f32 must be 0 or 1");
+  if (!(n.eps > 0.f) || !std::isfinite(n.eps)) return fail(FA4D_ERR_INVALID, "eps must be positive");
+  return FA4D_OK;
+}
+
+int check_rotary(const fa4d_rotary_args& a) {
+  int rc = check_table(a.table, a.positions_bits);
+  if (!rc) rc = check_dtype(a.dtype);
+  if (rc) return rc;
+  if (!a.q || !a.k || !a.q_out || !a.k_out || !a.positions)
+    return fail(FA4D_ERR_INVALID, "q, k, q_out, k_out and positions are required");
+  if (a.B < 1 || a.T < 1 || a.Hq < 1 || a.Hk < 1 || a.Hq > (1 << 20) || a.Hk > (1 << 20))
+    return fail(FA4D_ERR_INVALID, "sizes must be positive (B=%d T=%d Hq=%d Hk=%d)", a.B, a.T, a.Hq, a.Hk);
+  if (static_cast<int64_t>(a.B) * a.T > (1LL << 31)) return fail(FA4D_ERR_UNSUPPORTED, "more than 2^31 tokens");
+  return FA4D_OK;
+}
+
+int check_norm_rotary(const fa4d_rotary_args& a, const fa4d_head_norm& n) {
+  int rc = check_rotary(a);
+  if (!rc) rc = check_norm(n);
+  if (rc) return rc;
+  if (a.inverse) return fail(FA4D_ERR_INVALID, "inverse does not go with a norm");
+  if (a.Hq + a.Hk > 65535) return fail(FA4D_ERR_UNSUPPORTED, "more than 65535 heads");
+  return FA4D_OK;
+}
+
+bool rotary_vec(const fa4d_rotary_args& a) {
+  return table_vec(a.table) && rows16(a.q, a.q_stride, 3) && rows16(a.k, a.k_stride, 3) &&
+         rows16(a.q_out, a.q_out_stride, 3) && rows16(a.k_out, a.k_out_stride, 3);
+}
+
+int check_append(const fa4d_rotary_append_args& a) {
+  int rc = check_table(a.table, a.positions_bits);
+  if (!rc) rc = check_dtype(a.dtype);
+  if (rc) return rc;
+  if (!a.q || !a.k || !a.v || !a.q_out || !a.k_cache || !a.v_cache || !a.positions || !a.lengths || !a.lengths_out)
+    return fail(FA4D_ERR_INVALID, "q, k, v, q_out, the caches, positions, lengths and lengths_out are required");
+  if (a.lengths == a.lengths_out) return fail(FA4D_ERR_INVALID, "lengths_out may not be lengths");
+  if (a.B < 1 || a.T < 1 || a.Hq < 1 || a.Hk < 1 || a.C < 1)
+    return fail(FA4D_ERR_INVALID, "sizes must be positive (B=%d T=%d Hq=%d Hk=%d C=%d)", a.B, a.T, a.Hq, a.Hk, a.C);
+  if (static_cast<int64_t>(a.B) * a.T * (a.Hq + 2LL * a.Hk) > (1LL << 31))
+    return fail(FA4D_ERR_UNSUPPORTED, "more than 2^31 rows");
+  return FA4D_OK;
+}
+
+bool append_vec(const fa4d_rotary_append_args& a) {
+  return table_vec(a.table) && rows16(a.q, a.q_stride, 3) && rows16(a.k, a.k_stride, 3) && rows16(a.v, a.v_stride, 3) &&
+         rows16(a.q_out, a.q_out_stride, 3);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa4d_rotary(const fa4d_rotary_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  int rc = check_rotary(*a);
+  if (rc) return rc;
+  if ((rc = host_bind_device_of(a->q, "q"))) return rc;
+  return launched(fa4d::launch_rotary(*a, rotary_vec(*a), fa4d::host_sm_count(), static_cast<cudaStream_t>(stream)), "rotary");
+}
+
+int fa4d_rotary_append(const fa4d_rotary_append_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  int rc = check_append(*a);
+  if (rc) return rc;
+  if ((rc = host_bind_device_of(a->q, "q"))) return rc;
+  int* status = fa4d::host_status_word();
+  if (!status) return fail(FA4D_ERR_CUDA, "device status word is not available");
+  const bool vec = append_vec(*a) && rows16(a->k_cache, a->k_cache_stride, 3) && rows16(a->v_cache, a->v_cache_stride, 3);
+  return launched(fa4d::launch_rotary_append(*a, vec, status, static_cast<cudaStream_t>(stream)), "rotary append");
+}
+
+int fa4d_norm_rotary(const fa4d_norm_rotary_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  int rc = check_norm_rotary(a->rotary, a->norm);
+  if (rc) return rc;
+  if ((rc = host_bind_device_of(a->rotary.q, "q"))) return rc;
+  return launched(fa4d::launch_norm_rotary(*a, rotary_vec(a->rotary), fa4d::host_sm_count(), static_cast<cudaStream_t>(stream)),
+                  "norm and rotary");
+}
+
+size_t fa4d_norm_rotary_bwd_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D) {
+  if (B < 1 || T < 1 || Hq < 1 || Hk < 1 || D < 1 || Hq > 65535 || Hk > 65535 || D > 2 * FA4D_ROTARY_MAX_PAIRS) return 0;
+  return static_cast<size_t>(fa4d::norm_bwd_rows(Hq, Hk, fa4d::host_sm_count())) * D * sizeof(float);
+}
+
+int fa4d_norm_rotary_bwd(const fa4d_norm_rotary_bwd_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  const fa4d_rotary_args& r = a->rotary;
+  int rc = check_norm_rotary(r, a->norm);
+  if (rc) return rc;
+  if (!a->dq || !a->dk || !a->q_weight_grad || !a->k_weight_grad)
+    return fail(FA4D_ERR_INVALID, "dq, dk, q_weight_grad and k_weight_grad are required");
+  if ((rc = host_bind_device_of(r.q, "q"))) return rc;
+  const size_t need = fa4d_norm_rotary_bwd_workspace(r.B, r.T, r.Hq, r.Hk, r.table.D);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(FA4D_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", a->workspace_bytes, need);
+  if (!aligned16(a->workspace)) return fail(FA4D_ERR_LAYOUT, "workspace must be 16-byte aligned");
+  const bool vec = rotary_vec(r) && rows16(a->dq, a->dq_stride, 3) && rows16(a->dk, a->dk_stride, 3);
+  return launched(fa4d::launch_norm_rotary_bwd(*a, vec, fa4d::host_sm_count(), static_cast<cudaStream_t>(stream)),
+                  "norm and rotary backward");
+}
+
+int fa4d_norm_append(const fa4d_norm_append_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  const fa4d_rotary_append_args& r = a->append;
+  int rc = check_append(r);
+  if (rc) return rc;
+  const bool cache8 = a->cache_type != FA4D_CACHE_16BIT;
+  if (cache8 && (rc = check_cache_type(a->cache_type))) return rc;
+  if ((!cache8 || a->norm.q_weight || a->norm.k_weight) && (rc = check_norm(a->norm))) return rc;
+  if (r.Hq > 65535 || r.Hk > 65535) return fail(FA4D_ERR_UNSUPPORTED, "more than 65535 heads");
+  if (cache8) {
+    if (!a->k_scale || !a->v_scale) return fail(FA4D_ERR_INVALID, "k_scale and v_scale are required");
+    if (r.weights) return fail(FA4D_ERR_UNSUPPORTED, "weights go with 16-bit caches");
+    if (r.table.D % 16) return fail(FA4D_ERR_UNSUPPORTED, "8-bit caches need a head dim that is a multiple of 16, got %d", r.table.D);
+    if (!codes16(r.k_cache, r.k_cache_stride) || !codes16(r.v_cache, r.v_cache_stride))
+      return fail(FA4D_ERR_LAYOUT, "rows of 8-bit caches must start on 16-byte boundaries");
+  }
+  if ((rc = host_bind_device_of(r.q, "q"))) return rc;
+  int* status = fa4d::host_status_word();
+  if (!status) return fail(FA4D_ERR_CUDA, "device status word is not available");
+  const bool vec = append_vec(r) && (cache8 || (rows16(r.k_cache, r.k_cache_stride, 3) && rows16(r.v_cache, r.v_cache_stride, 3)));
+  return launched(fa4d::launch_norm_append(*a, vec, fa4d::host_sm_count(), status, static_cast<cudaStream_t>(stream)),
+                  "append with norm or to an 8-bit cache");
+}
+
+int fa4d_cache_values(const fa4d_cache_values_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  int rc = check_dtype(a->dtype);
+  if (!rc) rc = check_cache_type(a->cache_type);
+  if (rc) return rc;
+  if (!a->codes || !a->scale || !a->lengths || !a->out) return fail(FA4D_ERR_INVALID, "every pointer is required");
+  if (a->B < 1 || a->C < 1 || a->Hk < 1 || a->D < 16 || a->D % 16)
+    return fail(FA4D_ERR_INVALID, "sizes must be positive, D a multiple of 16 (B=%d C=%d Hk=%d D=%d)", a->B, a->C, a->Hk, a->D);
+  if (a->B > 65535 || static_cast<int64_t>(a->C) * a->Hk > (1LL << 35) / a->D)
+    return fail(FA4D_ERR_UNSUPPORTED, "cache too large (B <= 65535, C * Hk * D <= 2^35)");
+  if (!codes16(a->codes, a->codes_stride)) return fail(FA4D_ERR_LAYOUT, "codes: rows must start on 16-byte boundaries");
+  if (!rows16(a->out, a->out_stride, 3)) return fail(FA4D_ERR_LAYOUT, "out: rows must start on 16-byte boundaries");
+  if ((rc = host_bind_device_of(a->codes, "codes"))) return rc;
+  return launched(fa4d::launch_cache_values(*a, static_cast<cudaStream_t>(stream)), "cache values");
+}
+
+size_t fa4d_prefix_attention_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C,
+                                       int32_t weights) {
+  Plan plan;
+  return plan_prefix(B, T, Hq, Hk, D, P, C, weights != 0, false, &plan) ? 0 : plan.total;
+}
+
+int fa4d_prefix_attention(const fa4d_prefix_attention_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  return prefix_attention(*a, nullptr, stream);
+}
+
+size_t fa4d_prefix_attention_8bit_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C) {
+  Plan plan;
+  return plan_prefix(B, T, Hq, Hk, D, P, C, false, true, &plan) ? 0 : plan.total;
+}
+
+int fa4d_prefix_attention_8bit(const fa4d_prefix_attention_8bit_args* a, void* stream) {
+  if (!a) return fail(FA4D_ERR_INVALID, "args is NULL");
+  const int rc = check_cache_type(a->cache_type);
+  if (rc) return rc;
+  if (a->attention.weights) return fail(FA4D_ERR_UNSUPPORTED, "weights go with 16-bit caches");
+  if (!a->k_scale || !a->v_scale) return fail(FA4D_ERR_INVALID, "k_scale and v_scale are required");
+  return prefix_attention(a->attention, a, stream);
 }
 
 int fa4d_evict(const fa4d_evict_args* a, void* stream) {

@@ -7,7 +7,7 @@
 #include "fa4d.h"
 #include "fa4d_decode.h"
 #include "fa4d_launch.cuh"
-#include "fa4d_ptx.cuh"
+#include "fa4d_line.cuh"
 
 namespace fa4d {
 
@@ -60,155 +60,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ int length_of(const DecodeParams& p, int b) { return length_at(p.lengths, b, p.C); }
-// The division of `total` units.  Beside a prefix kernel the warps of the SMs that it leaves
-// free start at once, and the others when it is done: those get less, by its estimated time.
-template <int D>
-__device__ __forceinline__ Shares shares_of(const DecodeParams& p, int64_t total, int lane) {
-  const int least = p.min_units;
-  auto up = [](int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); };
-  if (p.load.items) {
-    const RunChoice c = choose_runs<D == 96 ? 128 : D>(p.load, total, lane);
-    const int free_sms = p.load.sms - p.load.items * c.runs;
-    if (free_sms > 0) {
-      const int early = p.warps / p.load.sms * free_sms, rest = p.warps - early;
-      // When all SMs work on the own keys; the late warps' part of that.
-      const float late_us = fmaxf(c.total_us - c.prefix_us - kDecodeMicros, 0.f);
-      const float part = fminf(late_us * c.rate * rest / p.warps, static_cast<float>(total));
-      const int late = static_cast<int>(part / max(rest, 1));
-      return Shares{early, max(up(total - static_cast<int64_t>(late) * rest, early), least), late, 0};
-    }
-  }
-  return Shares{p.warps, max(up(total, p.warps), least), 0, 0};
-}
-
-__device__ __forceinline__ int64_t warp_start(const Shares& s, int64_t warp) {
-  return min(warp, static_cast<int64_t>(s.early)) * s.each + max(warp - s.early, static_cast<int64_t>(0)) * s.late;
-}
-__device__ __forceinline__ int64_t warp_of(const Shares& s, int64_t unit) {
-  const int64_t early = static_cast<int64_t>(s.early) * s.each;
-  return unit < early ? unit / s.each : s.early + (unit - early) / max(s.late, 1);
-}
-
-// The lengths of the first 128 requests in a warp's registers (lane l: l, l + 32, ...), the
-// others in memory.
-struct Lengths {
-  int n[4];
-  __device__ __forceinline__ void load(const DecodeParams& p, int lane) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) n[x] = length_of(p, min(32 * x + lane, p.B - 1));
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (32 * x + lane >= p.B) n[x] = 0;
-  }
-  __device__ __forceinline__ int of(const DecodeParams& p, int b) const {
-    if (b >= 128) return length_of(p, b);
-    return __shfl_sync(0xffffffffu, b < 64 ? (b < 32 ? n[0] : n[1]) : (b < 96 ? n[2] : n[3]), b & 31);
-  }
-  // What all requests take of the line, per KV head and row tile.
-  __device__ __forceinline__ int64_t line(const DecodeParams& p, int lane) const {
-    int64_t all = 0;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) all += line_of(n[x]);
-    for (int i = 128 + lane; i < p.B; i += 32) all += line_of(length_of(p, i));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    return all;
-  }
-};
-
-// A place on the line, in a run with `left` of it to go.
-struct Place {
-  bool prefix;
-  int b, hk, tile;  // the item (b unused in the prefix)
-  int u, units;     // unit within the item, units of the item
-  int keys;         // keys of the item
-  int64_t left;
-
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  __device__ __forceinline__ int item(const DecodeParams& p) const {
-    return prefix ? hk * p.prefix_tiles + tile : (p.prefix_tiles + b * p.tiles) * p.Hk + hk * p.tiles + tile;
-  }
-  __device__ __forceinline__ void next_item(const DecodeParams& p, const Lengths& lengths) {
-    u = 0;
-    if (++tile < (prefix ? p.prefix_tiles : p.tiles)) return;
-    tile = 0;
-    if (++hk < p.Hk) return;
-    hk = 0;
-    b = prefix ? 0 : b + 1;
-    prefix = false;
-    for (; b < p.B; ++b) {  // the next request with keys
-      keys = lengths.of(p, b);
-      units = units_of(keys);
-      if (units) return;
-    }
-    left = 0;
-  }
-  // To the next unit; true if it is of another item.
-  __device__ __forceinline__ bool advance(const DecodeParams& p, const Lengths& lengths) {
-    --left;
-    if (++u < units) return false;
-    left -= prefix ? kPrefixItemUnits : kItemUnits;
-    next_item(p, lengths);
-    return true;
-  }
-};
-
-// The first unit at or after `at` on the line, in a run of `left`.
-__device__ __forceinline__ Place find_place(const DecodeParams& p, const Lengths& lengths, int64_t at, int64_t left,
-                                            int lane) {
-  Place w;
-  w.left = left;
-  w.b = 0;
-  int64_t line = p.prefix_units + kPrefixItemUnits;
-  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * line;
-  int tiles = p.tiles;
-  w.prefix = at < prefix_all;
-  if (w.prefix) {
-    w.keys = p.P;
-    tiles = p.prefix_tiles;
-  } else {
-    at -= prefix_all;
-    const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
-    bool found = false;
-    auto search = [&](int b0, int mine) {  // among the 32 requests from b0
-      int64_t upto = line_of(mine);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t before = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += before;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, upto * each > at);
-      found = past != 0;
-      const int l = found ? __ffs(past) - 1 : 31;
-      const int64_t to = __shfl_sync(0xffffffffu, upto, l);
-      if (!found) {
-        at -= to * each;
-        return;
-      }
-      w.b = b0 + l;
-      w.keys = __shfl_sync(0xffffffffu, mine, l);
-      line = line_of(w.keys);
-      at -= (to - line) * each;
-    };
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (!found && 32 * x < p.B) search(32 * x, lengths.n[x]);
-    for (int b0 = 128; !found && b0 < p.B; b0 += 32)
-      search(b0, b0 + lane < p.B ? length_of(p, b0 + lane) : 0);
-  }
-  w.units = units_of(w.keys);
-  const int64_t item = at / line;
-  w.hk = static_cast<int>(item / tiles);
-  w.tile = static_cast<int>(item - static_cast<int64_t>(w.hk) * tiles);
-  w.u = static_cast<int>(at - item * line);
-  if (w.u >= w.units) {  // in the item's change of rows
-    w.left -= line - w.u;
-    w.next_item(p, lengths);
-  }
-  return w;
-}
-
 // One warp: its units in order, each 16 keys of K and V brought by TMA into the warp's own ring
 // (no barrier between warps), x = Q K^T and P V by m16n8k16 products with the fp32 output row
 // tile in registers.  Memory bounds it, at 16 FLOP per byte of K and V for a row tile of 16: 1208
@@ -239,7 +90,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   if (!after_prefix) pdl_wait();
   pdl_launch();
 
-  Lengths lengths;
+  Lengths<kUnitShift> lengths;
   lengths.load(p, lane);
   const int64_t total = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kPrefixItemUnits) +
                         lengths.line(p, lane) * p.Hk * p.tiles;
@@ -251,13 +102,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kDecodeCtas<D>) decode_kern
   }
   const int64_t first = warp_start(shares, warp);
   const int64_t run = min(warp_start(shares, warp + 1), total) - first;
-  Place at;
+  Place<kUnitShift> at;
   at.left = 0;
   if (run > 0) at = find_place(p, lengths, first, run, lane);
   if (at.more()) {
     uint8_t* ring = smem + wid * S::kStages * S::kStage;
     uint8_t* queries = smem + S::kQ + wid * S::kTile;  // kQShared
-    Place in = at;
+    Place<kUnitShift> in = at;
 
     // K and V of the unit at `in` into a stage.  Rows past the item's keys come along (zeros past
     // the cache's end).
@@ -558,7 +409,7 @@ struct Joined {
     keys = length_of(p, b);
     each = static_cast<int64_t>(p.Hk) * p.tiles;
     first = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kPrefixItemUnits) +
-            line_before(p.lengths, p.C, b, lane) * each;
+            line_before(p.lengths, p.C, b, lane, p.unit_shift) * each;
   }
   // Of an item of `count` units that starts at `from` on the line.
   __device__ __forceinline__ Parts of_units(int64_t from, int count, int64_t item, int row) const {
@@ -577,7 +428,7 @@ struct Joined {
   // The parts of row r: of its own keys, and of the prefix.
   __device__ __forceinline__ Parts own(int r) const {
     const int64_t i = static_cast<int64_t>(hk) * p.tiles + r / 16;
-    return of_units(first + i * line_of(keys), units_of(keys), static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
+    return of_units(first + i * line_of(keys, p.unit_shift), units_of(keys, p.unit_shift), static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
   }
   __device__ __forceinline__ Parts prefix(int r) const {
     const int64_t row = static_cast<int64_t>(b) * p.R + r;

@@ -51,6 +51,7 @@ struct DecodeParams {
   int32_t tiles;         // row tiles of a (request, KV head)
   int32_t prefix_tiles;  // row tiles of a KV head's prefix in decode_kernel; 0: not done there
   int32_t prefix_units;  // units of a prefix item
+  int32_t unit_shift;    // keys of a unit, as a power of two: kUnitShift, or as the 8-bit kernel takes them
   int32_t seg_rows;      // rows kept of a segment: min(16, R or the batch's rows)
   int32_t warps;         // warps of decode_kernel's grid
   int32_t min_units;     // least units of a warp
@@ -71,6 +72,15 @@ struct DecodeParams {
   int* status;
 };
 
+// The same over caches in 8 bits (fa4d_decode8.cu): tm_k, tm_v over bytes, no weights, no prefix items.
+struct Decode8Params {
+  DecodeParams d;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_scale_stride[2], v_scale_stride[2];
+  int32_t q_bf16;
+};
+
 // Attention of all rows of each KV head over the prefix (fa4d_prefix.cu).
 struct PrefixParams {
   CUtensorMap tm_k;  // dims (D, P, Hk, 1), box (64, 128, 1, 1), 128-B swizzle
@@ -81,6 +91,7 @@ struct PrefixParams {
   int32_t parts;          // partial results per row, at most
   const int32_t* lengths;  // of the own keys that the decode kernel reads meanwhile
   int32_t B, C, Hk;
+  int32_t unit_shift;
   PrefixLoad load;
   Shares* shares;         // `parts` written: the partial results per row, at most p.parts
   int32_t d_in;           // head dim of the tensors (96 computes at 128)
@@ -91,7 +102,11 @@ struct PrefixParams {
 };
 
 constexpr int kDecodeWarps = 4;   // warps of a decode_kernel CTA
-constexpr int kUnitKeys = 16;
+constexpr int kUnitShift = 4;     // keys of a unit of decode_kernel, as a power of two
+constexpr int kUnitKeys = 1 << kUnitShift;
+// Of decode8_kernel: K and V of 8 KB, as decode_kernel's at head dim 128.
+template <int D>
+constexpr int kUnit8Shift = D == 64 ? 6 : D == 256 ? 4 : 5;
 constexpr int kItemUnits = 2;
 // The prefix's items lie together at the front: with a short prefix the first warps do little but
 // change rows, each time with a wait as long as memory is busy (128 requests, 918 MB of own keys,
@@ -135,18 +150,19 @@ struct RunChoice {
 // Read past L1 (as is everything that a kernel of the chain reads without a wait of its own):
 // what is complete is in L2, and an SM's L1 may still hold what an earlier kernel read there.
 __device__ __forceinline__ int length_at(const int32_t* lengths, int b, int C) { return min(max(__ldcg(lengths + b), 0), C); }
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnitKeys - 1) / kUnitKeys; }
+// Units of 2^shift keys.
+__device__ __forceinline__ int units_of(int keys, int shift) { return (keys + (1 << shift) - 1) >> shift; }
 
 // What an item of so many keys takes of the line.
-__device__ __forceinline__ int line_of(int keys) { return keys > 0 ? units_of(keys) + kItemUnits : 0; }
+__device__ __forceinline__ int line_of(int keys, int shift) { return keys > 0 ? units_of(keys, shift) + kItemUnits : 0; }
 
 // What the requests before b (all of them for b = B) take of the line, per KV head and row tile.
-__device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, int b, int lane) {
+__device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, int b, int lane, int shift) {
   int64_t n = 0;
   for (int i = lane; i < b; i += 128) {  // four loads in flight
     int u[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) u[x] = line_of(length_at(lengths, min(i + 32 * x, b - 1), C));
+    for (int x = 0; x < 4; ++x) u[x] = line_of(length_at(lengths, min(i + 32 * x, b - 1), C), shift);
 #pragma unroll
     for (int x = 0; x < 4; ++x) n += i + 32 * x < b ? u[x] : 0;
   }
@@ -205,6 +221,7 @@ __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t un
 #endif
 
 cudaError_t launch_decode(const DecodeParams& p, int D, bool bf16, int ctas, bool after_prefix, cudaStream_t s);
+cudaError_t launch_decode8(const Decode8Params& p, int D, bool int8, int ctas, bool after_prefix, cudaStream_t s);
 // `split_keys`: the rows of a KV head fit one slot (at most 128), and a run's slots take even
 // and odd key tiles; two parts per run then, one otherwise.
 cudaError_t launch_prefix(const PrefixParams& p, int D, bool bf16, int Hk, int splits, bool split_keys, cudaStream_t s);

@@ -236,6 +236,11 @@ cudaError_t launch_wait_timeout_check(int* status, long long limit, cudaStream_t
 // forms, the pairs and the copied rest divide into runs of 8).
 cudaError_t launch_rotary(const fa4d_rotary_args& a, bool vec, int sms, cudaStream_t s);
 cudaError_t launch_rotary_append(const fa4d_rotary_append_args& a, bool vec, int* status, cudaStream_t s);
+cudaError_t launch_norm_rotary(const fa4d_norm_rotary_args& a, bool vec, int sms, cudaStream_t s);
+cudaError_t launch_norm_rotary_bwd(const fa4d_norm_rotary_bwd_args& a, bool vec, int sms, cudaStream_t s);
+int64_t norm_bwd_rows(int Hq, int Hk, int sms);
+cudaError_t launch_norm_append(const fa4d_norm_append_args& a, bool vec, int sms, int* status, cudaStream_t s);
+cudaError_t launch_cache_values(const fa4d_cache_values_args& a, cudaStream_t s);
 cudaError_t launch_evict(const fa4d_evict_args& a, bool vec, int sms, cudaStream_t s);
 cudaError_t launch_exp2_check(float* out, int n, float lo, float hi, cudaStream_t s);
 

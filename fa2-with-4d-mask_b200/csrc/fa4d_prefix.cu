@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   // The start, side by side: the number of runs, barriers, tensor memory, Q.
   if (warp == 0) {
     pdl_wait();
-    const int64_t units = line_before(p.lengths, p.C, p.B, lane) * p.Hk * p.load.row_tiles;
+    const int64_t units = line_before(p.lengths, p.C, p.B, lane, p.unit_shift) * p.Hk * p.load.row_tiles;
     const int r = choose_runs<D>(p.load, units, lane).runs;
     if (lane == 0) *runs_shared = r;
   } else if (warp == 1) {

@@ -2,6 +2,7 @@
 // checks, output and workspace allocation, the current stream, and the calls into libfa4d.so.
 // A decode step's kernels take a few microseconds each, so the path from Python to the launch
 // is native: bound through ctypes the same checks took 25 to 35 us a call.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -37,7 +38,8 @@ std::string cat(const Args&... args) {
 
 std::string name_of(at::ScalarType t) {
   return cat("torch.", t == at::kBFloat16 ? "bfloat16" : t == at::kHalf ? "float16" : t == at::kFloat ? "float32"
-             : t == at::kDouble ? "float64" : t == at::kInt ? "int32" : t == at::kLong ? "int64" : at::toString(t));
+             : t == at::kDouble ? "float64" : t == at::kInt ? "int32" : t == at::kLong ? "int64" : t == at::kChar ? "int8"
+             : t == at::kFloat8_e4m3fn ? "float8_e4m3fn" : at::toString(t));
 }
 
 void check(int rc, const char* what) {
@@ -109,9 +111,17 @@ Tensor new_rows(const Tensor& x) {
 // have stride 0 either.
 Tensor rows16(const Tensor& x, bool walked = false) {
   const int n = static_cast<int>(x.dim());
+  const int64_t step = 16 / static_cast<int64_t>(x.element_size());
   bool ok = x.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  for (int i = 0; i + 1 < n; ++i) ok = ok && x.stride(i) % 8 == 0 && (!walked || x.stride(i) > 0 || x.size(i) == 1);
+  for (int i = 0; i + 1 < n; ++i) ok = ok && x.stride(i) % step == 0 && (!walked || x.stride(i) > 0 || x.size(i) == 1);
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// Whether all rows of 8-bit elements start on 16-byte boundaries.
+bool whole_rows(const Tensor& x) {
+  bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int i = 0; i + 1 < x.dim(); ++i) ok = ok && (x.size(i) == 1 || x.stride(i) % 16 == 0);
+  return ok;
 }
 
 void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
@@ -198,16 +208,15 @@ void set_positions(Args& a, const Tensor& p) {
   a.positions_bits = p.scalar_type() == at::kLong ? 64 : 32;
 }
 
-std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, const Tensor& positions, const Table& table, Layout l, bool inverse) {
-  q = unit_rows(q);
-  k = unit_rows(k);
-  Tensor qo = new_rows(q), ko = new_rows(k);
-  if (q.numel() == 0 || k.numel() == 0) {
-    if (q.numel() || k.numel()) refuse("query and key need at least one head");
-    return {qo, ko};
-  }
-  const c10::cuda::OptionalCUDAGuard guard(q.device());
-  fa4d_rotary_args a;
+// Nothing to do for empty tensors of tokens.
+bool no_tokens(const Tensor& q, const Tensor& k) {
+  if (q.numel() && k.numel()) return false;
+  if (q.numel() || k.numel()) refuse("query and key need at least one head");
+  return true;
+}
+
+void set_rotary(fa4d_rotary_args& a, const Tensor& q, const Tensor& k, const Tensor& qo, const Tensor& ko,
+                const Tensor& positions, const Table& table, Layout l, bool inverse) {
   a.table = table.t;
   a.q = q.data_ptr();
   a.k = k.data_ptr();
@@ -224,6 +233,16 @@ std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, const Tensor& positions, co
   a.Hk = small(k.size(l.head()), "heads");
   a.dtype = dtype_code(q);
   a.inverse = inverse;
+}
+
+std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, const Tensor& positions, const Table& table, Layout l, bool inverse) {
+  q = unit_rows(q);
+  k = unit_rows(k);
+  Tensor qo = new_rows(q), ko = new_rows(k);
+  if (no_tokens(q, k)) return {qo, ko};
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  fa4d_rotary_args a;
+  set_rotary(a, q, k, qo, ko, positions, table, l, inverse);
   check(fa4d_rotary(&a, stream_of(q)), "fa4d_rotary");
   return {qo, ko};
 }
@@ -252,6 +271,120 @@ struct Rotate : torch::autograd::Function<Rotate> {
   }
 };
 
+// The norms' weights [D], both in the tokens' type or both fp32, and their epsilon.
+struct Norm {
+  Tensor q, k;
+  double eps = 0;
+  bool defined() const { return q.defined(); }
+};
+
+Norm norm_arg(PyObject* q, PyObject* k, PyObject* eps, const Tensor& tokens) {
+  Norm n;
+  if ((q == Py_None) != (k == Py_None)) refuse("query_norm and key_norm go together");
+  if (q == Py_None) return n;
+  n.q = tensor_arg(q, "query_norm", 1);
+  n.k = tensor_arg(k, "key_norm", 1);
+  const std::pair<const char*, const Tensor*> all[] = {{"query_norm", &n.q}, {"key_norm", &n.k}};
+  for (const auto& [name, x] : all) {
+    if (x->size(0) != tokens.size(3)) refuse(cat(name, " must have ", tokens.size(3), " elements, got ", x->size(0)));
+    if ((x->scalar_type() != tokens.scalar_type() && x->scalar_type() != at::kFloat) || x->scalar_type() != n.q.scalar_type())
+      refuse("query_norm and key_norm must both be fp32 or both have the dtype of query");
+    if (x->device() != tokens.device()) refuse(cat(name, " must be on ", tokens.device(), ", got ", x->device()));
+  }
+  n.eps = PyFloat_AsDouble(eps);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse("eps must be a number");
+  }
+  if (!(static_cast<float>(n.eps) > 0.f) || !std::isfinite(static_cast<float>(n.eps))) refuse("eps must be positive");
+  return n;
+}
+
+// `q` and `k` are contiguous weights, which live as long as the call.
+void set_norm(fa4d_head_norm& a, const Tensor& q, const Tensor& k, double eps) {
+  a.q_weight = q.data_ptr();
+  a.k_weight = k.data_ptr();
+  a.weight_f32 = q.scalar_type() == at::kFloat;
+  a.eps = static_cast<float>(eps);
+}
+
+using Capsule = c10::intrusive_ptr<torch::CustomClassHolder>;
+
+std::pair<Tensor, Tensor> norm_rotate(Tensor q, Tensor k, const Tensor& wq, const Tensor& wk, const Tensor& positions,
+                                      const Table& table, Layout l, double eps) {
+  q = unit_rows(q);
+  k = unit_rows(k);
+  Tensor qo = new_rows(q), ko = new_rows(k);
+  if (no_tokens(q, k)) return {qo, ko};
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  const Tensor cq = wq.contiguous(), ck = wk.contiguous();
+  fa4d_norm_rotary_args a;
+  set_rotary(a.rotary, q, k, qo, ko, positions, table, l, false);
+  set_norm(a.norm, cq, ck, eps);
+  check(fa4d_norm_rotary(&a, stream_of(q)), "fa4d_norm_rotary");
+  return {qo, ko};
+}
+
+// The gradient of NormRotate, which has none of its own.
+struct NormRotateGrad : torch::autograd::Function<NormRotateGrad> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, Tensor dq, Tensor dk, Tensor q, Tensor k,
+                                                const Tensor& wq, const Tensor& wk, const Tensor& positions, Capsule table,
+                                                bool bhsd, double eps) {
+    const Layout l{bhsd};
+    const c10::cuda::OptionalCUDAGuard guard(q.device());
+    q = unit_rows(q);
+    k = unit_rows(k);
+    dq = unit_rows(dq);
+    dk = unit_rows(dk);
+    Tensor dxq = new_rows(q), dxk = new_rows(k);
+    if (no_tokens(q, k)) return {dxq, dxk, at::zeros_like(wq), at::zeros_like(wk)};
+    const Tensor cq = wq.contiguous(), ck = wk.contiguous();
+    Tensor dwq = at::empty_like(cq), dwk = at::empty_like(ck);
+    fa4d_norm_rotary_bwd_args a;
+    set_rotary(a.rotary, q, k, dxq, dxk, positions, static_cast<const Table&>(*table), l, false);
+    set_norm(a.norm, cq, ck, eps);
+    a.dq = dq.data_ptr();
+    a.dk = dk.data_ptr();
+    set3(a.dq_stride, dq, l);
+    set3(a.dk_stride, dk, l);
+    a.q_weight_grad = dwq.data_ptr();
+    a.k_weight_grad = dwk.data_ptr();
+    const fa4d_rotary_args& r = a.rotary;
+    a.workspace_bytes = fa4d_norm_rotary_bwd_workspace(r.B, r.T, r.Hq, r.Hk, r.table.D);
+    const Tensor workspace = at::empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+    check(fa4d_norm_rotary_bwd(&a, stream_of(q)), "fa4d_norm_rotary_bwd");
+    return {dxq, dxk, dwq, dwk};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "MultiAxisRotary with norms cannot be differentiated twice");
+  }
+};
+
+struct NormRotate : torch::autograd::Function<NormRotate> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const Tensor& wq, const Tensor& wk, const Tensor& positions, Capsule table,
+                                                bool bhsd, double eps) {
+    ctx->save_for_backward({q, k, wq, wk, positions});
+    ctx->saved_data["table"] = c10::IValue::make_capsule(table);
+    ctx->saved_data["bhsd"] = bhsd;
+    ctx->saved_data["eps"] = eps;
+    auto out = norm_rotate(q, k, wq, wk, positions, static_cast<const Table&>(*table), Layout{bhsd}, eps);
+    return {out.first, out.second};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    auto table = ctx->saved_data["table"].toCapsule();
+    try {
+      auto out = NormRotateGrad::apply(g[0], g[1], saved[0], saved[1], saved[2], saved[3], saved[4], table,
+                                       ctx->saved_data["bhsd"].toBool(), ctx->saved_data["eps"].toDouble());
+      return {out[0], out[1], out[2], out[3], Tensor(), Tensor(), Tensor(), Tensor()};
+    } catch (const Refused& e) {  // the engine's thread only knows torch's errors
+      TORCH_CHECK(false, e.text);
+    }
+  }
+};
+
 PyObject* pair_of(const Tensor& a, const Tensor& b) {
   PyObject* out = PyTuple_New(2);
   if (!out) return nullptr;
@@ -261,6 +394,44 @@ PyObject* pair_of(const Tensor& a, const Tensor& b) {
 }
 
 // ------------------------------------------------------------------ caches
+
+void check_slots(int64_t C, const Tensor& lengths, int64_t B, const Tensor& like) {
+  if (C < 1) refuse("the cache has no slots");
+  if (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B || lengths.device() != like.device() ||
+      !lengths.is_contiguous())
+    refuse(cat("lengths must be a contiguous int32 tensor of shape [", B, "] on ", like.device()));
+}
+
+bool code_type(const Tensor& x) { return x.scalar_type() == at::kFloat8_e4m3fn || x.scalar_type() == at::kChar; }
+int cache_code(const Tensor& x) { return x.scalar_type() == at::kChar ? FA4D_CACHE_INT8 : FA4D_CACHE_E4M3; }
+
+// The scales of an 8-bit cache of C slots.
+void check_scale(const char* name, const Tensor& s, int64_t B, int64_t Hk, int64_t C, const Tensor& like) {
+  const int64_t blocks = (C + FA4D_CACHE_BLOCK - 1) / FA4D_CACHE_BLOCK;
+  if (s.scalar_type() != at::kFloat || s.dim() != 3 || s.size(0) != B || s.size(1) != Hk || s.size(2) != blocks ||
+      s.device() != like.device() || (blocks > 1 && s.stride(2) != 1))
+    refuse(cat(name, " must be an fp32 tensor of shape [", B, ", ", Hk, ", ", blocks, "] (a scale for each ", FA4D_CACHE_BLOCK,
+               " slots) with unit block stride on ", like.device()));
+}
+
+// A batch's cache in 8 bits; returns its slots.
+int64_t check_cache8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& lengths, Layout l,
+                     int64_t B, int64_t Hk, int64_t D, const Tensor& like) {
+  const std::pair<const char*, const Tensor*> all[] = {{"key cache", &k}, {"value cache", &v}};
+  for (const auto& [name, x] : all) {
+    if (!code_type(*x) || x->scalar_type() != k.scalar_type() || x->device() != like.device())
+      refuse(cat(name, " must be float8_e4m3fn or int8, as the other, on ", like.device(), ", got ", name_of(x->scalar_type()),
+                 " on ", x->device()));
+    if (x->size(0) != B || x->size(l.head()) != Hk || x->size(3) != D || x->size(l.seq()) != k.size(l.seq()))
+      refuse(cat(name, " has shape ", x->sizes(), ", expected batch ", B, ", ", Hk, " heads of ", D,
+                 " and the same slots for keys and values"));
+  }
+  const int64_t C = k.size(l.seq());
+  check_slots(C, lengths, B, like);
+  check_scale("key_scale", ks, B, Hk, C, like);
+  check_scale("value_scale", vs, B, Hk, C, like);
+  return C;
+}
 
 // A batch's cache; returns its slots.
 int64_t check_cache(const Tensor& k, const Tensor& v, const Tensor& lengths, const Tensor& weights, Layout l, int64_t B,
@@ -274,10 +445,7 @@ int64_t check_cache(const Tensor& k, const Tensor& v, const Tensor& lengths, con
                  " and the same slots for keys and values"));
   }
   const int64_t C = k.size(l.seq());
-  if (C < 1) refuse("the cache has no slots");
-  if (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B || lengths.device() != like.device() ||
-      !lengths.is_contiguous())
-    refuse(cat("lengths must be a contiguous int32 tensor of shape [", B, "] on ", like.device()));
+  check_slots(C, lengths, B, like);
   if (weights.defined() &&
       (weights.scalar_type() != at::kFloat || weights.dim() != 3 || weights.size(0) != B || weights.size(1) != Hk ||
        weights.size(2) != C || weights.device() != like.device() || weights.stride(2) != 1))
@@ -290,6 +458,7 @@ void set_weights(int64_t (&out)[2], const Tensor& w) {
   out[1] = w.defined() ? w.stride(1) : 0;
 }
 
+const char* kScales = "key_scale and value_scale must be fp32 tensors";
 const char* kWeights = "weights must be an fp32 tensor";
 const char* kLengths = "lengths must be a contiguous int32 tensor";
 
@@ -356,22 +525,37 @@ PyObject* rotary(PyObject* const* args) {
   return pair_of(out.first, out.second);
 }
 
-// rotary_append(table, query, key, value, positions, key_cache, value_cache, lengths, weights,
-// layout) -> (query, lengths)
-PyObject* rotary_append(PyObject* const* args) {
+// Of both forms below: the arguments before `layout` are the same, those of norms and 8-bit caches
+// are None in the first.
+PyObject* append(PyObject* const* args, PyObject* layout, PyObject* query_norm, PyObject* key_norm, PyObject* eps,
+                 PyObject* key_scale, PyObject* value_scale) {
   Table* table = table_arg(args[0]);
-  const Layout l = layout_arg(args[9]);
+  const Layout l = layout_arg(layout);
   Tensor q = tensor_arg(args[1], "query", 4), k = tensor_arg(args[2], "key", 4), v = tensor_arg(args[3], "value", 4);
   check_tokens(q, k, v, l, table->t.D);
   const int64_t B = q.size(0), T = q.size(l.seq()), Hq = q.size(l.head()), Hk = k.size(l.head());
   const Tensor positions = check_positions(args[4], *table, B, T, q);
   const Tensor kc = tensor_arg(args[5], "key cache", 4), vc = tensor_arg(args[6], "value cache", 4);
   const Tensor lengths = any_tensor(args[7], kLengths), weights = optional_arg(args[8], kWeights);
-  const int64_t C = check_cache(kc, vc, lengths, weights, l, B, Hk, table->t.D, q);
-  no_gradient("append", {&q, &k, &v, &kc, &vc, &weights});
+  const Norm norm = norm_arg(query_norm, key_norm, eps, q);
+  if ((key_scale == Py_None) != (value_scale == Py_None)) refuse("key_scale and value_scale go together");
+  const Tensor ks = optional_arg(key_scale, kScales), vs = optional_arg(value_scale, kScales);
+  const bool cache8 = ks.defined();
+  if (cache8 && weights.defined()) refuse("weights go with 16-bit caches");
+  if (cache8 && table->t.D % 16) refuse(cat("8-bit caches need a head dim that is a multiple of 16, got ", table->t.D));
+  const int64_t C = cache8 ? check_cache8(kc, vc, ks, vs, lengths, l, B, Hk, table->t.D, q)
+                           : check_cache(kc, vc, lengths, weights, l, B, Hk, table->t.D, q);
+  no_gradient("append", {&q, &k, &v, &kc, &vc, &weights, &norm.q, &norm.k, &ks, &vs});
   if (kc.stride(3) != 1 || vc.stride(3) != 1) refuse("the caches are written in place and need unit head-dim stride");
   if (repeats(kc) || repeats(vc) || (weights.defined() && repeats(weights)))
     refuse("the caches and weights are written in place and may not repeat memory");
+  if (cache8) {
+    if (repeats(ks) || repeats(vs)) refuse("the scales are written in place and may not repeat memory");
+    if (kc.numel() && (kc.data_ptr() == vc.data_ptr() || ks.data_ptr() == vs.data_ptr()))
+      refuse("keys and values need caches and scales of their own");
+    for (const Tensor* x : {&kc, &vc})
+      if (!whole_rows(*x)) refuse("rows of 8-bit caches are written in place and must start on 16-byte boundaries");
+  }
   need_cuda("MultiAxisRotary", q);
   q = unit_rows(q);
   k = unit_rows(k);
@@ -380,7 +564,9 @@ PyObject* rotary_append(PyObject* const* args) {
   if (B == 0 || T == 0) return pair_of(qo, lengths.clone());
   Tensor lengths_out = at::empty_like(lengths);
   const c10::cuda::OptionalCUDAGuard guard(q.device());
-  fa4d_rotary_append_args a;
+  fa4d_norm_append_args n;
+  memset(&n, 0, sizeof(n));
+  fa4d_rotary_append_args& a = n.append;
   a.table = table->t;
   a.q = q.data_ptr();
   a.k = k.data_ptr();
@@ -405,15 +591,60 @@ PyObject* rotary_append(PyObject* const* args) {
   a.Hk = small(Hk, "heads");
   a.C = small(C, "cache");
   a.dtype = dtype_code(q);
-  check(fa4d_rotary_append(&a, stream_of(q)), "fa4d_rotary_append");
-  written({&kc, &vc, &weights});
+  if (!cache8 && !norm.defined()) {
+    check(fa4d_rotary_append(&a, stream_of(q)), "fa4d_rotary_append");
+  } else {
+    const Tensor wq = norm.defined() ? norm.q.contiguous() : Tensor(), wk = norm.defined() ? norm.k.contiguous() : Tensor();
+    if (norm.defined()) set_norm(n.norm, wq, wk, norm.eps);
+    if (cache8) {
+      n.cache_type = cache_code(kc);
+      for (int i = 0; i < 3; ++i) {  // a dimension of one is not stepped over
+        const int dim = i == 0 ? 0 : i == 1 ? l.seq() : l.head();
+        if (kc.size(dim) == 1) a.k_cache_stride[i] = 0;
+        if (vc.size(dim) == 1) a.v_cache_stride[i] = 0;
+      }
+      n.k_scale = ks.data_ptr<float>();
+      n.v_scale = vs.data_ptr<float>();
+      set_weights(n.k_scale_stride, ks);
+      set_weights(n.v_scale_stride, vs);
+    }
+    check(fa4d_norm_append(&n, stream_of(q)), "fa4d_norm_append");
+  }
+  written({&kc, &vc, &weights, &ks, &vs});
   return pair_of(qo, lengths_out);
 }
 
-// shared_prefix_attention(query, prefix_key, prefix_value, key, value, lengths, mask, weights,
-// scale, is_causal, layout) -> out
-PyObject* shared_prefix_attention(PyObject* const* args) {
-  const Layout l = layout_arg(args[10]);
+// norm_rotary(table, query, key, positions, query_norm, key_norm, eps, layout) -> (query, key)
+PyObject* norm_rotary(PyObject* const* args) {
+  Table* table = table_arg(args[0]);
+  const Layout l = layout_arg(args[7]);
+  const Tensor q = tensor_arg(args[1], "query", 4), k = tensor_arg(args[2], "key", 4);
+  check_tokens(q, k, Tensor(), l, table->t.D);
+  const Tensor positions = check_positions(args[3], *table, q.size(0), q.size(l.seq()), q);
+  const Norm n = norm_arg(args[4], args[5], args[6], q);
+  if (!n.defined()) refuse("query_norm and key_norm are required");
+  no_tangent("MultiAxisRotary", {&q, &k, &n.q, &n.k});
+  need_cuda("MultiAxisRotary", q);
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || n.q.requires_grad() || n.k.requires_grad())) {
+    auto holder = Capsule(c10::intrusive_ptr<Table>::unsafe_reclaim_from_nonowning(table));
+    auto out = NormRotate::apply(q, k, n.q, n.k, positions, holder, l.bhsd, n.eps);
+    return pair_of(out[0], out[1]);
+  }
+  auto out = norm_rotate(q, k, n.q, n.k, positions, *table, l, n.eps);
+  return pair_of(out.first, out.second);
+}
+
+// rotary_append(table, query, key, value, positions, key_cache, value_cache, lengths, weights,
+// layout) -> (query, lengths)
+PyObject* rotary_append(PyObject* const* args) { return append(args, args[9], Py_None, Py_None, Py_None, Py_None, Py_None); }
+
+// norm_append(table, query, key, value, positions, key_cache, value_cache, lengths, weights,
+// query_norm, key_norm, eps, key_scale, value_scale, layout) -> (query, lengths)
+PyObject* norm_append(PyObject* const* args) { return append(args, args[14], args[9], args[10], args[11], args[12], args[13]); }
+
+// Of both forms below; the scales of 8-bit caches are None in the first.
+PyObject* attend(PyObject* const* args, PyObject* layout, PyObject* key_scale, PyObject* value_scale) {
+  const Layout l = layout_arg(layout);
   Tensor q = tensor_arg(args[0], "query", 4);
   if (!half_type(q)) refuse(cat("query must be fp16 or bf16, got ", name_of(q.scalar_type())));
   Tensor k = tensor_arg(args[3], "key cache", 4), v = tensor_arg(args[4], "value cache", 4);
@@ -421,7 +652,11 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   if (Hk == 0 || Hq % Hk != 0) refuse(cat("query heads (", Hq, ") must be divisible by key/value heads (", Hk, ")"));
   if (D != 64 && D != 96 && D != 128 && D != 256) refuse(cat("head dim ", D, " is not built (64, 96, 128, 256)"));
   const Tensor lengths = any_tensor(args[5], kLengths), weights = optional_arg(args[7], kWeights);
-  const int64_t C = check_cache(k, v, lengths, weights, l, B, Hk, D, q);
+  if ((key_scale == Py_None) != (value_scale == Py_None)) refuse("key_scale and value_scale go together");
+  const Tensor ks = optional_arg(key_scale, kScales), vs = optional_arg(value_scale, kScales);
+  const bool cache8 = ks.defined();
+  if (cache8 && weights.defined()) refuse("weights go with 16-bit caches");
+  const int64_t C = cache8 ? check_cache8(k, v, ks, vs, lengths, l, B, Hk, D, q) : check_cache(k, v, lengths, weights, l, B, Hk, D, q);
   if (weights.defined() && repeats(weights)) refuse("weights are written in place and may not repeat memory");
   if ((args[1] == Py_None) != (args[2] == Py_None)) refuse("prefix_key and prefix_value go together");
   Tensor pk, pv;
@@ -458,7 +693,7 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   }
   if (!std::isfinite(scale)) refuse("scale must be finite");
   const int causal = PyObject_IsTrue(args[9]);
-  no_gradient("shared_prefix_attention", {&q, &pk, &pv, &k, &v, &weights});
+  no_gradient("shared_prefix_attention", {&q, &pk, &pv, &k, &v, &weights, &ks, &vs});
   need_cuda("shared_prefix_attention", q);
 
   const c10::cuda::OptionalCUDAGuard guard(q.device());
@@ -467,8 +702,9 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   if (out.numel() == 0) return THPVariable_Wrap(out);
   k = rows16(k, true);  // keys and values go through tensor maps
   v = rows16(v, true);
-  fa4d_prefix_attention_args a;
-  memset(&a, 0, sizeof(a));
+  fa4d_prefix_attention_8bit_args a8;
+  memset(&a8, 0, sizeof(a8));
+  fa4d_prefix_attention_args& a = a8.attention;
   if (P) {
     pk = rows16(pk, true);
     pv = rows16(pv, true);
@@ -507,12 +743,67 @@ PyObject* shared_prefix_attention(PyObject* const* args) {
   a.dtype = dtype_code(q);
   a.causal = causal;
   a.scale = static_cast<float>(scale);
-  a.workspace_bytes = fa4d_prefix_attention_workspace(a.B, a.T, a.Hq, a.Hk, a.D, a.P, a.C, weights.defined());
+  a.workspace_bytes = cache8 ? fa4d_prefix_attention_8bit_workspace(a.B, a.T, a.Hq, a.Hk, a.D, a.P, a.C)
+                             : fa4d_prefix_attention_workspace(a.B, a.T, a.Hq, a.Hk, a.D, a.P, a.C, weights.defined());
   if (!a.workspace_bytes) check(FA4D_ERR_INVALID, "fa4d_prefix_attention");
   const Tensor workspace = at::empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
   a.workspace = workspace.data_ptr();
-  check(fa4d_prefix_attention(&a, stream_of(q)), "fa4d_prefix_attention");
+  if (cache8) {
+    a8.cache_type = cache_code(k);
+    a8.k_scale = ks.data_ptr<float>();
+    a8.v_scale = vs.data_ptr<float>();
+    set_weights(a8.k_scale_stride, ks);
+    set_weights(a8.v_scale_stride, vs);
+    check(fa4d_prefix_attention_8bit(&a8, stream_of(q)), "fa4d_prefix_attention_8bit");
+  } else {
+    check(fa4d_prefix_attention(&a, stream_of(q)), "fa4d_prefix_attention");
+  }
   written({&weights});
+  return THPVariable_Wrap(out);
+}
+
+// shared_prefix_attention(query, prefix_key, prefix_value, key, value, lengths, mask, weights,
+// scale, is_causal, layout) -> out
+PyObject* shared_prefix_attention(PyObject* const* args) { return attend(args, args[10], Py_None, Py_None); }
+
+// shared_prefix_attention_8bit(query, prefix_key, prefix_value, key, value, lengths, mask, weights,
+// scale, is_causal, key_scale, value_scale, layout) -> out
+PyObject* shared_prefix_attention_8bit(PyObject* const* args) { return attend(args, args[12], args[10], args[11]); }
+
+// cache_values(cache, scale, lengths, dtype, layout) -> values
+PyObject* cache_values(PyObject* const* args) {
+  const Layout l = layout_arg(args[4]);
+  Tensor x = tensor_arg(args[0], "cache", 4);
+  if (!code_type(x)) refuse(cat("cache must be float8_e4m3fn or int8, got ", name_of(x.scalar_type())));
+  const Tensor scale = any_tensor(args[1], "scale must be an fp32 tensor"), lengths = any_tensor(args[2], kLengths);
+  const at::ScalarType type = THPDtype_Check(args[3]) ? reinterpret_cast<THPDtype*>(args[3])->scalar_type : at::kFloat;
+  if (type != at::kBFloat16 && type != at::kHalf) refuse("dtype must be torch.bfloat16 or torch.float16");
+  const int64_t B = x.size(0), Hk = x.size(l.head()), D = x.size(3), C = x.size(l.seq());
+  if (Hk == 0 || D == 0 || D % 16) refuse(cat("the cache needs at least one head, of a multiple of 16 elements, got ", D));
+  check_slots(C, lengths, B, x);
+  check_scale("scale", scale, B, Hk, C, x);
+  no_gradient("cache_values", {&x, &scale});
+  need_cuda("cache_values", x);
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const Tensor out = at::empty(x.sizes(), x.options().dtype(type));
+  if (B == 0) return THPVariable_Wrap(out);
+  x = rows16(x);
+  fa4d_cache_values_args a;
+  memset(&a, 0, sizeof(a));
+  a.codes = x.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  a.lengths = lengths.data_ptr<int32_t>();
+  a.out = out.data_ptr();
+  set3(a.codes_stride, x, l);
+  set_weights(a.scale_stride, scale);
+  set3(a.out_stride, out, l);
+  a.B = small(B, "batch");
+  a.C = small(C, "cache");
+  a.Hk = small(Hk, "heads");
+  a.D = small(D, "head dim");
+  a.dtype = dtype_code(out);
+  a.cache_type = cache_code(x);
+  check(fa4d_cache_values(&a, stream_of(x)), "fa4d_cache_values");
   return THPVariable_Wrap(out);
 }
 
@@ -691,7 +982,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {FA4D_ENTRY(make_table, 5),      FA4D_ENTRY(table_turns, 1),
                           FA4D_ENTRY(rotary, 5),
                           FA4D_ENTRY(rotary_append, 10),  FA4D_ENTRY(shared_prefix_attention, 11),
-                          FA4D_ENTRY(evict_by_weight, 9), {nullptr, nullptr, 0, nullptr}};
+                          FA4D_ENTRY(evict_by_weight, 9), FA4D_ENTRY(norm_rotary, 8),
+                          FA4D_ENTRY(norm_append, 15),    FA4D_ENTRY(shared_prefix_attention_8bit, 13),
+                          FA4D_ENTRY(cache_values, 5),    {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fa4d_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -3,8 +3,9 @@
 ``MultiAxisRotary`` turns pairs of a head's elements by angles that grow with the token's
 position; each pair follows one of several position axes (time, height and width of a
 video's patches, say), ``sections`` giving the number of pairs of each axis in order.  Text
-has the same position on every axis.  Calling it is differentiable; ``append`` is the
-serving form, which also stores the turned keys and the values in a cache.
+has the same position on every axis.  Each head can be normalised first, in the same pass.
+Calling it is differentiable; ``append`` is the serving form, which also stores the turned keys
+and the values in a cache of 16 or 8 bits.
 """
 
 from __future__ import annotations
@@ -68,20 +69,29 @@ class MultiAxisRotary:
         self._make_table()
 
     def __call__(self, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, *,
+                 query_norm: Optional[torch.Tensor] = None, key_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
                  layout: Layout = "bhsd") -> tuple:
-        """Turned (query, key), differentiable in both.
+        """Turned (query, key), differentiable in both, and in the norms' weights.
 
         Args:
             query/key: fp16/bf16 ``[B, H, T, D]`` ("bhsd") or ``[B, T, H, D]`` ("bshd"), any
                 strides; their head counts may differ.
             positions: integer ``[axes, B or 1, T]`` (int32 and int64 are read as they are).
+            query_norm/key_norm: weights ``[D]``, both fp32 or both in the tokens' dtype: each head x
+                becomes ``x * (mean(x**2) + eps) ** -0.5 * weight`` (in 32 bits, squares included)
+                before it is turned.  Gradients have no gradients of their own then.
         """
-        return self._host.rotary(self._table, query, key, positions, layout)
+        if query_norm is None and key_norm is None:
+            return self._host.rotary(self._table, query, key, positions, layout)
+        return self._host.norm_rotary(self._table, query, key, positions, query_norm, key_norm, eps, layout)
 
     def append(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
                key_cache: torch.Tensor, value_cache: torch.Tensor, lengths: torch.Tensor, *,
-               weights: Optional[torch.Tensor] = None, layout: Layout = "bhsd") -> tuple:
-        """Turns the new tokens' query and key and stores key and value in the caches.
+               weights: Optional[torch.Tensor] = None, query_norm: Optional[torch.Tensor] = None,
+               key_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, key_scale: Optional[torch.Tensor] = None,
+               value_scale: Optional[torch.Tensor] = None, layout: Layout = "bhsd") -> tuple:
+        """Turns the new tokens' query and key (normalised first, as in a call, where ``query_norm``
+        and ``key_norm`` are given) and stores key and value in the caches.
 
         Args:
             query/key/value: the T new tokens, as for a call (value has the key's heads).
@@ -91,13 +101,24 @@ class MultiAxisRotary:
             lengths: int32 ``[B]`` entries of each cache so far.
             weights: optional fp32 ``[B, Hk, C]`` attention weights of the cache entries, set
                 to 0 at the new slots.
+            key_scale/value_scale: of caches held in 8 bits (``torch.float8_e4m3fn`` or ``torch.int8``
+                codes, head dim a multiple of 16, rows on 16-byte boundaries, no ``weights``): fp32
+                ``[B, Hk, ceil(C / 64)]``, a scale for each 64 slots of a request and head,
+                updated in place.  A value is its code times its block's scale.  Scales written here
+                are powers of two: the least, 2**-126 or more, under which no value of the block
+                passes the largest code (448 or 127).  Where new tokens raise a block's scale, its
+                earlier codes are rounded anew; it does not sink until its first slot is written
+                again.  An infinity or NaN makes its block's scale NaN, and so the whole block.
 
         Returns:
             (turned query, new lengths).  Tokens past the capacity C are not stored: the new
             length stays at C and ``DEV_CACHE_FULL`` is set in ``device_status()``.
         """
-        return self._host.rotary_append(self._table, query, key, value, positions, key_cache, value_cache, lengths,
-                                        weights, layout)
+        if query_norm is None and key_norm is None and key_scale is None and value_scale is None:
+            return self._host.rotary_append(self._table, query, key, value, positions, key_cache, value_cache, lengths,
+                                            weights, layout)
+        return self._host.norm_append(self._table, query, key, value, positions, key_cache, value_cache, lengths, weights,
+                                      query_norm, key_norm, eps, key_scale, value_scale, layout)
 
 
 __all__ = ["MultiAxisRotary"]

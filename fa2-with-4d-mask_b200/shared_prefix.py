@@ -30,6 +30,8 @@ def shared_prefix_attention(
     weights: Optional[torch.Tensor] = None,
     scale: Optional[float] = None,
     is_causal: bool = True,
+    key_scale: Optional[torch.Tensor] = None,
+    value_scale: Optional[torch.Tensor] = None,
     layout: Layout = "bhsd",
 ) -> torch.Tensor:
     """Softmax attention of T new tokens per request over the shared prefix and the request's
@@ -48,6 +50,9 @@ def shared_prefix_attention(
             holds the own keys' logits, ``4 * B * Hq * T * C`` bytes by the caches' capacity C.
         scale: softmax scale, ``head_dim ** -0.5`` by default.
         is_causal: new token t sees the own entries up to its own, ``lengths - T + t``.
+        key_scale/value_scale: of own caches held in 8 bits, as ``MultiAxisRotary.append`` writes them
+            (codes ``torch.float8_e4m3fn`` or ``torch.int8``, fp32 scales ``[B, Hk, ceil(C / 64)]``,
+            any of them); the prefix stays in 16 bits, and there are no ``weights``.
 
     Returns:
         The output in the query's layout; rows that see no key are 0.  A row that sees a NaN, or
@@ -57,8 +62,37 @@ def shared_prefix_attention(
     Rows that are not on 16-byte boundaries are copied first.  There is no gradient, in either
     mode; ``weights`` is written as by an in-place operation.
     """
-    return _lib.host().shared_prefix_attention(query, prefix_key, prefix_value, key, value, lengths, mask, weights, scale,
-                                               is_causal, layout)
+    if key_scale is None and value_scale is None:
+        return _lib.host().shared_prefix_attention(query, prefix_key, prefix_value, key, value, lengths, mask, weights, scale,
+                                                   is_causal, layout)
+    return _lib.host().shared_prefix_attention_8bit(query, prefix_key, prefix_value, key, value, lengths, mask, weights, scale,
+                                                    is_causal, key_scale, value_scale, layout)
+
+
+def cache_values(
+    cache: torch.Tensor,
+    scale: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    dtype: torch.dtype = torch.bfloat16,
+    layout: Layout = "bhsd",
+) -> torch.Tensor:
+    """The values of a cache held in 8 bits, in 16: for what takes 16-bit caches (a request's cache
+    becomes a shared prefix, or is evicted from).
+
+    Args:
+        cache: codes, ``torch.float8_e4m3fn`` or ``torch.int8``, ``[B, Hk, C, D]`` ("bhsd") or
+            ``[B, C, Hk, D]`` ("bshd"), D a multiple of 16.
+        scale: fp32 ``[B, Hk, ceil(C / 64)]``.
+        lengths: int32 ``[B]`` entries of the cache.
+        dtype: ``torch.bfloat16``, which holds the values of caches written by
+            ``MultiAxisRotary.append`` exactly (magnitudes that a code rounds to 2**128 become
+            infinite), or ``torch.float16``.
+
+    Returns:
+        A new contiguous tensor of the cache's shape, 0 from a request's length on.
+    """
+    return _lib.host().cache_values(cache, scale, lengths, dtype, layout)
 
 
 def evict_by_weight(
@@ -95,4 +129,4 @@ def evict_by_weight(
     return _lib.host().evict_by_weight(key, value, weights, lengths, keep, sinks, recent, out, layout)
 
 
-__all__ = ["shared_prefix_attention", "evict_by_weight"]
+__all__ = ["shared_prefix_attention", "cache_values", "evict_by_weight"]

@@ -392,6 +392,98 @@ typedef struct fa4d_evict_args {
 } fa4d_evict_args;
 int fa4d_evict(const fa4d_evict_args* args, void* stream);
 
+/* ------------------------------------------------------------------ norms and 8-bit caches
+ * Models that normalise each head's query and key before the turn, and caches held in 8 bits. */
+
+/* The norm of a head x[D]: x (mean x^2 + eps)^-1/2 weight, computed in fp32. */
+typedef struct fa4d_head_norm {
+  const void* q_weight;      /* [D], unit stride */
+  const void* k_weight;
+  int32_t weight_f32;        /* 1: the weights are fp32; 0: they have the tokens' dtype */
+  float eps;                 /* positive */
+} fa4d_head_norm;
+
+typedef struct fa4d_norm_rotary_args {
+  fa4d_rotary_args rotary;   /* inverse must be 0 */
+  fa4d_head_norm norm;
+} fa4d_norm_rotary_args;
+
+/* q_out, k_out = q and k normalised, then turned, rounded once. */
+int fa4d_norm_rotary(const fa4d_norm_rotary_args* args, void* stream);
+
+/* The gradient: rotary.q, rotary.k are the forward's inputs, rotary.q_out, rotary.k_out are
+ * written with their gradients. */
+typedef struct fa4d_norm_rotary_bwd_args {
+  fa4d_rotary_args rotary;   /* inverse must be 0 */
+  fa4d_head_norm norm;
+  const void* dq;            /* [B, T, Hq, D] gradient of the forward's q_out */
+  const void* dk;            /* [B, T, Hk, D] */
+  int64_t dq_stride[3];      /* element strides (batch, seq, head), head-dim stride 1 */
+  int64_t dk_stride[3];
+  void* q_weight_grad;       /* [D] in the weights' type, written */
+  void* k_weight_grad;
+  void* workspace;           /* >= fa4d_norm_rotary_bwd_workspace() bytes, 16-B aligned */
+  size_t workspace_bytes;
+} fa4d_norm_rotary_bwd_args;
+
+/* Bytes of scratch (the weights' gradients of parts of the rows) for these sizes on the current
+ * device; 0 for invalid sizes. */
+size_t fa4d_norm_rotary_bwd_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D);
+int fa4d_norm_rotary_bwd(const fa4d_norm_rotary_bwd_args* args, void* stream);
+
+/* A cache in 8 bits: codes [B, C, Hk, D] (e4m3, or int8 from -127 to 127) and an fp32 scale for each
+ * block of FA4D_CACHE_BLOCK slots (from slot 0) of a request and head, [B, Hk, ceil(C / block)]; a
+ * value is its code times its scale. */
+#define FA4D_CACHE_BLOCK 64
+enum fa4d_cache_type { FA4D_CACHE_16BIT = 0, FA4D_CACHE_E4M3 = 1, FA4D_CACHE_INT8 = 2 };
+
+/* fa4d_rotary_append with a norm before the turn (norm.q_weight and norm.k_weight NULL: none), into
+ * caches of cache_type.  In a block of an 8-bit cache that holds no entry below lengths[b], the new
+ * tokens get the least scale 2^e, e >= -126, under which none of their values passes the largest
+ * code (448 or 127); in one that does, the larger of that and the block's scale, and where the scale
+ * grows the earlier codes are rounded anew.  An element that is not finite makes the scale of its
+ * block NaN until tokens enter the block anew.  Values are rounded to codes once, from fp32.
+ * 16-bit caches come with a norm (without: fa4d_rotary_append). */
+typedef struct fa4d_norm_append_args {
+  fa4d_rotary_append_args append; /* weights: must be NULL with an 8-bit cache */
+  fa4d_head_norm norm;
+  int32_t cache_type;        /* enum fa4d_cache_type */
+  float* k_scale;            /* 8-bit caches: [B, Hk, blocks], updated; NULL otherwise */
+  float* v_scale;
+  int64_t k_scale_stride[2]; /* (batch, head), block stride 1 */
+  int64_t v_scale_stride[2];
+} fa4d_norm_append_args;
+int fa4d_norm_append(const fa4d_norm_append_args* args, void* stream);
+
+/* out = the values of a cache in 16 bits, 0 from slot lengths[b] (clamped to [0, C]) on. */
+typedef struct fa4d_cache_values_args {
+  const void* codes;         /* [B, C, Hk, D] */
+  const float* scale;        /* [B, Hk, blocks] */
+  const int32_t* lengths;    /* [B] */
+  void* out;                 /* [B, C, Hk, D] 16-bit, written */
+  int64_t codes_stride[3];   /* element strides (batch, slot, head), head-dim stride 1 */
+  int64_t scale_stride[2];   /* (batch, head), block stride 1 */
+  int64_t out_stride[3];
+  int32_t B, C, Hk, D;
+  int32_t dtype;             /* of out */
+  int32_t cache_type;        /* FA4D_CACHE_E4M3 or FA4D_CACHE_INT8 */
+} fa4d_cache_values_args;
+int fa4d_cache_values(const fa4d_cache_values_args* args, void* stream);
+
+/* fa4d_prefix_attention over own caches in 8 bits (attention.k, attention.v: codes; the prefix stays
+ * in 16).  attention.weights must be NULL.  Codes that no token of a request may see can hold
+ * anything. */
+typedef struct fa4d_prefix_attention_8bit_args {
+  fa4d_prefix_attention_args attention;
+  int32_t cache_type;        /* FA4D_CACHE_E4M3 or FA4D_CACHE_INT8 */
+  const float* k_scale;      /* [B, Hk, blocks] */
+  const float* v_scale;
+  int64_t k_scale_stride[2]; /* (batch, head), block stride 1 */
+  int64_t v_scale_stride[2];
+} fa4d_prefix_attention_8bit_args;
+size_t fa4d_prefix_attention_8bit_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t P, int32_t C);
+int fa4d_prefix_attention_8bit(const fa4d_prefix_attention_8bit_args* args, void* stream);
+
 /* Message for the last non-zero return on this thread ("" if none). */
 const char* fa4d_last_error(void);
 

@@ -40,6 +40,7 @@ tilelang_attention_forward = _impl.tilelang_attention_forward
 tilelang_flash_attention = _impl.tilelang_flash_attention
 MultiAxisRotary = _impl.MultiAxisRotary
 shared_prefix_attention = _impl.shared_prefix_attention
+cache_values = _impl.cache_values
 evict_by_weight = _impl.evict_by_weight
 device_status = _impl.device_status
 DEV_CACHE_FULL = _impl.DEV_CACHE_FULL
@@ -50,6 +51,7 @@ __all__ = [
     "tilelang_flash_attention",
     "MultiAxisRotary",
     "shared_prefix_attention",
+    "cache_values",
     "evict_by_weight",
     "device_status",
     "DEV_CACHE_FULL",
