@@ -87,8 +87,9 @@ int bind_device_of(const void* ptr, const char* name) {
 
 // Tensor map over a [B, T, H, D] tensor of `esize`-byte elements given element strides (b, t, h):
 // dims (D, T, H, B), box (box, rows, 1, 1), zero fill out of bounds.
-int encode_tokens(CUtensorMap* m, CUtensorMapDataType type, int esize, int box0, CUtensorMapSwizzle swizzle, const void* ptr,
-                  int B, int T, int H, int D, const int64_t st[3], int rows, const char* name) {
+int encode_tokens(CUtensorMap* m, CUtensorMapDataType type, int esize, int box0, CUtensorMapSwizzle swizzle,
+                  CUtensorMapL2promotion promotion, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
+                  const char* name) {
   auto enc = tensor_map_encoder();
   if (!enc) return fail(FA4D_ERR_DRIVER, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   if (!aligned(ptr, 16)) return fail(FA4D_ERR_LAYOUT, "%s: base address is not 16-byte aligned", name);
@@ -110,7 +111,7 @@ int encode_tokens(CUtensorMap* m, CUtensorMapDataType type, int esize, int box0,
   cuuint32_t box[4] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, type, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FA4D_ERR_DRIVER, "%s: cuTensorMapEncodeTiled failed (%d)", name, int(r));
   return FA4D_OK;
 }
@@ -119,7 +120,7 @@ int encode_tokens(CUtensorMap* m, CUtensorMapDataType type, int esize, int box0,
 int encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
                 bool bf16, const char* name) {
   return encode_tokens(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, 64,
-                       CU_TENSOR_MAP_SWIZZLE_128B, ptr, B, T, H, D, st, rows, name);
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, ptr, B, T, H, D, st, rows, name);
 }
 
 // Tensor map over a [B or 1, H or 1, Tq, Tk] mask (1-byte) or score (4-byte) tensor
@@ -910,7 +911,14 @@ int host_encode_bthd(CUtensorMap* m, const void* ptr, int B, int T, int H, int D
 }
 int host_encode_bthd8(CUtensorMap* m, const void* ptr, int B, int T, int H, int D, const int64_t st[3], int rows,
                       const char* name) {
+  // Rows that lie apart (heads beside one another) are 64 to 256 bytes long: what L2 brings beyond them
+  // belongs to other heads, and is gone before it is asked for.
+  const bool apart = st[1] != D;
+  const auto promotion = !apart || D == 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                         : D == 128         ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                            : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
   return encode_tokens(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, D == 64 ? 64 : 128,
-                       D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, ptr, B, T, H, D, st, rows, name);
+                       D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, promotion, ptr, B, T, H, D, st, rows,
+                       name);
 }
 }  // namespace fa4d

@@ -36,7 +36,8 @@ __device__ __forceinline__ void settle_length(const fa4d_rotary_append_args& a, 
 
 // q's rows: a group of tokens and a range of heads.
 template <bool kBF16, bool kAdj, int VEC>
-__device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, const AppendGrid& g, int id) {
+__device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, const Turns<VEC>& turns, const Weights<VEC>& shared_w,
+                                         const AppendGrid& g, int id) {
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1);
   const int64_t n = static_cast<int64_t>(id % g.groups) * kRows + threadIdx.x / g.lanes;
@@ -44,11 +45,9 @@ __device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, cons
   const bool live = n < static_cast<int64_t>(a.B) * a.T;
   const int64_t b = n / a.T, t = n - b * a.T;
   const RowLane<VEC, kAdj> at(a.table, lane, g.chunks);
-  Pairs<VEC> w;
-  if (args.norm.q_weight) at.template vector<kBF16>(args.norm.q_weight, args.norm.weight_f32 != 0, w);
   const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1];
   uint16_t* dst = static_cast<uint16_t*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1];
-  norm_heads<kBF16, kAdj, VEC, 4>(a.table, at, args.norm.q_weight ? &w : nullptr, args.norm.eps, g.lanes, lane, live, src,
+  norm_heads<kBF16, kAdj, VEC, 4>(a.table, turns, at, args.norm.q_weight ? &shared_w : nullptr, args.norm.eps, g.lanes, lane, live, src,
                                   a.q_stride[2], dst, a.q_out_stride[2], first, min(first + g.q_each, a.Hq), a.positions,
                                   a.positions_bits, a.positions_stride, b, t);
 }
@@ -58,10 +57,17 @@ __device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, cons
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                           const __grid_constant__ AppendGrid g, int* status) {
+  __shared__ Turns<VEC> turns;
+  turns.template fill<kAdj>(args.append.table);
+  __syncthreads();
   pdl_wait();
   pdl_launch();
+  __shared__ Weights<VEC> shared_w;
   int id = blockIdx.x;
-  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, g, id - g.cache_blocks);
+  shared_w.template fill<kBF16, kAdj>(args.append.table, id >= g.cache_blocks ? args.norm.q_weight : args.norm.k_weight,
+                                      args.norm.weight_f32 != 0);
+  __syncthreads();
+  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, turns, shared_w, g, id - g.cache_blocks);
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1);
   const bool is_v = id >= g.cache_blocks / 2;
@@ -86,11 +92,9 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
       }
     return;
   }
-  Pairs<VEC> w;
-  at.template vector<kBF16>(args.norm.k_weight, args.norm.weight_f32 != 0, w);
   const uint16_t* src = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1];
   uint16_t* dst = static_cast<uint16_t*>(a.k_cache) + b * a.k_cache_stride[0] + slot * a.k_cache_stride[1];
-  norm_heads<kBF16, kAdj, VEC, 4>(a.table, at, &w, args.norm.eps, g.lanes, lane, live, src, a.k_stride[2], dst,
+  norm_heads<kBF16, kAdj, VEC, 4>(a.table, turns, at, &shared_w, args.norm.eps, g.lanes, lane, live, src, a.k_stride[2], dst,
                                   a.k_cache_stride[2], first, end, a.positions, a.positions_bits, a.positions_stride, b, t);
 }
 
@@ -103,10 +107,19 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
   constexpr int P = kRowPairs<VEC>;
   extern __shared__ float values[];  // [pass][2 P][threads]
   __shared__ uint32_t block_most;
+  __shared__ Turns<VEC> turns;
+  if (threadIdx.x == 0) block_most = 0;
+  turns.template fill<kAdj>(args.append.table);
+  __syncthreads();
   pdl_wait();
   pdl_launch();
+  __shared__ Weights<VEC> shared_w;
   int64_t id = blockIdx.x;
-  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, g, static_cast<int>(id - g.cache_blocks));
+  if (args.norm.q_weight)
+    shared_w.template fill<kBF16, kAdj>(args.append.table, id >= g.cache_blocks ? args.norm.q_weight : args.norm.k_weight,
+                                        args.norm.weight_f32 != 0);
+  __syncthreads();
+  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, turns, shared_w, g, static_cast<int>(id - g.cache_blocks));
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1), row = threadIdx.x / g.lanes, threads = blockDim.x;
   const bool is_v = id & 1;
@@ -120,8 +133,6 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
   const int64_t block = had / FA4D_CACHE_BLOCK + span, start = block * FA4D_CACHE_BLOCK;
   const int64_t from = max(had, start), to = min(min(had + a.T, static_cast<int64_t>(a.C)), start + FA4D_CACHE_BLOCK);
   if (from >= to) return;
-  if (threadIdx.x == 0) block_most = 0;
-  __syncthreads();
 
   const int64_t* ss = is_v ? args.v_scale_stride : args.k_scale_stride;
   float* scale_at = (is_v ? args.v_scale : args.k_scale) + b * ss[0] + h * ss[1] + block;
@@ -132,8 +143,6 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
   const uint16_t* x = static_cast<const uint16_t*>(is_v ? a.v : a.k) + b * xs[0] + h * xs[2];
   const RowLane<VEC, kAdj> at(a.table, lane, g.chunks);
   const bool norm = !is_v && args.norm.k_weight;
-  Pairs<VEC> w;
-  if (norm) at.template vector<kBF16>(args.norm.k_weight, args.norm.weight_f32 != 0, w);
   uint32_t most = 0;
   const int count = static_cast<int>(to - from);
 #pragma unroll 1
@@ -144,25 +153,26 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
     if (live) at.load(x + t * xs[1], raw);
     Pairs<VEC> p;
     unpack_pairs<kBF16, kAdj>(raw, p);
-    float cs[P], sn[P];
-    if (!is_v && live) at.angles(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, lane, cs, sn);
-    if (norm) {
-      const float r = rsqrtf(row_sum(p.squares(), g.lanes) * (1.f / a.table.D) + args.norm.eps);
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        p.a[j] = p.a[j] * r * w.a[j];
-        p.b[j] = p.b[j] * r * w.b[j];
-      }
-    }
+    if (norm) p.times(rsqrtf(row_sum(p.squares(), g.lanes) * (1.f / a.table.D) + args.norm.eps));
     if (!live) continue;
-    if (!is_v) at.turn(p, cs, sn, 1.f);
+    if (!is_v) {
+      Turn<VEC> turn;
+      at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
+      Pairs<VEC> w;
+      if (norm) at.weights(shared_w, lane, w);
+      Factors<VEC> factors;
+      factors.set(turn, norm ? &w : nullptr);
+      factors.turn(p, at.copied());
+    }
     float* v = values + i0 / kRows * (2 * P) * threads + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       // Dead chunks hold zeros.
-      most = max(most, max(__float_as_uint(p.a[j]) & 0x7fffffffu, __float_as_uint(p.b[j]) & 0x7fffffffu));
-      v[j * threads] = p.a[j];
-      v[(P + j) * threads] = p.b[j];
+      const float2 u = f2_split(p.a[j / 2]), z = f2_split(p.b[j / 2]);
+      const float x0 = j & 1 ? u.y : u.x, x1 = j & 1 ? z.y : z.x;
+      most = max(most, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu));
+      v[j * threads] = x0;
+      v[(P + j) * threads] = x1;
     }
   }
   most = __reduce_max_sync(0xffffffffu, most);

@@ -156,6 +156,8 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
     const int64_t each = p.min_units * fa4d::kDecodeWarps;
     out->ctas = static_cast<int>(std::min<int64_t>(out->ctas, (line + each - 1) / each));
   }
+  p.heads = 1;
+  p.groups = Hk;
   p.warps = out->ctas * fa4d::kDecodeWarps;
   p.logits_ld = (C + 3) / 4 * 4;
   const size_t seg = (static_cast<size_t>(items) + p.warps) * p.seg_rows;
@@ -243,6 +245,13 @@ int prefix_attention(const fa4d_prefix_attention_args& args, const fa4d_prefix_a
     return cache8 ? fa4d::host_encode_bthd8(m, ptr, a->B, a->C, a->Hk, a->D, st, 1 << p.unit_shift, name)
                   : encode(m, ptr, a->B, a->C, st, fa4d::kUnitKeys, name);
   };
+  // Codes of a slot's heads lie beside one another, 64 to 256 bytes each: the warps of a CTA take
+  // neighbouring heads of the same slots, whose bytes memory then reads together.
+  if (cache8 && a->k_stride[1] != a->D) {
+    p.heads = a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
+    p.groups /= p.heads;
+    p.warps /= p.heads;
+  }
   if ((rc = encode_own(&p.tm_k, a->k, a->k_stride, "k"))) return rc;
   if ((rc = encode_own(&p.tm_v, a->v, a->v_stride, "v"))) return rc;
   const int64_t ks[3] = {0, a->prefix_k_stride[0], a->prefix_k_stride[1]};

@@ -407,17 +407,17 @@ struct Joined {
   // Before the partial results are there: what the lengths tell.
   __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane) : p(params), b(b_), hk(hk_) {
     keys = length_of(p, b);
-    each = static_cast<int64_t>(p.Hk) * p.tiles;
-    first = static_cast<int64_t>(p.prefix_tiles) * p.Hk * (p.prefix_units + kPrefixItemUnits) +
+    each = static_cast<int64_t>(p.groups) * p.tiles;
+    first = static_cast<int64_t>(p.prefix_tiles) * p.groups * (p.prefix_units + kPrefixItemUnits) +
             line_before(p.lengths, p.C, b, lane, p.unit_shift) * each;
   }
   // Of an item of `count` units that starts at `from` on the line.
   __device__ __forceinline__ Parts of_units(int64_t from, int count, int64_t item, int row) const {
-    Parts x{p.seg_o, p.seg_ml, 0, p.seg_rows, 0};
+    Parts x{p.seg_o, p.seg_ml, 0, static_cast<int64_t>(p.heads) * p.seg_rows, 0};
     if (count > 0) {
       const int64_t w0 = warp_of(shares, from);
       x.n = static_cast<int>(warp_of(shares, from + count - 1) - w0 + 1);
-      x.first = (w0 + item) * p.seg_rows + row;
+      x.first = ((w0 + item) * p.heads + hk % p.heads) * p.seg_rows + row;
     }
     return x;
   }
@@ -427,8 +427,8 @@ struct Joined {
   }
   // The parts of row r: of its own keys, and of the prefix.
   __device__ __forceinline__ Parts own(int r) const {
-    const int64_t i = static_cast<int64_t>(hk) * p.tiles + r / 16;
-    return of_units(first + i * line_of(keys, p.unit_shift), units_of(keys, p.unit_shift), static_cast<int64_t>(p.prefix_tiles) * p.Hk + b * each + i, r % 16);
+    const int64_t i = static_cast<int64_t>(hk / p.heads) * p.tiles + r / 16;
+    return of_units(first + i * line_of(keys, p.unit_shift), units_of(keys, p.unit_shift), static_cast<int64_t>(p.prefix_tiles) * p.groups + b * each + i, r % 16);
   }
   __device__ __forceinline__ Parts prefix(int r) const {
     const int64_t row = static_cast<int64_t>(b) * p.R + r;

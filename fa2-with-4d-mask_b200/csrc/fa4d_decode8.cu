@@ -21,7 +21,7 @@ namespace {
 
 constexpr float kNegInf = -INFINITY;
 
-template <int D>
+template <int D, int kCols>
 struct Shape8 {
   static constexpr int kShift = kUnit8Shift<D>;
   static constexpr int kKeys = 1 << kShift;          // of a unit: 8 KB of K and V
@@ -31,8 +31,12 @@ struct Shape8 {
   static constexpr int kBox = kKeys * kRow;
   static constexpr int kTile = kBoxes * kBox;        // K or V of a unit
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = 3;
-  static constexpr int kBars = kDecodeWarps * kStages * kStage;
+  // With 16 rows of head dim 256 the queries stay in shared memory: in registers (64, beside 128 of
+  // output) they spilled.
+  static constexpr bool kQShared = D == 256 && kCols == 2;
+  static constexpr int kStages = kQShared ? 2 : 3;
+  static constexpr int kQ = kDecodeWarps * kStages * kStage;  // [warp][column tile][step][lane] 8 bytes
+  static constexpr int kBars = kQ + (kQShared ? kDecodeWarps * kCols * kWide * 16 : 0);
   static constexpr int kBytes = kBars + kDecodeWarps * kStages * 8 + 8 + 1024;  // aligned to 1024
   static constexpr int kKeyTiles = kKeys / 16;       // 16-key tiles of a unit
   static constexpr int kSteps = kWide / 64;          // 64 columns: four steps of the product with Q
@@ -47,25 +51,18 @@ struct Shape8 {
 // together find their chunks in different banks; what is done with the keys does not depend on it.
 __device__ __forceinline__ int key_of(int i) { return (i & 1) * 4 + (i >> 1); }
 
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-  return v;
-}
+// Plain loads and unordered products: the compiler interleaves them.
+__device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 lds8(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
 // An 8 x 8 matrix of 16-bit elements transposed, two elements of a row a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 // c (16 x 8, fp32) += a (16 x 16) b (16 x 8), fp16
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -78,14 +75,15 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 template <int D, bool kInt8, int kCols, bool kMask>
 __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __grid_constant__ Decode8Params p8,
                                                                        bool after_prefix) {
-  using S = Shape8<D>;
+  using S = Shape8<D, kCols>;
   constexpr int kShift = S::kShift;
   const DecodeParams& p = p8.d;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int g = lane >> 2, q4 = lane & 3;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kDecodeWarps + wid;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kDecodeWarps / p.heads) + wid / p.heads;
+  const int sub = wid % p.heads;  // of the heads that its neighbours take along
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars) + wid * S::kStages;
   int* abort_flag = reinterpret_cast<int*>(smem + S::kBars + kDecodeWarps * S::kStages * 8);
   if (lane < S::kStages) mbar_init(&full[lane], 1);
@@ -102,9 +100,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
 
   Lengths<kShift> lengths;
   lengths.load(p, lane);
-  const int64_t total = lengths.line(p, lane) * p.Hk * p.tiles;
+  const int64_t total = lengths.line(p, lane) * p.groups * p.tiles;
   const Shares shares = shares_of<D>(p, total, lane);
-  if (warp == 0 && lane == 0) {
+  if (warp == 0 && sub == 0 && lane == 0) {
     p.shares->early = shares.early;
     p.shares->each = shares.each;
     p.shares->late = shares.late;
@@ -127,15 +125,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
         uint8_t* dst = ring + brought % S::kStages * S::kStage;
 #pragma unroll
         for (int c = 0; c < S::kBoxes; ++c) {
-          tma_load_4d(dst + c * S::kBox, &p.tm_k, bar, c * S::kRow, in.u << kShift, in.hk, in.b);
-          tma_load_4d(dst + S::kTile + c * S::kBox, &p.tm_v, bar, c * S::kRow, in.u << kShift, in.hk, in.b);
+          tma_load_4d(dst + c * S::kBox, &p.tm_k, bar, c * S::kRow, in.u << kShift, in.hk * p.heads + sub, in.b);
+          tma_load_4d(dst + S::kTile + c * S::kBox, &p.tm_v, bar, c * S::kRow, in.u << kShift, in.hk * p.heads + sub, in.b);
         }
       }
       ++brought;
       in.advance(p, lengths);
     };
 
-    uint32_t qf[kCols][S::kSteps][8];
+    uint32_t qf[kCols][S::kQShared ? 1 : S::kSteps][8];
+    uint8_t* queries = smem + S::kQ + wid * kCols * S::kWide * 16 + lane * 8;  // kQShared
     float acc[S::kOutTiles][kCols][4];
     // Of columns 2 q4 and 2 q4 + 1 of each tile of 8 query rows:
     float qs[kCols][2];      // scale log2(e), and what the row was divided by for fp16
@@ -150,15 +149,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
     const float* vs;
 
     auto begin_item = [&]() {
+      const int hk = at.hk * p.heads + sub;
       seen = 0;
       whole = kMask ? 0 : p.causal ? at.keys - p.T + 1 : at.keys;
-      ks = p8.k_scale + at.b * p8.k_scale_stride[0] + at.hk * p8.k_scale_stride[1];
-      vs = p8.v_scale + at.b * p8.v_scale_stride[0] + at.hk * p8.v_scale_stride[1];
+      ks = p8.k_scale + at.b * p8.k_scale_stride[0] + hk * p8.k_scale_stride[1];
+      vs = p8.v_scale + at.b * p8.v_scale_stride[0] + hk * p8.v_scale_stride[1];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         const int r = at.tile * 16 + 8 * c + g;
         const bool valid = r < p.R;
-        const int t = r / p.G, h = at.hk * p.G + r % p.G;
+        const int t = r / p.G, h = hk * p.G + r % p.G;
         const uint16_t* row = static_cast<const uint16_t*>(p.q) + at.b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2];
         // Each lane 16 elements of every 64, the columns of the codes that it reads.
         uint4 raw[S::kSteps][2];
@@ -190,16 +190,21 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
 #pragma unroll
         for (int j = 0; j < S::kSteps; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 8; i += 2) {
             const float2 v = value(reinterpret_cast<const uint32_t*>(raw[j])[i]);
-            qf[c][j][i] = pack2<false>(v.x * f0 * f1, v.y * f0 * f1);
+            const float2 u = value(reinterpret_cast<const uint32_t*>(raw[j])[i + 1]);
+            const uint2 h = make_uint2(pack2<false>(v.x * f0 * f1, v.y * f0 * f1), pack2<false>(u.x * f0 * f1, u.y * f0 * f1));
+            if constexpr (S::kQShared)
+              *reinterpret_cast<uint2*>(queries + ((c * S::kSteps + j) * 4 + i / 2) * 256) = h;  // read by this lane alone
+            else
+              qf[c][j][i] = h.x, qf[c][j][i + 1] = h.y;
           }
         const float back = 1.f / f0 / f1;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           qs[c][x] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * q4 + 4 * x);
           const int rx = at.tile * 16 + 8 * c + 2 * q4 + x;
-          const int tx = rx / p.G, hx = at.hk * p.G + rx % p.G;
+          const int tx = rx / p.G, hx = hk * p.G + rx % p.G;
           lim[c][x] = rx >= p.R ? 0 : p.causal ? at.keys - p.T + tx + 1 : at.keys;
           if (kMask)
             mrow[c][x] = rx >= p.R ? nullptr
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
     };
 
     auto end_item = [&]() {
-      const int64_t seg = warp + at.item(p);
+      const int64_t seg = (warp + at.item(p)) * p.heads + sub;
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, o);
 #pragma unroll
@@ -250,12 +255,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
         }
     };
 
-    // Mask bits of a unit: bit (tile * kCols + column tile) * 4 + e for element e of that tile's
-    // logits in this lane.  They are loaded a unit ahead.
-    auto mask_bits = [&](int u) {
-      uint32_t bits = 0xffffffffu;
+    // The mask's bytes of this lane's logits of a unit, loaded a unit ahead and looked at then.
+    constexpr int kMaskBytes = kMask ? S::kKeyTiles * kCols * 4 : 1;
+    uint8_t mask_now[kMaskBytes], mask_next[kMaskBytes];
+    auto load_mask = [&](int u) {
       if constexpr (kMask) {
-        uint8_t v[S::kKeyTiles * kCols * 4];
 #pragma unroll
         for (int i = 0; i < S::kKeyTiles; ++i)
 #pragma unroll
@@ -263,26 +267,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = min((u << kShift) + 16 * i + 8 * (e >> 1) + key_of(g), at.keys - 1);
-              v[(i * kCols + c) * 4 + e] = mrow[c][e & 1] ? __ldcg(mrow[c][e & 1] + j) : 0;
+              mask_next[(i * kCols + c) * 4 + e] = mrow[c][e & 1] ? __ldcg(mrow[c][e & 1] + j) : 0;
             }
-        bits = 0;
-#pragma unroll
-        for (int i = 0; i < S::kKeyTiles * kCols * 4; ++i) bits |= (v[i] != 0 ? 1u : 0u) << i;
       }
-      return bits;
     };
+    auto keep_now = [&](int i, int c, int e) { return mask_now[kMask ? (i * kCols + c) * 4 + e : 0] != 0; };
     // Scales of a unit, loaded a unit ahead too.
     auto scales = [&](int u) {
       const int i = (u << kShift) / FA4D_CACHE_BLOCK;
       return make_float2(__ldcg(ks + i), __ldcg(vs + i));
     };
 
-    uint32_t keep_next = 0;
     float2 scale_next;
 #pragma unroll 1
     for (int i = 0; i < S::kStages - 1; ++i) bring_next();
     begin_item();
-    keep_next = mask_bits(at.u);
+    load_mask(at.u);
     scale_next = scales(at.u);
 #pragma unroll 1
     for (int it = 0; at.more(); ++it) {
@@ -292,13 +292,15 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
         break;
       }
       bring_next();  // into the stage of the unit before this one
-      const uint32_t keep_bits = keep_next;
+#pragma unroll
+      for (int i = 0; i < kMaskBytes; ++i) mask_now[i] = mask_next[i];
       const float2 scale = scale_next;
       if (at.u + 1 < at.units) {
-        keep_next = mask_bits(at.u + 1);
+        load_mask(at.u + 1);
         scale_next = scales(at.u + 1);
       }
-      const uint32_t sk = smem_u32(ring) + (it % S::kStages) * S::kStage, sv = sk + S::kTile;
+      const uint8_t* sk = ring + (it % S::kStages) * S::kStage;
+      const uint8_t* sv = sk + S::kTile;
 
       float x[S::kKeyTiles][kCols][4];
 #pragma unroll
@@ -318,25 +320,21 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
             codes_to_half2<kInt8>(wl[k], a0, a2);
             codes_to_half2<kInt8>(wh[k], a1, a3);
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) mma16(x[i][c], a0, a1, a2, a3, qf[c][j][2 * k], qf[c][j][2 * k + 1]);
+            for (int c = 0; c < kCols; ++c) {
+              uint2 q;
+              if constexpr (S::kQShared)
+                q = lds8(queries + ((c * S::kSteps + j) * 4 + k) * 256);
+              else
+                q = make_uint2(qf[c][j][2 * k], qf[c][j][2 * k + 1]);
+              mma16(x[i][c], a0, a1, a2, a3, q.x, q.y);
+            }
           }
         }
       }
 
-      // Scaled to log2 units; -inf where the row does not see the key.
+      // -inf where the row does not see the key.
       const int key0 = at.u << kShift;
       const bool all_seen = key0 + S::kKeys <= whole;
-      float f[kCols][2];
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) f[c][e] = qs[c][e] * scale.x;
-#pragma unroll
-      for (int i = 0; i < S::kKeyTiles; ++i)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][c][e] *= f[c][e & 1];
       if (all_seen) {
         seen = 0xffffffffu;
       } else {
@@ -348,7 +346,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int kj = 16 * i + 8 * (e >> 1) + key_of(g);
-              const bool keep = key0 + kj < lim[c][e & 1] && (!kMask || ((keep_bits >> ((i * kCols + c) * 4 + e)) & 1u));
+              const bool keep = key0 + kj < lim[c][e & 1] && (!kMask || keep_now(i, c, e));
               if (keep) {
                 live |= 1ull << kj;
                 seen |= 1u << (2 * c + (e & 1));
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
             for (int id = lane; id < S::kKeys * kChunks; id += 32) {
               const int row = id / kChunks, ch = id - row * kChunks;
               if (!(((row < 32 ? lo : hi) >> (row & 31)) & 1u))
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + S::at(row, ch)), "r"(0) : "memory");
+                *reinterpret_cast<uint4*>(const_cast<uint8_t*>(sv) + S::at(row, ch)) = make_uint4(0, 0, 0, 0);
             }
             fence_async_smem();  // before a copy into the stage
             __syncwarp();
@@ -377,8 +375,38 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
       }
 
       // Running maxima; sums and outputs are rescaled only where one grew.
-      const float zl = __log2f(scale.y);
-      float ol[kCols][2], oo[kCols][2], w_of[kCols][2];
+      float zl = __log2f(scale.y);
+      float f[kCols][2];  // to log2 units
+      bool odd = zl != zl;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          f[c][e] = qs[c][e] * scale.x;
+          odd = odd || !(f[c][e] > 0.f);
+        }
+      if (odd) {
+        // A factor below 0 goes to the logits, and one of 0, which -inf would make NaN; NaN, of it or of
+        // the scale of the values, reaches the sums of the rows that see one of the keys.
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& u = f[c][e];
+#pragma unroll
+            for (int i = 0; i < S::kKeyTiles; ++i)
+#pragma unroll
+              for (int h = 0; h < 4; h += 2) {
+                float& y = x[i][c][e + h];
+                if (y == kNegInf) continue;
+                if (u != u || zl != zl) l[c][e] = NAN;
+                y = u != u ? kNegInf : u < 0.f ? -y : u == 0.f ? 0.f : y;
+              }
+            u = u < 0.f ? -u : u > 0.f ? u : 1.f;
+          }
+        if (zl != zl) zl = kNegInf;
+      }
+      float ol[kCols][2], oo[kCols][2], w_of[kCols][2], sub[kCols][2];
       bool grew = false;
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
@@ -390,15 +418,16 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx *= f[c][e];
           const float m_new = fmaxf(m[c][e], mx), n_new = fmaxf(n[c][e], mx + zl);
           ol[c][e] = m[c][e] == m_new ? 1.f : ex2(m[c][e] - m_new);
           oo[c][e] = n[c][e] == n_new ? 1.f : ex2(n[c][e] - n_new);
           grew = grew || ol[c][e] != 1.f || oo[c][e] != 1.f;
           m[c][e] = m_new;
           n[c][e] = n_new;
+          sub[c][e] = m_new == kNegInf ? 0.f : m_new;
           // From a probability under m to a weight under n.  Past 2^126 the probability is 0.
-          const float up = (m_new == kNegInf ? 0.f : m_new) + zl - (n_new == kNegInf ? 0.f : n_new);
-          w_of[c][e] = ex2(up > 126.f ? 126.f : up);
+          w_of[c][e] = ex2(fminf(sub[c][e] + zl - (n_new == kNegInf ? 0.f : n_new), 126.f));
         }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -416,21 +445,17 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
       }
       uint32_t pf[S::kKeyTiles][kCols][2];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const float s0 = m[c][0] == kNegInf ? 0.f : m[c][0], s1 = m[c][1] == kNegInf ? 0.f : m[c][1];
+      for (int c = 0; c < kCols; ++c)
 #pragma unroll
         for (int i = 0; i < S::kKeyTiles; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float x0 = x[i][c][2 * h], x1 = x[i][c][2 * h + 1];
-            const float p0 = ex2(x0 - s0), p1 = ex2(x1 - s1);
+            const float p0 = ex2(fmaf(x[i][c][2 * h], f[c][0], -sub[c][0]));
+            const float p1 = ex2(fmaf(x[i][c][2 * h + 1], f[c][1], -sub[c][1]));
             l[c][0] += p0;
             l[c][1] += p1;
-            // A scale that is NaN reaches only the rows that see the key.
-            const float w0 = x0 == kNegInf ? 0.f : p0 * w_of[c][0], w1 = x1 == kNegInf ? 0.f : p1 * w_of[c][1];
-            pf[i][c][h] = transpose8(pack2<false>(w0, w1));
+            pf[i][c][h] = transpose8(pack2<false>(p0 * w_of[c][0], p1 * w_of[c][1]));
           }
-      }
 
 #pragma unroll
       for (int i = 0; i < S::kKeyTiles; ++i) {
@@ -479,7 +504,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
       if (at.u + 1 == at.units || at.left == 1) end_item();
       if (at.advance(p, lengths) && at.more()) {
         begin_item();
-        keep_next = mask_bits(at.u);
+        load_mask(at.u);
         scale_next = scales(at.u);
       }
     }
@@ -492,9 +517,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
 template <int D, bool kInt8, int kCols, bool kMask>
 cudaError_t launch_t(const Decode8Params& p, int ctas, bool after_prefix, cudaStream_t s) {
   auto kern = decode8_kernel<D, kInt8, kCols, kMask>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape8<D>::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape8<D, kCols>::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_chained(kern, dim3(ctas), 32 * kDecodeWarps, Shape8<D>::kBytes, 1, s, p, after_prefix);
+  return launch_chained(kern, dim3(ctas), 32 * kDecodeWarps, Shape8<D, kCols>::kBytes, 1, s, p, after_prefix);
 }
 
 template <int D, bool kInt8>

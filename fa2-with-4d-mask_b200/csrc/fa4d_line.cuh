@@ -14,7 +14,8 @@ __device__ __forceinline__ Shares shares_of(const DecodeParams& p, int64_t total
   const int least = p.min_units;
   auto up = [](int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); };
   if (p.load.items) {
-    const RunChoice c = choose_runs<D == 96 ? 128 : D>(p.load, total, lane);
+    RunChoice c = choose_runs<D == 96 ? 128 : D>(p.load, total * p.heads, lane);
+    c.rate /= p.heads;
     const int free_sms = p.load.sms - p.load.items * c.runs;
     if (free_sms > 0) {
       const int early = p.warps / p.load.sms * free_sms, rest = p.warps - early;
@@ -68,20 +69,20 @@ struct Lengths {
 template <int kShift>
 struct Place {
   bool prefix;
-  int b, hk, tile;  // the item (b unused in the prefix)
+  int b, hk, tile;  // the item (b unused in the prefix); hk: the group of heads
   int u, units;     // unit within the item, units of the item
   int keys;         // keys of the item
   int64_t left;
 
   __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ int item(const DecodeParams& p) const {
-    return prefix ? hk * p.prefix_tiles + tile : (p.prefix_tiles + b * p.tiles) * p.Hk + hk * p.tiles + tile;
+    return prefix ? hk * p.prefix_tiles + tile : (p.prefix_tiles + b * p.tiles) * p.groups + hk * p.tiles + tile;
   }
   __device__ __forceinline__ void next_item(const DecodeParams& p, const Lengths<kShift>& lengths) {
     u = 0;
     if (++tile < (prefix ? p.prefix_tiles : p.tiles)) return;
     tile = 0;
-    if (++hk < p.Hk) return;
+    if (++hk < p.groups) return;
     hk = 0;
     b = prefix ? 0 : b + 1;
     prefix = false;
@@ -110,7 +111,7 @@ __device__ __forceinline__ Place<kShift> find_place(const DecodeParams& p, const
   w.left = left;
   w.b = 0;
   int64_t line = p.prefix_units + kPrefixItemUnits;
-  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.Hk * line;
+  const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.groups * line;
   int tiles = p.tiles;
   w.prefix = at < prefix_all;
   if (w.prefix) {
@@ -118,7 +119,7 @@ __device__ __forceinline__ Place<kShift> find_place(const DecodeParams& p, const
     tiles = p.prefix_tiles;
   } else {
     at -= prefix_all;
-    const int64_t each = static_cast<int64_t>(p.Hk) * p.tiles;
+    const int64_t each = static_cast<int64_t>(p.groups) * p.tiles;
     bool found = false;
     auto search = [&](int b0, int mine) {  // among the 32 requests from b0
       int64_t upto = line_of(mine, kShift);

@@ -7,6 +7,8 @@
 //
 // Bound by memory: the forward reads and writes each element once, the backward reads x and dy and
 // writes dx.
+#include <algorithm>
+
 #include "fa4d.h"
 #include "fa4d_kernels.h"
 #include "fa4d_launch.cuh"
@@ -18,133 +20,315 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// A block's part of the heads: q's first `q_parts` blocks along y, then k's.
-struct HeadRange {
+// Blocks of an SM, and ranges of at most so many heads (their angles are worked out once).  The grid
+// fills the GPU once; with many tokens it is kWaves times as large, which evens out what the SMs are
+// apart (B2 T16385 Hq16 Hk8 D256: forward 150 us once, 130 three times; B1 T8192 Hq32 Hk8 D128, whose
+// blocks have two rounds, 34 and 35; backward 204 and 192, 49 and 57).
+constexpr int kFwdPerSm = 5, kBwdPerSm = 3, kHeadsEach = 16;
+constexpr int kFwdWaves = 3, kBwdWaves = 2;
+constexpr int kLong = 8;  // rounds of a block
+
+// The grid: `q_blocks` blocks for q, then those for k, in proportion to their heads; of each, `parts`
+// ranges of heads side by side, and over those the tokens.
+struct NormGrid {
+  int lanes, chunks;
+  int q_blocks, q_parts, q_each;
+  int k_blocks, k_parts, k_each;
+};
+
+// A block's part.
+struct Part {
   bool is_q;
-  int first, end;
-  __device__ __forceinline__ HeadRange(int part, int q_parts, int each, int Hq, int Hk) {
-    is_q = part < q_parts;
-    first = (is_q ? part : part - q_parts) * each;
+  int first, end;      // heads
+  uint32_t x, across;  // which of so many blocks that share the tokens
+  __device__ __forceinline__ Part(const NormGrid& g, int Hq, int Hk) {
+    is_q = blockIdx.x < g.q_blocks;
+    const int id = is_q ? blockIdx.x : blockIdx.x - g.q_blocks, parts = is_q ? g.q_parts : g.k_parts;
+    const int each = is_q ? g.q_each : g.k_each;
+    first = id % parts * each;
     end = min(first + each, is_q ? Hq : Hk);
+    x = id / parts;
+    across = (is_q ? g.q_blocks : g.k_blocks) / parts;
   }
 };
 
-// One thread: a lane of a token's rows, for a range of q's or of k's heads, so that angles and
-// weights serve several heads.
-constexpr int kHeads = 4;
+// One thread: a lane of a token's rows, for a range of q's or of k's heads (angles serve them all),
+// token after token, `across` blocks apart.  What it reads comes into places of its own in shared
+// memory, kDepth rows ahead (no barrier between threads): with loads into registers, four rows at a
+// time, a warp had none on their way while it computed (fed so, forward and backward together 431 us
+// at B2 T16385 Hq16 Hk8 D256; the packed arithmetic is in both figures' favour: 335 now).
+constexpr int kFwdDepth = 6, kBwdDepth = 4;
+template <int VEC, bool kAdj, int kStreams, int kDepth>
+class Feed {
+ public:
+  static constexpr int kBytes = VEC == 8 ? kDepth * kStreams * 2 * 16 * kThreads : 0;
 
-template <bool kBF16, bool kAdj, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_rotary_kernel(const __grid_constant__ fa4d_norm_rotary_args args, int chunks,
-                                                               int lanes, int q_parts, int heads_each) {
-  const fa4d_rotary_args& a = args.rotary;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
-  const bool live = n < static_cast<int64_t>(a.B) * a.T;
-  const int64_t b = n / a.T, t = n - b * a.T;
-  const HeadRange heads(blockIdx.y, q_parts, heads_each, a.Hq, a.Hk);
-  const RowLane<VEC, kAdj> at(a.table, lane, chunks);
-  pdl_wait();
-  pdl_launch();
-  Pairs<VEC> w;
-  at.template vector<kBF16>(heads.is_q ? args.norm.q_weight : args.norm.k_weight, args.norm.weight_f32 != 0, w);
-  const int64_t* si = heads.is_q ? a.q_stride : a.k_stride;
-  const int64_t* so = heads.is_q ? a.q_out_stride : a.k_out_stride;
-  const uint16_t* src = static_cast<const uint16_t*>(heads.is_q ? a.q : a.k) + b * si[0] + t * si[1];
-  uint16_t* dst = static_cast<uint16_t*>(heads.is_q ? a.q_out : a.k_out) + b * so[0] + t * so[1];
-  norm_heads<kBF16, kAdj, VEC, kHeads>(a.table, at, &w, args.norm.eps, lanes, lane, live, src, si[2], dst, so[2], heads.first,
-                                       heads.end, a.positions, a.positions_bits, a.positions_stride, b, t);
-}
-
-// The gradient.  A block takes tokens gridDim.x * (rows of a block) apart and adds the weights'
-// gradient up over all of them in registers, then over its rows in shared memory: one row of D sums
-// a block, which weight_grad_kernel adds (always in the same order).
-constexpr int kBwdHeads = 2;
-
-template <bool kBF16, bool kAdj, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_rotary_grad_kernel(const __grid_constant__ fa4d_norm_rotary_bwd_args args,
-                                                                   int chunks, int lanes, int q_parts, int heads_each) {
-  constexpr int P = kRowPairs<VEC>;
-  __shared__ float sums[kThreads * 2 * P];  // [rows][D]
-  const fa4d_rotary_args& a = args.rotary;
-  const int lane = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes, rows = kThreads / lanes;
-  const HeadRange heads(blockIdx.y, q_parts, heads_each, a.Hq, a.Hk);
-  const RowLane<VEC, kAdj> at(a.table, lane, chunks);
-  pdl_wait();
-  pdl_launch();
-  Pairs<VEC> w, dw;
-  at.template vector<kBF16>(heads.is_q ? args.norm.q_weight : args.norm.k_weight, args.norm.weight_f32 != 0, w);
+  __device__ __forceinline__ Feed(uint8_t* smem, const RowLane<VEC, kAdj>& at_, const fa4d_rotary_args& a, uint32_t first_token,
+                                  uint32_t step_, int first_, int end_)
+      : at(at_), ring(reinterpret_cast<uint4*>(smem) + threadIdx.x), n(first_token), step(step_), tokens(a.B * static_cast<uint32_t>(a.T)),
+        T(a.T), h(first_), first(first_), end(end_) {}
+  __device__ __forceinline__ void add(int s, const void* base, const int64_t (&stride)[3]) {
+    all[s] = static_cast<const uint16_t*>(base) + first * stride[2];
+    batch[s] = stride[0];
+    seq[s] = stride[1];
+    head[s] = stride[2];
+  }
+  __device__ __forceinline__ void start() {
+    place();
+    if constexpr (VEC == 8)
 #pragma unroll
-  for (int j = 0; j < P; ++j) dw.a[j] = dw.b[j] = 0.f;
-  const int64_t* si = heads.is_q ? a.q_stride : a.k_stride;
-  const int64_t* sd = heads.is_q ? args.dq_stride : args.dk_stride;
-  const int64_t* so = heads.is_q ? a.q_out_stride : a.k_out_stride;
-  const uint16_t* x_all = static_cast<const uint16_t*>(heads.is_q ? a.q : a.k);
-  const uint16_t* dy_all = static_cast<const uint16_t*>(heads.is_q ? args.dq : args.dk);
-  uint16_t* dx_all = static_cast<uint16_t*>(heads.is_q ? a.q_out : a.k_out);
-  const float mean = 1.f / a.table.D;
-  const int64_t tokens = static_cast<int64_t>(a.B) * a.T;
-  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * rows; n0 < tokens; n0 += static_cast<int64_t>(gridDim.x) * rows) {
-    const int64_t n = n0 + row;
-    const bool live = n < tokens;
-    const int64_t b = n / a.T, t = n - b * a.T;
-    const uint16_t* x = x_all + b * si[0] + t * si[1];
-    const uint16_t* dy = dy_all + b * sd[0] + t * sd[1];
-    uint16_t* dx = dx_all + b * so[0] + t * so[1];
-    float cs[P], sn[P];
-    for (int h0 = heads.first; h0 < heads.end; h0 += kBwdHeads) {
-      Raw<VEC> rx[kBwdHeads], rd[kBwdHeads];
+      for (int i = 0; i < kDepth; ++i) bring(i);
+  }
+  // The row at `stage` (they come round in order), all streams.
+  __device__ __forceinline__ void take(int stage, Raw<VEC> (&r)[kStreams]) {
+    if constexpr (VEC == 8) {
+      cp_async_wait<kDepth - 1>();
 #pragma unroll
-      for (int u = 0; u < kBwdHeads; ++u)
-        if (live && h0 + u < heads.end) {
-          at.load(x + (h0 + u) * si[2], rx[u]);
-          at.load(dy + (h0 + u) * sd[2], rd[u]);
-        }
-      if (h0 == heads.first && live) at.angles(a.table, a.positions, a.positions_bits, a.positions_stride, b, t, lane, cs, sn);
-#pragma unroll
-      for (int u = 0; u < kBwdHeads; ++u) {
-        const bool here = live && h0 + u < heads.end;
-        Pairs<VEC> xv, g;
-        unpack_pairs<kBF16, kAdj>(rx[u], xv);
-        unpack_pairs<kBF16, kAdj>(rd[u], g);
-        if (here) at.turn(g, cs, sn, -1.f);
-        float dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < P; ++j) dot = fmaf(xv.a[j], w.a[j] * g.a[j], fmaf(xv.b[j], w.b[j] * g.b[j], dot));
-        float square = xv.squares();
-        for (int o = lanes / 2; o; o >>= 1) {
-          square += __shfl_xor_sync(0xffffffffu, square, o);
-          dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        }
-        if (!here) continue;
-        const float r = rsqrtf(square * mean + args.norm.eps), c = r * r * (dot * mean);
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          dw.a[j] = fmaf(g.a[j], xv.a[j] * r, dw.a[j]);
-          dw.b[j] = fmaf(g.b[j], xv.b[j] * r, dw.b[j]);
-          g.a[j] = r * (w.a[j] * g.a[j] - xv.a[j] * c);
-          g.b[j] = r * (w.b[j] * g.b[j] - xv.b[j] * c);
-        }
-        pack_pairs<kBF16, kAdj>(g, rx[u]);
-        at.store(dx + (h0 + u) * so[2], rx[u]);
+      for (int s = 0; s < kStreams; ++s) {
+        const uint4* p = ring + (stage * kStreams + s) * 2 * kThreads;
+        r[s].x[0] = at.live ? p[0] : make_uint4(0, 0, 0, 0);
+        r[s].y[0] = at.live ? p[kThreads] : make_uint4(0, 0, 0, 0);
       }
+    } else {
+#pragma unroll
+      for (int s = 0; s < kStreams; ++s)
+        if (n < tokens) at.load(src[s], r[s]);
     }
   }
-  // Over the block's rows.
+  // After the last use of what take() gave.
+  __device__ __forceinline__ void next(int stage) {
+    if constexpr (VEC == 8)
+      bring(stage);
+    else
+      advance();
+  }
+
+ private:
+  const RowLane<VEC, kAdj>& at;
+  uint4* ring;  // [kDepth][kStreams][2], kThreads apart
+  uint32_t n, step, tokens, T;
+  int h, first, end;
+  const uint16_t* all[kStreams];
+  const uint16_t* src[kStreams];
+  int64_t batch[kStreams], seq[kStreams], head[kStreams];
+
+  __device__ __forceinline__ void place() {
+    const uint32_t b = n / T, t = n - b * T;
 #pragma unroll
-  for (int i = 0; i < kRowChunks<VEC>; ++i)
-    if ((at.live >> i) & 1u) {
+    for (int s = 0; s < kStreams; ++s) src[s] = all[s] + b * batch[s] + t * seq[s];
+  }
+  __device__ __forceinline__ void advance() {
+    if (++h < end) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int e0 = kAdj && VEC == 8 ? at.at0[i] + 2 * j : at.at0[i] + j, e1 = kAdj && VEC == 8 ? e0 + 1 : at.at1[i] + j;
-        sums[row * a.table.D + e0] = dw.a[VEC * i + j];
-        sums[row * a.table.D + e1] = dw.b[VEC * i + j];
+      for (int s = 0; s < kStreams; ++s) src[s] += head[s];
+      return;
+    }
+    h = first;
+    n += step;
+    place();
+  }
+  __device__ __forceinline__ void bring(int stage) {
+    if (at.live && n < tokens) {
+#pragma unroll
+      for (int s = 0; s < kStreams; ++s) {
+        uint4* p = ring + (stage * kStreams + s) * 2 * kThreads;
+        cp_async16(p, src[s] + at.at0[0], 16);
+        cp_async16(p + kThreads, src[s] + at.at1[0], 16);
       }
     }
+    cp_async_commit();
+    advance();
+  }
+};
+
+// The rows that a thread goes through: `live` ones of tokens (b, t), heads from `first` on.
+struct Rows {
+  uint32_t n, step;
+  int iterations;
+  __device__ __forceinline__ Rows(const fa4d_rotary_args& a, int lanes, const Part& part) {
+    const uint32_t rows = kThreads / lanes, tokens = a.B * static_cast<uint32_t>(a.T), n0 = part.x * rows;
+    step = part.across * rows;
+    n = n0 + threadIdx.x / lanes;
+    iterations = static_cast<int>((tokens - n0 + step - 1) / step) * (part.end - part.first);  // the same for all threads
+  }
+};
+
+template <bool kBF16, bool kAdj, int VEC, int kLanes>
+__global__ void __launch_bounds__(kThreads, kFwdPerSm) norm_rotary_kernel(
+    const __grid_constant__ fa4d_norm_rotary_args args, const __grid_constant__ NormGrid grid) {
+  const int lanes = kLanes ? kLanes : grid.lanes;
+  using F = Feed<VEC, kAdj, 1, kFwdDepth>;
+  extern __shared__ uint4 ring4[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ring4);  // [F::kBytes]
+  __shared__ Turns<VEC> turns;
+  __shared__ Weights<VEC> weights;
+  const fa4d_rotary_args& a = args.rotary;
+  turns.template fill<kAdj>(a.table);
+  const int lane = threadIdx.x & (lanes - 1);
+  const Part heads(grid, a.Hq, a.Hk);
+  const RowLane<VEC, kAdj> at(a.table, lane, grid.chunks);
+  Rows rows(a, lanes, heads);
+  F feed(ring, at, a, rows.n, rows.step, heads.first, heads.end);
+  pdl_wait();
+  pdl_launch();
+  if (heads.is_q)
+    feed.add(0, a.q, a.q_stride);
+  else
+    feed.add(0, a.k, a.k_stride);
+  feed.start();
+  weights.template fill<kBF16, kAdj>(a.table, heads.is_q ? args.norm.q_weight : args.norm.k_weight, args.norm.weight_f32 != 0);
   __syncthreads();
-  float* part = static_cast<float*>(args.workspace) + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * a.table.D;
+  const int64_t* so = heads.is_q ? a.q_out_stride : a.k_out_stride;
+  const uint32_t tokens = a.B * static_cast<uint32_t>(a.T);
+  const float mean = 1.f / a.table.D;
+  uint16_t* dst = nullptr;
+  bool live = false;
+  Factors<VEC> factors;
+  const bool copied = at.copied();
+  int h = heads.first, stage = 0;
+#pragma unroll 1
+  for (int it = 0; it < rows.iterations; ++it) {
+    Raw<VEC> raw[1];
+    feed.take(stage, raw);
+    if (h == heads.first) {
+      live = rows.n < tokens;
+      const uint32_t b = rows.n / a.T, t = rows.n - b * a.T;
+      dst = static_cast<uint16_t*>(heads.is_q ? a.q_out : a.k_out) + b * so[0] + t * so[1] + h * so[2];
+      if (live) {
+        Turn<VEC> turn;
+        at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
+        Pairs<VEC> w;
+        at.weights(weights, lane, w);
+        factors.set(turn, &w);
+      }
+    }
+    Pairs<VEC> p;
+    unpack_pairs<kBF16, kAdj>(raw[0], p);
+    p.times(rsqrtf(row_sum<kLanes>(p.squares(), lanes) * mean + args.norm.eps));
+    if (live) {
+      factors.turn(p, copied);
+      pack_pairs<kBF16, kAdj>(p, raw[0]);
+      at.store(dst, raw[0]);
+    }
+    feed.next(stage);
+    if (++stage == kFwdDepth) stage = 0;
+    dst += so[2];
+    if (++h == heads.end) {
+      h = heads.first;
+      rows.n += rows.step;
+    }
+  }
+  if constexpr (VEC == 8) cp_async_wait_all();
+}
+
+// The gradient.  A thread adds the weights' gradient up over all its rows in registers, then the
+// block over its threads in shared memory: one row of D sums a block, which weight_grad_kernel adds
+// (always in the same order).
+template <bool kBF16, bool kAdj, int VEC, int kLanes>
+__global__ void __launch_bounds__(kThreads, kBwdPerSm) norm_rotary_grad_kernel(
+    const __grid_constant__ fa4d_norm_rotary_bwd_args args, const __grid_constant__ NormGrid grid) {
+  const int lanes = kLanes ? kLanes : grid.lanes;
+  using F = Feed<VEC, kAdj, 2, kBwdDepth>;
+  constexpr int P = kRowPairs<VEC> / 2;
+  constexpr int kSums = kThreads * 4 * P * 4;
+  extern __shared__ uint4 ring4[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ring4);  // [max(F::kBytes, kSums)]; in the end the sums, [rows][D]
+  __shared__ Turns<VEC> turns;
+  __shared__ Weights<VEC> weights;
+  const fa4d_rotary_args& a = args.rotary;
+  turns.template fill<kAdj>(a.table);
+  const int lane = threadIdx.x & (lanes - 1);
+  const Part heads(grid, a.Hq, a.Hk);
+  const RowLane<VEC, kAdj> at(a.table, lane, grid.chunks);
+  Rows rows(a, lanes, heads);
+  F feed(ring, at, a, rows.n, rows.step, heads.first, heads.end);
+  pdl_wait();
+  pdl_launch();
+  if (heads.is_q) {
+    feed.add(0, a.q, a.q_stride);
+    feed.add(1, args.dq, args.dq_stride);
+  } else {
+    feed.add(0, a.k, a.k_stride);
+    feed.add(1, args.dk, args.dk_stride);
+  }
+  feed.start();
+  weights.template fill<kBF16, kAdj>(a.table, heads.is_q ? args.norm.q_weight : args.norm.k_weight, args.norm.weight_f32 != 0);
+  __syncthreads();
+  const int64_t* so = heads.is_q ? a.q_out_stride : a.k_out_stride;
+  const uint32_t tokens = a.B * static_cast<uint32_t>(a.T);
+  const float mean = 1.f / a.table.D;
+  uint16_t* dx = nullptr;
+  bool live = false;
+  Turn<VEC> turn;
+  const bool copied = at.copied();
+  Pairs<VEC> dw;
+#pragma unroll
+  for (int j = 0; j < P; ++j) dw.a[j] = dw.b[j] = f2(0.f, 0.f);
+  int h = heads.first, stage = 0;
+#pragma unroll 1
+  for (int it = 0; it < rows.iterations; ++it) {
+    Raw<VEC> raw[2];
+    feed.take(stage, raw);
+    if (h == heads.first) {
+      live = rows.n < tokens;
+      const uint32_t b = rows.n / a.T, t = rows.n - b * a.T;
+      dx = static_cast<uint16_t*>(heads.is_q ? a.q_out : a.k_out) + b * so[0] + t * so[1] + h * so[2];
+      if (live) at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
+    }
+    Pairs<VEC> x, d, g, w;
+    unpack_pairs<kBF16, kAdj>(raw[0], x);
+    unpack_pairs<kBF16, kAdj>(raw[1], d);
+    at.weights(weights, lane, w);
+    uint64_t dots = f2(0.f, 0.f);
+    turn.back(d, g, copied);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      w.a[j] = fmul2(w.a[j], g.a[j]);
+      w.b[j] = fmul2(w.b[j], g.b[j]);
+      dots = ffma2(x.a[j], w.a[j], ffma2(x.b[j], w.b[j], dots));
+    }
+    const float2 both = f2_split(dots);
+    const float square = row_sum<kLanes>(x.squares(), lanes), dot = row_sum<kLanes>(both.x + both.y, lanes);
+    if (live) {
+      const float r = rsqrtf(square * mean + args.norm.eps), c = -(r * r * (dot * mean));
+      const uint64_t rr = f2(r, r), cc = f2(c, c);
+      x.times(r);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        dw.a[j] = ffma2(g.a[j], x.a[j], dw.a[j]);
+        dw.b[j] = ffma2(g.b[j], x.b[j], dw.b[j]);
+        g.a[j] = ffma2(x.a[j], cc, fmul2(w.a[j], rr));
+        g.b[j] = ffma2(x.b[j], cc, fmul2(w.b[j], rr));
+      }
+      pack_pairs<kBF16, kAdj>(g, raw[0]);
+      at.store(dx, raw[0]);
+    }
+    feed.next(stage);
+    if (++stage == kBwdDepth) stage = 0;
+    dx += so[2];
+    if (++h == heads.end) {
+      h = heads.first;
+      rows.n += rows.step;
+    }
+  }
+  if constexpr (VEC == 8) cp_async_wait_all();
+  __syncthreads();
+  // Over the block's rows.
+  float* sums = reinterpret_cast<float*>(ring);
+  const int row = threadIdx.x / lanes;
+#pragma unroll
+  for (int j = 0; j < 2 * P; ++j)
+    if ((at.live >> (j / VEC)) & 1u) {
+      const float2 u = f2_split(dw.a[j / 2]), v = f2_split(dw.b[j / 2]);
+      const PairAt<VEC, kAdj> e(a.table, lane + 32 * (j / VEC), j % VEC);
+      sums[row * a.table.D + e.e0] = j & 1 ? u.y : u.x;
+      sums[row * a.table.D + e.e1] = j & 1 ? v.y : v.x;
+    }
+  __syncthreads();
+  float* part = static_cast<float*>(args.workspace) + static_cast<int64_t>(blockIdx.x) * a.table.D;
   for (int e = threadIdx.x; e < a.table.D; e += kThreads) {
     float s = 0.f;
-    for (int r = 0; r < rows; ++r) s += sums[r * a.table.D + e];
+    for (int r = 0; r < kThreads / lanes; ++r) s += sums[r * a.table.D + e];
     part[e] = s;
   }
 }
@@ -177,70 +361,85 @@ __global__ void __launch_bounds__(256) weight_grad_kernel(const float* parts, in
   }
 }
 
-struct NormGrid {
-  int lanes, q_parts, each;
-  dim3 grid;
-};
-
-NormGrid grid_of(const fa4d_rotary_args& a, int vec, int per_sm, int most_each, bool all_tokens, int sms) {
+NormGrid grid_of(const fa4d_rotary_args& a, int vec, int per_sm, int waves, int sms) {
   NormGrid g;
   g.lanes = row_lanes(a.table, vec);
-  const int rows = kThreads / g.lanes;
-  const int64_t blocks = (static_cast<int64_t>(a.B) * a.T + rows - 1) / rows;
+  g.chunks = chunks_of(a.table, vec);
+  const int rows = kThreads / g.lanes, all = a.Hq + a.Hk;
+  const int64_t blocks = (static_cast<int64_t>(a.B) * a.T + rows - 1) / rows, once = static_cast<int64_t>(sms) * per_sm;
   // Heads are split until the blocks fill the GPU, down to one head.
-  const int64_t full = static_cast<int64_t>(sms) * per_sm;
-  g.each = most_each;
-  while (g.each > 1 && blocks * ((a.Hq + g.each - 1) / g.each + (a.Hk + g.each - 1) / g.each) < full) g.each /= 2;
-  g.q_parts = (a.Hq + g.each - 1) / g.each;
-  const int parts = g.q_parts + (a.Hk + g.each - 1) / g.each;
-  const int64_t x = all_tokens ? blocks : min(blocks, max(full / parts, static_cast<int64_t>(1)));
-  g.grid = dim3(static_cast<unsigned>(x), parts);
+  auto parts_of = [](int heads, int each) { return (heads + each - 1) / each; };
+  int each = kHeadsEach;
+  while (each > 1 && blocks * (parts_of(a.Hq, each) + parts_of(a.Hk, each)) < once) each /= 2;
+  const int64_t full = blocks * (parts_of(a.Hq, each) + parts_of(a.Hk, each)) < kLong * once ? once : waves * once;
+  auto set = [&](int heads, int& n, int& parts, int& share) {
+    parts = parts_of(heads, each);
+    share = parts_of(heads, parts);
+    n = static_cast<int>(std::min(blocks, std::max<int64_t>(full * heads / all / parts, 1))) * parts;
+  };
+  set(a.Hq, g.q_blocks, g.q_parts, g.q_each);
+  set(a.Hk, g.k_blocks, g.k_parts, g.k_each);
   return g;
 }
 
-constexpr int kFwdPerSm = 12, kFwdEach = 8;
-constexpr int kBwdPerSm = 4, kBwdEach = 8;
 
-template <int VEC, bool kBF16>
-cudaError_t launch_fwd_t(const fa4d_norm_rotary_args& a, int sms, cudaStream_t s) {
-  const NormGrid g = grid_of(a.rotary, VEC, kFwdPerSm, kFwdEach, true, sms);
-  auto kern = a.rotary.table.pairing == FA4D_PAIR_ADJACENT ? norm_rotary_kernel<kBF16, true, VEC>
-                                                           : norm_rotary_kernel<kBF16, false, VEC>;
-  return launch_chained(kern, g.grid, kThreads, 0, 1, s, a, chunks_of(a.rotary.table, VEC), g.lanes, g.q_parts, g.each);
+template <int VEC, bool kBF16, int kLanes>
+cudaError_t launch_fwd_t(const fa4d_norm_rotary_args& a, const NormGrid& g, cudaStream_t s) {
+  auto kern = a.rotary.table.pairing == FA4D_PAIR_ADJACENT ? norm_rotary_kernel<kBF16, true, VEC, kLanes>
+                                                           : norm_rotary_kernel<kBF16, false, VEC, kLanes>;
+  constexpr int smem = Feed<VEC, true, 1, kFwdDepth>::kBytes;
+  static_assert(smem <= 40 * 1024, "with what is static, more needs leave");
+  return launch_chained(kern, dim3(g.q_blocks + g.k_blocks), kThreads, smem, 1, s, a, g);
 }
 
-template <int VEC, bool kBF16>
-cudaError_t launch_bwd_t(const fa4d_norm_rotary_bwd_args& a, int sms, cudaStream_t s) {
-  const NormGrid g = grid_of(a.rotary, VEC, kBwdPerSm, kBwdEach, false, sms);
-  auto kern = a.rotary.table.pairing == FA4D_PAIR_ADJACENT ? norm_rotary_grad_kernel<kBF16, true, VEC>
-                                                           : norm_rotary_grad_kernel<kBF16, false, VEC>;
+template <int VEC, bool kBF16, int kLanes>
+cudaError_t launch_bwd_t(const fa4d_norm_rotary_bwd_args& a, const NormGrid& g, cudaStream_t s) {
+  auto kern = a.rotary.table.pairing == FA4D_PAIR_ADJACENT ? norm_rotary_grad_kernel<kBF16, true, VEC, kLanes>
+                                                           : norm_rotary_grad_kernel<kBF16, false, VEC, kLanes>;
+  constexpr int sums = kThreads * 2 * kRowPairs<VEC> * 4, feed = Feed<VEC, true, 2, kBwdDepth>::kBytes;
+  constexpr int smem = feed > sums ? feed : sums;
+  static_assert(smem <= 40 * 1024, "with what is static, more needs leave");
   const cudaError_t e =
-      launch_chained(kern, g.grid, kThreads, 0, 1, s, a, chunks_of(a.rotary.table, VEC), g.lanes, g.q_parts, g.each);
+      launch_chained(kern, dim3(g.q_blocks + g.k_blocks), kThreads, smem, 1, s, a, g);
   if (e != cudaSuccess) return e;
-  const int D = a.rotary.table.D, q_rows = g.q_parts * static_cast<int>(g.grid.x);
-  const int k_rows = static_cast<int>(g.grid.y - g.q_parts) * static_cast<int>(g.grid.x);
+  const int D = a.rotary.table.D;
   return launch_chained(weight_grad_kernel<kBF16>, dim3((D + 7) / 8, 2), 256, 0, 1, s, static_cast<const float*>(a.workspace), D,
-                        q_rows, k_rows, a.q_weight_grad, a.k_weight_grad, a.norm.weight_f32 != 0);
+                        g.q_blocks, g.k_blocks, a.q_weight_grad, a.k_weight_grad, a.norm.weight_f32 != 0);
+}
+
+// The kernels of 4, 8 and 16 lanes a row (head dims from 33 to 256) know it, which saves the loops of
+// their sums.
+template <bool kBF16>
+cudaError_t launch_fwd_b(const fa4d_norm_rotary_args& a, bool vec, int sms, cudaStream_t s) {
+  const NormGrid g = grid_of(a.rotary, vec ? 8 : 1, kFwdPerSm, kFwdWaves, sms);
+  if (!vec) return launch_fwd_t<1, kBF16, 32>(a, g, s);
+  if (g.lanes == 16) return launch_fwd_t<8, kBF16, 16>(a, g, s);
+  if (g.lanes == 8) return launch_fwd_t<8, kBF16, 8>(a, g, s);
+  if (g.lanes == 4) return launch_fwd_t<8, kBF16, 4>(a, g, s);
+  return launch_fwd_t<8, kBF16, 0>(a, g, s);
+}
+template <bool kBF16>
+cudaError_t launch_bwd_b(const fa4d_norm_rotary_bwd_args& a, bool vec, int sms, cudaStream_t s) {
+  const NormGrid g = grid_of(a.rotary, vec ? 8 : 1, kBwdPerSm, kBwdWaves, sms);
+  if (!vec) return launch_bwd_t<1, kBF16, 32>(a, g, s);
+  if (g.lanes == 16) return launch_bwd_t<8, kBF16, 16>(a, g, s);
+  if (g.lanes == 8) return launch_bwd_t<8, kBF16, 8>(a, g, s);
+  if (g.lanes == 4) return launch_bwd_t<8, kBF16, 4>(a, g, s);
+  return launch_bwd_t<8, kBF16, 0>(a, g, s);
 }
 
 }  // namespace
 
-// Rows of partial sums that a backward pass writes at most, whichever way its rows are divided.
-int64_t norm_bwd_rows(int Hq, int Hk, int sms) {
-  const int64_t parts = Hq + Hk;  // one head each
-  return max(static_cast<int64_t>(sms) * kBwdPerSm, parts);
-}
+// Rows of partial sums that a backward pass writes at most, whichever way its rows are divided: a
+// block each (see grid_of: one a part where that is more than its share).
+int64_t norm_bwd_rows(int Hq, int Hk, int sms) { return static_cast<int64_t>(sms) * kBwdPerSm * kBwdWaves + Hq + Hk; }
 
 cudaError_t launch_norm_rotary(const fa4d_norm_rotary_args& a, bool vec, int sms, cudaStream_t s) {
-  const bool bf16 = a.rotary.dtype == FA4D_BF16;
-  if (vec) return bf16 ? launch_fwd_t<8, true>(a, sms, s) : launch_fwd_t<8, false>(a, sms, s);
-  return bf16 ? launch_fwd_t<1, true>(a, sms, s) : launch_fwd_t<1, false>(a, sms, s);
+  return a.rotary.dtype == FA4D_BF16 ? launch_fwd_b<true>(a, vec, sms, s) : launch_fwd_b<false>(a, vec, sms, s);
 }
 
 cudaError_t launch_norm_rotary_bwd(const fa4d_norm_rotary_bwd_args& a, bool vec, int sms, cudaStream_t s) {
-  const bool bf16 = a.rotary.dtype == FA4D_BF16;
-  if (vec) return bf16 ? launch_bwd_t<8, true>(a, sms, s) : launch_bwd_t<8, false>(a, sms, s);
-  return bf16 ? launch_bwd_t<1, true>(a, sms, s) : launch_bwd_t<1, false>(a, sms, s);
+  return a.rotary.dtype == FA4D_BF16 ? launch_bwd_b<true>(a, vec, sms, s) : launch_bwd_b<false>(a, vec, sms, s);
 }
 
 }  // namespace fa4d

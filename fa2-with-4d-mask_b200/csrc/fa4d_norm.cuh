@@ -10,9 +10,30 @@ namespace fa4d {
 // VEC = 8 each has a chunk of 8 pairs (lanes past the last chunk idle), with VEC = 1 all 32 have up
 // to 4 chunks of one pair, 32 apart.
 template <int VEC>
-constexpr int kRowChunks = VEC == 8 ? 1 : 4;
+constexpr int kRowChunks = VEC == 1 ? 4 : 1;
 template <int VEC>
 constexpr int kRowPairs = VEC * kRowChunks<VEC>;  // of a lane
+
+// Elements of pair j of chunk c of a row (past the pairs, of elements that are copied).  With VEC = 8
+// a chunk is 8 elements of the first half of what is turned and 8 of the second, whichever the
+// pairing, so that neighbouring lanes read neighbouring 16 bytes (with 32 bytes a lane, 16 at a time,
+// every sector was asked for twice).
+template <int VEC, bool kAdj>
+struct PairAt {
+  int e0, e1;
+  __device__ __forceinline__ PairAt(const fa4d_rotary_table& tab, int c, int j) {
+    const int pairs = tab.rotary_dim / 2, turned = pairs / VEC;
+    const int at0 = c < turned ? c * (kAdj && VEC == 1 ? 2 : VEC) : tab.rotary_dim + (c - turned) * 2 * VEC;
+    const int at1 = c < turned ? (kAdj && VEC == 1 ? at0 + 1 : pairs + c * VEC) : at0 + VEC;
+    if (kAdj && VEC > 1) {
+      e0 = j < VEC / 2 ? at0 + 2 * j : at1 + 2 * j - VEC;
+      e1 = e0 + 1;
+    } else {
+      e0 = at0 + j;
+      e1 = at1 + j;
+    }
+  }
+};
 
 inline int chunks_of(const fa4d_rotary_table& tab, int vec) {
   return tab.rotary_dim / 2 / vec + (tab.D - tab.rotary_dim) / (2 * vec);
@@ -25,22 +46,40 @@ inline int row_lanes(const fa4d_rotary_table& tab, int vec) {
   return lanes;
 }
 
-// The sum over a row's lanes, in all of them; every lane of the warp takes part.
+// The sum over a row's lanes, in all of them; every lane of the warp takes part.  kLanes: known lanes
+// of a row, or 0.
+template <int kLanes = 0>
 __device__ __forceinline__ float row_sum(float x, int lanes) {
-  for (int o = lanes / 2; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if constexpr (kLanes > 0) {
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  } else {
+    for (int o = lanes / 2; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  }
   return x;
 }
 
-// What a lane holds of a row: pair j is (a[j], b[j]) (past the pairs, elements that are copied).
+// What a lane holds of a row: pair j is (a_j, b_j) (past the pairs, elements that are copied); two
+// pairs beside one another lie packed, for the packed arithmetic.
 template <int VEC>
 struct Pairs {
-  float a[kRowPairs<VEC>], b[kRowPairs<VEC>];
+  static constexpr int kTwo = kRowPairs<VEC> / 2;
+  uint64_t a[kTwo], b[kTwo];
 
   __device__ __forceinline__ float squares() const {
-    float s = 0.f;
+    uint64_t s = f2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < kRowPairs<VEC>; ++j) s = fmaf(a[j], a[j], fmaf(b[j], b[j], s));
-    return s;
+    for (int j = 0; j < kTwo; ++j) s = ffma2(a[j], a[j], ffma2(b[j], b[j], s));
+    const float2 t = f2_split(s);
+    return t.x + t.y;
+  }
+  __device__ __forceinline__ void times(float r) {
+    const uint64_t rr = f2(r, r);
+#pragma unroll
+    for (int j = 0; j < kTwo; ++j) {
+      a[j] = fmul2(a[j], rr);
+      b[j] = fmul2(b[j], rr);
+    }
   }
 };
 
@@ -48,6 +87,116 @@ struct Pairs {
 template <int VEC>
 struct Raw {
   typename Run<VEC>::T x[kRowChunks<VEC>], y[kRowChunks<VEC>];
+};
+
+// The table's turns and axes in shared memory, laid so that the lanes of a row read neighbours (a
+// kernel parameter is read one address at a time).
+template <int VEC>
+struct Turns {
+  uint64_t turn[FA4D_ROTARY_MAX_PAIRS];
+  uint8_t axis[FA4D_ROTARY_MAX_PAIRS];
+  static constexpr int kChunks = FA4D_ROTARY_MAX_PAIRS / VEC;
+  static __device__ __forceinline__ int at(int chunk, int j) { return j * kChunks + chunk; }
+  // All threads of the block; a barrier follows.
+  template <bool kAdj>
+  __device__ __forceinline__ void fill(const fa4d_rotary_table& tab) {
+    for (int i = threadIdx.x; i < tab.rotary_dim / 2; i += blockDim.x) {
+      const int c = i / VEC, j = i % VEC;
+      const PairAt<VEC, kAdj> e(tab, c, j);
+      const int pair = kAdj ? e.e0 / 2 : e.e0;
+      turn[at(c, j)] = tab.turn[pair];
+      axis[at(c, j)] = tab.axis[pair];
+    }
+  }
+};
+
+// A norm's weights in shared memory: of each chunk its pairs' first elements, then the second ones,
+// four at a time, so that the lanes of a row read neighbours.  They stay there, since registers are
+// what the kernels lack (and each lane reading its elements from memory took as many requests as
+// eight heads' tokens).
+template <int VEC>
+struct Weights {
+  static constexpr int kQuads = VEC == 1 ? 1 : VEC / 2;  // of a chunk (one pair: half of one)
+  static constexpr int kChunks = FA4D_ROTARY_MAX_PAIRS / VEC;
+  float4 w[kQuads * kChunks];
+  // All threads of the block; a barrier follows.
+  template <bool kBF16, bool kAdj>
+  __device__ __forceinline__ void fill(const fa4d_rotary_table& tab, const void* from, bool f32) {
+    for (int i = threadIdx.x; i < FA4D_ROTARY_MAX_PAIRS; i += blockDim.x) {
+      const int c = i / VEC, j = i % VEC;
+      if (i >= tab.D / 2) {  // lanes past the last chunk take part in sums
+        set(c, j, 0.f);
+        set(c, VEC + j, 0.f);
+        continue;
+      }
+      const PairAt<VEC, kAdj> e(tab, c, j);
+      auto get = [&](int e) {
+        return f32 ? __ldcg(static_cast<const float*>(from) + e) : to_f<kBF16>(__ldcg(static_cast<const uint16_t*>(from) + e));
+      };
+      set(c, j, get(e.e0));
+      set(c, VEC + j, get(e.e1));
+    }
+  }
+  __device__ __forceinline__ void set(int c, int k, float x) {
+    reinterpret_cast<float*>(&w[(k / 4) * kChunks + c])[k % 4] = x;
+  }
+  __device__ __forceinline__ float of(int c, int k) const { return reinterpret_cast<const float*>(&w[(k / 4) * kChunks + c])[k % 4]; }
+};
+
+__device__ __forceinline__ uint64_t minus(uint64_t x) { return x ^ 0x8000000080000000ull; }
+
+// a A + b B, or a A where B is 0 (an infinite b and B = 0 make NaN).
+__device__ __forceinline__ uint64_t mix_apart(uint64_t a, uint64_t A, uint64_t b, uint64_t B) {
+  const float2 x = f2_split(a), u = f2_split(A), y = f2_split(b), v = f2_split(B);
+  return f2(v.x == 0.f ? x.x * u.x : fmaf(x.x, u.x, y.x * v.x), v.y == 0.f ? x.y * u.y : fmaf(x.y, u.y, y.y * v.y));
+}
+
+// The cosines and sines of a lane's pairs.
+template <int VEC>
+struct Turn {
+  uint64_t c[kRowPairs<VEC> / 2], s[kRowPairs<VEC> / 2];
+  // Turned back.  `copied`: pairs with sine 0 are not to be mixed (see RowLane::copied).
+  __device__ __forceinline__ void back(const Pairs<VEC>& d, Pairs<VEC>& g, bool copied) const {
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      if (copied) {
+        g.a[j] = mix_apart(d.a[j], c[j], d.b[j], s[j]);
+        g.b[j] = mix_apart(d.b[j], c[j], d.a[j], minus(s[j]));
+      } else {
+        g.a[j] = ffma2(d.a[j], c[j], fmul2(d.b[j], s[j]));
+        g.b[j] = ffma2(d.b[j], c[j], fmul2(d.a[j], minus(s[j])));
+      }
+    }
+  }
+};
+
+// The turn with a norm's weights: (a, b) becomes (a A + b B, b C + a E).
+template <int VEC>
+struct Factors {
+  uint64_t A[kRowPairs<VEC> / 2], B[kRowPairs<VEC> / 2], C[kRowPairs<VEC> / 2], E[kRowPairs<VEC> / 2];
+  __device__ __forceinline__ void set(const Turn<VEC>& t, const Pairs<VEC>* w) {
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      A[j] = w ? fmul2(w->a[j], t.c[j]) : t.c[j];
+      B[j] = minus(w ? fmul2(w->b[j], t.s[j]) : t.s[j]);
+      C[j] = w ? fmul2(w->b[j], t.c[j]) : t.c[j];
+      E[j] = w ? fmul2(w->a[j], t.s[j]) : t.s[j];
+    }
+  }
+  // `copied`: as for Turn::back.
+  __device__ __forceinline__ void turn(Pairs<VEC>& p, bool copied) const {
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      const uint64_t a = p.a[j], b = p.b[j];
+      if (copied) {
+        p.a[j] = mix_apart(a, A[j], b, B[j]);
+        p.b[j] = mix_apart(b, C[j], a, E[j]);
+      } else {
+        p.a[j] = ffma2(a, A[j], fmul2(b, B[j]));
+        p.b[j] = ffma2(b, C[j], fmul2(a, E[j]));
+      }
+    }
+  }
 };
 
 // A lane's place in its row.
@@ -60,12 +209,11 @@ struct RowLane {
 #pragma unroll
     for (int i = 0; i < kRowChunks<VEC>; ++i) {
       const int c = lane + 32 * i;
-      const Chunk<VEC, kAdj> ch(tab, c);
-      at0[i] = ch.at0;
-      at1[i] = ch.at1;
+      at0[i] = PairAt<VEC, kAdj>(tab, c, 0).e0;
+      at1[i] = kAdj && VEC > 1 ? PairAt<VEC, kAdj>(tab, c, VEC / 2).e0 : PairAt<VEC, kAdj>(tab, c, 0).e1;
       if (c < chunks) {
         live |= 1u << i;
-        if (!ch.copied) turned |= 1u << i;
+        if (c < tab.rotary_dim / 2 / VEC) turned |= 1u << i;
       }
     }
   }
@@ -87,128 +235,144 @@ struct RowLane {
         Run<VEC>::store(row + at1[i], r.y[i]);
       }
   }
-  // A vector of D elements (a norm's weights), fp32 or 16-bit.
-  template <bool kBF16>
-  __device__ __forceinline__ void vector(const void* w, bool f32, Pairs<VEC>& p) const {
+  // This lane's elements of a norm's weights.
+  __device__ __forceinline__ void weights(const Weights<VEC>& w, int lane, Pairs<VEC>& p) const {
+    if constexpr (VEC == 1) {
 #pragma unroll
-    for (int i = 0; i < kRowChunks<VEC>; ++i)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const bool ok = (live >> i) & 1u;
-        const int e0 = kAdj && VEC == 8 ? at0[i] + 2 * j : at0[i] + j, e1 = kAdj && VEC == 8 ? e0 + 1 : at1[i] + j;
-        auto at = [&](int e) {
-          if (!ok) return 0.f;
-          return f32 ? __ldcg(static_cast<const float*>(w) + e) : to_f<kBF16>(__ldcg(static_cast<const uint16_t*>(w) + e));
-        };
-        p.a[VEC * i + j] = at(e0);
-        p.b[VEC * i + j] = at(e1);
+      for (int i = 0; i < 4; i += 2) {
+        const bool u = (live >> i) & 1u, v = (live >> (i + 1)) & 1u;
+        p.a[i / 2] = f2(u ? w.of(lane + 32 * i, 0) : 0.f, v ? w.of(lane + 32 * i + 32, 0) : 0.f);
+        p.b[i / 2] = f2(u ? w.of(lane + 32 * i, 1) : 0.f, v ? w.of(lane + 32 * i + 32, 1) : 0.f);
       }
+    } else {
+#pragma unroll
+      for (int q = 0; q < VEC / 4; ++q) {
+        const float4 x = w.w[q * Weights<VEC>::kChunks + lane], y = w.w[(VEC / 4 + q) * Weights<VEC>::kChunks + lane];
+        p.a[2 * q] = f2(x.x, x.y), p.a[2 * q + 1] = f2(x.z, x.w);
+        p.b[2 * q] = f2(y.x, y.y), p.b[2 * q + 1] = f2(y.z, y.w);
+      }
+    }
   }
   // The cosines and sines of the row's pairs at token (b, t).
-  __device__ __forceinline__ void angles(const fa4d_rotary_table& tab, const void* positions, int bits,
-                                         const int64_t (&ps)[3], int64_t b, int64_t t, int lane,
-                                         float (&cs)[kRowPairs<VEC>], float (&sn)[kRowPairs<VEC>]) const {
+  __device__ __forceinline__ void angles(const Turns<VEC>& turns, const void* positions, int bits, const int64_t (&ps)[3],
+                                         int64_t b, int64_t t, int lane, Turn<VEC>& out) const {
+    float cs[kRowPairs<VEC>], sn[kRowPairs<VEC>];
 #pragma unroll
     for (int i = 0; i < kRowChunks<VEC>; ++i)
       if ((turned >> i) & 1u) {
-        Chunk<VEC, kAdj> ch(tab, lane + 32 * i);
-        ch.turn_to(tab, positions, bits, ps, b, t, lane + 32 * i, false);
+        const int64_t here = b * ps[1] + t * ps[2];
+        uint64_t p = 0;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          cs[VEC * i + j] = ch.cs[j];
-          sn[VEC * i + j] = ch.sn[j];
+          const int at = turns.at(lane + 32 * i, j);
+          // Pairs beside one another mostly follow the same axis.
+          const int axis = turns.axis[at];
+          if (j == 0 || axis != turns.axis[turns.at(lane + 32 * i, j - 1)])
+            p = position_at(positions, bits, axis * ps[0] + here);
+          // Nearest multiple of 2^-32 turns, as a signed fraction of half a turn (see fa4d_rotary.cu).
+          const int32_t frac = static_cast<int32_t>((p * turns.turn[at] + 0x80000000ull) >> 32);
+          sincospif(static_cast<float>(frac) * 4.656612873077393e-10f, &sn[VEC * i + j], &cs[VEC * i + j]);  // 2^-31
         }
-      }
-  }
-  // Turned by the angles (sign 1) or back (sign -1).
-  __device__ __forceinline__ void turn(Pairs<VEC>& p, const float (&cs)[kRowPairs<VEC>], const float (&sn)[kRowPairs<VEC>],
-                                       float sign) const {
+      } else {
 #pragma unroll
-    for (int i = 0; i < kRowChunks<VEC>; ++i)
-      if ((turned >> i) & 1u) {
-#pragma unroll
-        for (int j = VEC * i; j < VEC * (i + 1); ++j) {
-          const float2 u = turned_pair(p.a[j], p.b[j], cs[j], sign * sn[j]);
-          p.a[j] = u.x;
-          p.b[j] = u.y;
-        }
+        for (int j = 0; j < VEC; ++j) cs[VEC * i + j] = 1.f, sn[VEC * i + j] = 0.f;
       }
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      out.c[j] = f2(cs[2 * j], cs[2 * j + 1]);
+      out.s[j] = f2(sn[2 * j], sn[2 * j + 1]);
+    }
   }
-  static __device__ __forceinline__ float2 turned_pair(float a, float b, float c, float s) { return fa4d::turned(a, b, c, s); }
+  // Chunks that are copied keep apart what the turn would mix: 0 * infinity is not a number.
+  __device__ __forceinline__ bool copied() const { return turned != live; }
 };
 
-template <bool kBF16, bool kAdj>
-__device__ __forceinline__ void unpack_pairs(const Raw<8>& r, Pairs<8>& p) {
-  const uint32_t* x = reinterpret_cast<const uint32_t*>(&r.x[0]);
-  const uint32_t* y = reinterpret_cast<const uint32_t*>(&r.y[0]);
+template <bool kBF16, bool kAdj, int VEC>
+__device__ __forceinline__ void unpack_pairs(const Raw<VEC>& r, Pairs<VEC>& p) {
+  if constexpr (VEC == 1) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float2 u = unpack2<kBF16>(x[w]), v = unpack2<kBF16>(y[w]);
-    if (kAdj) {
-      p.a[w] = u.x, p.b[w] = u.y;
-      p.a[w + 4] = v.x, p.b[w + 4] = v.y;
+    for (int i = 0; i < 4; i += 2) {
+      p.a[i / 2] = f2(to_f<kBF16>(r.x[i]), to_f<kBF16>(r.x[i + 1]));
+      p.b[i / 2] = f2(to_f<kBF16>(r.y[i]), to_f<kBF16>(r.y[i + 1]));
+    }
+  } else {
+    constexpr int W = VEC / 2;  // words of a run
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(&r.x[0]);
+    const uint32_t* y = reinterpret_cast<const uint32_t*>(&r.y[0]);
+    if constexpr (kAdj) {
+#pragma unroll
+      for (int w = 0; w < W; w += 2) {
+        const float2 u = unpack2<kBF16>(x[w]), v = unpack2<kBF16>(x[w + 1]), s = unpack2<kBF16>(y[w]), t = unpack2<kBF16>(y[w + 1]);
+        p.a[w / 2] = f2(u.x, v.x), p.b[w / 2] = f2(u.y, v.y);
+        p.a[(w + W) / 2] = f2(s.x, t.x), p.b[(w + W) / 2] = f2(s.y, t.y);
+      }
     } else {
-      p.a[2 * w] = u.x, p.a[2 * w + 1] = u.y;
-      p.b[2 * w] = v.x, p.b[2 * w + 1] = v.y;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float2 u = unpack2<kBF16>(x[w]), v = unpack2<kBF16>(y[w]);
+        p.a[w] = f2(u.x, u.y);
+        p.b[w] = f2(v.x, v.y);
+      }
     }
   }
 }
-template <bool kBF16, bool kAdj>
-__device__ __forceinline__ void unpack_pairs(const Raw<1>& r, Pairs<1>& p) {
+template <bool kBF16, bool kAdj, int VEC>
+__device__ __forceinline__ void pack_pairs(const Pairs<VEC>& p, Raw<VEC>& r) {
+  if constexpr (VEC == 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p.a[i] = to_f<kBF16>(r.x[i]);
-    p.b[i] = to_f<kBF16>(r.y[i]);
-  }
-}
-template <bool kBF16, bool kAdj>
-__device__ __forceinline__ void pack_pairs(const Pairs<8>& p, Raw<8>& r) {
-  uint32_t* x = reinterpret_cast<uint32_t*>(&r.x[0]);
-  uint32_t* y = reinterpret_cast<uint32_t*>(&r.y[0]);
+    for (int i = 0; i < 4; i += 2) {
+      const float2 a = f2_split(p.a[i / 2]), b = f2_split(p.b[i / 2]);
+      r.x[i] = to_h<kBF16>(a.x), r.x[i + 1] = to_h<kBF16>(a.y);
+      r.y[i] = to_h<kBF16>(b.x), r.y[i + 1] = to_h<kBF16>(b.y);
+    }
+  } else {
+    constexpr int W = VEC / 2;
+    uint32_t* x = reinterpret_cast<uint32_t*>(&r.x[0]);
+    uint32_t* y = reinterpret_cast<uint32_t*>(&r.y[0]);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    x[w] = kAdj ? pack2<kBF16>(p.a[w], p.b[w]) : pack2<kBF16>(p.a[2 * w], p.a[2 * w + 1]);
-    y[w] = kAdj ? pack2<kBF16>(p.a[w + 4], p.b[w + 4]) : pack2<kBF16>(p.b[2 * w], p.b[2 * w + 1]);
-  }
-}
-template <bool kBF16, bool kAdj>
-__device__ __forceinline__ void pack_pairs(const Pairs<1>& p, Raw<1>& r) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r.x[i] = to_h<kBF16>(p.a[i]);
-    r.y[i] = to_h<kBF16>(p.b[i]);
+    for (int j = 0; j < W; ++j) {
+      const float2 a = f2_split(p.a[j]), b = f2_split(p.b[j]);
+      if constexpr (kAdj) {
+        uint32_t* z = j < W / 2 ? x + 2 * j : y + 2 * j - W;
+        z[0] = pack2<kBF16>(a.x, b.x);
+        z[1] = pack2<kBF16>(a.y, b.y);
+      } else {
+        x[j] = pack2<kBF16>(a.x, a.y);
+        y[j] = pack2<kBF16>(b.x, b.y);
+      }
+    }
   }
 }
 
-// The heads [first, end) of a token, normalised (w; null: not) and turned.
+// The heads [first, end) of a token, normalised (weights; null: not) and turned.
 // kHeads rows' loads are in flight together.
 template <bool kBF16, bool kAdj, int VEC, int kHeads>
-__device__ __forceinline__ void norm_heads(const fa4d_rotary_table& tab, const RowLane<VEC, kAdj>& at, const Pairs<VEC>* w,
+__device__ __forceinline__ void norm_heads(const fa4d_rotary_table& tab, const Turns<VEC>& turns, const RowLane<VEC, kAdj>& at, const Weights<VEC>* weights,
                                            float eps, int lanes, int lane, bool live, const uint16_t* src, int64_t src_head,
                                            uint16_t* dst, int64_t dst_head, int first, int end, const void* positions, int bits,
                                            const int64_t (&ps)[3], int64_t b, int64_t t) {
-  float cs[kRowPairs<VEC>], sn[kRowPairs<VEC>];
+  Factors<VEC> factors;
+  const bool copied = at.copied();
   for (int h0 = first; h0 < end; h0 += kHeads) {
     Raw<VEC> raw[kHeads];
 #pragma unroll
     for (int u = 0; u < kHeads; ++u)
       if (live && h0 + u < end) at.load(src + (h0 + u) * src_head, raw[u]);
     // The angles, while the first heads are on their way.
-    if (h0 == first && live) at.angles(tab, positions, bits, ps, b, t, lane, cs, sn);
+    if (h0 == first && live) {
+      Turn<VEC> turn;
+      at.angles(turns, positions, bits, ps, b, t, lane, turn);
+      Pairs<VEC> w;
+      if (weights) at.weights(*weights, lane, w);
+      factors.set(turn, weights ? &w : nullptr);
+    }
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       Pairs<VEC> p;
       unpack_pairs<kBF16, kAdj>(raw[u], p);
-      if (w) {
-        const float r = rsqrtf(row_sum(p.squares(), lanes) * (1.f / tab.D) + eps);
-#pragma unroll
-        for (int j = 0; j < kRowPairs<VEC>; ++j) {
-          p.a[j] = p.a[j] * r * w->a[j];
-          p.b[j] = p.b[j] * r * w->b[j];
-        }
-      }
+      if (weights) p.times(rsqrtf(row_sum(p.squares(), lanes) * (1.f / tab.D) + eps));
       if (!live || h0 + u >= end) continue;
-      at.turn(p, cs, sn, 1.f);
+      factors.turn(p, copied);
       pack_pairs<kBF16, kAdj>(p, raw[u]);
       at.store(dst + (h0 + u) * dst_head, raw[u]);
     }

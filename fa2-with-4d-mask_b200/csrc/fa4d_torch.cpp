@@ -325,36 +325,40 @@ std::pair<Tensor, Tensor> norm_rotate(Tensor q, Tensor k, const Tensor& wq, cons
   return {qo, ko};
 }
 
-// The gradient of NormRotate, which has none of its own.
+torch::autograd::variable_list norm_rotate_grad(Tensor dq, Tensor dk, Tensor q, Tensor k, const Tensor& wq, const Tensor& wk,
+                                                const Tensor& positions, const Table& table, Layout l, double eps) {
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  q = unit_rows(q);
+  k = unit_rows(k);
+  dq = unit_rows(dq);
+  dk = unit_rows(dk);
+  Tensor dxq = new_rows(q), dxk = new_rows(k);
+  if (no_tokens(q, k)) return {dxq, dxk, at::zeros_like(wq), at::zeros_like(wk)};
+  const Tensor cq = wq.contiguous(), ck = wk.contiguous();
+  Tensor dwq = at::empty_like(cq), dwk = at::empty_like(ck);
+  fa4d_norm_rotary_bwd_args a;
+  set_rotary(a.rotary, q, k, dxq, dxk, positions, table, l, false);
+  set_norm(a.norm, cq, ck, eps);
+  a.dq = dq.data_ptr();
+  a.dk = dk.data_ptr();
+  set3(a.dq_stride, dq, l);
+  set3(a.dk_stride, dk, l);
+  a.q_weight_grad = dwq.data_ptr();
+  a.k_weight_grad = dwk.data_ptr();
+  const fa4d_rotary_args& r = a.rotary;
+  a.workspace_bytes = fa4d_norm_rotary_bwd_workspace(r.B, r.T, r.Hq, r.Hk, r.table.D);
+  const Tensor workspace = at::empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
+  a.workspace = workspace.data_ptr();
+  check(fa4d_norm_rotary_bwd(&a, stream_of(q)), "fa4d_norm_rotary_bwd");
+  return {dxq, dxk, dwq, dwk};
+}
+
+// The gradient of NormRotate where it is itself part of a graph: it has none of its own.
 struct NormRotateGrad : torch::autograd::Function<NormRotateGrad> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, Tensor dq, Tensor dk, Tensor q, Tensor k,
-                                                const Tensor& wq, const Tensor& wk, const Tensor& positions, Capsule table,
-                                                bool bhsd, double eps) {
-    const Layout l{bhsd};
-    const c10::cuda::OptionalCUDAGuard guard(q.device());
-    q = unit_rows(q);
-    k = unit_rows(k);
-    dq = unit_rows(dq);
-    dk = unit_rows(dk);
-    Tensor dxq = new_rows(q), dxk = new_rows(k);
-    if (no_tokens(q, k)) return {dxq, dxk, at::zeros_like(wq), at::zeros_like(wk)};
-    const Tensor cq = wq.contiguous(), ck = wk.contiguous();
-    Tensor dwq = at::empty_like(cq), dwk = at::empty_like(ck);
-    fa4d_norm_rotary_bwd_args a;
-    set_rotary(a.rotary, q, k, dxq, dxk, positions, static_cast<const Table&>(*table), l, false);
-    set_norm(a.norm, cq, ck, eps);
-    a.dq = dq.data_ptr();
-    a.dk = dk.data_ptr();
-    set3(a.dq_stride, dq, l);
-    set3(a.dk_stride, dk, l);
-    a.q_weight_grad = dwq.data_ptr();
-    a.k_weight_grad = dwk.data_ptr();
-    const fa4d_rotary_args& r = a.rotary;
-    a.workspace_bytes = fa4d_norm_rotary_bwd_workspace(r.B, r.T, r.Hq, r.Hk, r.table.D);
-    const Tensor workspace = at::empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
-    a.workspace = workspace.data_ptr();
-    check(fa4d_norm_rotary_bwd(&a, stream_of(q)), "fa4d_norm_rotary_bwd");
-    return {dxq, dxk, dwq, dwk};
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const Tensor& dq, const Tensor& dk,
+                                                const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk,
+                                                const Tensor& positions, Capsule table, bool bhsd, double eps) {
+    return norm_rotate_grad(dq, dk, q, k, wq, wk, positions, static_cast<const Table&>(*table), Layout{bhsd}, eps);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
     TORCH_CHECK(false, "MultiAxisRotary with norms cannot be differentiated twice");
@@ -375,9 +379,16 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     const auto saved = ctx->get_saved_variables();
     auto table = ctx->saved_data["table"].toCapsule();
+    const bool bhsd = ctx->saved_data["bhsd"].toBool();
+    const double eps = ctx->saved_data["eps"].toDouble();
     try {
-      auto out = NormRotateGrad::apply(g[0], g[1], saved[0], saved[1], saved[2], saved[3], saved[4], table,
-                                       ctx->saved_data["bhsd"].toBool(), ctx->saved_data["eps"].toDouble());
+      // Mostly no graph of the gradient is wanted, and a function of its own would cost as much as its kernels.
+      const bool tangent = c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+                           (g[0]._fw_grad(0).defined() || g[1]._fw_grad(0).defined());
+      auto out = !at::GradMode::is_enabled() && !tangent
+                     ? norm_rotate_grad(g[0], g[1], saved[0], saved[1], saved[2], saved[3], saved[4],
+                                        static_cast<const Table&>(*table), Layout{bhsd}, eps)
+                     : NormRotateGrad::apply(g[0], g[1], saved[0], saved[1], saved[2], saved[3], saved[4], table, bhsd, eps);
       return {out[0], out[1], out[2], out[3], Tensor(), Tensor(), Tensor(), Tensor()};
     } catch (const Refused& e) {  // the engine's thread only knows torch's errors
       TORCH_CHECK(false, e.text);
