@@ -17,9 +17,9 @@ constexpr int kRows = 16;  // rows of a block
 // The blocks of a grid: first those of the caches, then q's.
 struct AppendGrid {
   int chunks, lanes;
-  int cache_blocks;
-  int spans;                // 8-bit caches: 64-slot blocks that T tokens can touch
-  int groups;               // of kRows tokens
+  uint32_t cache_blocks;
+  uint32_t spans;                // 8-bit caches: 64-slot blocks that T tokens can touch
+  uint32_t groups;          // of kRows tokens
   int q_each, k_each;       // heads of a block, of q and (16-bit caches) of k and of v
   int q_parts, k_parts;
 };
@@ -35,19 +35,18 @@ __device__ __forceinline__ void settle_length(const fa4d_rotary_append_args& a, 
 }
 
 // q's rows: a group of tokens and a range of heads.
-template <bool kBF16, bool kAdj, int VEC>
+template <bool kBF16, bool kAdj, int VEC, int kHeads>
 __device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, const Turns<VEC>& turns, const Weights<VEC>& shared_w,
-                                         const AppendGrid& g, int id) {
+                                         const AppendGrid& g, uint32_t id) {
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1);
-  const int64_t n = static_cast<int64_t>(id % g.groups) * kRows + threadIdx.x / g.lanes;
+  const uint32_t n = static_cast<uint32_t>(id % g.groups) * kRows + threadIdx.x / g.lanes, T = a.T, b = n / T, t = n - b * T;
   const int first = id / g.groups * g.q_each;
-  const bool live = n < static_cast<int64_t>(a.B) * a.T;
-  const int64_t b = n / a.T, t = n - b * a.T;
+  const bool live = n < a.B * T;
   const RowLane<VEC, kAdj> at(a.table, lane, g.chunks);
   const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1];
   uint16_t* dst = static_cast<uint16_t*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1];
-  norm_heads<kBF16, kAdj, VEC, 4>(a.table, turns, at, args.norm.q_weight ? &shared_w : nullptr, args.norm.eps, g.lanes, lane, live, src,
+  norm_heads<kBF16, kAdj, VEC, kHeads>(a.table, turns, at, args.norm.q_weight ? &shared_w : nullptr, args.norm.eps, g.lanes, lane, live, src,
                                   a.q_stride[2], dst, a.q_out_stride[2], first, min(first + g.q_each, a.Hq), a.positions,
                                   a.positions_bits, a.positions_stride, b, t);
 }
@@ -63,19 +62,18 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
   pdl_wait();
   pdl_launch();
   __shared__ Weights<VEC> shared_w;
-  int id = blockIdx.x;
+  uint32_t id = blockIdx.x;
   shared_w.template fill<kBF16, kAdj>(args.append.table, id >= g.cache_blocks ? args.norm.q_weight : args.norm.k_weight,
                                       args.norm.weight_f32 != 0);
   __syncthreads();
-  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, turns, shared_w, g, id - g.cache_blocks);
+  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC, 2>(args, turns, shared_w, g, id - g.cache_blocks);
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1);
   const bool is_v = id >= g.cache_blocks / 2;
   id -= is_v ? g.cache_blocks / 2 : 0;
-  const int64_t n = static_cast<int64_t>(id % g.groups) * kRows + threadIdx.x / g.lanes;
+  const uint32_t n = static_cast<uint32_t>(id % g.groups) * kRows + threadIdx.x / g.lanes, T = a.T, b = n / T, t = n - b * T;
   const int first = id / g.groups * g.k_each, end = min(first + g.k_each, a.Hk);
-  bool live = n < static_cast<int64_t>(a.B) * a.T;
-  const int64_t b = n / a.T, t = n - b * a.T;
+  bool live = n < a.B * T;
   const int64_t had = live ? entries_of(a, b) : 0, slot = had + t;
   if (live && !is_v && first == 0 && t == 0 && lane == 0) settle_length(a, b, had, status);
   live = live && slot < a.C;
@@ -94,7 +92,7 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
   }
   const uint16_t* src = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1];
   uint16_t* dst = static_cast<uint16_t*>(a.k_cache) + b * a.k_cache_stride[0] + slot * a.k_cache_stride[1];
-  norm_heads<kBF16, kAdj, VEC, 4>(a.table, turns, at, &shared_w, args.norm.eps, g.lanes, lane, live, src, a.k_stride[2], dst,
+  norm_heads<kBF16, kAdj, VEC, 2>(a.table, turns, at, &shared_w, args.norm.eps, g.lanes, lane, live, src, a.k_stride[2], dst,
                                   a.k_cache_stride[2], first, end, a.positions, a.positions_bits, a.positions_stride, b, t);
 }
 
@@ -105,29 +103,26 @@ template <bool kBF16, bool kAdj, int VEC, bool kInt8>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                       const __grid_constant__ AppendGrid g, int* status) {
   constexpr int P = kRowPairs<VEC>;
-  extern __shared__ float values[];  // [pass][2 P][threads]
+  extern __shared__ uint4 values[];  // [pass][P / 2][threads]: four values, two pairs
   __shared__ uint32_t block_most;
   __shared__ Turns<VEC> turns;
+  uint32_t id = blockIdx.x;
+  const bool is_v = id < g.cache_blocks && (id & 1);
   if (threadIdx.x == 0) block_most = 0;
-  turns.template fill<kAdj>(args.append.table);
-  __syncthreads();
+  if (!is_v) turns.template fill<kAdj>(args.append.table);
   pdl_wait();
   pdl_launch();
   __shared__ Weights<VEC> shared_w;
-  int64_t id = blockIdx.x;
-  if (args.norm.q_weight)
+  if (!is_v && args.norm.q_weight)
     shared_w.template fill<kBF16, kAdj>(args.append.table, id >= g.cache_blocks ? args.norm.q_weight : args.norm.k_weight,
                                         args.norm.weight_f32 != 0);
   __syncthreads();
-  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC>(args, turns, shared_w, g, static_cast<int>(id - g.cache_blocks));
+  if (id >= g.cache_blocks) return append_q<kBF16, kAdj, VEC, 4>(args, turns, shared_w, g, id - g.cache_blocks);
   const fa4d_rotary_append_args& a = args.append;
   const int lane = threadIdx.x & (g.lanes - 1), row = threadIdx.x / g.lanes, threads = blockDim.x;
-  const bool is_v = id & 1;
   id >>= 1;
-  const int span = static_cast<int>(id % g.spans);
-  id /= g.spans;
-  const int h = static_cast<int>(id % a.Hk);
-  const int64_t b = id / a.Hk;
+  const uint32_t row_of = id / g.spans, b = row_of / a.Hk;
+  const int span = id - row_of * g.spans, h = row_of - b * a.Hk;
   const int64_t had = entries_of(a, b);
   if (h == 0 && span == 0 && !is_v && threadIdx.x == 0) settle_length(a, b, had, status);
   const int64_t block = had / FA4D_CACHE_BLOCK + span, start = block * FA4D_CACHE_BLOCK;
@@ -143,39 +138,38 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
   const uint16_t* x = static_cast<const uint16_t*>(is_v ? a.v : a.k) + b * xs[0] + h * xs[2];
   const RowLane<VEC, kAdj> at(a.table, lane, g.chunks);
   const bool norm = !is_v && args.norm.k_weight;
-  uint32_t most = 0;
+  float largest = 0.f;
   const int count = static_cast<int>(to - from);
+  Raw<VEC> raw;
+  if (row < count) at.load(x + (from - had + row) * xs[1], raw);
 #pragma unroll 1
   for (int i0 = 0; i0 < count; i0 += kRows) {
     const bool live = i0 + row < count;
     const int64_t t = from - had + i0 + row;
-    Raw<VEC> raw;
-    if (live) at.load(x + t * xs[1], raw);
     Pairs<VEC> p;
     unpack_pairs<kBF16, kAdj>(raw, p);
-    if (norm) p.times(rsqrtf(row_sum(p.squares(), g.lanes) * (1.f / a.table.D) + args.norm.eps));
+    if (i0 + kRows + row < count) at.load(x + (t + kRows) * xs[1], raw);  // on its way meanwhile
+    if (norm) {
+      p.times(rsqrtf(row_sum(p.squares(), g.lanes) * (1.f / a.table.D) + args.norm.eps));
+      Pairs<VEC> w;
+      at.weights(shared_w, lane, w);
+      p.times(w);
+    }
     if (!live) continue;
     if (!is_v) {
       Turn<VEC> turn;
       at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
-      Pairs<VEC> w;
-      if (norm) at.weights(shared_w, lane, w);
-      Factors<VEC> factors;
-      factors.set(turn, norm ? &w : nullptr);
-      factors.turn(p, at.copied());
+      turn.on(p, at.copied());
     }
-    float* v = values + i0 / kRows * (2 * P) * threads + threadIdx.x;
+    uint4* v = values + i0 / kRows * (P / 2) * threads + threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      // Dead chunks hold zeros.
-      const float2 u = f2_split(p.a[j / 2]), z = f2_split(p.b[j / 2]);
-      const float x0 = j & 1 ? u.y : u.x, x1 = j & 1 ? z.y : z.x;
-      most = max(most, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu));
-      v[j * threads] = x0;
-      v[(P + j) * threads] = x1;
+    for (int j = 0; j < P / 2; ++j) {
+      const float2 x0 = f2_split(p.a[j]), x1 = f2_split(p.b[j]);  // chunks past the last are zeros
+      largest = max_abs_nan(max_abs_nan(largest, x0.x, x0.y), x1.x, x1.y);
+      v[j * threads] = make_uint4(__float_as_uint(x0.x), __float_as_uint(x0.y), __float_as_uint(x1.x), __float_as_uint(x1.y));
     }
   }
-  most = __reduce_max_sync(0xffffffffu, most);
+  uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));  // NaN is above infinity
   if ((threadIdx.x & 31) == 0 && most) atomicMax(&block_most, most);
   __syncthreads();
   most = block_most;
@@ -202,16 +196,21 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
     }
   }
   const bool number = scale == scale;  // codes under a scale that is not are 0
-  const float inverse = 1.f / scale;
+  const float inverse = number ? 1.f / scale : 0.f;
+  const uint64_t inverse2 = f2(inverse, inverse);
 #pragma unroll 1
   for (int i0 = 0; i0 + row < count; i0 += kRows) {
-    const float* v = values + i0 / kRows * (2 * P) * threads + threadIdx.x;
+    const uint4* v = values + i0 / kRows * (P / 2) * threads + threadIdx.x;
     uint8_t* dst = cache + (from + i0 + row) * st[1];
     float u[P], z[P];
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      u[j] = number ? v[j * threads] * inverse : 0.f;
-      z[j] = number ? v[(P + j) * threads] * inverse : 0.f;
+    for (int j = 0; j < P / 2; ++j) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (number) x = v[j * threads];
+      const float2 a2 = f2_split(fmul2(f2(__uint_as_float(x.x), __uint_as_float(x.y)), inverse2));
+      const float2 b2 = f2_split(fmul2(f2(__uint_as_float(x.z), __uint_as_float(x.w)), inverse2));
+      u[2 * j] = a2.x, u[2 * j + 1] = a2.y;
+      z[2 * j] = b2.x, z[2 * j + 1] = b2.y;
     }
     if constexpr (VEC == 8) {
       if (!at.live) continue;
@@ -236,39 +235,61 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
   }
 }
 
-// One thread: 16 codes of a slot and head.  Bound by memory: 1 byte read and 2 written an element.
+// n / d for n below 2^31 and d from 1: n * mul / 2^(32 + shift), with mul = ceil(2^(32 + shift) / d),
+// 2^shift >= d / 2 (then mul < 2^32, and what it is too large by, times n, stays below 2^(32 + shift) / d).
+struct Divisor {
+  uint32_t mul, shift, d;
+  explicit Divisor(uint32_t by) : mul(0), shift(0), d(by) {
+    if (d == 1) return;
+    while ((2u << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << (32 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+
+// One thread: kPieces times 8 codes, a block's threads apart, whose loads are in flight together.
+// Bound by memory: 1 byte read and 2 written an element.
+constexpr int kPieces = 4, kValuesThreads = 128;
 template <bool kBF16, bool kInt8>
-__global__ void __launch_bounds__(256) cache_values_kernel(const __grid_constant__ fa4d_cache_values_args a, int parts) {
+__global__ void __launch_bounds__(kValuesThreads) cache_values_kernel(const __grid_constant__ fa4d_cache_values_args a, Divisor parts,
+                                                           Divisor inner, bool heads_inner, uint32_t pieces) {
   pdl_wait();
   pdl_launch();
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
   const int64_t b = blockIdx.y;
-  // In the order of out's memory: heads within a slot where their stride is the smaller one.
-  const bool heads_inner = a.out_stride[2] < a.out_stride[1];
-  const uint32_t row = id / parts, part = id - row * parts;
-  const uint32_t inner = heads_inner ? a.Hk : a.C;
-  const uint32_t o = row / inner, i = row - o * inner;
-  if (o >= static_cast<uint32_t>(heads_inner ? a.C : a.Hk)) return;
-  const int64_t slot = heads_inner ? o : i, h = heads_inner ? i : o;
-  uint4 out[2] = {};
-  if (slot < __ldcg(a.lengths + b)) {
-    const uint4 c = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.codes) + b * a.codes_stride[0] +
-                                                          slot * a.codes_stride[1] + h * a.codes_stride[2]) + part);
-    const float scale = __ldcg(a.scale + b * a.scale_stride[0] + h * a.scale_stride[1] + slot / FA4D_CACHE_BLOCK);
-    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-    uint32_t* to = reinterpret_cast<uint32_t*>(out);
+  const int64_t length = __ldcg(a.lengths + b);
+  const uint8_t* codes = static_cast<const uint8_t*>(a.codes) + b * a.codes_stride[0];
+  const float* scales = a.scale + b * a.scale_stride[0];
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_stride[0];
+  const uint32_t first = blockIdx.x * (kValuesThreads * kPieces) + threadIdx.x;
+  uint2 c[kPieces];
+  float scale[kPieces];
+  int64_t to[kPieces];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float f[4];
-      codes_to_float<kInt8>(words[k], f);
-      to[2 * k] = pack2<kBF16>(f[0] * scale, f[1] * scale);
-      to[2 * k + 1] = pack2<kBF16>(f[2] * scale, f[3] * scale);
-    }
+  for (int k = 0; k < kPieces; ++k) {
+    const uint32_t id = first + kValuesThreads * k, row = parts.of(id), part = id - row * parts.d;
+    const uint32_t o = inner.of(row), i = row - o * inner.d;
+    const int64_t slot = heads_inner ? o : i, h = heads_inner ? i : o;
+    c[k] = make_uint2(0, 0);
+    scale[k] = 0.f;
+    if (id >= pieces) continue;
+    to[k] = slot * a.out_stride[1] + h * a.out_stride[2] + 8 * part;
+    if (slot >= length) continue;
+    c[k] = __ldcg(reinterpret_cast<const uint2*>(codes + slot * a.codes_stride[1] + h * a.codes_stride[2]) + part);
+    scale[k] = __ldcg(scales + h * a.scale_stride[1] + slot / FA4D_CACHE_BLOCK);
   }
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + b * a.out_stride[0] + slot * a.out_stride[1] +
-                                        h * a.out_stride[2]) + 2 * part;
-  dst[0] = out[0];
-  dst[1] = out[1];
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    if (first + kValuesThreads * k >= pieces) continue;
+    float f[4], g[4];
+    codes_to_float<kInt8>(c[k].x, f);
+    codes_to_float<kInt8>(c[k].y, g);
+    uint4 v;
+    v.x = pack2<kBF16>(f[0] * scale[k], f[1] * scale[k]);
+    v.y = pack2<kBF16>(f[2] * scale[k], f[3] * scale[k]);
+    v.z = pack2<kBF16>(g[0] * scale[k], g[1] * scale[k]);
+    v.w = pack2<kBF16>(g[2] * scale[k], g[3] * scale[k]);
+    *reinterpret_cast<uint4*>(out + to[k]) = v;
+  }
 }
 
 template <int VEC, bool kBF16, bool kAdj>
@@ -279,11 +300,11 @@ cudaError_t launch_append_t(const fa4d_norm_append_args& args, int sms, int* sta
   g.lanes = std::max(row_lanes(a.table, VEC), 2);  // whole warps
   const int threads = kRows * g.lanes;
   const int64_t tokens = static_cast<int64_t>(a.B) * a.T;
-  g.groups = static_cast<int>((tokens + kRows - 1) / kRows);
-  // One head a block until the blocks fill the GPU, then up to 8, which share the angles.
+  g.groups = static_cast<uint32_t>((tokens + kRows - 1) / kRows);
+  // One head a block until the blocks fill the GPU, then up to 16, which share the angles.
   auto each = [&](int heads) {
     int e = 1;
-    while (e < 8 && static_cast<int64_t>(g.groups) * heads / (2 * e) >= 8LL * sms) e *= 2;
+    while (e < 16 && static_cast<int64_t>(g.groups) * heads / (2 * e) >= 4LL * sms) e *= 2;
     return e;
   };
   g.q_each = each(a.Hq);
@@ -300,12 +321,12 @@ cudaError_t launch_append_t(const fa4d_norm_append_args& args, int sms, int* sta
     cache_blocks = 2LL * a.B * a.Hk * g.spans;
   }
   if (cache_blocks + q_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  g.cache_blocks = static_cast<int>(cache_blocks);
+  g.cache_blocks = static_cast<uint32_t>(cache_blocks);
   const dim3 grid(static_cast<unsigned>(cache_blocks + q_blocks));
   if (args.cache_type == FA4D_CACHE_16BIT)
     return launch_chained(norm_append_kernel<kBF16, kAdj, VEC>, grid, threads, 0, 1, s, args, g, status);
   const int passes = std::min((a.T + kRows - 1) / kRows, FA4D_CACHE_BLOCK / kRows);
-  const size_t smem = static_cast<size_t>(passes) * 2 * kRowPairs<VEC> * threads * sizeof(float);
+  const size_t smem = static_cast<size_t>(passes) * (kRowPairs<VEC> / 2) * threads * sizeof(uint4);
   auto kern = args.cache_type == FA4D_CACHE_INT8 ? append8_kernel<kBF16, kAdj, VEC, true> : append8_kernel<kBF16, kAdj, VEC, false>;
   if (smem > 32 * 1024) {  // with what is static, 48 KB need no leave
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
@@ -327,13 +348,15 @@ cudaError_t launch_norm_append(const fa4d_norm_append_args& a, bool vec, int sms
 }
 
 cudaError_t launch_cache_values(const fa4d_cache_values_args& a, cudaStream_t s) {
-  const int parts = a.D / 16;
-  const int64_t threads = static_cast<int64_t>(a.C) * a.Hk * parts;  // fewer than 2^31, B at most 65535
-  const dim3 grid(static_cast<unsigned>((threads + 255) / 256), a.B);
+  // In the order of out's memory: heads within a slot where their stride is the smaller one.
+  const bool heads_inner = a.out_stride[2] < a.out_stride[1];
+  const Divisor parts(a.D / 8), inner(heads_inner ? a.Hk : a.C);
+  const uint32_t pieces = static_cast<uint32_t>(static_cast<int64_t>(a.C) * a.Hk * (a.D / 8));  // fewer than 2^31 - 1024
+  const dim3 grid((pieces + kValuesThreads * kPieces - 1) / (kValuesThreads * kPieces), a.B);
   const bool bf16 = a.dtype == FA4D_BF16, i8 = a.cache_type == FA4D_CACHE_INT8;
   auto kern = bf16 ? (i8 ? cache_values_kernel<true, true> : cache_values_kernel<true, false>)
                    : (i8 ? cache_values_kernel<false, true> : cache_values_kernel<false, false>);
-  return launch_chained(kern, grid, 256, 0, 1, s, a, parts);
+  return launch_chained(kern, grid, kValuesThreads, 0, 1, s, a, parts, inner, heads_inner, pieces);
 }
 
 }  // namespace fa4d

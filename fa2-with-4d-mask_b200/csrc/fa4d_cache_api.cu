@@ -443,8 +443,8 @@ int fa4d_cache_values(const fa4d_cache_values_args* a, void* stream) {
   if (!a->codes || !a->scale || !a->lengths || !a->out) return fail(FA4D_ERR_INVALID, "every pointer is required");
   if (a->B < 1 || a->C < 1 || a->Hk < 1 || a->D < 16 || a->D % 16)
     return fail(FA4D_ERR_INVALID, "sizes must be positive, D a multiple of 16 (B=%d C=%d Hk=%d D=%d)", a->B, a->C, a->Hk, a->D);
-  if (a->B > 65535 || static_cast<int64_t>(a->C) * a->Hk > (1LL << 35) / a->D)
-    return fail(FA4D_ERR_UNSUPPORTED, "cache too large (B <= 65535, C * Hk * D <= 2^35)");
+  if (a->B > 65535 || static_cast<int64_t>(a->C) * a->Hk > (1LL << 33) / a->D)
+    return fail(FA4D_ERR_UNSUPPORTED, "cache too large (B <= 65535, C * Hk * D <= 2^33)");
   if (!codes16(a->codes, a->codes_stride)) return fail(FA4D_ERR_LAYOUT, "codes: rows must start on 16-byte boundaries");
   if (!rows16(a->out, a->out_stride, 3)) return fail(FA4D_ERR_LAYOUT, "out: rows must start on 16-byte boundaries");
   if ((rc = host_bind_device_of(a->codes, "codes"))) return rc;

@@ -197,9 +197,10 @@ __global__ void __launch_bounds__(kThreads, kFwdPerSm) norm_rotary_kernel(
       if (live) {
         Turn<VEC> turn;
         at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
+        factors.set(turn);
         Pairs<VEC> w;
         at.weights(weights, lane, w);
-        factors.set(turn, &w);
+        factors.weigh(w);
       }
     }
     Pairs<VEC> p;

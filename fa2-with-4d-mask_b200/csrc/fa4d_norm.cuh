@@ -73,6 +73,13 @@ struct Pairs {
     const float2 t = f2_split(s);
     return t.x + t.y;
   }
+  __device__ __forceinline__ void times(const Pairs& w) {
+#pragma unroll
+    for (int j = 0; j < kTwo; ++j) {
+      a[j] = fmul2(a[j], w.a[j]);
+      b[j] = fmul2(b[j], w.b[j]);
+    }
+  }
   __device__ __forceinline__ void times(float r) {
     const uint64_t rr = f2(r, r);
 #pragma unroll
@@ -89,12 +96,43 @@ struct Raw {
   typename Run<VEC>::T x[kRowChunks<VEC>], y[kRowChunks<VEC>];
 };
 
+// Cosines and sines of two angles, each in 2^-32 turns, packed: y, what is left beside the nearest
+// quarter turn (at most 1/8, rounded to 24 bits), goes to polynomials in y^2, sin(2 pi y) = y S(y^2) and
+// cos(2 pi y) = 1 + y^2 C(y^2), and the quarter swaps them and sets their signs.  The coefficients
+// were fitted for this library (least squares on Chebyshev nodes, reweighted toward the minimax; 3e-9
+// and 3e-10 off); with the arithmetic's rounding the results are off by at most 1.1e-7 (2^-23), over
+// 2 million angles.  About 20 instructions an angle: with sincospif, whose argument has to hold whole
+// half turns as well, angles were a third of what these kernels execute.
+__device__ __forceinline__ void cos_sin2(uint32_t f0, uint32_t f1, uint64_t& c, uint64_t& s) {
+  const uint32_t q0 = f0 + 0x20000000u, q1 = f1 + 0x20000000u;  // the nearest quarter in the top two bits
+  const int32_t r0 = static_cast<int32_t>(f0 - (q0 & 0xC0000000u)), r1 = static_cast<int32_t>(f1 - (q1 & 0xC0000000u));
+  auto both = [](float x) { return f2(x, x); };
+  const uint64_t y = fmul2(f2(static_cast<float>(r0), static_cast<float>(r1)), both(2.3283064365386963e-10f));  // 2^-32
+  const uint64_t u = fmul2(y, y);
+  uint64_t S = ffma2(both(-75.40207f), u, both(81.59255f));
+  S = fmul2(ffma2(ffma2(S, u, both(-41.341663f)), u, both(6.2831855f)), y);
+  uint64_t C = ffma2(both(59.475986f), u, both(-85.4502f));
+  C = ffma2(ffma2(ffma2(C, u, both(64.93938f)), u, both(-19.739208f)), u, both(1.f));
+  const float2 si = f2_split(S), co = f2_split(C);
+  auto place = [](uint32_t q, float si, float co, float& cq, float& sq) {
+    const bool swap = q & 0x40000000u;
+    sq = __uint_as_float(__float_as_uint(swap ? co : si) ^ (q & 0x80000000u));
+    cq = __uint_as_float(__float_as_uint(swap ? si : co) ^ ((q + 0x40000000u) & 0x80000000u));
+  };
+  float c0, c1, s0, s1;
+  place(q0, si.x, co.x, c0, s0);
+  place(q1, si.y, co.y, c1, s1);
+  c = f2(c0, c1);
+  s = f2(s0, s1);
+}
+
 // The table's turns and axes in shared memory, laid so that the lanes of a row read neighbours (a
 // kernel parameter is read one address at a time).
 template <int VEC>
 struct Turns {
   uint64_t turn[FA4D_ROTARY_MAX_PAIRS];
   uint8_t axis[FA4D_ROTARY_MAX_PAIRS];
+  uint8_t several[FA4D_ROTARY_MAX_PAIRS / VEC];  // whether a chunk's pairs follow several axes
   static constexpr int kChunks = FA4D_ROTARY_MAX_PAIRS / VEC;
   static __device__ __forceinline__ int at(int chunk, int j) { return j * kChunks + chunk; }
   // All threads of the block; a barrier follows.
@@ -102,10 +140,17 @@ struct Turns {
   __device__ __forceinline__ void fill(const fa4d_rotary_table& tab) {
     for (int i = threadIdx.x; i < tab.rotary_dim / 2; i += blockDim.x) {
       const int c = i / VEC, j = i % VEC;
-      const PairAt<VEC, kAdj> e(tab, c, j);
-      const int pair = kAdj ? e.e0 / 2 : e.e0;
-      turn[at(c, j)] = tab.turn[pair];
-      axis[at(c, j)] = tab.axis[pair];
+      auto pair = [&](int k) {
+        const PairAt<VEC, kAdj> e(tab, c, k);
+        return kAdj ? e.e0 / 2 : e.e0;
+      };
+      turn[at(c, j)] = tab.turn[pair(j)];
+      axis[at(c, j)] = tab.axis[pair(j)];
+      if (j == 0) {
+        bool differ = false;
+        for (int k = 1; k < VEC; ++k) differ = differ || tab.axis[pair(k)] != tab.axis[pair(0)];
+        several[c] = differ;
+      }
     }
   }
 };
@@ -155,6 +200,20 @@ __device__ __forceinline__ uint64_t mix_apart(uint64_t a, uint64_t A, uint64_t b
 template <int VEC>
 struct Turn {
   uint64_t c[kRowPairs<VEC> / 2], s[kRowPairs<VEC> / 2];
+  // Turned in place; `copied` as for back.
+  __device__ __forceinline__ void on(Pairs<VEC>& p, bool copied) const {
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      const uint64_t a = p.a[j], b = p.b[j];
+      if (copied) {
+        p.a[j] = mix_apart(a, c[j], b, minus(s[j]));
+        p.b[j] = mix_apart(b, c[j], a, s[j]);
+      } else {
+        p.a[j] = ffma2(a, c[j], fmul2(b, minus(s[j])));
+        p.b[j] = ffma2(b, c[j], fmul2(a, s[j]));
+      }
+    }
+  }
   // Turned back.  `copied`: pairs with sine 0 are not to be mixed (see RowLane::copied).
   __device__ __forceinline__ void back(const Pairs<VEC>& d, Pairs<VEC>& g, bool copied) const {
 #pragma unroll
@@ -174,13 +233,21 @@ struct Turn {
 template <int VEC>
 struct Factors {
   uint64_t A[kRowPairs<VEC> / 2], B[kRowPairs<VEC> / 2], C[kRowPairs<VEC> / 2], E[kRowPairs<VEC> / 2];
-  __device__ __forceinline__ void set(const Turn<VEC>& t, const Pairs<VEC>* w) {
+  __device__ __forceinline__ void set(const Turn<VEC>& t) {
 #pragma unroll
     for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
-      A[j] = w ? fmul2(w->a[j], t.c[j]) : t.c[j];
-      B[j] = minus(w ? fmul2(w->b[j], t.s[j]) : t.s[j]);
-      C[j] = w ? fmul2(w->b[j], t.c[j]) : t.c[j];
-      E[j] = w ? fmul2(w->a[j], t.s[j]) : t.s[j];
+      A[j] = C[j] = t.c[j];
+      B[j] = minus(t.s[j]);
+      E[j] = t.s[j];
+    }
+  }
+  __device__ __forceinline__ void weigh(const Pairs<VEC>& w) {
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      A[j] = fmul2(w.a[j], A[j]);
+      B[j] = fmul2(w.b[j], B[j]);
+      C[j] = fmul2(w.b[j], C[j]);
+      E[j] = fmul2(w.a[j], E[j]);
     }
   }
   // `copied`: as for Turn::back.
@@ -256,32 +323,27 @@ struct RowLane {
   // The cosines and sines of the row's pairs at token (b, t).
   __device__ __forceinline__ void angles(const Turns<VEC>& turns, const void* positions, int bits, const int64_t (&ps)[3],
                                          int64_t b, int64_t t, int lane, Turn<VEC>& out) const {
-    float cs[kRowPairs<VEC>], sn[kRowPairs<VEC>];
+    uint32_t f[kRowPairs<VEC>];  // nearest multiples of 2^-32 turns
 #pragma unroll
     for (int i = 0; i < kRowChunks<VEC>; ++i)
       if ((turned >> i) & 1u) {
         const int64_t here = b * ps[1] + t * ps[2];
-        uint64_t p = 0;
+        const int c = lane + 32 * i;
+        const uint64_t first = position_at(positions, bits, turns.axis[turns.at(c, 0)] * ps[0] + here);
+        const bool several = turns.several[c];  // mostly a chunk follows one axis
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const int at = turns.at(lane + 32 * i, j);
-          // Pairs beside one another mostly follow the same axis.
-          const int axis = turns.axis[at];
-          if (j == 0 || axis != turns.axis[turns.at(lane + 32 * i, j - 1)])
-            p = position_at(positions, bits, axis * ps[0] + here);
-          // Nearest multiple of 2^-32 turns, as a signed fraction of half a turn (see fa4d_rotary.cu).
-          const int32_t frac = static_cast<int32_t>((p * turns.turn[at] + 0x80000000ull) >> 32);
-          sincospif(static_cast<float>(frac) * 4.656612873077393e-10f, &sn[VEC * i + j], &cs[VEC * i + j]);  // 2^-31
+          const int at = turns.at(c, j);
+          uint64_t p = first;
+          if (several) p = position_at(positions, bits, turns.axis[at] * ps[0] + here);
+          f[VEC * i + j] = static_cast<uint32_t>((p * turns.turn[at] + 0x80000000ull) >> 32);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) cs[VEC * i + j] = 1.f, sn[VEC * i + j] = 0.f;
+        for (int j = 0; j < VEC; ++j) f[VEC * i + j] = 0;  // cosine 1 and sine 0, exactly
       }
 #pragma unroll
-    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
-      out.c[j] = f2(cs[2 * j], cs[2 * j + 1]);
-      out.s[j] = f2(sn[2 * j], sn[2 * j + 1]);
-    }
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) cos_sin2(f[2 * j], f[2 * j + 1], out.c[j], out.s[j]);
   }
   // Chunks that are copied keep apart what the turn would mix: 0 * infinity is not a number.
   __device__ __forceinline__ bool copied() const { return turned != live; }
@@ -362,9 +424,12 @@ __device__ __forceinline__ void norm_heads(const fa4d_rotary_table& tab, const T
     if (h0 == first && live) {
       Turn<VEC> turn;
       at.angles(turns, positions, bits, ps, b, t, lane, turn);
-      Pairs<VEC> w;
-      if (weights) at.weights(*weights, lane, w);
-      factors.set(turn, weights ? &w : nullptr);
+      factors.set(turn);
+      if (weights) {
+        Pairs<VEC> w;
+        at.weights(*weights, lane, w);
+        factors.weigh(w);
+      }
     }
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
