@@ -112,6 +112,19 @@ int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, boo
 // 24.7 / 18.9 at 32768; Hq16 Hk4 D256, 128 rows: 16.9 / 18.1 at 512 and 24.5 / 21.8 at 2048.
 constexpr int64_t kDecodePrefix = 1 << 22;
 
+// Keys of a unit (as a power of two) and CTAs of an SM of decode8_kernel.
+struct Shape8 {
+  int shift, ctas;
+};
+template <int D>
+Shape8 shape8_of(int cols) {
+  return {fa4d::kUnit8Shift<D>, cols == 1 ? fa4d::kCtas8<D, 1> : fa4d::kCtas8<D, 2>};
+}
+Shape8 shape8_of(int D, int64_t R) {
+  const int cols = fa4d::decode8_cols(R);
+  return D == 64 ? shape8_of<64>(cols) : D == 96 ? shape8_of<96>(cols) : D == 128 ? shape8_of<128>(cols) : shape8_of<256>(cols);
+}
+
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights, bool cache8, Plan* out) {
@@ -130,7 +143,7 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   p.G = Hq / Hk;
   p.R = T * p.G;
   p.tiles = (p.R + 15) / 16;
-  p.unit_shift = !cache8 ? fa4d::kUnitShift : D == 64 ? fa4d::kUnit8Shift<64> : D == 256 ? fa4d::kUnit8Shift<256> : fa4d::kUnit8Shift<128>;
+  p.unit_shift = cache8 ? shape8_of(D, p.R).shift : fa4d::kUnitShift;
   const int sms = fa4d::host_sm_count();
   if (cache8 ? P > 0 : (rows + 15) / 16 * P * Hk * D > kDecodePrefix) {
     out->split_keys = D != 256 && rows <= 128;
@@ -145,7 +158,7 @@ int plan_prefix(int B, int T, int Hq, int Hk, int D, int P, int C, bool weights,
   }
   p.prefix_units = (P + fa4d::kUnitKeys - 1) / fa4d::kUnitKeys;
   p.seg_rows = static_cast<int>(std::min<int64_t>(16, p.prefix_tiles ? rows : p.R));
-  out->ctas = sms * (D == 256 && !cache8 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
+  out->ctas = sms * (cache8 ? shape8_of(D, p.R).ctas : D == 256 ? fa4d::kDecodeCtas<256> : fa4d::kDecodeCtas<128>);
   p.min_units = 2;
   const int64_t items = static_cast<int64_t>(p.prefix_tiles) * Hk + static_cast<int64_t>(B) * Hk * p.tiles;
   if (items > (1 << 30)) return fail(FA4D_ERR_UNSUPPORTED, "too many row tiles");

@@ -109,6 +109,12 @@ constexpr int kUnitKeys = 1 << kUnitShift;
 // Of decode8_kernel: K and V of 8 KB, as decode_kernel's at head dim 128.
 template <int D>
 constexpr int kUnit8Shift = D == 64 ? 6 : D == 256 ? 4 : 5;
+// Its column tiles of 8 rows, and its CTAs of an SM: as many as the registers allow, since a unit is a
+// chain of waits (about 1600 clocks) that only other warps fill (1.2 GB of codes, B64 Hk8 D128, 4 rows:
+// 231 us with two CTAs and three stages a warp, 186 with three and two).
+inline int decode8_cols(int64_t R) { return R <= 8 ? 1 : 2; }
+template <int D, int kCols>
+constexpr int kCtas8 = kCols == 1 && D <= 128 ? 3 : 2;
 constexpr int kItemUnits = 2;
 // The prefix's items lie together at the front: with a short prefix the first warps do little but
 // change rows, each time with a wait as long as memory is busy (128 requests, 918 MB of own keys,

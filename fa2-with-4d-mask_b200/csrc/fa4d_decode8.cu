@@ -31,10 +31,10 @@ struct Shape8 {
   static constexpr int kBox = kKeys * kRow;
   static constexpr int kTile = kBoxes * kBox;        // K or V of a unit
   static constexpr int kStage = 2 * kTile;
-  // With 16 rows of head dim 256 the queries stay in shared memory: in registers (64, beside 128 of
-  // output) they spilled.
-  static constexpr bool kQShared = D == 256 && kCols == 2;
-  static constexpr int kStages = kQShared ? 2 : 3;
+  // Where the output takes 128 registers the queries stay in shared memory: in registers (64) they
+  // spilled.
+  static constexpr bool kQShared = kWide * kCols == 512;
+  static constexpr int kStages = (kQShared || kCtas8<D, kCols> == 3 ? 16384 : 24576) / kStage;
   static constexpr int kQ = kDecodeWarps * kStages * kStage;  // [warp][column tile][step][lane] 8 bytes
   static constexpr int kBars = kQ + (kQShared ? kDecodeWarps * kCols * kWide * 16 : 0);
   static constexpr int kBytes = kBars + kDecodeWarps * kStages * 8 + 8 + 1024;  // aligned to 1024
@@ -73,7 +73,7 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 // product's operands (of V, two keys' bytes are interleaved first, which transposes it), and P^T
 // turns between the products by movmatrix.
 template <int D, bool kInt8, int kCols, bool kMask>
-__global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __grid_constant__ Decode8Params p8,
+__global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_kernel(const __grid_constant__ Decode8Params p8,
                                                                        bool after_prefix) {
   using S = Shape8<D, kCols>;
   constexpr int kShift = S::kShift;
@@ -281,11 +281,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
     float2 scale_next;
 #pragma unroll 1
     for (int i = 0; i < S::kStages - 1; ++i) bring_next();
-    begin_item();
-    load_mask(at.u);
-    scale_next = scales(at.u);
+    bool fresh = true;  // at an item's first unit (one copy of that code, too)
 #pragma unroll 1
     for (int it = 0; at.more(); ++it) {
+      if (fresh) {
+        begin_item();
+        load_mask(at.u);
+        scale_next = scales(at.u);
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&full[it % S::kStages], (it / S::kStages) & 1, abort_flag))) {
         // Given up: what is still on its way must land before the CTA ends.
         for (int j = it; j < brought; ++j) mbar_wait_short(&full[j % S::kStages], (j / S::kStages) & 1);
@@ -302,15 +305,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
       const uint8_t* sk = ring + (it % S::kStages) * S::kStage;
       const uint8_t* sv = sk + S::kTile;
 
-      float x[S::kKeyTiles][kCols][4];
+      // Few tiles would be few chains of dependent products: those have two sums.
+      constexpr int kChains = S::kKeyTiles * kCols <= 2 ? 2 : 1;
+      float x[S::kKeyTiles][kCols][4], x2[kChains == 2 ? S::kKeyTiles : 1][kCols][4];
 #pragma unroll
-      for (int i = 0; i < S::kKeyTiles; ++i) {
+      for (int i = 0; i < S::kKeyTiles; ++i)
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][c][e] = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            x[i][c][e] = 0.f;
+            if (kChains == 2) x2[kChains == 2 ? i : 0][c][e] = 0.f;
+          }
 #pragma unroll
-        for (int j = 0; j < S::kSteps; ++j) {
+      for (int j = 0; j < S::kSteps; ++j) {
+#pragma unroll
+        for (int i = 0; i < S::kKeyTiles; ++i) {
           const uint4 lo = lds16(sk + S::at(16 * i + key_of(g), 4 * j + q4));
           const uint4 hi = lds16(sk + S::at(16 * i + 8 + key_of(g), 4 * j + q4));
           const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -326,11 +336,18 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
                 q = lds8(queries + ((c * S::kSteps + j) * 4 + k) * 256);
               else
                 q = make_uint2(qf[c][j][2 * k], qf[c][j][2 * k + 1]);
-              mma16(x[i][c], a0, a1, a2, a3, q.x, q.y);
+              mma16(kChains == 2 && (k & 1) ? x2[kChains == 2 ? i : 0][c] : x[i][c], a0, a1, a2, a3, q.x, q.y);
             }
           }
         }
       }
+      if (kChains == 2)
+#pragma unroll
+        for (int i = 0; i < S::kKeyTiles; ++i)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][c][e] += x2[kChains == 2 ? i : 0][c][e];
 
       // -inf where the row does not see the key.
       const int key0 = at.u << kShift;
@@ -406,43 +423,56 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
           }
         if (zl != zl) zl = kNegInf;
       }
-      float ol[kCols][2], oo[kCols][2], w_of[kCols][2], sub[kCols][2];
-      bool grew = false;
+      // A maximum follows the logits only when they pass it by more than 2^kSlack (so weights stay far
+      // below fp16's largest), which one vote over the lanes' own maxima tells: then they are brought
+      // together, and sums and output rescaled.
+      constexpr float kSlack = 8.f;
+      float mx[kCols][2];
+      bool past = false;
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = kNegInf;
+          float x_max = kNegInf;
 #pragma unroll
-          for (int i = 0; i < S::kKeyTiles; ++i) mx = fmaxf(mx, fmaxf(x[i][c][e], x[i][c][e + 2]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx *= f[c][e];
-          const float m_new = fmaxf(m[c][e], mx), n_new = fmaxf(n[c][e], mx + zl);
-          ol[c][e] = m[c][e] == m_new ? 1.f : ex2(m[c][e] - m_new);
-          oo[c][e] = n[c][e] == n_new ? 1.f : ex2(n[c][e] - n_new);
-          grew = grew || ol[c][e] != 1.f || oo[c][e] != 1.f;
-          m[c][e] = m_new;
-          n[c][e] = n_new;
-          sub[c][e] = m_new == kNegInf ? 0.f : m_new;
-          // From a probability under m to a weight under n.  Past 2^126 the probability is 0.
-          w_of[c][e] = ex2(fminf(sub[c][e] + zl - (n_new == kNegInf ? 0.f : n_new), 126.f));
+          for (int i = 0; i < S::kKeyTiles; ++i) x_max = fmaxf(x_max, fmaxf(x[i][c][e], x[i][c][e + 2]));
+          mx[c][e] = x_max * f[c][e];
+          past = past || mx[c][e] > m[c][e] + kSlack || mx[c][e] + zl > n[c][e] + kSlack;
         }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
-          l[c][0] *= ol[c][0];
-          l[c][1] *= ol[c][1];
+          float to[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = mx[c][e];
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+            const float m_new = fmaxf(m[c][e], y), n_new = fmaxf(n[c][e], y + zl);
+            l[c][e] *= m[c][e] == m_new ? 1.f : ex2(m[c][e] - m_new);
+            to[e] = n[c][e] == n_new ? 1.f : ex2(n[c][e] - n_new);
+            m[c][e] = m_new;
+            n[c][e] = n_new;
+          }
 #pragma unroll
           for (int i = 0; i < S::kOutTiles; ++i) {
-            acc[i][c][0] *= oo[c][0];
-            acc[i][c][1] *= oo[c][1];
-            acc[i][c][2] *= oo[c][0];
-            acc[i][c][3] *= oo[c][1];
+            acc[i][c][0] *= to[0];
+            acc[i][c][1] *= to[1];
+            acc[i][c][2] *= to[0];
+            acc[i][c][3] *= to[1];
           }
         }
       }
+      float w_of[kCols][2], sub[kCols][2];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sub[c][e] = m[c][e] == kNegInf ? 0.f : m[c][e];
+          // From a probability under m to a weight under n.  Past 2^126 the probability is 0.
+          w_of[c][e] = ex2(fminf(sub[c][e] + zl - (n[c][e] == kNegInf ? 0.f : n[c][e]), 126.f));
+        }
       uint32_t pf[S::kKeyTiles][kCols][2];
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
@@ -502,11 +532,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 2) decode8_kernel(const __g
         }
       }
       if (at.u + 1 == at.units || at.left == 1) end_item();
-      if (at.advance(p, lengths) && at.more()) {
-        begin_item();
-        load_mask(at.u);
-        scale_next = scales(at.u);
-      }
+      fresh = at.advance(p, lengths);
     }
   }
   if (lane == 0 && *reinterpret_cast<volatile int*>(abort_flag)) atomicOr(p.status, FA4D_DEV_TIMEOUT_PREFIX);
@@ -524,8 +550,7 @@ cudaError_t launch_t(const Decode8Params& p, int ctas, bool after_prefix, cudaSt
 
 template <int D, bool kInt8>
 cudaError_t launch_d(const Decode8Params& p, int ctas, bool after_prefix, cudaStream_t s) {
-  // One column tile serves up to 8 rows of a request and KV head; of more, 16 at a time.
-  if (p.d.R <= 8)
+  if (decode8_cols(p.d.R) == 1)
     return p.d.mask ? launch_t<D, kInt8, 1, true>(p, ctas, after_prefix, s) : launch_t<D, kInt8, 1, false>(p, ctas, after_prefix, s);
   return p.d.mask ? launch_t<D, kInt8, 2, true>(p, ctas, after_prefix, s) : launch_t<D, kInt8, 2, false>(p, ctas, after_prefix, s);
 }

@@ -84,6 +84,11 @@ CASES = [
     (3, 2, 12, 2, 96, 400, 66, BF16, E4M3, "bshd"),
     (2, 1, 16, 1, 128, 0, 3000, BF16, E4M3, "bhsd"),
     (140, 1, 2, 1, 128, 0, 200, FP16, E4M3, "bshd"),
+    (2, 3, 16, 2, 128, 0, 150, BF16, E4M3, "bshd"),  # 24 rows
+    (1, 5, 14, 1, 96, 0, 130, FP16, INT8, "bhsd"),  # 70 rows, the last tile with 6
+    (2, 1, 33, 1, 64, 0, 200, FP16, E4M3, "bhsd"),  # 33 rows
+    (3, 2, 12, 1, 96, 0, 65, BF16, E4M3, "bshd"),
+    (2, 9, 8, 4, 64, 70, 100, BF16, INT8, "bshd"),
 ]
 
 
