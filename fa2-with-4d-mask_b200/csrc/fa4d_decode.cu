@@ -404,12 +404,15 @@ struct Joined {
   int64_t each, first;
   Shares shares;
 
-  // Before the partial results are there: what the lengths tell.
-  __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane) : p(params), b(b_), hk(hk_) {
+  // Before the partial results are there: what the lengths tell.  `divide`: the division too, as
+  // decode_kernel works it out where no prefix kernel runs beside it.
+  __device__ __forceinline__ Joined(const DecodeParams& params, int b_, int hk_, int lane, bool divide) : p(params), b(b_), hk(hk_) {
     keys = length_of(p, b);
     each = static_cast<int64_t>(p.groups) * p.tiles;
-    first = static_cast<int64_t>(p.prefix_tiles) * p.groups * (p.prefix_units + kPrefixItemUnits) +
-            line_before(p.lengths, p.C, b, lane, p.unit_shift) * each;
+    const int64_t prefix_all = static_cast<int64_t>(p.prefix_tiles) * p.groups * (p.prefix_units + kPrefixItemUnits);
+    first = prefix_all + line_before(p.lengths, p.C, b, lane, p.unit_shift) * each;
+    if (divide)
+      shares = even_shares(prefix_all + line_before(p.lengths, p.C, p.B, lane, p.unit_shift) * each, p.warps, p.min_units);
   }
   // Of an item of `count` units that starts at `from` on the line.
   __device__ __forceinline__ Parts of_units(int64_t from, int count, int64_t item, int row) const {
@@ -448,19 +451,21 @@ __device__ __forceinline__ float log2_sum(float m, float l) {
 // latency: partial rows are loaded ahead of the maximum that scales them (about 3 us for 42 parts
 // of 32 rows, 8 us behind a decode kernel of 296 CTAs at B32 Hq32).
 template <int D, bool kBF16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_warps) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_warps, bool divide) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  Joined at(p, blockIdx.z, blockIdx.y, lane);
-  pdl_wait();
-  pdl_launch();
-  at.load_shares();
-
+  Joined at(p, blockIdx.z, blockIdx.y, lane, divide);
   const int r = (blockIdx.x * (blockDim.x / 32) + wid) / row_warps;
   Parts x{}, y{};
+  if (!divide) {
+    pdl_wait();
+    at.load_shares();
+  }
   if (r < p.R) {
     x = at.prefix(r);
     y = at.own(r);
   }
+  pdl_wait();
+  pdl_launch();
   const int share = (x.n + y.n + row_warps - 1) / row_warps;
   const int n0 = min(wid % row_warps * share, x.n + y.n), n = min(n0 + share, x.n + y.n);
   float acc[D / 32];
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) weigh_kernel(const __grid_con
   constexpr int kRows = 64;
   __shared__ float lse[kRows];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  Joined at(p, blockIdx.z, blockIdx.y, lane);
+  Joined at(p, blockIdx.z, blockIdx.y, lane, false);
   const int key0 = blockIdx.x * kWeighTimes * kWeighKeys + 4 * threadIdx.x;
   float* weights = p.weights + at.b * p.weights_stride[0] + at.hk * p.weights_stride[1];
   if (blockIdx.x * kWeighTimes * kWeighKeys < at.keys) {
@@ -697,7 +702,12 @@ cudaError_t launch_join_d(const DecodeParams& p, bool bf16, int sms, cudaStream_
     warps = ((all + blocks - 1) / blocks + row_warps - 1) / row_warps * row_warps;
   const dim3 grid(blocks, p.Hk, p.B);
   auto kern = bf16 ? join_kernel<D, true> : join_kernel<D, false>;
-  const cudaError_t e = launch_chained(kern, grid, 32 * warps, 0, 1, s, p, row_warps);
+  // Few blocks work the division out while decode_kernel's last CTAs run, which spares them a wait
+  // (1 request, 4000 own keys in 8 bits: 10.8 us a call so for 9.8, 16 requests of 24 rows 39.2 and
+  // 38.3); of many the division holds up what is still running (48 requests of 64 rows, 384 blocks:
+  // 33.6 us and 37.0).
+  const bool divide = !p.load.items && static_cast<int64_t>(blocks) * p.Hk * p.B <= 2LL * sms;
+  const cudaError_t e = launch_chained(kern, grid, 32 * warps, 0, 1, s, p, row_warps, divide);
   if (e != cudaSuccess || !p.weights) return e;
   const dim3 weigh((p.C + kWeighTimes * kWeighKeys - 1) / (kWeighTimes * kWeighKeys), p.Hk, p.B);
   return launch_chained(weigh_kernel, weigh, kJoinThreads, 0, 1, s, p);

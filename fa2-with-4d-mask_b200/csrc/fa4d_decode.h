@@ -164,6 +164,16 @@ __device__ __forceinline__ int units_of(int keys, int shift) { return (keys + (1
 // What an item of so many keys takes of the line.
 __device__ __forceinline__ int line_of(int keys, int shift) { return keys > 0 ? units_of(keys, shift) + kItemUnits : 0; }
 
+// a / b for a >= 0, b > 0, in 32 bits where that does (a 64-bit division is five times as long).
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+  return a >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
+
+// The division of `total` units among so many warps where no prefix kernel runs beside them.
+__device__ __forceinline__ Shares even_shares(int64_t total, int warps, int least) {
+  return Shares{warps, max(static_cast<int>(quotient(total + warps - 1, warps)), least), 0, 0};
+}
+
 // What the requests before b (all of them for b = B) take of the line, per KV head and row tile.
 __device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, int b, int lane, int shift) {
   int64_t n = 0;

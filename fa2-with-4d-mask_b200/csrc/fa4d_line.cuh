@@ -26,7 +26,7 @@ __device__ __forceinline__ Shares shares_of(const DecodeParams& p, int64_t total
       return Shares{early, max(up(total - static_cast<int64_t>(late) * rest, early), least), late, 0};
     }
   }
-  return Shares{p.warps, max(up(total, p.warps), least), 0, 0};
+  return even_shares(total, p.warps, least);
 }
 
 __device__ __forceinline__ int64_t warp_start(const Shares& s, int64_t warp) {
@@ -34,7 +34,7 @@ __device__ __forceinline__ int64_t warp_start(const Shares& s, int64_t warp) {
 }
 __device__ __forceinline__ int64_t warp_of(const Shares& s, int64_t unit) {
   const int64_t early = static_cast<int64_t>(s.early) * s.each;
-  return unit < early ? unit / s.each : s.early + (unit - early) / max(s.late, 1);
+  return unit < early ? quotient(unit, s.each) : s.early + quotient(unit - early, max(s.late, 1));
 }
 
 // The lengths of the first 128 requests in a warp's registers (lane l: l, l + 32, ...), the
