@@ -261,7 +261,8 @@ int prefix_attention(const fa4d_prefix_attention_args& args, const fa4d_prefix_a
   // Codes of a slot's heads lie beside one another, 64 to 256 bytes each: the warps of a CTA take
   // neighbouring heads of the same slots, whose bytes memory then reads together.
   if (cache8 && a->k_stride[1] != a->D) {
-    p.heads = a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
+    p.head_shift = a->Hk % 4 == 0 ? 2 : a->Hk % 2 == 0 ? 1 : 0;
+    p.heads = 1 << p.head_shift;
     p.groups /= p.heads;
     p.warps /= p.heads;
   }

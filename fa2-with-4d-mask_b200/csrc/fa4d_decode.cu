@@ -420,7 +420,7 @@ struct Joined {
     if (count > 0) {
       const int64_t w0 = warp_of(shares, from);
       x.n = static_cast<int>(warp_of(shares, from + count - 1) - w0 + 1);
-      x.first = ((w0 + item) * p.heads + hk % p.heads) * p.seg_rows + row;
+      x.first = (((w0 + item) << p.head_shift) + (hk & (p.heads - 1))) * p.seg_rows + row;
     }
     return x;
   }
@@ -430,7 +430,7 @@ struct Joined {
   }
   // The parts of row r: of its own keys, and of the prefix.
   __device__ __forceinline__ Parts own(int r) const {
-    const int64_t i = static_cast<int64_t>(hk / p.heads) * p.tiles + r / 16;
+    const int64_t i = static_cast<int64_t>(hk >> p.head_shift) * p.tiles + r / 16;
     return of_units(first + i * line_of(keys, p.unit_shift), units_of(keys, p.unit_shift), static_cast<int64_t>(p.prefix_tiles) * p.groups + b * each + i, r % 16);
   }
   __device__ __forceinline__ Parts prefix(int r) const {
@@ -450,22 +450,25 @@ __device__ __forceinline__ float log2_sum(float m, float l) {
 // Joins the output: row_warps warps a row, each a share of its parts.  Everything here is
 // latency: partial rows are loaded ahead of the maximum that scales them (about 3 us for 42 parts
 // of 32 rows, 8 us behind a decode kernel of 296 CTAs at B32 Hq32).
-template <int D, bool kBF16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_warps, bool divide) {
+template <int D, bool kBF16, bool kDivide>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int row_warps) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  Joined at(p, blockIdx.z, blockIdx.y, lane, divide);
+  Joined at(p, blockIdx.z, blockIdx.y, lane, kDivide);
   const int r = (blockIdx.x * (blockDim.x / 32) + wid) / row_warps;
   Parts x{}, y{};
-  if (!divide) {
+  if constexpr (!kDivide) {
     pdl_wait();
+    pdl_launch();
     at.load_shares();
   }
   if (r < p.R) {
     x = at.prefix(r);
     y = at.own(r);
   }
-  pdl_wait();
-  pdl_launch();
+  if constexpr (kDivide) {
+    pdl_wait();
+    pdl_launch();
+  }
   const int share = (x.n + y.n + row_warps - 1) / row_warps;
   const int n0 = min(wid % row_warps * share, x.n + y.n), n = min(n0 + share, x.n + y.n);
   float acc[D / 32];
@@ -701,13 +704,14 @@ cudaError_t launch_join_d(const DecodeParams& p, bool bf16, int sms, cudaStream_
   if (static_cast<int64_t>(blocks) * p.Hk * p.B > 3LL * sms)
     warps = ((all + blocks - 1) / blocks + row_warps - 1) / row_warps * row_warps;
   const dim3 grid(blocks, p.Hk, p.B);
-  auto kern = bf16 ? join_kernel<D, true> : join_kernel<D, false>;
   // Few blocks work the division out while decode_kernel's last CTAs run, which spares them a wait
   // (1 request, 4000 own keys in 8 bits: 10.8 us a call so for 9.8, 16 requests of 24 rows 39.2 and
   // 38.3); of many the division holds up what is still running (48 requests of 64 rows, 384 blocks:
   // 33.6 us and 37.0).
   const bool divide = !p.load.items && static_cast<int64_t>(blocks) * p.Hk * p.B <= 2LL * sms;
-  const cudaError_t e = launch_chained(kern, grid, 32 * warps, 0, 1, s, p, row_warps, divide);
+  auto kern = divide ? (bf16 ? join_kernel<D, true, true> : join_kernel<D, false, true>)
+                     : (bf16 ? join_kernel<D, true, false> : join_kernel<D, false, false>);
+  const cudaError_t e = launch_chained(kern, grid, 32 * warps, 0, 1, s, p, row_warps);
   if (e != cudaSuccess || !p.weights) return e;
   const dim3 weigh((p.C + kWeighTimes * kWeighKeys - 1) / (kWeighTimes * kWeighKeys), p.Hk, p.B);
   return launch_chained(weigh_kernel, weigh, kJoinThreads, 0, 1, s, p);

@@ -53,7 +53,8 @@ struct DecodeParams {
   int32_t prefix_units;  // units of a prefix item
   int32_t unit_shift;    // keys of a unit, as a power of two: kUnitShift, or as the 8-bit kernel takes them
   int32_t seg_rows;      // rows kept of a segment: min(16, R or the batch's rows)
-  int32_t heads;         // KV heads that neighbouring warps take side by side (decode8_kernel; otherwise 1)
+  int32_t heads;         // KV heads that neighbouring warps take side by side (decode8_kernel: 1, 2 or 4; otherwise 1)
+  int32_t head_shift;    // log2(heads)
   int32_t groups;        // Hk / heads
   int32_t warps;         // warps of the grid / heads: those that take runs of the line
   int32_t min_units;     // least units of a warp
