@@ -18,10 +18,9 @@ constexpr int kRows = 16;  // rows of a block
 struct AppendGrid {
   int chunks, lanes;
   uint32_t cache_blocks;
-  uint32_t spans;                // 8-bit caches: 64-slot blocks that T tokens can touch
-  uint32_t groups;          // of kRows tokens
-  int q_each, k_each;       // heads of a block, of q and (16-bit caches) of k and of v
-  int q_parts, k_parts;
+  uint32_t spans;      // 8-bit caches: 64-slot blocks that T tokens can touch
+  uint32_t groups;     // of kRows tokens
+  int q_each, k_each;  // heads of a block, of q and (16-bit caches) of k and of v
 };
 
 __device__ __forceinline__ int64_t entries_of(const fa4d_rotary_append_args& a, int64_t b) {
@@ -46,13 +45,14 @@ __device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, cons
   const RowLane<VEC, kAdj> at(a.table, lane, g.chunks);
   const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1];
   uint16_t* dst = static_cast<uint16_t*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1];
-  norm_heads<kBF16, kAdj, VEC, kHeads>(a.table, turns, at, args.norm.q_weight ? &shared_w : nullptr, args.norm.eps, g.lanes, lane, live, src,
-                                  a.q_stride[2], dst, a.q_out_stride[2], first, min(first + g.q_each, a.Hq), a.positions,
-                                  a.positions_bits, a.positions_stride, b, t);
+  norm_heads<kBF16, kAdj, VEC, kHeads>(a.table, turns, at, args.norm.q_weight ? &shared_w : nullptr, args.norm.eps, g.lanes,
+                                       lane, live, src, a.q_stride[2], dst, a.q_out_stride[2], first,
+                                       min(first + g.q_each, a.Hq), a.positions, a.positions_bits, a.positions_stride, b, t);
 }
 
 // 16-bit caches.  A decode step has few tokens: everything is spread over the grid, and latency
-// bounds it.
+// bounds it (160 tokens, Hq16 Hk4 D256: 4.0 us back to back; with four rows of q in flight, whose
+// registers leave fewer blocks an SM, 4.5).
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                           const __grid_constant__ AppendGrid g, int* status) {
@@ -98,7 +98,10 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
 
 // 8-bit caches: a block of threads has a 64-slot block of one request, head and cache.  The new
 // tokens' values wait in shared memory, in 32 bits, until their largest magnitude is known; then the
-// scale, the earlier codes anew where it grows, and the new codes.
+// scale, the earlier codes anew where it grows, and the new codes.  One token: latency, 3.1 us; 64
+// tokens 6.9.  Two prompts of 4097 tokens (Hq32 Hk8 D128, 185 MB): 54 us, half of it q's rows, where
+// about 30 M warp instructions at 45% of the issue slots bound it (the angles of each KV head's keys
+// and the two passes over their values; q by a kernel of its own, as in training: 56 us).
 template <bool kBF16, bool kAdj, int VEC, bool kInt8>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                       const __grid_constant__ AppendGrid g, int* status) {
@@ -247,8 +250,10 @@ struct Divisor {
   __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
 };
 
-// One thread: kPieces times 8 codes, a block's threads apart, whose loads are in flight together.
-// Bound by memory: 1 byte read and 2 written an element.
+// One thread: kPieces times 8 codes, a block's threads apart, whose loads are in flight together.  1
+// byte read and 2 written an element; two waits, for the length and for the codes, are a good part of
+// a call's time (64 caches of 300 slots, Hk8 D128, half full: 12.9 us for 10 + 39 MB; 16 bytes a
+// thread, one piece, 17 us; three to seven pieces differ by 8%).
 constexpr int kPieces = 4, kValuesThreads = 128;
 template <bool kBF16, bool kInt8>
 __global__ void __launch_bounds__(kValuesThreads) cache_values_kernel(const __grid_constant__ fa4d_cache_values_args a, Divisor parts,
@@ -284,10 +289,12 @@ __global__ void __launch_bounds__(kValuesThreads) cache_values_kernel(const __gr
     codes_to_float<kInt8>(c[k].x, f);
     codes_to_float<kInt8>(c[k].y, g);
     uint4 v;
-    v.x = pack2<kBF16>(f[0] * scale[k], f[1] * scale[k]);
-    v.y = pack2<kBF16>(f[2] * scale[k], f[3] * scale[k]);
-    v.z = pack2<kBF16>(g[0] * scale[k], g[1] * scale[k]);
-    v.w = pack2<kBF16>(g[2] * scale[k], g[3] * scale[k]);
+    const uint64_t by = f2(scale[k], scale[k]);
+    auto two = [&](float x, float y) {
+      const float2 r = f2_split(fmul2(f2(x, y), by));
+      return pack2<kBF16>(r.x, r.y);
+    };
+    v = make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(g[0], g[1]), two(g[2], g[3]));
     *reinterpret_cast<uint4*>(out + to[k]) = v;
   }
 }
@@ -309,13 +316,11 @@ cudaError_t launch_append_t(const fa4d_norm_append_args& args, int sms, int* sta
   };
   g.q_each = each(a.Hq);
   g.k_each = each(a.Hk);
-  g.q_parts = (a.Hq + g.q_each - 1) / g.q_each;
-  g.k_parts = (a.Hk + g.k_each - 1) / g.k_each;
-  const int64_t q_blocks = static_cast<int64_t>(g.groups) * g.q_parts;
+  const int64_t q_blocks = static_cast<int64_t>(g.groups) * ((a.Hq + g.q_each - 1) / g.q_each);
   int64_t cache_blocks;
   if (args.cache_type == FA4D_CACHE_16BIT) {
     g.spans = 0;
-    cache_blocks = 2LL * g.groups * g.k_parts;
+    cache_blocks = 2LL * g.groups * ((a.Hk + g.k_each - 1) / g.k_each);
   } else {
     g.spans = (a.T + FA4D_CACHE_BLOCK - 2) / FA4D_CACHE_BLOCK + 1;
     cache_blocks = 2LL * a.B * a.Hk * g.spans;

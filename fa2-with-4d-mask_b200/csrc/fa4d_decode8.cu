@@ -63,8 +63,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // c (16 x 8, fp32) += a (16 x 16) b (16 x 8), fp16
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // One warp: its units in order, each 8 KB of K and V brought by TMA into the warp's own ring, keys
@@ -72,9 +72,16 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 // O^T = V^T P^T.  A lane reads 16 codes of a key at once, converts them in registers to the
 // product's operands (of V, two keys' bytes are interleaved first, which transposes it), and P^T
 // turns between the products by movmatrix.
+//
+// With up to 8 rows memory bounds it: 1.21 GB of e4m3 codes (B64 Hk8 D128, 2048 to 16384 entries, 4
+// rows) 186 us with the join, 6.5 TB/s, 99% of the measured copy rate, in both layouts; int8 188.  With
+// 16 rows a unit's conversions, softmax and waits do (about 1000 instructions and 1.7 us of two warps a
+// scheduler, D 64): 48 requests of 64 rows, 26 MB read four times, 33.6 us, of which the join 7 and the
+// start 4; tiles of 32 rows, which read the keys half as often, took 41, for fewer warps share the
+// work.  Units of head dim 256 (16 keys) take 1.9 us: 16 requests of 24 rows, own up to 2050, 38 us.
 template <int D, bool kInt8, int kCols, bool kMask>
-__global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_kernel(const __grid_constant__ Decode8Params p8,
-                                                                       bool after_prefix) {
+__global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_kernel(
+    const __grid_constant__ Decode8Params p8, bool after_prefix) {
   using S = Shape8<D, kCols>;
   constexpr int kShift = S::kShift;
   const DecodeParams& p = p8.d;

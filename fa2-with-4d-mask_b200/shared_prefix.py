@@ -4,7 +4,7 @@ received.
 
 A decode step rotates and appends the new tokens (``MultiAxisRotary.append``), attends
 (``shared_prefix_attention``, which can accumulate ``weights``) and, when caches run full,
-shrinks them (``evict_by_weight``).  Everything is enqueued on the current stream without a
+shrinks them (``evict_by_weight``); caches held in 8 bits are read back by ``cache_values``.  Everything is enqueued on the current stream without a
 host synchronisation, so a step can be captured in a CUDA graph.
 """
 
@@ -51,8 +51,9 @@ def shared_prefix_attention(
         scale: softmax scale, ``head_dim ** -0.5`` by default.
         is_causal: new token t sees the own entries up to its own, ``lengths - T + t``.
         key_scale/value_scale: of own caches held in 8 bits, as ``MultiAxisRotary.append`` writes them
-            (codes ``torch.float8_e4m3fn`` or ``torch.int8``, fp32 scales ``[B, Hk, ceil(C / 64)]``,
-            any of them); the prefix stays in 16 bits, and there are no ``weights``.
+            (codes ``torch.float8_e4m3fn`` or ``torch.int8``, fp32 scales ``[B, Hk, ceil(C / 64)]``, 0
+            or positive, powers of two or not); the prefix stays in 16 bits, and there are no
+            ``weights``.  Weights go to the product with V in fp16, whatever the query's dtype.
 
     Returns:
         The output in the query's layout; rows that see no key are 0.  A row that sees a NaN, or

@@ -432,8 +432,8 @@ size_t fa4d_norm_rotary_bwd_workspace(int32_t B, int32_t T, int32_t Hq, int32_t 
 int fa4d_norm_rotary_bwd(const fa4d_norm_rotary_bwd_args* args, void* stream);
 
 /* A cache in 8 bits: codes [B, C, Hk, D] (e4m3, or int8 from -127 to 127) and an fp32 scale for each
- * block of FA4D_CACHE_BLOCK slots (from slot 0) of a request and head, [B, Hk, ceil(C / block)]; a
- * value is its code times its scale. */
+ * block of FA4D_CACHE_BLOCK slots (from slot 0) of a request and head, [B, Hk, ceil(C / block)], 0
+ * or positive, or NaN; a value is its code times its scale.  e4m3 codes are not the NaN codes. */
 #define FA4D_CACHE_BLOCK 64
 enum fa4d_cache_type { FA4D_CACHE_16BIT = 0, FA4D_CACHE_E4M3 = 1, FA4D_CACHE_INT8 = 2 };
 
@@ -443,7 +443,8 @@ enum fa4d_cache_type { FA4D_CACHE_16BIT = 0, FA4D_CACHE_E4M3 = 1, FA4D_CACHE_INT
  * code (448 or 127); in one that does, the larger of that and the block's scale, and where the scale
  * grows the earlier codes are rounded anew.  An element that is not finite makes the scale of its
  * block NaN until tokens enter the block anew.  Values are rounded to codes once, from fp32.
- * 16-bit caches come with a norm (without: fa4d_rotary_append). */
+ * 16-bit caches come with a norm (without: fa4d_rotary_append).  A cosine or sine is off by at most
+ * 2^-23, beside the angle's own 2^-33 turns. */
 typedef struct fa4d_norm_append_args {
   fa4d_rotary_append_args append; /* weights: must be NULL with an 8-bit cache */
   fa4d_head_norm norm;
@@ -471,8 +472,9 @@ typedef struct fa4d_cache_values_args {
 int fa4d_cache_values(const fa4d_cache_values_args* args, void* stream);
 
 /* fa4d_prefix_attention over own caches in 8 bits (attention.k, attention.v: codes; the prefix stays
- * in 16).  attention.weights must be NULL.  Codes that no token of a request may see can hold
- * anything. */
+ * in 16).  attention.weights must be NULL.  Codes and scales that no token of a request may see can
+ * hold anything; a block whose scale is NaN makes the rows NaN that see one of its entries.  Queries
+ * and codes go to the products exactly, weights are rounded to fp16. */
 typedef struct fa4d_prefix_attention_8bit_args {
   fa4d_prefix_attention_args attention;
   int32_t cache_type;        /* FA4D_CACHE_E4M3 or FA4D_CACHE_INT8 */
