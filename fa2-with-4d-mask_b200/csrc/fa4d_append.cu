@@ -152,17 +152,23 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
     Pairs<VEC> p;
     unpack_pairs<kBF16, kAdj>(raw, p);
     if (i0 + kRows + row < count) at.load(x + (t + kRows) * xs[1], raw);  // on its way meanwhile
+    // Keys with what roundings leave out, so that few of them come to lie on the wrong side of the border
+    // of two codes.  Two prompts of 4097 tokens: of 8.4 million e4m3 keys 12.8 did without, 9.6 do
+    // (means of 20 draws), for 55.6 us against 54.4; shorter appends take as long as without.
+    Pairs<VEC> low;
+#pragma unroll
+    for (int j = 0; j < P / 2; ++j) low.a[j] = low.b[j] = f2(0.f, 0.f);
     if (norm) {
-      p.times(rsqrtf(row_sum(p.squares(), g.lanes) * (1.f / a.table.D) + args.norm.eps));
+      const float square = row_sum(p.squares(), g.lanes);
       Pairs<VEC> w;
       at.weights(shared_w, lane, w);
-      p.times(w);
+      p.normalise(square * (1.f / a.table.D) + args.norm.eps, w, low);
     }
     if (!live) continue;
     if (!is_v) {
       Turn<VEC> turn;
       at.angles(turns, a.positions, a.positions_bits, a.positions_stride, b, t, lane, turn);
-      turn.on(p, at.copied());
+      turn.on_exact(p, low, at.copied());
     }
     uint4* v = values + i0 / kRows * (P / 2) * threads + threadIdx.x;
 #pragma unroll

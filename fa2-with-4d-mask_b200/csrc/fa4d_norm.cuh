@@ -59,6 +59,8 @@ __device__ __forceinline__ float row_sum(float x, int lanes) {
   return x;
 }
 
+__device__ __forceinline__ uint64_t minus(uint64_t x) { return x ^ 0x8000000080000000ull; }
+
 // What a lane holds of a row: pair j is (a_j, b_j) (past the pairs, elements that are copied); two
 // pairs beside one another lie packed, for the packed arithmetic.
 template <int VEC>
@@ -73,11 +75,22 @@ struct Pairs {
     const float2 t = f2_split(s);
     return t.x + t.y;
   }
-  __device__ __forceinline__ void times(const Pairs& w) {
+  // Times w / sqrt(v), and into `low` what the roundings leave out.
+  __device__ __forceinline__ void normalise(float v, const Pairs& w, Pairs& low) {
+    const float r = rsqrtf(v), h = v * r;
+    // One step of Newton's.  Squares beyond fp32 give r = 0, whose step would be 0 times infinity.
+    const float e = fmaf(-h, r, 1.f) - fmaf(v, r, -h) * r, r_low = r > 0.f ? 0.5f * r * e : 0.f;
+    const uint64_t rr = f2(r, r), rl = f2(r_low, r_low);
 #pragma unroll
     for (int j = 0; j < kTwo; ++j) {
-      a[j] = fmul2(a[j], w.a[j]);
-      b[j] = fmul2(b[j], w.b[j]);
+      auto one = [&](uint64_t& x, uint64_t weight, uint64_t& rest) {
+        const uint64_t n = fmul2(x, rr), nl = ffma2(x, rl, ffma2(x, rr, minus(n)));
+        const uint64_t y = fmul2(n, weight);
+        rest = ffma2(nl, weight, ffma2(n, weight, minus(y)));
+        x = y;
+      };
+      one(a[j], w.a[j], low.a[j]);
+      one(b[j], w.b[j], low.b[j]);
     }
   }
   __device__ __forceinline__ void times(float r) {
@@ -188,8 +201,6 @@ struct Weights {
   __device__ __forceinline__ float of(int c, int k) const { return reinterpret_cast<const float*>(&w[(k / 4) * kChunks + c])[k % 4]; }
 };
 
-__device__ __forceinline__ uint64_t minus(uint64_t x) { return x ^ 0x8000000080000000ull; }
-
 // a A + b B, or a A where B is 0 (an infinite b and B = 0 make NaN).
 __device__ __forceinline__ uint64_t mix_apart(uint64_t a, uint64_t A, uint64_t b, uint64_t B) {
   const float2 x = f2_split(a), u = f2_split(A), y = f2_split(b), v = f2_split(B);
@@ -212,6 +223,22 @@ struct Turn {
         p.a[j] = ffma2(a, c[j], fmul2(b, minus(s[j])));
         p.b[j] = ffma2(b, c[j], fmul2(a, s[j]));
       }
+    }
+  }
+  // Turned in place with what roundings left out of p so far (`low`) and of the turn's first products.
+  __device__ __forceinline__ void on_exact(Pairs<VEC>& p, const Pairs<VEC>& low, bool copied) const {
+    if (copied) {  // (a chunk of them is not turned, or single pairs are)
+      on(p, true);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kRowPairs<VEC> / 2; ++j) {
+      const uint64_t a = p.a[j], b = p.b[j], m = minus(s[j]);
+      const uint64_t u = fmul2(b, m), v = fmul2(a, s[j]);
+      const uint64_t lu = ffma2(low.b[j], m, ffma2(low.a[j], c[j], ffma2(b, m, minus(u))));
+      const uint64_t lv = ffma2(low.a[j], s[j], ffma2(low.b[j], c[j], ffma2(a, s[j], minus(v))));
+      p.a[j] = fadd2(ffma2(a, c[j], u), lu);
+      p.b[j] = fadd2(ffma2(b, c[j], v), lv);
     }
   }
   // Turned back.  `copied`: pairs with sine 0 are not to be mixed (see RowLane::copied).

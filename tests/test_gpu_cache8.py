@@ -219,6 +219,25 @@ def test_infinities_and_nan_make_their_block_nan_until_it_starts_anew(code):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("code", [E4M3, INT8])
+def test_squares_beyond_32_bits_become_rows_of_zeros(code):
+    """Finite tokens whose sum of squares is infinite in 32 bits: r = 0, as in a plain norm in 32
+    bits; their neighbours in the block keep a finite scale."""
+    g = torch.Generator().manual_seed(10)
+    rope, (q, k, v, pos, kc, vc, ks, vs) = plain(g, T=5, code=code)
+    k[0, 1, 2] = 1e30
+    k[1, 0, :, 7] = -3e38
+    n = torch.tensor([0, 63], dtype=torch.int32, device=DEV)
+    w = torch.ones(64, device=DEV)
+    rope.append(q, k, v, pos, kc, vc, n, key_scale=ks, value_scale=vs, query_norm=w, key_norm=w)
+    got = [api.cache_values(kc, ks, n + 5)[b, :, n[b]:n[b] + 5].float() for b in range(2)]
+    assert all(bool(torch.isfinite(x).all()) for x in got)
+    assert not got[0][1, 2].any() and not got[1][0].any()
+    for x in (got[0][0], got[0][1, 3], got[1][1]):
+        assert bool((x != 0).any(-1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", [E4M3, INT8])
 def test_full_and_odd_lengths(code):
     """Tokens past the capacity are dropped and count for nothing, in a block that ends there too."""
     g = torch.Generator().manual_seed(10)
