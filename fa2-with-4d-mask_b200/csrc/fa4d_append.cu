@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
 // 8-bit caches: a block of threads has a 64-slot block of one request, head and cache.  The new
 // tokens' values wait in shared memory, in 32 bits, until their largest magnitude is known; then the
 // scale, the earlier codes anew where it grows, and the new codes.  One token: latency, 3.1 us; 64
-// tokens 6.9.  Two prompts of 4097 tokens (Hq32 Hk8 D128, 185 MB): 54 us, half of it q's rows, where
+// tokens 6.9.  Two prompts of 4097 tokens (Hq32 Hk8 D128, 185 MB): 55.6 us, half of it q's rows, where
 // about 30 M warp instructions at 45% of the issue slots bound it (the angles of each KV head's keys
-// and the two passes over their values; q by a kernel of its own, as in training: 56 us).
+// and the two passes over their values; q by a kernel of its own, as in training: 2 us more).
 template <bool kBF16, bool kAdj, int VEC, bool kInt8>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                       const __grid_constant__ AppendGrid g, int* status) {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __g
     for (int i = threadIdx.x; i < all; i += threads) {
       const int r = i / parts;
       uint4* at16 = reinterpret_cast<uint4*>(cache + (start + r) * st[1]) + (i - r * parts);
-      uint4 c = *at16;
+      uint4 c = __ldcg(at16);  // (a sector may hold another head's codes too, written by another SM)
       uint32_t* words = reinterpret_cast<uint32_t*>(&c);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {

@@ -13,14 +13,8 @@
 
 namespace fa4d {
 
-// Two codes to fp16 (exact: e4m3 has 4 significant bits and exponents -9 to 8, int8 7 and a sign),
-// low byte to the low half.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(two));
-  return h;
-}
-// The four codes of a word: a = codes 0 and 1, b = codes 2 and 3.
+// The four codes of a word to fp16 (exact: e4m3 has 4 significant bits and exponents -9 to 8, int8 7
+// and a sign): a = codes 0 and 1, b = codes 2 and 3.
 template <bool kInt8>
 __device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& a, uint32_t& b) {
   if constexpr (kInt8) {

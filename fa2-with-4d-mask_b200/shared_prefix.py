@@ -4,8 +4,9 @@ received.
 
 A decode step rotates and appends the new tokens (``MultiAxisRotary.append``), attends
 (``shared_prefix_attention``, which can accumulate ``weights``) and, when caches run full,
-shrinks them (``evict_by_weight``); caches held in 8 bits are read back by ``cache_values``.  Everything is enqueued on the current stream without a
-host synchronisation, so a step can be captured in a CUDA graph.
+shrinks them (``evict_by_weight``); caches held in 8 bits are read back by ``cache_values``.
+Everything is enqueued on the current stream without a host synchronisation, so a step can be
+captured in a CUDA graph.
 """
 
 from __future__ import annotations
