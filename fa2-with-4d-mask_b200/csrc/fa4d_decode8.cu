@@ -20,6 +20,9 @@ namespace fa4d {
 namespace {
 
 constexpr float kNegInf = -INFINITY;
+// Probabilities are computed 2^kRaise times as large, so that their factors to weights (up to 2^126, where
+// V's scales are far apart) reach all that 32 bits hold.
+constexpr int kRaise = 16;
 
 template <int D, int kCols>
 struct Shape8 {
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_k
     float qs[kCols][2];      // scale log2(e), and what the row was divided by for fp16
     float m[kCols][2];       // running maximum of the logits
     float n[kCols][2];       // of the weights that go to the product with V
-    float l[kCols][2];       // this lane's part of the sum
+    float l[kCols][2];       // this lane's part of the sum, 2^kRaise times as large
     int lim[kCols][2];       // keys below it are seen
     const uint8_t* mrow[kCols][2];
     unsigned seen;           // bit 2 c + e: the column has seen one of this lane's keys
@@ -240,6 +243,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_k
           for (int o = 4; o < 32; o <<= 1) l[c][x] += __shfl_xor_sync(0xffffffffu, l[c][x], o);
           // The output row under the maximum of the logits; a part without weights is 0.
           const float to = n[c][x] == kNegInf ? 1.f : ex2(n[c][x] - m[c][x]);
+          l[c][x] *= 1.f / (1 << kRaise);
           if ((seen >> (2 * c + x)) & 1u) part_of_keys(m[c][x], l[c][x]);
           const int r = 8 * c + 2 * q4 + x;
           if (r >= p.seg_rows) continue;
@@ -434,6 +438,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_k
       // below fp16's largest), which one vote over the lanes' own maxima tells: then they are brought
       // together, and sums and output rescaled.
       constexpr float kSlack = 8.f;
+      static_assert(kRaise > kSlack, "the factors of weights whose probability is above 2^-126 stay below 2^126");
       float mx[kCols][2];
       bool past = false;
 #pragma unroll
@@ -476,8 +481,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_k
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sub[c][e] = m[c][e] == kNegInf ? 0.f : m[c][e];
-          // From a probability under m to a weight under n.  Past 2^126 the probability is 0.
+          sub[c][e] = (m[c][e] == kNegInf ? 0.f : m[c][e]) - kRaise;
+          // From a probability under m to a weight under n.  A weight is at most 2^kSlack (see above), so a
+          // probability whose factor is cut off here is below 2^(kSlack - 126 - kRaise) = 2^-134: 0 in 32 bits.
           w_of[c][e] = ex2(fminf(sub[c][e] + zl - (n[c][e] == kNegInf ? 0.f : n[c][e]), 126.f));
         }
       uint32_t pf[S::kKeyTiles][kCols][2];

@@ -176,3 +176,33 @@ def test_logits_and_scales_that_rise_and_fall(swing, D, Hq, Hk, code):
     lengths = torch.randint(C // 2, C + 1, (B,), generator=g, dtype=torch.int32)
     assert units_of_a_warp(lengths, C, Hq // Hk, D, Hk) >= 6
     check(a, lengths.to(DEV), "bhsd", scale=swing * math.log(2) / (96 * D))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("D,Hq", [(64, 1), (64, 8), (64, 16), (96, 8), (128, 8), (128, 16), (256, 8), (256, 16)])
+@pytest.mark.parametrize("below,above", [(120.5, 28), (125.5, 33)])
+def test_scales_of_values_far_apart(below, above, D, Hq, code):
+    """A block of values of 2^-100 whose logits are 0, then one of 2^above whose logits are -below (in powers
+    of two): the second has 2^7.5 times the first one's part of the output, although its probabilities are
+    near 32 bits' least.  Every request holds the same, and the line is divided between and within them:
+    the bound holds wherever.  (Row tiles that are full: the rows beside have logits of 0.)"""
+    B, C = 2400, 128
+    g = torch.Generator(DEV).manual_seed(5)
+    v = codes(g, (1, 1, C, D), code)
+    k = torch.zeros(1, 1, C, D, device=DEV)
+    k[:, :, 64:, 0] = -96.0
+    k = k.to(torch.int8) if code == INT8 else k.to(E4M3)
+    q = torch.zeros(1, Hq, 1, D, dtype=BF16, device=DEV)
+    q[..., 0] = 1.0
+    ks, vs = torch.tensor([1.0, below / 96], device=DEV), torch.tensor([2.0 ** -100, 2.0 ** above], device=DEV)
+    every = lambda x: x.view(torch.uint8).repeat(B, 1, 1, 1).view(x.dtype)  # noqa: E731
+    a = dict(q=q.repeat(B, 1, 1, 1), pk=None, pv=None, k=every(k), v=every(v), ks=ks.repeat(B, 1, 1), vs=vs.repeat(B, 1, 1))
+    lengths = torch.full((B,), C, dtype=torch.int32, device=DEV)
+    out = call(a, lengths, "bhsd", scale=math.log(2)).double()
+    one = {n: None if x is None else x[:1] for n, x in a.items()}
+    ref, size, top, biggest = formula(one, lengths[:1], "bhsd", scale=math.log(2))
+    e = (D + 16) * 2.0 ** -24 * biggest
+    bound = U[BF16] * ref.abs() + (2.0 ** -11 + 2 * e + 2.0 ** -20) * size + 2.0 ** -25 * C * LARGEST[code] * top
+    off = ((out - ref).abs() / bound).amax((1, 2, 3))
+    assert bool((off <= 1).all()), (float(off.max()), int(off.argmax()))
