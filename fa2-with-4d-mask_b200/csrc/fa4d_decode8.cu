@@ -484,7 +484,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, kCtas8<D, kCols>) decode8_k
           sub[c][e] = (m[c][e] == kNegInf ? 0.f : m[c][e]) - kRaise;
           // From a probability under m to a weight under n.  A weight is at most 2^kSlack (see above), so a
           // probability whose factor is cut off here is below 2^(kSlack - 126 - kRaise) = 2^-134: 0 in 32 bits.
-          w_of[c][e] = ex2(fminf(sub[c][e] + zl - (n[c][e] == kNegInf ? 0.f : n[c][e]), 126.f));
+          // The maxima's difference first, which is exact or nearly: added to V's scale, large logits would lose
+          // the last bits of either.
+          w_of[c][e] = ex2(fminf(sub[c][e] - (n[c][e] == kNegInf ? 0.f : n[c][e]) + zl, 126.f));
         }
       uint32_t pf[S::kKeyTiles][kCols][2];
 #pragma unroll

@@ -206,3 +206,24 @@ def test_scales_of_values_far_apart(below, above, D, Hq, code):
     bound = U[BF16] * ref.abs() + (2.0 ** -11 + 2 * e + 2.0 ** -20) * size + 2.0 ** -25 * C * LARGEST[code] * top
     off = ((out - ref).abs() / bound).amax((1, 2, 3))
     assert bool((off <= 1).all()), (float(off.max()), int(off.argmax()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_large_logits_and_scales_that_are_no_powers_of_two(dtype, code):
+    """Equal keys: every logit is the same, 1.2 million, so the output is the values' mean, whatever a logit's
+    error.  The exponents that weights are made of are differences of logits, and keep their bits."""
+    a = make(6, 3, 1, 4, 2, 64, 0, 1000, dtype, code, "bhsd")
+    a["q"].fill_(64.0)
+    a["k"] = torch.full(a["k"].shape, 96.0, device=DEV).to(code)
+    a["v"] = (a["v"].view(torch.uint8) & 0x7F).view(code)  # positive
+    a["ks"].fill_(2.0)
+    lengths = torch.tensor([1000, 300, 65], dtype=torch.int32)
+    out = call(a, lengths.to(DEV), "bhsd", scale=1.0).double()
+    for b, n in enumerate(lengths.tolist()):
+        v = values_ref(a["v"][b:b + 1], a["vs"][b:b + 1], lengths[b:b + 1].to(DEV))[0, :, :n].repeat_interleave(2, 0)
+        mean, size = v.mean(1, keepdim=True), v.abs().mean(1, keepdim=True)
+        bound = U[dtype] * mean.abs() + (2.0 ** -11 + 2.0 ** -20) * size + 2.0 ** -25 * 448 * float(a["vs"].max()) + 2.0 ** -24
+        off = (out[b] - mean).abs() - bound
+        assert bool((off <= 0).all()), (b, float(off.max()))
