@@ -295,7 +295,9 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) norm_rotary_grad_kernel(
     const float2 both = f2_split(dots);
     const float square = row_sum<kLanes>(x.squares(), lanes), dot = row_sum<kLanes>(both.x + both.y, lanes);
     if (live) {
-      const float r = rsqrtf(square * mean + args.norm.eps), c = -(r * r * (dot * mean));
+      // r times the dot product is of the gradient's size: r^2 alone passes fp32 beside the least epsilons.
+      // Where the squares do (r = 0), the row's output is 0 whatever it holds, and so is its gradient.
+      const float r = rsqrtf(square * mean + args.norm.eps), c = r > 0.f ? -(r * (r * (dot * mean))) : 0.f;
       const uint64_t rr = f2(r, r), cc = f2(c, c);
       x.times(r);
 #pragma unroll

@@ -121,3 +121,27 @@ def test_gradients_of_inputs_that_are_broadcast(dtype):
     d2 = d2.double()
     want, size = d2.sum((0, 1), keepdim=True), d2.abs().sum((0, 1), keepdim=True)
     close(d1, want, U[dtype] * want.abs() + 8 * 2.0 ** -24 * size + 2.0 ** -25)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 22])
+def test_gradients_where_squares_leave_32_bits(D):
+    """Rows of zeros beside the least epsilon, whose r^2 is beyond fp32: dx = r w g.  Rows whose squares are
+    infinite in 32 bits are normalised to zeros whatever they hold, so their gradient is 0."""
+    rope = api.MultiAxisRotary(D, (D // 2,))
+    x = torch.ones(1, 1, 4, D, dtype=BF16, device=DEV)
+    x[0, 0, 1] = 0
+    x[0, 0, 2] = 3e38
+    x[0, 0, 3] = 2.0 ** -100
+    w = torch.linspace(0.5, 1.5, D, device=DEV)
+    pos = torch.zeros(1, 1, 4, dtype=torch.int64, device=DEV)
+    dy = torch.ones_like(x)
+    dy[..., ::2] = 0.5
+    eps = 2.0 ** -130
+    leaf, v = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y, _ = rope(leaf, x, pos, query_norm=v, key_norm=v, eps=eps)
+    assert not y[0, 0, 1:3].any()
+    dx, dw = torch.autograd.grad(y, (leaf, v), dy)
+    rows = [0, 1, 3]
+    gradients_close(dx[:, :, rows], dw, x[:, :, rows], w, dy[:, :, rows], pos[..., rows], (D // 2,), eps, base=1e4)
+    assert not dx[0, 0, 2].any()
