@@ -227,3 +227,20 @@ def test_large_logits_and_scales_that_are_no_powers_of_two(dtype, code):
         bound = U[dtype] * mean.abs() + (2.0 ** -11 + 2.0 ** -20) * size + 2.0 ** -25 * 448 * float(a["vs"].max()) + 2.0 ** -24
         off = (out[b] - mean).abs() - bound
         assert bool((off <= 0).all()), (b, float(off.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hq", [(64, 4), (128, 12), (256, 4)])
+@pytest.mark.parametrize("power", [-126, -118, 100])
+def test_values_of_any_size(power, D, Hq):
+    """Scales of V down to the least that appending writes; steps of bf16's least exponent, and of partial
+    rows in 32 bits, beside the bound."""
+    a = make(7, 12, 1, Hq, 1, D, 0, 1000, BF16, E4M3, "bhsd")
+    a["vs"].fill_(2.0 ** power)
+    a["ks"] *= 16.0  # logits of up to 60 or so: maxima move
+    lengths = torch.randint(1, 1001, (12,), generator=torch.Generator().manual_seed(7), dtype=torch.int32).to(DEV)
+    ref, size, top, biggest = formula(a, lengths, "bhsd")
+    e = (D + 16) * 2.0 ** -24 * biggest
+    bound = U[BF16] * ref.abs() + (2.0 ** -11 + 2 * e + 2.0 ** -20) * size + 2.0 ** -25 * 1000 * 448 * top + 2.0 ** -133
+    off = (call(a, lengths, "bhsd").double() - ref).abs() / bound
+    assert bool((off <= 1).all()), float(off.max())
