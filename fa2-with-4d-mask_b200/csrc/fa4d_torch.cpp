@@ -469,6 +469,81 @@ void set_weights(int64_t (&out)[2], const Tensor& w) {
   out[1] = w.defined() ? w.stride(1) : 0;
 }
 
+// Whether two tensors share a byte.  A byte of x lies at its base + the sum of index * stride +
+// the byte within its element, so they do where whole numbers c, each within the range that the
+// indices leave it, solve  sum c * stride = base of y - base of x  (c of x's dimensions from 0
+// up, of y's from 0 down).
+class Meeting {
+ public:
+  static bool of(const Tensor& x, const Tensor& y) {
+    if (x.numel() == 0 || y.numel() == 0) return false;
+    Meeting m;
+    m.add(x, 1);
+    m.add(y, -1);
+    m.terms.push_back({1, 1 - static_cast<int64_t>(y.element_size()), static_cast<int64_t>(x.element_size()) - 1});
+    return m.solve(static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(x.data_ptr()));
+  }
+
+ private:
+  struct Term {
+    int64_t stride, lo, hi;  // of the number that multiplies the stride
+    // Of the sums of this term and the shorter strides' behind it: the least and the largest, and
+    // whether every number between them is one.
+    int64_t least = 0, most = 0;
+    bool dense = false;
+  };
+  c10::SmallVector<Term, 16> terms;
+  int steps = 0;
+
+  void add(const Tensor& x, int sign) {
+    for (int i = 0; i < x.dim(); ++i) {
+      if (x.size(i) == 1 || x.stride(i) == 0) continue;
+      const int64_t stride = x.stride(i) * static_cast<int64_t>(x.element_size()), last = x.size(i) - 1;
+      terms.push_back({stride, sign > 0 ? 0 : -last, sign > 0 ? last : 0});
+    }
+  }
+
+  bool solve(int64_t sum) {
+    std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.stride > b.stride; });
+    size_t n = 0;  // equal strides make one term
+    for (size_t i = 1; i < terms.size(); ++i) {
+      if (terms[i].stride == terms[n].stride) {
+        terms[n].lo += terms[i].lo;
+        terms[n].hi += terms[i].hi;
+      } else {
+        terms[++n] = terms[i];
+      }
+    }
+    terms.resize(n + 1);
+    int64_t least = 0, most = 0;
+    bool dense = true;
+    for (size_t i = terms.size(); i-- > 0;) {
+      Term& t = terms[i];
+      dense = dense && (t.lo == t.hi || t.stride <= most - least + 1);
+      t.least = least += t.lo * t.stride;
+      t.most = most += t.hi * t.stride;
+      t.dense = dense;
+    }
+    return search(0, sum);
+  }
+
+  // From the longest stride down.  Where strides are nested few numbers fit at each; what is not
+  // decided within the steps counts as shared.
+  bool search(size_t i, int64_t sum) {
+    if (i == terms.size()) return sum == 0;
+    const Term& t = terms[i];
+    if (sum < t.least || sum > t.most) return false;
+    if (t.dense || ++steps > 10000) return true;
+    const int64_t rest_least = t.least - t.lo * t.stride, rest_most = t.most - t.hi * t.stride;
+    auto down = [&](int64_t v) { return v / t.stride - (v % t.stride < 0); };
+    const int64_t from = std::max(t.lo, -down(rest_most - sum)), to = std::min(t.hi, down(sum - rest_least));
+    for (int64_t c = from; c <= to; ++c)
+      if (search(i + 1, sum - c * t.stride)) return true;
+    return false;
+  }
+};
+bool meet(const Tensor& x, const Tensor& y) { return Meeting::of(x, y); }
+
 const char* kScales = "key_scale and value_scale must be fp32 tensors";
 const char* kWeights = "weights must be an fp32 tensor";
 const char* kLengths = "lengths must be a contiguous int32 tensor";
@@ -562,8 +637,10 @@ PyObject* append(PyObject* const* args, PyObject* layout, PyObject* query_norm, 
     refuse("the caches and weights are written in place and may not repeat memory");
   if (cache8) {
     if (repeats(ks) || repeats(vs)) refuse("the scales are written in place and may not repeat memory");
-    if (kc.numel() && (kc.data_ptr() == vc.data_ptr() || ks.data_ptr() == vs.data_ptr()))
-      refuse("keys and values need caches and scales of their own");
+    const Tensor* out[] = {&kc, &vc, &ks, &vs};
+    for (int i = 0; i < 4; ++i)
+      for (int j = i + 1; j < 4; ++j)
+        if (meet(*out[i], *out[j])) refuse("keys and values need caches and scales of their own");
     for (const Tensor* x : {&kc, &vc})
       if (!whole_rows(*x)) refuse("rows of 8-bit caches are written in place and must start on 16-byte boundaries");
   }
@@ -817,81 +894,6 @@ PyObject* cache_values(PyObject* const* args) {
   check(fa4d_cache_values(&a, stream_of(x)), "fa4d_cache_values");
   return THPVariable_Wrap(out);
 }
-
-// Whether two tensors share a byte.  A byte of x lies at its base + the sum of index * stride +
-// the byte within its element, so they do where whole numbers c, each within the range that the
-// indices leave it, solve  sum c * stride = base of y - base of x  (c of x's dimensions from 0
-// up, of y's from 0 down).
-class Meeting {
- public:
-  static bool of(const Tensor& x, const Tensor& y) {
-    if (x.numel() == 0 || y.numel() == 0) return false;
-    Meeting m;
-    m.add(x, 1);
-    m.add(y, -1);
-    m.terms.push_back({1, 1 - static_cast<int64_t>(y.element_size()), static_cast<int64_t>(x.element_size()) - 1});
-    return m.solve(static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(x.data_ptr()));
-  }
-
- private:
-  struct Term {
-    int64_t stride, lo, hi;  // of the number that multiplies the stride
-    // Of the sums of this term and the shorter strides' behind it: the least and the largest, and
-    // whether every number between them is one.
-    int64_t least = 0, most = 0;
-    bool dense = false;
-  };
-  c10::SmallVector<Term, 16> terms;
-  int steps = 0;
-
-  void add(const Tensor& x, int sign) {
-    for (int i = 0; i < x.dim(); ++i) {
-      if (x.size(i) == 1 || x.stride(i) == 0) continue;
-      const int64_t stride = x.stride(i) * static_cast<int64_t>(x.element_size()), last = x.size(i) - 1;
-      terms.push_back({stride, sign > 0 ? 0 : -last, sign > 0 ? last : 0});
-    }
-  }
-
-  bool solve(int64_t sum) {
-    std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.stride > b.stride; });
-    size_t n = 0;  // equal strides make one term
-    for (size_t i = 1; i < terms.size(); ++i) {
-      if (terms[i].stride == terms[n].stride) {
-        terms[n].lo += terms[i].lo;
-        terms[n].hi += terms[i].hi;
-      } else {
-        terms[++n] = terms[i];
-      }
-    }
-    terms.resize(n + 1);
-    int64_t least = 0, most = 0;
-    bool dense = true;
-    for (size_t i = terms.size(); i-- > 0;) {
-      Term& t = terms[i];
-      dense = dense && (t.lo == t.hi || t.stride <= most - least + 1);
-      t.least = least += t.lo * t.stride;
-      t.most = most += t.hi * t.stride;
-      t.dense = dense;
-    }
-    return search(0, sum);
-  }
-
-  // From the longest stride down.  Where strides are nested few numbers fit at each; what is not
-  // decided within the steps counts as shared.
-  bool search(size_t i, int64_t sum) {
-    if (i == terms.size()) return sum == 0;
-    const Term& t = terms[i];
-    if (sum < t.least || sum > t.most) return false;
-    if (t.dense || ++steps > 10000) return true;
-    const int64_t rest_least = t.least - t.lo * t.stride, rest_most = t.most - t.hi * t.stride;
-    auto down = [&](int64_t v) { return v / t.stride - (v % t.stride < 0); };
-    const int64_t from = std::max(t.lo, -down(rest_most - sum)), to = std::min(t.hi, down(sum - rest_least));
-    for (int64_t c = from; c <= to; ++c)
-      if (search(i + 1, sum - c * t.stride)) return true;
-    return false;
-  }
-};
-bool meet(const Tensor& x, const Tensor& y) { return Meeting::of(x, y); }
 
 // evict_by_weight(key, value, weights, lengths, keep, sinks, recent, out, layout) -> (key,
 // value, weights, lengths, index)
