@@ -52,7 +52,8 @@ __device__ __forceinline__ void append_q(const fa4d_norm_append_args& args, cons
 
 // 16-bit caches.  A decode step has few tokens: everything is spread over the grid, and latency
 // bounds it (160 tokens, Hq16 Hk4 D256: 4.0 us back to back; with four rows of q in flight, whose
-// registers leave fewer blocks an SM, 4.5).
+// registers leave fewer blocks an SM, 4.5).  Two prompts of 4097 tokens (Hq32 Hk8 D128, 201 MB): 51.7 us,
+// 59% of the measured copy rate; loads wait two heads at a time, with none fed ahead as in training.
 template <bool kBF16, bool kAdj, int VEC>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                           const __grid_constant__ AppendGrid g, int* status) {
@@ -99,9 +100,10 @@ __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) norm_append_kernel(const
 // 8-bit caches: a block of threads has a 64-slot block of one request, head and cache.  The new
 // tokens' values wait in shared memory, in 32 bits, until their largest magnitude is known; then the
 // scale, the earlier codes anew where it grows, and the new codes.  One token: latency, 3.1 us; 64
-// tokens 6.9.  Two prompts of 4097 tokens (Hq32 Hk8 D128, 185 MB): 55.6 us, half of it q's rows, where
-// about 30 M warp instructions at 45% of the issue slots bound it (the angles of each KV head's keys
-// and the two passes over their values; q by a kernel of its own, as in training: 2 us more).
+// tokens 6.9.  Two prompts of 4097 tokens (Hq32 Hk8 D128, 185 MB): 55.6 us, half of it q's rows.  Nothing
+// is saturated there (issue slots 45%, DRAM 29%, 23% of the warps that an SM holds): 30 M warp
+// instructions, the angles again for each KV head, and the waits of the two passes over their values (q by
+// a kernel of its own, as in training: 2 us more).
 template <bool kBF16, bool kAdj, int VEC, bool kInt8>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 512) append8_kernel(const __grid_constant__ fa4d_norm_append_args args,
                                                                       const __grid_constant__ AppendGrid g, int* status) {

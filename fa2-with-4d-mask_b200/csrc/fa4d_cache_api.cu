@@ -1,7 +1,7 @@
 // fa4d_cache_api.cu — the C ABI of the operators around the attention: rotary positions and
 // their serving form, with and without norms, attention over a shared prefix and own caches of 16
-// or 8 bits, the values of 8-bit caches, eviction.  Argument
-// checks, the division of work and dispatch; nothing is allocated here.
+// or 8 bits, the values of 8-bit caches, eviction.  Argument checks, the division of work and
+// dispatch; nothing is allocated here.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -110,6 +110,11 @@ int prefix_splits(int64_t row_tiles, int Hk, int tiles, int64_t rows, int D, boo
 // caches of 100, Hq32 Hk8 D128: 16 rows 14.0 / 15.2 at P 2048 and 23.2 / 19.8 at 8192; 64 rows
 // 15.5 / 15.5 at 512 and 19.0 / 17.3 at 2048; Hq64 Hk1 D64, 128 rows: 11.0 / 14.2 at 2048 and
 // 24.7 / 18.9 at 32768; Hq16 Hk4 D256, 128 rows: 16.9 / 18.1 at 512 and 24.5 / 21.8 at 2048.
+//
+// decode8_kernel takes no prefix: before own caches in 8 bits the prefix kernel does every one, and the grid
+// behind it is full.  Hq32 Hk8 D128, own 300, 8 bits / 16 bits: 1 request without a prefix 9.0 / 8.6, prefix 16
+// 14.8 / 8.5, 2048 15.3 / 10.1; 8 requests 10.0 / 10.1, 15.4 / 10.9 and 15.9 / 16.7; 32 requests 12.8 / 18.2,
+// 16.6 / 18.4 and 19.4 / 20.6.
 constexpr int64_t kDecodePrefix = 1 << 22;
 
 // Keys of a unit (as a power of two) and CTAs of an SM of decode8_kernel.

@@ -201,7 +201,10 @@ __device__ __forceinline__ int64_t line_before(const int32_t* lengths, int C, in
 // partial rows to join is taken.  Over 18 calls (8 to 256 requests, 1024 to 30000 prefix keys,
 // head dims 64 to 256), each timed with every number of runs, the choice is 1.0% above the best
 // on average and 4% at most (3.3% and 25% with the larger of equal numbers of runs and without
-// that part).
+// that part).  Those calls had 16-bit caches.  Before own caches in 8 bits the choice is made with the same
+// numbers, which are not fitted to decode8_kernel: a unit is 8 KB there for head dims 64, 128 and 256 (4,
+// 8 and 16 KB here), takes 1.6 to 1.9 us of a warp, and an SM holds three CTAs up to 8 rows.  That costs
+// time at most: both kernels divide by what is found here, whatever it is.
 template <int D>
 __device__ __forceinline__ RunChoice choose_runs(const PrefixLoad& w, int64_t units, int lane) {
   const float all = static_cast<float>(units);

@@ -5,10 +5,11 @@
 // g = turn^-1(dy):  dw = sum over rows of g x r,  dx = r (w g - x r^2 mean(w g x)).
 // The backward pass works r out again from x, which it reads in any case.
 //
-// Bound by memory: the forward reads and writes each element once, the backward reads x and dy and
-// writes dx.  Measured, forward and backward: B1 T8192 Hq32 Hk8 D128 bf16 33 and 49 us (168 and 252
-// MB: 5.1 TB/s, 78% of the measured copy rate; two rounds of a block, the second not full), B2 T16385
-// Hq16 Hk8 D256 fp16 130 and 205 us (805 and 1208 MB: 6.2 and 5.9 TB/s).
+// The forward reads and writes each element once, the backward reads x and dy and writes dx, which bounds
+// long inputs.  Measured, forward and backward: B2 T16385 Hq16 Hk8 D256 fp16 130 and 205 us (805 and 1208
+// MB: 6.2 and 5.9 TB/s, 95% and 90% of the measured copy rate).  B1 T8192 Hq32 Hk8 D128 bf16 33 and 49 us
+// (168 and 252 MB: 5.1 TB/s, 78%): there the division bounds it, 512 groups of tokens over 296 blocks of
+// q in two rounds, the second 73% full.
 #include <algorithm>
 
 #include "fa4d.h"
@@ -235,9 +236,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm) norm_rotary_grad_kernel(
   const int lanes = kLanes ? kLanes : grid.lanes;
   using F = Feed<VEC, kAdj, 2, kBwdDepth>;
   constexpr int P = kRowPairs<VEC> / 2;
-  constexpr int kSums = kThreads * 4 * P * 4;
   extern __shared__ uint4 ring4[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>(ring4);  // [max(F::kBytes, kSums)]; in the end the sums, [rows][D]
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ring4);  // [F::kBytes], and in the end the sums, [rows][D]
   __shared__ Turns<VEC> turns;
   __shared__ Weights<VEC> weights;
   const fa4d_rotary_args& a = args.rotary;
@@ -388,7 +388,6 @@ NormGrid grid_of(const fa4d_rotary_args& a, int vec, int per_sm, int waves, int 
   set(a.Hk, g.k_blocks, g.k_parts, g.k_each);
   return g;
 }
-
 
 template <int VEC, bool kBF16, int kLanes>
 cudaError_t launch_fwd_t(const fa4d_norm_rotary_args& a, const NormGrid& g, cudaStream_t s) {

@@ -113,9 +113,10 @@ struct Raw {
 // quarter turn (at most 1/8, rounded to 24 bits), goes to polynomials in y^2, sin(2 pi y) = y S(y^2) and
 // cos(2 pi y) = 1 + y^2 C(y^2), and the quarter swaps them and sets their signs.  The coefficients
 // were fitted for this library (least squares on Chebyshev nodes, reweighted toward the minimax; 3e-9
-// and 3e-10 off); with the arithmetic's rounding the results are off by at most 1.1e-7 (2^-23), over
-// 2 million angles.  About 20 instructions an angle: with sincospif, whose argument has to hold whole
-// half turns as well, angles were a third of what these kernels execute.
+// and 3e-10 off, with the coefficients rounded to fp32 2.4e-8 and 1.3e-8); with the arithmetic's
+// rounding the results are off by at most 2^-23 (1.1e-7 over 2 million angles), and whole quarters are
+// exact.  About 20 instructions an angle: with sincospif, whose argument has to hold whole half turns
+// as well, angles were a third of what these kernels execute.
 __device__ __forceinline__ void cos_sin2(uint32_t f0, uint32_t f1, uint64_t& c, uint64_t& s) {
   const uint32_t q0 = f0 + 0x20000000u, q1 = f1 + 0x20000000u;  // the nearest quarter in the top two bits
   const int32_t r0 = static_cast<int32_t>(f0 - (q0 & 0xC0000000u)), r1 = static_cast<int32_t>(f1 - (q1 & 0xC0000000u));

@@ -110,6 +110,8 @@ class MultiAxisRotary:
                 passes the largest code (448 or 127).  Where new tokens raise a block's scale, its
                 earlier codes are rounded anew; it does not sink until its first slot is written
                 again.  An infinity or NaN makes its block's scale NaN, and so the whole block.
+                The caches and scales may not share memory.  Cosines and sines are those of the form
+                with norms, with or without them: the query can differ in its last bit from a call's.
 
         Returns:
             (turned query, new lengths).  Tokens past the capacity C are not stored: the new

@@ -80,7 +80,8 @@ def cache_values(
     layout: Layout = "bhsd",
 ) -> torch.Tensor:
     """The values of a cache held in 8 bits, in 16: for what takes 16-bit caches (a request's cache
-    becomes a shared prefix, or is evicted from).
+    becomes a shared prefix; or it is evicted from, by weights of the caller's own, since attention
+    over 8-bit caches adds none up).
 
     Args:
         cache: codes, ``torch.float8_e4m3fn`` or ``torch.int8``, ``[B, Hk, C, D]`` ("bhsd") or

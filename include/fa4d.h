@@ -444,7 +444,7 @@ enum fa4d_cache_type { FA4D_CACHE_16BIT = 0, FA4D_CACHE_E4M3 = 1, FA4D_CACHE_INT
  * grows the earlier codes are rounded anew.  An element that is not finite makes the scale of its
  * block NaN until tokens enter the block anew.  Values are rounded to codes once, from fp32.
  * 16-bit caches come with a norm (without: fa4d_rotary_append).  A cosine or sine is off by at most
- * 2^-23, beside the angle's own 2^-33 turns. */
+ * 2^-23, beside the angle's own 2^-33 turns.  8-bit caches and their scales share no memory. */
 typedef struct fa4d_norm_append_args {
   fa4d_rotary_append_args append; /* weights: must be NULL with an 8-bit cache */
   fa4d_head_norm norm;
@@ -473,8 +473,10 @@ int fa4d_cache_values(const fa4d_cache_values_args* args, void* stream);
 
 /* fa4d_prefix_attention over own caches in 8 bits (attention.k, attention.v: codes; the prefix stays
  * in 16).  attention.weights must be NULL.  Codes and scales that no token of a request may see can
- * hold anything; a block whose scale is NaN makes the rows NaN that see one of its entries.  Queries
- * and codes go to the products exactly, weights are rounded to fp16. */
+ * hold anything; a block whose scale is NaN makes the rows NaN that see one of its entries.  Codes go
+ * to the products exactly, and so do queries but for bf16 elements below 2^-32 of the row's largest, which
+ * are rounded to multiples of at most 2^-39 of that; weights are rounded to fp16.  Probabilities below 2^-126
+ * may count as 0. */
 typedef struct fa4d_prefix_attention_8bit_args {
   fa4d_prefix_attention_args attention;
   int32_t cache_type;        /* FA4D_CACHE_E4M3 or FA4D_CACHE_INT8 */
