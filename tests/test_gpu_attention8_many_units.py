@@ -50,13 +50,13 @@ def formula(a, lengths, layout, mask=None, scale=None, causal=True):
         one = torch.tensor([n])
         k, v = (values_ref(x[b:b + 1], s[b:b + 1], one.to(DEV))[0, :, :n] for x, s in ((kc, a["ks"]), (vc, a["vs"])))
         z = a["vs"][b].double().repeat_interleave(BLOCK, 1)[:, :n]
-        rows = q[b].view(Hk, -1, T, D)  # [Hk, G, T, D]
+        rows = q[b].reshape(Hk, Hq // Hk, T, D)  # [Hk, G, T, D]
         seen = torch.ones(T, n, dtype=torch.bool, device=DEV)
         if causal:
             seen = torch.arange(n, device=DEV)[None] < n - T + 1 + torch.arange(T, device=DEV)[:, None]
         seen = seen.expand(Hk, Hq // Hk, T, n)
         if mask is not None:
-            seen = seen & mask[b % mask.shape[0], :, :, :n].expand(Hq, T, n).view(Hk, -1, T, n)
+            seen = seen & mask[b % mask.shape[0], :, :, :n].expand(Hq, T, n).reshape(Hk, Hq // Hk, T, n)
         some = seen.any(2).any(1)  # [Hk, n]: others may hold anything
         k, v = (x.masked_fill(~some[..., None], 0.0) for x in (k, v))
         z = z.masked_fill(~some, 0.0)
